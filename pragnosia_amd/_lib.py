@@ -82,7 +82,19 @@ _RET_I64 = {"pragnosia_aspin_delta_bwd_workspace_bytes", "pragnosia_aspin_prep_t
             "pragnosia_layer_norm_partials", "pragnosia_wgrad_workspace_bytes",
             "pragnosia_aspin_exact_chunk_bwd_workspace_bytes", "pragnosia_aspin_delta_par_bwd_workspace_bytes"}
 
+# the entry points of include/lm/pragnosia_lm.h, in header order
+LM_SIGNATURES = {
+    "pragnosia_lm_abi_version": [],
+    "pragnosia_head_fwd_workspace_bytes": [_i64] * 4,
+    "pragnosia_head_fwd": [_p] * 5 + [_f32] + [_p] * 9 + [_i64] * 5 + [_p],
+    "pragnosia_head_bwd_workspace_bytes": [_i64] * 3,
+    "pragnosia_head_bwd": [_p] * 12 + [_f32] + [_p] * 2 + [_i32, _p] + [_i64] * 5 + [_p],
+}
+
+_LM_RET_I64 = {"pragnosia_head_fwd_workspace_bytes", "pragnosia_head_bwd_workspace_bytes"}
+
 _lib = None
+_lm_lib = None
 
 
 class PragnosiaError(RuntimeError):
@@ -104,6 +116,19 @@ def lib():
                           _i64 if name in _RET_I64 else _i32)
         _lib = L
     return _lib
+
+
+def lm_lib():
+    """The loaded library with the language model's entry points (include/lm/pragnosia_lm.h) set up too."""
+    global _lm_lib
+    if _lm_lib is None:
+        L = lib()
+        for name, args in LM_SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.argtypes = args
+            fn.restype = _i64 if name in _LM_RET_I64 else _i32
+        _lm_lib = L
+    return _lm_lib
 
 
 def check(code: int, what: str) -> None:
