@@ -49,6 +49,20 @@ int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd,
                        const float* p, const float* zl, float tau, void* dh, void* dW, int dw_f32, void* workspace,
                        int64_t workspace_bytes, int64_t n, int64_t V, int64_t d, int64_t K, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Rows of a token table: y_i = scale W[ids_i], n rows; an id outside [0, V) gives a zero row. W (V, d) and y (n, d) fp32
+ * or bf16 (w_bf16, y_bf16), d a multiple of 8; ids (n) int64. n = 0 does nothing. Replaces nn.Embedding of
+ * src/model.py:822-826 (scale 1). */
+int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16, int64_t n,
+                        int64_t V, int64_t d, void* stream);
+
+/* Its gradient: dW[v] = scale sum of g_i over the tokens with ids_i = v, in fp32 in the order of their positions (blocks
+ * of 32 where there are more), zero where there is none; g (n, d) and dW (V, d) fp32 or bf16. No atomics on values, no
+ * memset: the same bits each time, also in a captured step. */
+int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d);
+int pragnosia_embed_bwd(const void* g, int g_bf16, const int64_t* ids, float scale, void* dW, int w_bf16,
+                        void* workspace, int64_t workspace_bytes, int64_t n, int64_t V, int64_t d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

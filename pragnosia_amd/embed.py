@@ -1,0 +1,100 @@
+"""Lookup of token rows with a scale, and its gradient by sorted tokens, on hand-written kernels (csrc/embed.hip; C ABI in
+include/lm/pragnosia_lm.h).
+
+    y = embedding(ids, W, scale)
+
+is scale * W[ids] with a zero row where an id is outside the table (padding). The gradient of W is summed in fp32 over a
+stable order of the tokens by id: no atomics on values, so the same bits each time, and no memset in a captured step,
+where torch's embedding sorts with one past 3072 indices (`src/model.py:822-826` is the reference's lookup)."""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from ._lib import PragnosiaError, check, lm_lib
+from .head import _FLOATS, _INTS, _aligned
+from .ops import _expect, _ptr, _require_gpu, _stream
+
+
+def _check_embed(op: str, ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype) -> None:
+    if ids.dtype not in _INTS:
+        raise PragnosiaError(f"{op}: ids must be integers, got {ids.dtype}")
+    _expect(op, W.device, ids=(ids, (None,)), W=(W, (None, None)))
+    if W.dtype not in _FLOATS or dtype not in _FLOATS:
+        raise PragnosiaError(f"{op}: the table and the rows must be bf16 or fp32, got {W.dtype} and {dtype}")
+    if W.shape[0] == 0 or W.shape[1] == 0 or W.shape[1] % 8:
+        raise PragnosiaError(f"{op}: a table (V, d) with V > 0 and d a multiple of 8 expected, got {tuple(W.shape)}")
+    if not math.isfinite(scale):
+        raise PragnosiaError(f"{op}: scale must be finite, got {scale}")
+
+
+@torch.library.custom_op("pragnosia::embed", mutates_args=())
+def embed(ids: Tensor, W: Tensor, scale: float, bf16: bool) -> Tensor:
+    """ids (n), W (V, d) -> scale W[ids] (n, d), bf16 or fp32."""
+    _require_gpu(ids, W)
+    dtype = torch.bfloat16 if bf16 else torch.float32
+    _check_embed("embed", ids, W, scale, dtype)
+    n, (V, d) = ids.shape[0], W.shape
+    y = torch.empty(n, d, device=W.device, dtype=dtype)
+    ids, Wc = ids.to(torch.int64).contiguous(), _aligned(W)
+    with torch.cuda.device(W.device):
+        check(lm_lib().pragnosia_embed_fwd(_ptr(ids), _ptr(Wc), int(W.dtype == torch.bfloat16), float(scale), _ptr(y),
+                                           int(bf16), n, V, d, _stream(W)), "pragnosia_embed_fwd")
+    return y
+
+
+@embed.register_fake
+def _(ids, W, scale, bf16):
+    return W.new_empty(ids.shape[0], W.shape[1], dtype=torch.bfloat16 if bf16 else torch.float32)
+
+
+@torch.library.custom_op("pragnosia::embed_bwd", mutates_args=())
+def embed_bwd(g: Tensor, ids: Tensor, V: int, scale: float, bf16: bool) -> Tensor:
+    """g (n, d), ids (n) -> dW (V, d), bf16 or fp32."""
+    _require_gpu(g, ids)
+    if g.dtype not in _FLOATS or g.dim() != 2 or g.shape[1] % 8 or g.shape[1] == 0 or V <= 0:
+        raise PragnosiaError(f"embed_bwd: gradients (n, d) in bf16 or fp32 expected, got {tuple(g.shape)} {g.dtype}")
+    _expect("embed_bwd", g.device, ids=(ids, (g.shape[0],)))
+    n, d = g.shape
+    dW = torch.empty(V, d, device=g.device, dtype=torch.bfloat16 if bf16 else torch.float32)
+    g, ids = _aligned(g), ids.to(torch.int64).contiguous()
+    with torch.cuda.device(g.device):
+        L = lm_lib()
+        nbytes = L.pragnosia_embed_bwd_workspace_bytes(n, V, d)
+        if nbytes < 0:
+            raise PragnosiaError(f"embed_bwd: shape n={n} V={V} d={d} rejected")
+        ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
+        check(L.pragnosia_embed_bwd(_ptr(g), int(g.dtype == torch.bfloat16), _ptr(ids), float(scale), _ptr(dW),
+                                    int(bf16), _ptr(ws), nbytes, n, V, d, _stream(g)), "pragnosia_embed_bwd")
+    return dW
+
+
+@embed_bwd.register_fake
+def _(g, ids, V, scale, bf16):
+    return g.new_empty(V, g.shape[1], dtype=torch.bfloat16 if bf16 else torch.float32)
+
+
+def _embed_setup(ctx, inputs, output):
+    ids, W, scale, _ = inputs
+    ctx.save_for_backward(ids)
+    ctx.V, ctx.scale, ctx.bf16 = W.shape[0], scale, W.dtype == torch.bfloat16
+
+
+def _embed_backward(ctx, g):
+    ids, = ctx.saved_tensors
+    return None, embed_bwd(g, ids, ctx.V, ctx.scale, ctx.bf16), None, None
+
+
+embed.register_autograd(_embed_backward, setup_context=_embed_setup)
+
+
+def embedding(ids: Tensor, W: Tensor, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> Tensor:
+    """scale * W[ids], (..., d) in `dtype` (W's by default; the product is rounded once). W (V, d) bf16 or fp32, d a
+    multiple of 8. An id outside [0, V) gives a row of zeros and takes no part in W's gradient."""
+    dtype = dtype or W.dtype
+    if dtype not in _FLOATS:
+        raise PragnosiaError(f"embedding: the rows must be bf16 or fp32, got {dtype}")
+    return embed(ids.reshape(-1), W, float(scale), dtype == torch.bfloat16).view(*ids.shape, W.shape[-1])
