@@ -1,36 +1,40 @@
 // A workgroup's bf16 matrix product over a tile of outputs, shared by the head's kernels: acc(x, y) = sum_k X(x, k) Y(y, k)
-// for 256 x 256 outputs, 8 waves of 128 x 64, v_mfma_f32_16x16x32_bf16.
+// on v_mfma_f32_16x16x32_bf16, WX x WY waves of 16 NA x 16 NB outputs each.
 //
 // Either operand comes in one of two layouts: with the contracted index k running along its rows in memory (KR = false:
 // h, W or dl read along their rows), or down its rows (KR = true: the same matrices contracted over tokens or words).
-// Each step stages 64 values of k of both operands (32 KB each) into one of two LDS buffers, straight from memory
-// (buffer loads to LDS, 16 bytes a lane), while the other buffer is multiplied: one barrier a step, and the loads of a
-// step have the whole step before it to arrive.
+//
+// A step contracts 64 values of k, staged into one of NS LDS buffers straight from memory (buffer loads to LDS, 16 bytes
+// a lane). Step s, in a wave (its first half's fragments are in registers already):
+//     read the second half's fragments;  multiply the first half
+//     wait until stage s + 1 has arrived; barrier (every wave has read all of stage s)
+//     issue the loads of stage s + NS into the buffer of stage s;  read stage s + 1's first half;  multiply the second
+// so that fragment reads run beside products (spread among them by the scheduler's group barriers: 1268 TFLOP/s at 8192^3
+// against 1217 with the reads first), one barrier a step, and a stage has NS - 1 steps to arrive. Stages past the
+// last are issued too, from offsets past the resource (zeros, no memory traffic), so that the wait counts are constants.
 //
 // A buffer load to LDS writes its 64 lanes' 16 bytes consecutively, so the arrangement against bank conflicts is made by
 // which 16 bytes each lane fetches:
 //   KR = false: an LDS row is one row's 64 k (128 bytes, eight segments of 16); segment s of row r holds k segment
-//     s ^ (r / 2 % 8), so that the 16 rows a fragment read touches spread over all segments.
-//   KR = true: an LDS row is one k's 256 columns (512 bytes, 16 granules of 32); granule s of row k holds columns
-//     16 (s ^ f(k)).., f(k) = k % 4 + 4 (k / 8 % 2): the eight rows that half a transposing read touches (k = 8 g +
-//     0 .. 3 for two values of g) lie in eight granules. Read with ds_read_b64_tr_b16.
-// Within a 32-wide k block lane group g holds k = 8 g .. 8 g + 7 of both operands.
+//     s ^ (r % 8).
+//   KR = true: an LDS row is one k's columns, in granules of 16 columns (32 bytes); granule s of row k holds granule
+//     s ^ f(k), read with ds_read_b64_tr_b16. Half a read touches the rows k = 0 .. 3 and 8 .. 11 (of 16), which f
+//     spreads over all banks: f = k % 4 + 4 (k / 8 % 2) where a row is a multiple of 256 bytes, and k / 2 % 2 +
+//     2 (k / 8 % 2) where it is an odd multiple of 128 (odd rows then start in the other half of the banks).
+// Both measured 240 - 250 bytes a clock and compute unit, the rate of consecutive reads. Within a 32-wide k block lane
+// group g holds k = 8 g .. 8 g + 7 of both operands.
 //
 // Range checks: a buffer resource covers exactly the rows that exist, so rows past the operand read as zero; a k segment
-// past the end of a row is fetched from an offset past the resource (zero) for both operands, whatever follows there.
+// past the end of a row, or a column past it, is fetched from an offset past the resource (zero), whatever follows there.
 #pragma once
 #include "mfma_tile.h"
 
 namespace pgn {
 
-constexpr int kGemmTile = 256;      // outputs a side
-constexpr int kGemmK = 64;          // k a step
-constexpr int kGemmStage = kGemmTile * kGemmK * 2;  // bytes of one operand's buffer
-constexpr int kGemmLds = 4 * kGemmStage;
-constexpr int kGemmThreads = 512;
-constexpr int kXcdCount = 8;        // XCDs of an MI355X, taking workgroups in turn
+constexpr int kGemmK = 64;    // k a step
+constexpr int kXcdCount = 8;  // XCDs of an MI355X, taking workgroups in turn
 
-typedef __attribute__((address_space(3))) void lds_ptr_t;
+typedef __attribute__((address_space(3))) void lds_void;
 
 // A matrix operand: `rows` rows of pitch `ld` elements (a multiple of 8) at p (16-byte aligned).
 struct Operand {
@@ -38,93 +42,303 @@ struct Operand {
   int64_t ld, rows;
 };
 
-// The 64 x 256 or 256 x 64 block of `o` that a step contracts: KR = false: rows x0 .., k columns k0 .. (those below
-// k_end); KR = true: k rows k0 .. (below k_end, itself at most o.rows), columns x0 ...
-template <bool KR>
-PGN_DEVICE void stage_operand(const Operand& o, int64_t x0, int64_t k0, int64_t k_end, unsigned char* lds, int tid) {
-  constexpr int kBeyond = 0x7ffffff0;  // past any resource
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if constexpr (!KR) {
-    const int64_t left = min((int64_t)kGemmTile, o.rows - x0);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<__bf16*>(o.p + x0 * o.ld), (short)0, (int)(left * o.ld * 2), 0x00020000);
+// One operand's staging: R rows (KR = false) or columns (KR = true) of the tile, T threads.
+template <bool KR, int R, int T>
+struct Stager {
+  static constexpr int kBytes = R * kGemmK * 2;
+  static constexpr int kLoads = kBytes / (T * 16);
+  static constexpr int kRowBytes = KR ? 2 * R : 128;
+  // Rows that a load of all threads covers: where they are whole and the arrangement repeats after them, a lane's offset
+  // is the same for every load, from a base that moves by kLoadRows rows.
+  static constexpr int kLoadRows = T * 16 / kRowBytes;
+  static constexpr bool kSame = T * 16 % kRowBytes == 0 && kLoadRows % 16 == 0;
+  static constexpr int kOffs = kSame ? 1 : kLoads;
+  static_assert(kBytes % (T * 16) == 0, "whole loads");
+  static_assert(!KR || R % 64 == 0, "the granules of a row are exchanged within aligned groups of four or eight");
+
+  const __bf16* base;  // the tile's first row (KR = false), or row k_begin
+  int64_t bytes;       // from there to the operand's end
+  int64_t step;        // bytes from one stage to the next
+  int pitch;           // bytes of a row
+  int off[kOffs];      // a lane's bytes from base, or past any resource
+  int k_seg;           // KR = false: the lane's first k in a stage
+
+  static PGN_DEVICE int swizzle(int k) {
+    return kRowBytes % 256 == 0 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+  }
+
+  // The tile at x0, k from k_begin to k_end. KR = false: lanes() once, then any number of tiles.
+  PGN_DEVICE void lanes(const Operand& o, int tid) {
+    static_assert(!KR, "");
+    k_seg = 8 * ((tid & 7) ^ ((tid >> 3) & 7));
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = 64 * u + (tid >> 3), seg = (tid & 7) ^ ((tid >> 4) & 7);
-      const int k = (int)k0 + 8 * seg;
-      const int off = k < (int)k_end ? row * (int)o.ld * 2 + 2 * k : kBeyond;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t*)(lds + u * 8192 + w * 1024), 16, off, 0, 0, 0);
-    }
-  } else {
-    const int64_t left = min((int64_t)kGemmK, k_end - k0);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<__bf16*>(o.p + k0 * o.ld), (short)0, (int)(left * o.ld * 2), 0x00020000);
+    for (int u = 0; u < kOffs; ++u) off[u] = ((T / 8) * u + (tid >> 3)) * (int)o.ld * 2 + 2 * k_seg;
+    step = kGemmK * 2;
+    pitch = (int)o.ld * 2;
+  }
+  PGN_DEVICE void tile(const Operand& o, int64_t x0, int64_t k_begin) {
+    base = o.p + x0 * o.ld + k_begin;
+    bytes = (min((int64_t)R, o.rows - x0) * o.ld - k_begin) * 2;
+  }
+  PGN_DEVICE void init(const Operand& o, int64_t x0, int64_t k_begin, int64_t k_end, int tid) {
+    if constexpr (!KR) {
+      lanes(o, tid);
+      tile(o, x0, k_begin);
+    } else {
+      base = o.p + k_begin * o.ld;
+      bytes = (k_end - k_begin) * o.ld * 2;
+      step = kGemmK * o.ld * 2;
+      k_seg = 0;
+      pitch = (int)o.ld * 2;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int k = 16 * u + (tid >> 5), s = tid & 31;
-      const int f = (k & 3) | ((k >> 1) & 4);
-      const int col = (int)x0 + 8 * (s ^ (2 * f));
-      const int off = col < (int)o.ld ? (k * (int)o.ld + col) * 2 : kBeyond;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t*)(lds + u * 8192 + w * 1024), 16, off, 0, 0, 0);
+      for (int u = 0; u < kOffs; ++u) {
+        const int e = u * T + tid, k = e / (kRowBytes / 16), s = e - k * (kRowBytes / 16);
+        const int col = (int)x0 + 8 * (s ^ (2 * swizzle(k)));
+        off[u] = col < (int)o.ld ? (k * (int)o.ld + col) * 2 : 0x7ffffff0;
+      }
     }
   }
-}
 
-// Fragment of 16 rows x0 .. x0 + 15 of an operand for k block kb (32 wide) of a staged buffer.
-template <bool KR>
-PGN_DEVICE bf16x8 staged_frag(const unsigned char* lds, int x0, int kb, int g, int i) {
-  if constexpr (!KR) {
-    return *reinterpret_cast<const bf16x8*>(lds + (x0 + i) * 128 + ((4 * kb + g) ^ ((i >> 1) & 7)) * 16);
-  } else {
-    const int f = (i >> 2) | ((g & 1) << 2);
-    const unsigned char* q = lds + (32 * kb + 8 * g + (i >> 2)) * 512 + (((x0 >> 4) ^ f) * 32) + 8 * (i & 3);
-    return cat8(ds_read_tr(reinterpret_cast<const __bf16*>(q)), ds_read_tr(reinterpret_cast<const __bf16*>(q + 2048)));
+  // Stage s of the range [k_begin, k_end) into lds (wave w's share). A stage past the last loads nothing.
+  PGN_DEVICE void load(int s, int64_t k_count, unsigned char* lds, int w) const {
+    const int64_t at = s * step;
+    const char* p = reinterpret_cast<const char*>(base) + at;
+    const int records = (int)max((int64_t)0, min(bytes - at, (int64_t)0x7fff0000));
+    int beyond = 0;
+    if constexpr (!KR) {
+      // all ones past the range's end: the offset is then past the resource
+      const int room = (int)min(k_count - (int64_t)s * kGemmK, (int64_t)kGemmK);
+      beyond = ((room - 1 - k_seg) >> 31) & 0x7ffffff0;
+    }
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int ahead = kSame ? u * kLoadRows * pitch : 0;
+      const __amdgpu_buffer_rsrc_t r =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p + ahead), (short)0, max(0, records - ahead), 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + u * T * 16 + w * 1024), 16,
+                                               off[kSame ? 0 : u] | beyond, 0, 0, 0);
+    }
   }
+};
+
+// A wave's fragments of a staged operand: 16 rows (or columns) x0 .. of k block kb.
+template <bool KR, int R>
+struct Reader {
+  static constexpr int kRowBytes = KR ? 2 * R : 128;
+  int at[KR ? 8 : 2];  // byte offsets: KR = false: by k block; KR = true: by granule within an aligned eight (or four)
+
+  PGN_DEVICE void init(int x0, int g, int i) {
+    if constexpr (!KR) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) at[kb] = (x0 + i) * 128 + ((4 * kb + g) ^ (i & 7)) * 16;
+    } else {
+      const int f = kRowBytes % 256 == 0 ? (i >> 2) | ((g & 1) << 2) : ((i >> 3) & 1) | ((g & 1) << 1);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        at[q] = (8 * g + (i >> 2)) * kRowBytes + (((x0 >> 4) + q) ^ f) * 32 + 8 * (i & 3);
+    }
+  }
+
+  // fragment q: rows (columns) x0 + 16 q ..; q < 8
+  template <int Q, int KB>
+  PGN_DEVICE bf16x8 get(const unsigned char* lds) const {
+    if constexpr (!KR) {
+      return *reinterpret_cast<const bf16x8*>(lds + at[KB] + Q * 16 * 128);
+    } else {
+      const __bf16* p = reinterpret_cast<const __bf16*>(lds + at[Q] + 32 * KB * kRowBytes);
+      return cat8(ds_read_tr(p), ds_read_tr(p + 4 * kRowBytes / 2));
+    }
+  }
+};
+
+template <int NA_, int NB_, int WX_, int WY_, int NS_>
+struct Tile {
+  static constexpr int NA = NA_, NB = NB_, WX = WX_, WY = WY_, NS = NS_;
+  static constexpr int X = 16 * NA * WX, Y = 16 * NB * WY, kThreads = 64 * WX * WY;
+  static constexpr int kStage = (X + Y) * kGemmK * 2, kLds = NS * kStage;
+  static constexpr int kLdsInfo = kLds + 2 * kThreads * 16;  // with gemm_tiles' row data
+  static constexpr int kLoads = kStage / (kThreads * 16);  // a thread's loads of a stage
+  static_assert(kLdsInfo <= 160 * 1024 && NS >= 2, "");
+};
+
+template <int N>
+PGN_DEVICE void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-// acc[a][b] (a < 8, b < 4): outputs x = x0 + 128 wx + 16 a + 4 g + r, y = y0 + 64 wy + 16 b + i of wave (wx, wy) =
-// (w % 2, w / 2), summed over k in [k_begin, k_end); k_begin a multiple of 64 (for KR = false also k_end <= ld).
-template <bool XKR, bool YKR>
+// Fragments of both halves of a stage, and their products.
+template <class C, bool XKR, bool YKR>
+struct Frags {
+  static constexpr int kX = C::X * kGemmK * 2;  // bytes of X's part of a buffer
+  Reader<XKR, C::X> rx;
+  Reader<YKR, C::Y> ry;
+  bf16x8 fx[2][C::NA], fy[2][C::NB];
+
+  PGN_DEVICE void init(const WaveIdx& t) {
+    rx.init(16 * C::NA * (t.w % C::WX), t.g, t.i), ry.init(16 * C::NB * (t.w / C::WX), t.g, t.i);
+  }
+  template <int KB>
+  PGN_DEVICE void read(const unsigned char* p) {
+    static_for<0, C::NB>([&](auto b) { fy[KB][b.value] = ry.template get<b.value, KB>(p + kX); });
+    static_for<0, C::NA>([&](auto a) { fx[KB][a.value] = rx.template get<a.value, KB>(p); });
+  }
+  // The products of half KB, the reads of the other half (issued before) spread among them: one read, then products.
+  template <int KB>
+  PGN_DEVICE void multiply(f32x4 (&acc)[C::NA][C::NB]) {
+#pragma unroll
+    for (int a = 0; a < C::NA; ++a)
+#pragma unroll
+      for (int b = 0; b < C::NB; ++b) acc[a][b] = pgn_mfma(fx[KB][a], fy[KB][b], acc[a][b]);
+    constexpr int kReads = C::NA * (XKR ? 2 : 1) + C::NB * (YKR ? 2 : 1), kEach = C::NA * C::NB / kReads;
+    static_for<0, kReads>([&](auto) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+      __builtin_amdgcn_sched_group_barrier(0x8, kEach > 0 ? kEach : 1, 0);  // products
+    });
+  }
+};
+
+template <class C>
+PGN_DEVICE void zero_acc(f32x4 (&acc)[C::NA][C::NB]) {
+#pragma unroll
+  for (int a = 0; a < C::NA; ++a)
+#pragma unroll
+    for (int b = 0; b < C::NB; ++b) acc[a][b] = zero4();
+}
+
+// acc[a][b]: outputs x = x0 + 16 NA wx + 16 a + 4 g + r, y = y0 + 16 NB wy + 16 b + i of wave (wx, wy) = (w % WX, w / WX),
+// summed over k in [k_begin, k_end); for KR = false k_end <= ld.
+template <class C, bool XKR, bool YKR>
 PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_t y0, int64_t k_begin, int64_t k_end,
-                          unsigned char* lds, f32x4 (&acc)[8][4]) {
+                          unsigned char* lds, f32x4 (&acc)[C::NA][C::NB]) {
   const WaveIdx t = wave_idx();
-  const int wx = t.w & 1, wy = t.w >> 1, tid = threadIdx.x;
-#pragma unroll
-  for (int a = 0; a < 8; ++a)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) acc[a][b] = zero4();
-  const int steps = (int)((k_end - k_begin + kGemmK - 1) / kGemmK);
-  auto stage = [&](int s) {
-    unsigned char* buf = lds + (s & 1) * kGemmStage;
-    stage_operand<XKR>(X, x0, k_begin + (int64_t)s * kGemmK, k_end, buf, tid);
-    stage_operand<YKR>(Y, y0, k_begin + (int64_t)s * kGemmK, k_end, buf + 2 * kGemmStage, tid);
+  const int tid = threadIdx.x;
+  typedef Frags<C, XKR, YKR> F;
+  Stager<XKR, C::X, C::kThreads> sx;
+  Stager<YKR, C::Y, C::kThreads> sy;
+  sx.init(X, x0, k_begin, k_end, tid), sy.init(Y, y0, k_begin, k_end, tid);
+  F f;
+  f.init(t);
+  const int64_t k_count = k_end - k_begin;
+  const int steps = (int)((k_count + kGemmK - 1) / kGemmK);
+  zero_acc<C>(acc);
+  auto stage = [&](int s, int buf) {
+    unsigned char* p = lds + buf * C::kStage;
+    sx.load(s, k_count, p, t.w), sy.load(s, k_count, p + F::kX, t.w);
   };
-  if (steps > 0) stage(0);
-  for (int s = 0; s < steps; ++s) {
-    // this step's loads have arrived and every wave's reads of the other buffer are done
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (s + 1 < steps) stage(s + 1);
-    const unsigned char* xs = lds + (s & 1) * kGemmStage;
-    const unsigned char* ys = xs + 2 * kGemmStage;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      bf16x8 fx[8], fy[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) fy[b] = staged_frag<YKR>(ys, 64 * wy + 16 * b, kb, t.g, t.i);
-#pragma unroll
-      for (int a = 0; a < 8; ++a) fx[a] = staged_frag<XKR>(xs, 128 * wx + 16 * a, kb, t.g, t.i);
-#pragma unroll
-      for (int a = 0; a < 8; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] = pgn_mfma(fx[a], fy[b], acc[a][b]);
-    }
-  }
-  // the buffers may be written again
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int s = 0; s < C::NS; ++s) stage(s, s);
+  wait_loads<C::kLoads * (C::NS - 1)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  f.template read<0>(lds);
+  int buf = 0;
+  for (int s = 0; s < steps; ++s) {
+    f.template read<1>(lds + buf * C::kStage);
+    f.template multiply<0>(acc);
+    wait_loads<C::kLoads * (C::NS - 2)>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    stage(s + C::NS, buf);
+    buf = buf + 1 == C::NS ? 0 : buf + 1;
+    f.template read<0>(lds + buf * C::kStage);
+    f.template multiply<1>(acc);
+  }
+  // nothing in flight into the buffers, nothing being read: they may be used again
+  wait_loads<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The same for a run of tiles with both operands along their rows, k from 0 to d: tiles at(item) = (x0, y0) for item =
+// first, first + stride, .. below items (first < items), epilogue(acc, x0, y0, info) after each. The stages of the next
+// tile are under way while a tile's last steps and its epilogue run.
+//
+// info: kInfo bytes of data of each of the tile's Y rows (row y's at rows + y kInfo, row_count of them; the rest reads as
+// zero), copied to LDS a tile ahead: into one of two places by the tile's parity, from a tile's first barrier on, when
+// the tile before, that place's last reader, is done; complete at the tile's own first barrier.
+//
+// kStores: how many stores every wave's epilogue issues, last of all. They need not have left before the next tile's first
+// stages are read: those loads were issued before them, and memory operations are counted in order.
+template <class C, int kInfo, int kStores, class At, class Epilogue>
+PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const void* rows, int64_t row_count,
+                           int64_t first, int64_t stride, int64_t items, unsigned char* lds, At&& at,
+                           Epilogue&& epilogue) {
+  static_assert(C::Y * kInfo <= C::kThreads * 16 && kInfo % 8 == 0, "one load a thread");
+  const WaveIdx t = wave_idx();
+  const int tid = threadIdx.x, steps = (int)((d + kGemmK - 1) / kGemmK);
+  typedef Frags<C, false, false> F;
+  Stager<false, C::X, C::kThreads> sx;
+  Stager<false, C::Y, C::kThreads> sy;
+  sx.lanes(X, tid), sy.lanes(Y, tid);
+  F f;
+  f.init(t);
+  // the next stage to load: step ls of tile item `li`
+  int64_t li = first;
+  int ls = 0;
+  auto aim = [&]() {
+    int64_t x0 = 0, y0 = 0;
+    if (li < items) at(li, x0, y0);
+    sx.tile(X, x0, 0), sy.tile(Y, y0, 0);
+    if (li >= items) sx.bytes = sy.bytes = 0;  // loads nothing
+  };
+  auto stage = [&](int buf) {
+    unsigned char* p = lds + buf * C::kStage;
+    sx.load(ls, d, p, t.w), sy.load(ls, d, p + F::kX, t.w);
+    if (++ls == steps) {
+      ls = 0, li += stride;
+      aim();
+    }
+  };
+  unsigned char* const info = lds + C::kLds;
+  auto load_info = [&](int64_t item, int place) {
+    int64_t x0 = 0, y0 = 0;
+    if (item < items) at(item, x0, y0);
+    const int64_t left = item < items && rows != nullptr ? min((int64_t)C::Y, row_count - y0) : 0;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(static_cast<const char*>(rows) + (left > 0 ? y0 * kInfo : 0)), (short)0, (int)(left * kInfo),
+        0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(info + place * C::kThreads * 16 + t.w * 1024), 16, tid * 16,
+                                             0, 0, 0);
+  };
+  aim();
+  load_info(first, 0);
+  for (int s = 0; s < C::NS; ++s) stage(s);
+  wait_loads<C::kLoads * (C::NS - 1)>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  int buf = 0, place = 0;
+  for (int64_t item = first; item < items; item += stride) {
+    int64_t x0, y0;
+    at(item, x0, y0);
+    f32x4 acc[C::NA][C::NB];
+    zero_acc<C>(acc);
+    auto half = [&](int s) {
+      f.template read<1>(lds + buf * C::kStage);
+      f.template multiply<0>(acc);
+      if (s == 0 && item == first)
+        wait_loads<0>();
+      else if (s == 0)
+        wait_loads<kStores>();
+      else
+        wait_loads<C::kLoads * (C::NS - 2)>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s == 0) load_info(item + stride, place ^ 1);
+      stage(buf);
+      buf = buf + 1 == C::NS ? 0 : buf + 1;
+    };
+    f.template read<0>(lds + buf * C::kStage);
+    for (int s = 0; s + 1 < steps; ++s) {
+      half(s);
+      f.template read<0>(lds + buf * C::kStage);
+      f.template multiply<1>(acc);
+    }
+    // the next tile's first fragments are read after the epilogue, which needs their registers
+    half(steps - 1);
+    f.template multiply<1>(acc);
+    epilogue(acc, x0, y0, info + place * C::kThreads * 16);
+    place ^= 1;
+  }
+  wait_loads<0>();
 }
 
 // Tile `item` of a grid of tx x ty tiles (x tiles, y tiles), so ordered that consecutive items share operands: bands of
@@ -136,15 +350,20 @@ PGN_DEVICE void band_tile(int64_t item, int64_t tx, int64_t ty, int64_t& ix, int
   iy = y0 + in - ix * h;
 }
 
-// The item of workgroup `wg` of `items`, the grid rounded up to a multiple of the XCD count: workgroup wg runs on XCD
-// wg % 8, which takes a contiguous run of the items, so neighbours share operands in its L2. -1: none.
-PGN_DEVICE int64_t xcd_item(int64_t wg, int64_t items) {
-  const int64_t per = (items + kXcdCount - 1) / kXcdCount, item = (wg % kXcdCount) * per + wg / kXcdCount;
-  return item < items && wg / kXcdCount < per ? item : -1;
+// Workgroup `wg` runs on XCD wg % 8. An XCD takes a contiguous run of the items, its workgroups neighbours in it at any
+// time, so they share operands in its L2: the items are first, first + stride, .. below end.
+struct XcdRun {
+  int64_t first, stride, end;
+};
+PGN_DEVICE XcdRun xcd_run(int64_t items) {
+  const int64_t per = (items + kXcdCount - 1) / kXcdCount, x = blockIdx.x % kXcdCount;
+  return {x * per + blockIdx.x / kXcdCount, gridDim.x / kXcdCount, min(items, (x + 1) * per)};
 }
 
-inline unsigned xcd_grid(int64_t items) {
-  return (unsigned)((items + kXcdCount - 1) / kXcdCount * kXcdCount);
+// Workgroups for `items` items with one each, or at most `most`, a whole number an XCD.
+inline unsigned xcd_grid(int64_t items, int64_t most = (int64_t)1 << 30) {
+  const int64_t per = (items + kXcdCount - 1) / kXcdCount;
+  return (unsigned)((per < most / kXcdCount ? per : most / kXcdCount) * kXcdCount);
 }
 
 }  // namespace pgn

@@ -18,25 +18,86 @@ using namespace pgn;
 
 namespace {
 
-constexpr int kWaveWords = 128;  // words a wave reduces: one piece of a row's softmax
+// Tiles of the logits (words x tokens), and of the gradients' products (columns of h or W x rows). A large one reaches the
+// matrix cores' rate; smaller ones fill the chip where there are few tokens (choose_logits, choose_grads).
+typedef Tile<8, 4, 2, 4, 2> Large;  // 256 x 256, 8 waves
+typedef Tile<6, 4, 2, 4, 2> Wide;   // 192 x 256, 8 waves: four cover widths of 704 and 768 with less left over
+typedef Tile<4, 4, 2, 2, 2> Mid;    // 128 x 128, 4 waves, two workgroups a compute unit
+typedef Tile<2, 2, 2, 2, 4> Small;  // 64 x 64, 4 waves, two workgroups a compute unit
+enum Kind { kLarge, kWide, kMid, kSmall };
+
+struct KindInfo {
+  int x, y, slots;    // tile, and workgroups that run at once
+  float step, fixed;  // microseconds of a step of 64, and of a tile beside its steps, as measured on a full chip
+};
+constexpr KindInfo kLogitsKinds[] = {{Large::X, Large::Y, 256, 1.7f, 6.f},
+                                     {0, 0, 0, 0.f, 0.f},
+                                     {Mid::X, Mid::Y, 512, 1.2f, 3.f},
+                                     {Small::X, Small::Y, 512, 0.45f, 1.5f}};
+constexpr KindInfo kGradKinds[] = {{Large::X, Large::Y, 256, 1.95f, 8.f},
+                                   {Wide::X, Wide::Y, 256, 1.55f, 7.f},
+                                   {Mid::X, Mid::Y, 512, 1.3f, 4.f}};
+
+int64_t tiles(int64_t x, int64_t m) { return (x + m - 1) / m; }
+int64_t round_up(int64_t x, int64_t m) { return tiles(x, m) * m; }
+
+// The tile kind of the logits of n tokens and V words: the least time by rounds of tiles.
+Kind choose_logits(int64_t n, int64_t V, int64_t d) {
+  Kind best = kLarge;
+  float least = INFINITY;
+  for (Kind k : {kLarge, kMid, kSmall}) {
+    const KindInfo& i = kLogitsKinds[k];
+    const float t = (float)tiles(tiles(n, i.y) * tiles(V, i.x), i.slots) * (tiles(d, kGemmK) * i.step + i.fixed);
+    if (t < least) least = t, best = k;
+  }
+  return best;
+}
 
 // The workspace of one piece's dl: at most this many bytes (but at least one column of tiles).
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+constexpr int64_t kPieceBytes = (int64_t)128 << 20;
+constexpr int64_t kPad = 256;  // dl's rows and columns are padded to whole tiles of any kind
 
-struct Plan {
+// How the gradients' products are laid out: the pieces of the vocabulary; the tile; the ranges that the contracted
+// dimension is cut into (words for dh, tokens for dW), each a multiple of 64, so that few output tiles still fill the
+// chip: the ranges' partial sums, fp32, are added in order by head_sum.
+struct GradPlan {
   int64_t n_pad, v_piece, pieces;
+  Kind kind;
+  int64_t len_h, split_h, len_w, split_w;
+  int64_t dl_bytes, part_h, part_w;  // bytes of the workspace's three parts
 };
 
-int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-
-Plan plan(int64_t n, int64_t V) {
-  Plan p;
-  p.n_pad = round_up(n, kGemmTile);
-  const int64_t v_pad = round_up(V, kGemmTile);
-  const int64_t most = std::max<int64_t>(kGemmTile, kPieceBytes / (2 * p.n_pad) / kGemmTile * kGemmTile);
-  p.pieces = (v_pad + most - 1) / most;
-  p.v_piece = round_up((v_pad + p.pieces - 1) / p.pieces, kGemmTile);
-  p.pieces = (v_pad + p.v_piece - 1) / p.v_piece;
+GradPlan choose_grads(int64_t n, int64_t V, int64_t d) {
+  GradPlan p;
+  p.n_pad = round_up(n, kPad);
+  const int64_t v_pad = round_up(V, kPad), most = std::max(kPad, kPieceBytes / (2 * p.n_pad) / kPad * kPad);
+  p.v_piece = round_up(tiles(v_pad, tiles(v_pad, most)), kPad);
+  p.pieces = tiles(v_pad, p.v_piece);
+  const int64_t words = std::min(V, p.v_piece), steps_h = tiles(words, kGemmK), steps_w = tiles(n, kGemmK);
+  float least = INFINITY;
+  for (Kind k : {kLarge, kWide, kMid}) {
+    const KindInfo& i = kGradKinds[k];
+    const int64_t tx = tiles(d, i.x), th = tx * tiles(n, i.y), tw = tx * tiles(words, i.y);
+    for (int64_t len = 4; ; len *= 2) {  // steps of an item, at most
+      const int64_t sh = tiles(steps_h, len), sw = tiles(steps_w, len);
+      const int64_t lh = tiles(steps_h, sh), lw = tiles(steps_w, sw);
+      const float ch = lh * i.step + i.fixed, cw = lw * i.step + i.fixed, sum = th * sh * ch + tw * sw * cw;
+      float t = std::max(ch, cw);
+      if (th * sh + tw * sw > i.slots) t = std::max(t, sum / i.slots + 0.5f * std::min(ch, cw));
+      // partial sums: written and read at about 4 bytes a picosecond, and a launch
+      const float part = (sh > 1 ? 8.f * sh * n * d : 0.f) + (sw > 1 ? 8.f * sw * words * d : 0.f);
+      if (part > 0.f) t += part * 0.25e-6f + 3.f;
+      if (sh <= 64 && sw <= 64 && t < least) {
+        least = t;
+        p.kind = k;
+        p.len_h = lh * kGemmK, p.split_h = tiles(steps_h, lh), p.len_w = lw * kGemmK, p.split_w = tiles(steps_w, lw);
+      }
+      if (sh == 1 && sw == 1) break;
+    }
+  }
+  p.dl_bytes = p.n_pad * p.v_piece * 2;
+  p.part_h = p.split_h > 1 || p.pieces > 1 ? p.split_h * n * d * 4 : 0;
+  p.part_w = p.split_w > 1 ? p.split_w * words * d * 4 : 0;
   return p;
 }
 
@@ -113,101 +174,128 @@ struct FwdOut {
   float* label;        // n: the label's logit (written only where the label is in range)
 };
 
-// One tile's logits reduced. NEXP sums of exponentials, of scale0 l and scale1 l.
-template <int NEXP>
-__global__ __launch_bounds__(kGemmThreads) void head_logits(Operand h, Operand W, const int64_t* __restrict__ y,
-                                                            float scale0, float scale1, FwdOut out, int64_t d) {
+// Tiles of logits, reduced: a wave's words are one piece of its tokens' rows. NEXP sums of exponentials, of scale0 l and
+// scale1 l. y: labels, or null.
+template <class C, int NEXP>
+__global__ __launch_bounds__(C::kThreads) void head_logits(Operand h, Operand W, const int64_t* __restrict__ y,
+                                                           float scale0, float scale1, FwdOut out, int64_t d) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t tx = (W.rows + kGemmTile - 1) / kGemmTile, ty = (h.rows + kGemmTile - 1) / kGemmTile;
-  const int64_t item = xcd_item(blockIdx.x, tx * ty);
-  if (item < 0) return;
-  int64_t ix, iy;
-  band_tile(item, tx, ty, ix, iy);
-  f32x4 acc[8][4];
-  gemm_tile<false, false>(W, h, ix * kGemmTile, iy * kGemmTile, 0, d, smem, acc);
+  const int64_t tx = (W.rows + C::X - 1) / C::X, ty = (h.rows + C::Y - 1) / C::Y, n = h.rows;
+  const XcdRun run = xcd_run(tx * ty);
+  if (run.first >= run.end) return;
   const WaveIdx t = wave_idx();
-  const int64_t v0 = ix * kGemmTile + (t.w & 1) * kWaveWords, i0 = iy * kGemmTile + (t.w >> 1) * 64, n = h.rows;
+  const int wx = t.w % C::WX, wy = t.w / C::WX;
+  constexpr int kWords = 16 * C::NA;
   const float c0 = scale0 * kLog2e, c1 = scale1 * kLog2e;
-  if (v0 + kWaveWords > W.rows) {
+  gemm_tiles<C, 8, 0>(
+      W, h, d, y, n, run.first, run.stride, run.end, smem,
+      [&](int64_t item, int64_t& x0, int64_t& y0) {
+        band_tile(item, tx, ty, x0, y0);
+        x0 *= C::X, y0 *= C::Y;
+      },
+      [&](f32x4(&acc)[C::NA][C::NB], int64_t x0, int64_t y0, const unsigned char* info) {
+        const int64_t v0 = x0 + kWords * wx;
+        if (v0 + kWords > W.rows) {
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
+          for (int a = 0; a < C::NA; ++a)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (v0 + 16 * a + 4 * t.g + r >= W.rows)
+            for (int r = 0; r < 4; ++r)
+              if (v0 + 16 * a + 4 * t.g + r >= W.rows)
 #pragma unroll
-          for (int b = 0; b < 4; ++b) acc[a][b][r] = -INFINITY;
-  }
+                for (int b = 0; b < C::NB; ++b) acc[a][b][r] = -INFINITY;
+        }
+        const int64_t piece = (v0 / kWords) * n;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int64_t row = i0 + 16 * b + t.i;
-    if (y != nullptr) {
-      const int64_t at = row < n ? y[row] - v0 : -1;
-      if (__ballot(at >= 0 && at < kWaveWords)) {
-        const int own = (at >= 0 && at < kWaveWords) ? (int)at - 4 * t.g : -1;
+        for (int b = 0; b < C::NB; ++b) {
+          const int local = 16 * C::NB * wy + 16 * b + t.i;
+          const int64_t row = y0 + local;
+          if (y != nullptr) {
+            const int64_t label = reinterpret_cast<const int64_t*>(info)[local], at = label - v0;
+            const bool here = row < n && at >= 0 && at < kWords && label < W.rows;
+            if (__ballot(here)) {
+              const int own = here ? (int)at - 4 * t.g : -1;
 #pragma unroll
-        for (int a = 0; a < 8; ++a)
+              for (int a = 0; a < C::NA; ++a)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (own == 16 * a + r && v0 + at < W.rows) out.label[row] = acc[a][b][r];
-      }
-    }
-    float m = acc[0][b][0];
+                for (int r = 0; r < 4; ++r)
+                  if (own == 16 * a + r) out.label[row] = acc[a][b][r];
+            }
+          }
+          float m = acc[0][b][0];
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
+          for (int a = 0; a < C::NA; ++a)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[a][b][r]);
-    m = column_max(m);
-    const float base = m > -INFINITY ? m : 0.f;
-    float s0 = 0.f, s1 = 0.f;
+            for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[a][b][r]);
+          m = column_max(m);
+          const float base = m > -INFINITY ? m : 0.f, b0 = base * c0, b1 = base * c1;
+          float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
+          for (int a = 0; a < C::NA; ++a)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s0 += exp2_hw((acc[a][b][r] - base) * c0);
-        if constexpr (NEXP == 2) s1 += exp2_hw((acc[a][b][r] - base) * c1);
-      }
-    s0 = column_sum(s0);
-    if constexpr (NEXP == 2) s1 = column_sum(s1);
-    if (t.g == 0 && row < n) {
-      const int64_t o = (v0 / kWaveWords) * n + row;
-      out.m[o] = m;
-      out.s0[o] = s0;
-      if constexpr (NEXP == 2) out.s1[o] = s1;
-    }
-  }
+            for (int r = 0; r < 4; ++r) {
+              s0 += exp2_hw(__builtin_fmaf(acc[a][b][r], c0, -b0));
+              if constexpr (NEXP == 2) s1 += exp2_hw(__builtin_fmaf(acc[a][b][r], c1, -b1));
+            }
+          s0 = column_sum(s0);
+          if constexpr (NEXP == 2) s1 = column_sum(s1);
+          if (t.g == 0 && row < n) {
+            out.m[piece + row] = m;
+            out.s0[piece + row] = s0;
+            if constexpr (NEXP == 2) out.s1[piece + row] = s1;
+          }
+        }
+      });
 }
 
-// A row's pieces joined: a thread a row.
-__global__ __launch_bounds__(64) void head_join(FwdOut in, int64_t pieces, float scale0, float scale1,
-                                                const int64_t* __restrict__ y, float* __restrict__ ce,
-                                                float* __restrict__ lse, const float* __restrict__ ent,
-                                                const float* __restrict__ psum, const float* __restrict__ p,
-                                                const float* __restrict__ zl, float tau, float* __restrict__ kd,
-                                                float* __restrict__ lse_t, int second, int64_t n, int64_t V,
-                                                int64_t K) {
-  const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (row >= n) return;
-  float m = -INFINITY;
-  for (int64_t q = 0; q < pieces; ++q) m = fmaxf(m, in.m[q * n + row]);
-  float s0 = 0.f, s1 = 0.f;
-  for (int64_t q = 0; q < pieces; ++q) {
-    const float mq = in.m[q * n + row] - m;
-    s0 += in.s0[q * n + row] * expf(mq * scale0);
-    if (second) s1 += in.s1[q * n + row] * expf(mq * scale1);
-  }
-  const float l0 = m * scale0 + logf(s0), l1 = second ? m * scale1 + logf(s1) : l0;
-  if (y != nullptr) {
-    lse[row] = l0;
-    ce[row] = y[row] >= 0 && y[row] < V ? l0 - in.label[row] : 0.f;
-  }
-  if (K > 0) {
-    float dot = 0.f;
-    for (int64_t k = 0; k < K; ++k) {
-      const float pk = p[row * K + k];
-      if (pk > 0.f) dot += pk * zl[row * K + k];
+// Rows' pieces joined: 16 rows a workgroup, 16 threads a row (thread 16 q + r: every 16th piece of row r from q).
+struct JoinArgs {
+  const int64_t* y;
+  float *ce, *lse;
+  const float *ent, *psum, *p, *zl;
+  float *kd, *lse_t;
+  float tau, scale0, scale1;
+  int second;
+  int64_t pieces, n, V, K;
+};
+
+__global__ __launch_bounds__(256) void head_join(FwdOut in, JoinArgs j) {
+  __shared__ float parts[4][16][17];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t row = (int64_t)blockIdx.x * 16 + r, n = j.n;
+  const bool live = row < n;
+  float m = -INFINITY, s0 = 0.f, s1 = 0.f, dot = 0.f;
+  if (live) {
+    for (int64_t k = q; k < j.pieces; k += 16) m = fmaxf(m, in.m[k * n + row]);
+    for (int64_t k = q; k < j.K; k += 16) {
+      const float pk = j.p[row * j.K + k];
+      if (pk > 0.f) dot += pk * j.zl[row * j.K + k];
     }
-    lse_t[row] = l1;
-    kd[row] = psum[row] > 0.f ? tau * tau * (ent[row] - dot / tau + l1) : 0.f;
+  }
+  parts[0][q][r] = m;
+  parts[3][q][r] = dot;
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) m = fmaxf(m, parts[0][k][r]);
+  if (live)
+    for (int64_t k = q; k < j.pieces; k += 16) {
+      const float mk = in.m[k * n + row] - m;
+      s0 += in.s0[k * n + row] * expf(mk * j.scale0);
+      if (j.second) s1 += in.s1[k * n + row] * expf(mk * j.scale1);
+    }
+  parts[1][q][r] = s0;
+  parts[2][q][r] = s1;
+  __syncthreads();
+  if (q != 0 || !live) return;
+  s0 = s1 = dot = 0.f;
+  for (int k = 0; k < 16; ++k) s0 += parts[1][k][r], s1 += parts[2][k][r], dot += parts[3][k][r];
+  const float l0 = m * j.scale0 + logf(s0), l1 = j.second ? m * j.scale1 + logf(s1) : l0;
+  if (j.y != nullptr) {
+    const int64_t label = j.y[row];
+    j.lse[row] = l0;
+    j.ce[row] = label >= 0 && label < j.V ? l0 - in.label[row] : 0.f;
+  }
+  if (j.K > 0) {
+    j.lse_t[row] = l1;
+    j.kd[row] = j.psum[row] > 0.f ? j.tau * j.tau * (j.ent[row] - dot / j.tau + l1) : 0.f;
   }
 }
 
@@ -218,58 +306,108 @@ struct BwdIn {
   float tau;
 };
 
-// dl of a piece of the vocabulary: words v_begin .. v_begin + ld of the workspace's rows (n_pad, ld). Word and token
-// rows past the ends get zeros.
-template <int NEXP>
-__global__ __launch_bounds__(kGemmThreads) void head_dlogits(Operand h, Operand W, BwdIn in, float scale0,
-                                                             float scale1, __bf16* __restrict__ dl, int64_t ld,
-                                                             int64_t v_begin, int64_t d) {
+// What dl takes of a row: dl = w0 exp(l scale0 - l0) + w1 exp(l scale1 - l1) - gc [v = label], the exponents in base 2;
+// zero where not live.
+struct RowInfo {
+  float w0, l0, w1, l1, gc;
+  int32_t label, live, unused;
+};
+
+__global__ __launch_bounds__(256) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows, int64_t n,
+                                                 int64_t V) {
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row >= n) return;
+  RowInfo o{};
+  const int64_t label = in.y != nullptr ? in.y[row] : -1;
+  const bool labelled = label >= 0 && label < V;
+  o.label = labelled ? (int32_t)label : -1;
+  o.gc = labelled && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
+  const float w_ce = o.gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f);
+  const float w_kd = in.g_kd != nullptr ? in.g_kd[row] * in.tau * in.psum[row] : 0.f;
+  o.w0 = second ? w_ce : w_ce + w_kd;
+  o.w1 = w_kd;
+  o.l0 = (in.lse != nullptr ? in.lse[row] : in.lse_t[row]) * kLog2e;
+  o.l1 = second ? in.lse_t[row] * kLog2e : 0.f;
+  o.live = w_ce != 0.f || w_kd != 0.f || o.gc != 0.f;
+  rows[row] = o;
+}
+
+// Two adjacent accumulator tiles (rows 0 .. 15 and 16 .. 31 of a 32-row block; lane (i, g) holds rows 4 g .. 4 g + 3 of
+// column i of both) rounded to bf16, exchanged between lane groups so that a lane ends with eight consecutive rows of its
+// column, first_of(g) ..: one 16-byte store, 64 bytes a column.
+PGN_DEVICE int first_of(int g) { return 16 * (g & 1) + 8 * (g >> 1); }
+PGN_DEVICE bf16x8 eight_rows(f32x4 lo, f32x4 hi) {
+  const i32x2 x = __builtin_bit_cast(i32x2, to_bf16x4(lo)), y = __builtin_bit_cast(i32x2, to_bf16x4(hi));
+  const auto p = __builtin_amdgcn_permlane16_swap((unsigned)x[0], (unsigned)y[0], false, false);
+  const auto q = __builtin_amdgcn_permlane16_swap((unsigned)x[1], (unsigned)y[1], false, false);
+  const unsigned p0 = p[0], p1 = p[1], q0 = q[0], q1 = q[1];
+  return __builtin_bit_cast(bf16x8, i32x4{(int)p0, (int)q0, (int)p1, (int)q1});
+}
+
+// dl of a piece of the vocabulary: words v_begin .. v_begin + ld (ld a multiple of kPad) of the workspace's rows (n
+// padded likewise). Word and token rows past the ends get zeros.
+template <class C, int NEXP>
+__global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W, const RowInfo* __restrict__ rows,
+                                                            float scale0, float scale1, __bf16* __restrict__ dl,
+                                                            int64_t ld, int64_t v_begin, int64_t n_pad, int64_t d) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t tx = ld / kGemmTile, ty = (h.rows + kGemmTile - 1) / kGemmTile;
-  const int64_t item = xcd_item(blockIdx.x, tx * ty);
-  if (item < 0) return;
-  int64_t ix, iy;
-  band_tile(item, tx, ty, ix, iy);
-  f32x4 acc[8][4];
-  gemm_tile<false, false>(W, h, v_begin + ix * kGemmTile, iy * kGemmTile, 0, d, smem, acc);
+  const int64_t tx = ld / C::X, ty = n_pad / C::Y, words = min(ld, W.rows - v_begin);
+  const XcdRun run = xcd_run(tx * ty);
+  if (run.first >= run.end) return;
   const WaveIdx t = wave_idx();
-  const int64_t c0 = ix * kGemmTile + (t.w & 1) * kWaveWords, v0 = v_begin + c0;
-  const int64_t i0 = iy * kGemmTile + (t.w >> 1) * 64, n = h.rows;
+  const int wx = t.w % C::WX, wy = t.w / C::WX;
   const float e0 = scale0 * kLog2e, e1 = scale1 * kLog2e;
+  const Operand Wp{W.p + v_begin * W.ld, W.ld, words};
+  gemm_tiles<C, sizeof(RowInfo), C::NB * C::NA / 2>(
+      Wp, h, d, rows, h.rows, run.first, run.stride, run.end, smem,
+      [&](int64_t item, int64_t& x0, int64_t& y0) {
+        band_tile(item, tx, ty, x0, y0);
+        x0 *= C::X, y0 *= C::Y;
+      },
+      [&](f32x4(&acc)[C::NA][C::NB], int64_t x0, int64_t y0, const unsigned char* info) {
+        const int64_t c0 = x0 + 16 * C::NA * wx;
+        const bool partial = c0 + 16 * C::NA > words;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int64_t row = i0 + 16 * b + t.i;
-    const bool live = row < n;
-    // weights of the two softmaxes in dl, and the label
-    const int64_t label = live && in.y != nullptr ? in.y[row] : -1;
-    const bool labelled = label >= 0 && label < W.rows;
-    const float gc = live && labelled && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
-    const float w_ce = gc + (live && in.g_lse != nullptr ? in.g_lse[row] : 0.f);
-    const float w_kd = live && in.g_kd != nullptr ? in.g_kd[row] * in.tau * in.psum[row] : 0.f;
-    float w0, w1 = 0.f, l0, l1 = 0.f;
-    if constexpr (NEXP == 2) {
-      w0 = w_ce, w1 = w_kd;
-      l0 = live ? in.lse[row] * kLog2e : 0.f, l1 = live ? in.lse_t[row] * kLog2e : 0.f;
-    } else {
-      w0 = w_ce + w_kd;
-      l0 = live ? (in.lse != nullptr ? in.lse[row] : in.lse_t[row]) * kLog2e : 0.f;
-    }
-    const bool any = w_ce != 0.f || w_kd != 0.f || gc != 0.f;
-    const int at = labelled && gc != 0.f && label >= v0 && label < v0 + kWaveWords ? (int)(label - v0) - 4 * t.g : -1;
-    const bool hit = __ballot(at >= 0) != 0;
+        for (int b = 0; b < C::NB; ++b) {
+          const int local = 16 * C::NB * wy + 16 * b + t.i;
+          const RowInfo o = reinterpret_cast<const RowInfo*>(info)[local];
+          const int at = o.label - (int)(v_begin + c0);
+          const bool here = o.gc != 0.f && at >= 0 && at < 16 * C::NA, hit = __ballot(here) != 0;
+          const int own = here ? at - 4 * t.g : -1;
 #pragma unroll
-    for (int a = 0; a < 8; ++a) {
-      f32x4 x;
+          for (int a = 0; a < C::NA; ++a) {
+            f32x4 x = acc[a][b];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = w0 * exp2_hw(acc[a][b][r] * e0 - l0);
-        if constexpr (NEXP == 2) x[r] += w1 * exp2_hw(acc[a][b][r] * e1 - l1);
-        if (hit && at == 16 * a + r) x[r] -= gc;
-        if (!any || v0 + 16 * a + 4 * t.g + r >= W.rows) x[r] = 0.f;
-      }
-      *reinterpret_cast<bf16x4*>(dl + row * ld + c0 + 16 * a + 4 * t.g) = to_bf16x4(x);
-    }
-  }
+            for (int r = 0; r < 4; ++r) {
+              float z = o.w0 * exp2_hw(__builtin_fmaf(x[r], e0, -o.l0));
+              if constexpr (NEXP == 2) z += o.w1 * exp2_hw(__builtin_fmaf(x[r], e1, -o.l1));
+              x[r] = o.live ? z : 0.f;
+            }
+            acc[a][b] = x;
+          }
+          if (hit) {
+#pragma unroll
+            for (int a = 0; a < C::NA; ++a)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (own == 16 * a + r) acc[a][b][r] -= o.gc;
+          }
+          if (partial) {
+#pragma unroll
+            for (int a = 0; a < C::NA; ++a)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (c0 + 16 * a + 4 * t.g + r >= words) acc[a][b][r] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < C::NB; ++b) {
+          __bf16* p = dl + (y0 + 16 * C::NB * wy + 16 * b + t.i) * ld + c0 + first_of(t.g);
+#pragma unroll
+          for (int a = 0; a < C::NA; a += 2)
+            *reinterpret_cast<bf16x8*>(p + 16 * a) = eight_rows(acc[a][b], acc[a + 1][b]);
+        }
+      });
 }
 
 // dl at the teacher's entries, whole: a thread an entry. Repeated ids write the same value.
@@ -299,78 +437,122 @@ __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const int32_t* __
   dl[row * ld + (v - v_begin)] = (__bf16)x;
 }
 
-// dh (+)= dl W over a piece (the first workgroups) and dW = dl^T h of the piece (the others).
+// dh = dl W over a piece and dW = dl^T h of the piece, in one launch; either whole, or as fp32 partial sums by range of
+// the contracted dimension.
+struct GradSide {
+  int64_t rows, k, len, split;  // output rows; contracted length, its ranges
+  void* out;                    // rows x d, where one range is all
+  float* part;                  // split x rows x d
+  int f32, add;                 // out's type; whether part holds earlier pieces' sums
+};
 struct GradArgs {
-  Operand dl_rows, dl_words;  // dl by its rows (n_pad), contracted over words / over tokens
-  Operand W, h;               // W's rows of the piece; h
-  int64_t n, d, words, n_pad, ld;
-  __bf16* dh;
-  float* dh_acc;   // fp32 sums where there are several pieces
-  int first, last;
-  void* dW;        // the piece's rows
-  int dw_f32;
-  int64_t items_h, items_w;
+  Operand dl, W, h;  // dl by rows (n_pad); W's rows of the piece
+  int64_t d;
+  GradSide side[2];  // dh, dW
+  int first;         // the side whose items are longer, launched first
 };
 
-__global__ __launch_bounds__(kGemmThreads) void head_grads(GradArgs q) {
+template <class C>
+__global__ __launch_bounds__(C::kThreads) void head_grads(GradArgs q) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t tx = (q.d + kGemmTile - 1) / kGemmTile;
-  f32x4 acc[8][4];
-  int64_t item = xcd_item(blockIdx.x, q.items_h + q.items_w);
-  if (item < 0) return;
-  const WaveIdx t = wave_idx();
-  int64_t ix, iy;
-  if (item < q.items_h) {
-    iy = item / tx, ix = item - iy * tx;
-    gemm_tile<true, false>(q.W, q.dl_rows, ix * kGemmTile, iy * kGemmTile, 0, q.words, smem, acc);
-    const int64_t c0 = ix * kGemmTile + (t.w & 1) * 128, i0 = iy * kGemmTile + (t.w >> 1) * 64;
+  const int64_t tx = (q.d + C::X - 1) / C::X;
+  // each XCD takes a contiguous eighth of the first side's items, then of the second's
+  int which = q.first;
+  int64_t j = blockIdx.x / kXcdCount;
+  for (int u = 0; u < 2; ++u, which ^= 1) {
+    const GradSide& s = q.side[which];
+    const int64_t items = s.out == nullptr ? 0 : tx * ((s.rows + C::Y - 1) / C::Y) * s.split;
+    const int64_t per = (items + kXcdCount - 1) / kXcdCount;
+    if (j < per) {
+      const int64_t item = blockIdx.x % kXcdCount * per + j;
+      if (item >= items) return;
+      const int64_t range = item / (items / s.split), tile = item - range * (items / s.split), iy = tile / tx;
+      const int64_t x0 = (tile - iy * tx) * C::X, y0 = iy * C::Y;
+      const int64_t k0 = range * s.len, k1 = max(k0, min(s.k, k0 + s.len));
+      f32x4 acc[C::NA][C::NB];
+      if (which == 0)
+        gemm_tile<C, true, false>(q.W, q.dl, x0, y0, k0, k1, smem, acc);
+      else
+        gemm_tile<C, true, true>(q.h, q.dl, x0, y0, k0, k1, smem, acc);
+      const WaveIdx t = wave_idx();
+      const int64_t c0 = x0 + 16 * C::NA * (t.w % C::WX);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int64_t row = i0 + 16 * b + t.i;
-      if (row >= q.n) continue;
+      for (int b = 0; b < C::NB; ++b) {
+        const int64_t row = y0 + 16 * C::NB * (t.w / C::WX) + 16 * b + t.i;
+        if (s.part != nullptr || s.f32) {
+          float* p = (s.part != nullptr ? s.part + (range * s.rows + row) * q.d : (float*)s.out + row * q.d);
 #pragma unroll
-      for (int a = 0; a < 8; ++a) {
-        const int64_t c = c0 + 16 * a + 4 * t.g;
-        if (c >= q.d) continue;
-        f32x4 x = acc[a][b];
-        if (!q.first) x += *reinterpret_cast<const f32x4*>(q.dh_acc + row * q.d + c);
-        if (q.last)
-          *reinterpret_cast<bf16x4*>(q.dh + row * q.d + c) = to_bf16x4(x);
-        else
-          *reinterpret_cast<f32x4*>(q.dh_acc + row * q.d + c) = x;
+          for (int a = 0; a < C::NA; ++a) {
+            const int64_t c = c0 + 16 * a + 4 * t.g;
+            if (row >= s.rows || c >= q.d) continue;
+            f32x4 x = acc[a][b];
+            if (s.part != nullptr && s.add) x += *reinterpret_cast<const f32x4*>(p + c);
+            *reinterpret_cast<f32x4*>(p + c) = x;
+          }
+        } else {
+#pragma unroll
+          for (int a = 0; a < C::NA; a += 2) {
+            const bf16x8 x = eight_rows(acc[a][b], acc[a + 1][b]);
+            const int64_t c = c0 + 16 * a + first_of(t.g);
+            if (row < s.rows && c < q.d) *reinterpret_cast<bf16x8*>((__bf16*)s.out + row * q.d + c) = x;
+          }
+        }
       }
+      return;
     }
-  } else {
-    item -= q.items_h;
-    iy = item / tx, ix = item - iy * tx;
-    gemm_tile<true, true>(q.h, q.dl_words, ix * kGemmTile, iy * kGemmTile, 0, q.n, smem, acc);
-    const int64_t c0 = ix * kGemmTile + (t.w & 1) * 128, i0 = iy * kGemmTile + (t.w >> 1) * 64;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int64_t row = i0 + 16 * b + t.i;
-      if (row >= q.words) continue;
-#pragma unroll
-      for (int a = 0; a < 8; ++a) {
-        const int64_t c = c0 + 16 * a + 4 * t.g;
-        if (c >= q.d) continue;
-        if (q.dw_f32)
-          *reinterpret_cast<f32x4*>((float*)q.dW + row * q.d + c) = acc[a][b];
-        else
-          *reinterpret_cast<bf16x4*>((__bf16*)q.dW + row * q.d + c) = to_bf16x4(acc[a][b]);
-      }
-    }
+    j -= per;
   }
+}
+
+// out = the ranges' partial sums in order, four elements a thread.
+__global__ __launch_bounds__(256) void head_sum(const float* __restrict__ part, void* __restrict__ out, int f32,
+                                                int64_t split, int64_t count) {
+  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < count; e += (int64_t)gridDim.x * 1024) {
+    f32x4 x = *reinterpret_cast<const f32x4*>(part + e);
+    for (int64_t k = 1; k < split; ++k) x += *reinterpret_cast<const f32x4*>(part + k * count + e);
+    if (f32)
+      *reinterpret_cast<f32x4*>((float*)out + e) = x;
+    else
+      *reinterpret_cast<bf16x4*>((__bf16*)out + e) = to_bf16x4(x);
+  }
+}
+
+// Logits kernels by tile kind: F<C> with the tile type.
+template <class F>
+auto by_kind(Kind k, F&& f) {
+  return k == kLarge ? f(Large{}) : k == kMid ? f(Mid{}) : f(Small{});
+}
+
+int launch_sum(const float* part, void* out, int f32, int64_t split, int64_t count, hipStream_t st) {
+  hipLaunchKernelGGL(head_sum, dim3((unsigned)std::min<int64_t>(tiles(count, 1024), 4096)), dim3(256), 0, st, part, out,
+                     f32, split, count);
+  return (int)hipGetLastError();
+}
+
+template <class C>
+int launch_grads(const GradArgs& ga, hipStream_t st) {
+  const hipError_t e = pgn_lds_limit((const void*)head_grads<C>, C::kLds);
+  if (e != hipSuccess) return (int)e;
+  int64_t groups = 0;
+  for (const GradSide& s : ga.side)
+    if (s.out != nullptr) groups += xcd_grid(tiles(ga.d, C::X) * tiles(s.rows, C::Y) * s.split);
+  hipLaunchKernelGGL(head_grads<C>, dim3((unsigned)groups), dim3(C::kThreads), C::kLds, st, ga);
+  return (int)hipGetLastError();
 }
 
 bool head_shape_ok(int64_t n, int64_t V, int64_t d, int64_t K) {
   return n > 0 && n <= (int64_t)1 << 24 && V > 0 && V <= (int64_t)1 << 24 && d > 0 && d % 8 == 0 && d <= 65536 &&
-         K >= 0 && K <= 65536 && round_up(n, kGemmTile) / kGemmTile * (round_up(V, kGemmTile) / kGemmTile) < 1 << 22 &&
-         n * K < (int64_t)1 << 31;  // launches of fewer than 2^32 threads
+         K >= 0 && K <= 65536 && n * K < (int64_t)1 << 31;  // launches of fewer than 2^32 threads
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
-int64_t head_pieces(int64_t V) { return round_up(V, kGemmTile) / kWaveWords; }
+// Pieces of a row's softmax: the words of a wave of the tile.
+int64_t head_pieces(int64_t n, int64_t V, int64_t d) {
+  const Kind k = choose_logits(n, V, d);
+  return tiles(V, kLogitsKinds[k].x) * 2;
+}
+static_assert(Large::WX == 2 && Mid::WX == 2 && Small::WX == 2, "two waves along the words");
 
 }  // namespace
 
@@ -378,7 +560,7 @@ extern "C" int pragnosia_lm_abi_version(void) { return 1; }
 
 extern "C" int64_t pragnosia_head_fwd_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t K) {
   if (!head_shape_ok(n, V, d, K)) return -1;
-  return (3 * head_pieces(V) + 2) * n * (int64_t)sizeof(float);
+  return (3 * head_pieces(n, V, d) + 2) * n * (int64_t)sizeof(float);
 }
 
 extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y, const int64_t* ids, const float* z,
@@ -393,38 +575,39 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
   PGN_CHECK_ARG(tau > 0.f && tau < INFINITY);
   PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_head_fwd_workspace_bytes(n, V, d, K));
   hipStream_t st = (hipStream_t)stream;
-  const int64_t pieces = head_pieces(V);
+  const int64_t pieces = head_pieces(n, V, d);
   float* f = (float*)workspace;
   const FwdOut out{f, f + pieces * n, f + 2 * pieces * n, f + 3 * pieces * n};
   float* ent = f + (3 * pieces + 1) * n;
   const Operand ho{(const __bf16*)h, d, n}, Wo{(const __bf16*)W, d, V};
-  hipError_t e = pgn_lds_limit((const void*)head_logits<1>, kGemmLds);
-  if (e == hipSuccess) e = pgn_lds_limit((const void*)head_logits<2>, kGemmLds);
-  if (e != hipSuccess) return (int)e;
   if (K > 0) {
-    hipLaunchKernelGGL(head_teacher, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, ids, z, 1.f / tau, entry, p, psum,
+    hipLaunchKernelGGL(head_teacher, dim3((unsigned)tiles(n, 4)), dim3(256), 0, st, ids, z, 1.f / tau, entry, p, psum,
                        ent, n, V, K);
-    hipLaunchKernelGGL(head_entry_logits, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, ho.p, Wo.p, entry, zl, n, d,
+    hipLaunchKernelGGL(head_entry_logits, dim3((unsigned)tiles(n, 4)), dim3(256), 0, st, ho.p, Wo.p, entry, zl, n, d,
                        K);
   }
   const int second = y && K > 0 && tau != 1.f;
   const float scale0 = y ? 1.f : 1.f / tau, scale1 = 1.f / tau;
-  const int64_t items = round_up(V, kGemmTile) / kGemmTile * (round_up(n, kGemmTile) / kGemmTile);
-  if (second)
-    hipLaunchKernelGGL(head_logits<2>, dim3(xcd_grid(items)), dim3(kGemmThreads), kGemmLds, st, ho, Wo, y, scale0,
-                       scale1, out, d);
-  else
-    hipLaunchKernelGGL(head_logits<1>, dim3(xcd_grid(items)), dim3(kGemmThreads), kGemmLds, st, ho, Wo, y, scale0,
-                       scale1, out, d);
-  hipLaunchKernelGGL(head_join, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st, out, pieces, scale0, scale1, y, ce,
-                     lse, ent, psum, p, zl, tau, kd, lse_t, second, n, V, K);
+  const Kind kind = choose_logits(n, V, d);
+  const int rc = by_kind(kind, [&](auto c) {
+    typedef decltype(c) C;
+    const auto fn = second ? head_logits<C, 2> : head_logits<C, 1>;
+    const hipError_t e = pgn_lds_limit((const void*)fn, C::kLdsInfo);
+    if (e != hipSuccess) return (int)e;
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(tiles(V, C::X) * tiles(n, C::Y), kLogitsKinds[kind].slots)), dim3(C::kThreads),
+                       C::kLdsInfo, st, ho, Wo, y, scale0, scale1, out, d);
+    return (int)hipGetLastError();
+  });
+  if (rc) return rc;
+  const JoinArgs j{y, ce, lse, ent, psum, p, zl, kd, lse_t, tau, scale0, scale1, second, pieces, n, V, K};
+  hipLaunchKernelGGL(head_join, dim3((unsigned)tiles(n, 16)), dim3(256), 0, st, out, j);
   PGN_RETURN_LAUNCH();
 }
 
 extern "C" int64_t pragnosia_head_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!head_shape_ok(n, V, d, 0)) return -1;
-  const Plan pl = plan(n, V);
-  return pl.n_pad * pl.v_piece * 2 + (pl.pieces > 1 ? n * d * 4 : 0);
+  const GradPlan pl = choose_grads(n, V, d);
+  return pl.dl_bytes + pl.part_h + pl.part_w + n * (int64_t)sizeof(RowInfo);
 }
 
 extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd, const void* h,
@@ -441,40 +624,47 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   PGN_CHECK_ARG(tau > 0.f && tau < INFINITY);
   PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_head_bwd_workspace_bytes(n, V, d));
   hipStream_t st = (hipStream_t)stream;
-  const Plan pl = plan(n, V);
+  const GradPlan pl = choose_grads(n, V, d);
   const bool ce = g_ce || g_lse;
   const int second = ce && g_kd && tau != 1.f;
   const float scale0 = ce ? 1.f : 1.f / tau, scale1 = 1.f / tau;
   const BwdIn in{g_ce, g_lse, g_kd, ce ? lse : nullptr, lse_t, psum, y, tau};
   const Operand ho{(const __bf16*)h, d, n}, Wo{(const __bf16*)W, d, V};
-  __bf16* dl = (__bf16*)workspace;
-  float* acc = (float*)(dl + pl.n_pad * pl.v_piece);
-  hipError_t e = pgn_lds_limit((const void*)head_dlogits<1>, kGemmLds);
-  if (e == hipSuccess) e = pgn_lds_limit((const void*)head_dlogits<2>, kGemmLds);
-  if (e == hipSuccess) e = pgn_lds_limit((const void*)head_grads, kGemmLds);
-  if (e != hipSuccess) return (int)e;
-  const int64_t ty = pl.n_pad / kGemmTile, td = round_up(d, kGemmTile) / kGemmTile;
+  unsigned char* ws = (unsigned char*)workspace;
+  __bf16* dl = (__bf16*)ws;
+  float *part_h = (float*)(ws + pl.dl_bytes), *part_w = (float*)(ws + pl.dl_bytes + pl.part_h);
+  RowInfo* rows = (RowInfo*)(ws + pl.dl_bytes + pl.part_h + pl.part_w);
+  hipLaunchKernelGGL(head_rows, dim3((unsigned)tiles(n, 256)), dim3(256), 0, st, in, second, rows, n, V);
+  const Kind kind = choose_logits(n, pl.v_piece, d);
   for (int64_t q = 0; q < pl.pieces; ++q) {
-    const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0), ld = round_up(words, kGemmTile);
-    const int64_t items = ld / kGemmTile * ty;
-    if (second)
-      hipLaunchKernelGGL(head_dlogits<2>, dim3(xcd_grid(items)), dim3(kGemmThreads), kGemmLds, st, ho, Wo, in, scale0,
-                         scale1, dl, ld, v0, d);
-    else
-      hipLaunchKernelGGL(head_dlogits<1>, dim3(xcd_grid(items)), dim3(kGemmThreads), kGemmLds, st, ho, Wo, in, scale0,
-                         scale1, dl, ld, v0, d);
+    const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0), ld = round_up(words, kPad);
+    int rc = by_kind(kind, [&](auto c) {
+      typedef decltype(c) C;
+      const auto fn = second ? head_dlogits<C, 2> : head_dlogits<C, 1>;
+      const hipError_t e = pgn_lds_limit((const void*)fn, C::kLdsInfo);
+      if (e != hipSuccess) return (int)e;
+      hipLaunchKernelGGL(fn, dim3(xcd_grid(ld / C::X * (pl.n_pad / C::Y), kLogitsKinds[kind].slots)),
+                         dim3(C::kThreads), C::kLdsInfo, st, ho, Wo, rows, scale0, scale1, dl, ld, v0, pl.n_pad, d);
+      return (int)hipGetLastError();
+    });
+    if (rc) return rc;
     if (g_kd)
-      hipLaunchKernelGGL(head_entry_dl, dim3((unsigned)((n * K + 255) / 256)), dim3(256), 0, st, in, entry, p, zl, dl,
-                         ld, v0, n, V, K);
-    GradArgs ga;
-    ga.dl_rows = ga.dl_words = Operand{dl, ld, pl.n_pad};
-    ga.W = Operand{Wo.p + v0 * d, d, words};
-    ga.h = ho;
-    ga.n = n, ga.d = d, ga.words = words, ga.n_pad = pl.n_pad, ga.ld = ld;
-    ga.dh = (__bf16*)dh, ga.dh_acc = acc, ga.first = q == 0, ga.last = q == pl.pieces - 1;
-    ga.dW = dw_f32 ? (void*)((float*)dW + v0 * d) : (void*)((__bf16*)dW + v0 * d), ga.dw_f32 = dw_f32;
-    ga.items_h = dh ? ty * td : 0, ga.items_w = dW ? ld / kGemmTile * td : 0;
-    hipLaunchKernelGGL(head_grads, dim3(xcd_grid(ga.items_h + ga.items_w)), dim3(kGemmThreads), kGemmLds, st, ga);
+      hipLaunchKernelGGL(head_entry_dl, dim3((unsigned)tiles(n * K, 256)), dim3(256), 0, st, in, entry, p, zl, dl, ld,
+                         v0, n, V, K);
+    void* dW_q = dW == nullptr ? nullptr
+                               : dw_f32 ? (void*)((float*)dW + v0 * d) : (void*)((__bf16*)dW + v0 * d);
+    GradArgs ga{Operand{dl, ld, pl.n_pad}, Operand{Wo.p + v0 * d, d, words}, ho, d,
+                {{n, words, pl.len_h, pl.split_h, dh, pl.part_h ? part_h : nullptr, 0, q > 0},
+                 {words, n, pl.len_w, pl.split_w, dW_q, pl.part_w ? part_w : nullptr, dw_f32, 0}},
+                pl.len_h >= pl.len_w ? 0 : 1};
+    rc = pl.kind == kLarge ? launch_grads<Large>(ga, st)
+                           : pl.kind == kWide ? launch_grads<Wide>(ga, st) : launch_grads<Mid>(ga, st);
+    if (rc) return rc;
+    if (dW && pl.part_w && (rc = launch_sum(part_w, dW_q, dw_f32, pl.split_w, words * d, st))) return rc;
+  }
+  if (dh && pl.part_h) {
+    const int rc = launch_sum(part_h, dh, 0, pl.split_h, n * d, st);
+    if (rc) return rc;
   }
   PGN_RETURN_LAUNCH();
 }
