@@ -15,11 +15,12 @@ import torch
 from torch import Tensor
 
 from ._lib import PragnosiaError, check, lm_lib
-from .head import _FLOATS, _INTS, _aligned
-from .ops import _expect, _ptr, _require_gpu, _stream
+from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _on
+from .ops import _expect, _require_gpu
 
 
 def _check_embed(op: str, ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype) -> None:
+    _require_gpu(ids, W)
     if ids.dtype not in _INTS:
         raise PragnosiaError(f"{op}: ids must be integers, got {ids.dtype}")
     _expect(op, W.device, ids=(ids, (None,)), W=(W, (None, None)))
@@ -31,24 +32,60 @@ def _check_embed(op: str, ids: Tensor, W: Tensor, scale: float, dtype: torch.dty
         raise PragnosiaError(f"{op}: scale must be finite, got {scale}")
 
 
+def _forward(ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
+    """ids (n) int64, W (V, d), both contiguous."""
+    n, (V, d) = ids.shape[0], W.shape
+    y = torch.empty(n, d, device=W.device, dtype=dtype)
+    with _on(W) as stream:
+        check(lm_lib().pragnosia_embed_fwd(_at(ids), _at(W), W.dtype == _BF16, scale, _at(y), dtype == _BF16, n, V, d,
+                                           stream), "pragnosia_embed_fwd")
+    return y
+
+
+def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) -> Tensor:
+    """g (n, d), ids (n) int64 -> dW (V, d) in `dtype`."""
+    g = _as(g, g.dtype)
+    n, d = g.shape
+    dW = torch.empty(V, d, device=g.device, dtype=dtype)
+    L = lm_lib()
+    nbytes = L.pragnosia_embed_bwd_workspace_bytes(n, V, d)
+    if nbytes < 0:
+        raise PragnosiaError(f"embed_bwd: shape n={n} V={V} d={d} rejected")
+    ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
+    with _on(g) as stream:
+        check(L.pragnosia_embed_bwd(_at(g), g.dtype == _BF16, _at(ids), scale, _at(dW), dtype == _BF16, _at(ws), nbytes,
+                                    n, V, d, stream), "pragnosia_embed_bwd")
+    return dW
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, W, scale, dtype):
+        ids = _as(ids, _I64)
+        ctx.save_for_backward(ids)
+        ctx.V, ctx.scale, ctx.dtype = W.shape[0], scale, W.dtype
+        return _forward(ids, _as(W, W.dtype), scale, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        ids, = ctx.saved_tensors
+        return None, _backward(g, ids, ctx.V, ctx.scale, ctx.dtype), None, None
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the same as custom ops, for traces
 @torch.library.custom_op("pragnosia::embed", mutates_args=())
 def embed(ids: Tensor, W: Tensor, scale: float, bf16: bool) -> Tensor:
     """ids (n), W (V, d) -> scale W[ids] (n, d), bf16 or fp32."""
-    _require_gpu(ids, W)
-    dtype = torch.bfloat16 if bf16 else torch.float32
+    dtype = _BF16 if bf16 else _F32
     _check_embed("embed", ids, W, scale, dtype)
-    n, (V, d) = ids.shape[0], W.shape
-    y = torch.empty(n, d, device=W.device, dtype=dtype)
-    ids, Wc = ids.to(torch.int64).contiguous(), _aligned(W)
-    with torch.cuda.device(W.device):
-        check(lm_lib().pragnosia_embed_fwd(_ptr(ids), _ptr(Wc), int(W.dtype == torch.bfloat16), float(scale), _ptr(y),
-                                           int(bf16), n, V, d, _stream(W)), "pragnosia_embed_fwd")
-    return y
+    return _forward(_as(ids, _I64), _as(W, W.dtype), float(scale), dtype)
 
 
 @embed.register_fake
 def _(ids, W, scale, bf16):
-    return W.new_empty(ids.shape[0], W.shape[1], dtype=torch.bfloat16 if bf16 else torch.float32)
+    return W.new_empty(ids.shape[0], W.shape[1], dtype=_BF16 if bf16 else _F32)
 
 
 @torch.library.custom_op("pragnosia::embed_bwd", mutates_args=())
@@ -57,30 +94,21 @@ def embed_bwd(g: Tensor, ids: Tensor, V: int, scale: float, bf16: bool) -> Tenso
     _require_gpu(g, ids)
     if g.dtype not in _FLOATS or g.dim() != 2 or g.shape[1] % 8 or g.shape[1] == 0 or V <= 0:
         raise PragnosiaError(f"embed_bwd: gradients (n, d) in bf16 or fp32 expected, got {tuple(g.shape)} {g.dtype}")
+    if ids.dtype not in _INTS:
+        raise PragnosiaError(f"embed_bwd: ids must be integers, got {ids.dtype}")
     _expect("embed_bwd", g.device, ids=(ids, (g.shape[0],)))
-    n, d = g.shape
-    dW = torch.empty(V, d, device=g.device, dtype=torch.bfloat16 if bf16 else torch.float32)
-    g, ids = _aligned(g), ids.to(torch.int64).contiguous()
-    with torch.cuda.device(g.device):
-        L = lm_lib()
-        nbytes = L.pragnosia_embed_bwd_workspace_bytes(n, V, d)
-        if nbytes < 0:
-            raise PragnosiaError(f"embed_bwd: shape n={n} V={V} d={d} rejected")
-        ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
-        check(L.pragnosia_embed_bwd(_ptr(g), int(g.dtype == torch.bfloat16), _ptr(ids), float(scale), _ptr(dW),
-                                    int(bf16), _ptr(ws), nbytes, n, V, d, _stream(g)), "pragnosia_embed_bwd")
-    return dW
+    return _backward(g, _as(ids, _I64), V, float(scale), _BF16 if bf16 else _F32)
 
 
 @embed_bwd.register_fake
 def _(g, ids, V, scale, bf16):
-    return g.new_empty(V, g.shape[1], dtype=torch.bfloat16 if bf16 else torch.float32)
+    return g.new_empty(V, g.shape[1], dtype=_BF16 if bf16 else _F32)
 
 
 def _embed_setup(ctx, inputs, output):
     ids, W, scale, _ = inputs
     ctx.save_for_backward(ids)
-    ctx.V, ctx.scale, ctx.bf16 = W.shape[0], scale, W.dtype == torch.bfloat16
+    ctx.V, ctx.scale, ctx.bf16 = W.shape[0], scale, W.dtype == _BF16
 
 
 def _embed_backward(ctx, g):
@@ -94,7 +122,13 @@ embed.register_autograd(_embed_backward, setup_context=_embed_setup)
 def embedding(ids: Tensor, W: Tensor, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> Tensor:
     """scale * W[ids], (..., d) in `dtype` (W's by default; the product is rounded once). W (V, d) bf16 or fp32, d a
     multiple of 8. An id outside [0, V) gives a row of zeros and takes no part in W's gradient."""
-    dtype = dtype or W.dtype
-    if dtype not in _FLOATS:
-        raise PragnosiaError(f"embedding: the rows must be bf16 or fp32, got {dtype}")
-    return embed(ids.reshape(-1), W, float(scale), dtype == torch.bfloat16).view(*ids.shape, W.shape[-1])
+    dtype, scale = dtype or W.dtype, float(scale)
+    flat = ids if ids.dim() == 1 else ids.reshape(-1)
+    _check_embed("embedding", flat, W, scale, dtype)
+    if torch.compiler.is_compiling():
+        y = embed(flat, W, scale, dtype == _BF16)
+    elif torch.is_grad_enabled() and W.requires_grad:
+        y = _Embedding.apply(flat, W, scale, dtype)
+    else:
+        y = _forward(_as(flat, _I64), _as(W, W.dtype), scale, dtype)
+    return y if ids.dim() == 1 else y.view(*ids.shape, W.shape[-1])

@@ -5,18 +5,20 @@ top logits, forward and backward on hand-written kernels (csrc/head_loss.hip; C 
     kd, ce = linear_distill(h, W, ids, logits, tau, y)
 
 h (..., d) are hidden rows and W (V, d) the head's weight (the LM's tied table), d a multiple of 8. The logits h W^T are
-formed on the bf16 matrix cores in pieces of the vocabulary: h and W in another type are rounded to bf16, as autocast
-rounds a Linear's operands. The reference's LM forms its logits in chunks of rows under activation checkpointing
+formed on the bf16 matrix cores in pieces of the vocabulary: fp32 h and W are rounded to bf16, as autocast rounds a
+Linear's operands. The reference's LM forms its logits in chunks of rows under activation checkpointing
 (`src/model.py:563-567`); LM.loss does so here too, unless the model was built with fused_ends.
 
 Every loss comes per token in fp32, so a mean, a mask or weights are the caller's own: the kernels take the per-token
 gradients that autograd hands back. The gradients of logits are rounded to bf16 once, before the two products that dh
 (in h's type) and dW (in W's; an fp32 W gets the unrounded fp32 sums) are; sums are held in fp32 throughout and taken in
 a fixed order, so the same call gives the same bits.
+
+An eager call goes through an autograd function straight to the C ABI; a traced one (torch.compile) through the custom
+ops, whose dispatch costs tens of microseconds a call.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional
 
@@ -24,22 +26,47 @@ import torch
 from torch import Tensor
 
 from ._lib import PragnosiaError, check, lm_lib
-from .ops import _bf16, _expect, _f32, _ptr, _require_gpu, _stream
+from .ops import _expect, _require_gpu
 
 _FLOATS = (torch.bfloat16, torch.float32)
 _INTS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
+_F32, _BF16, _I64 = torch.float32, torch.bfloat16, torch.int64
 
 
-def _aligned(t: Optional[Tensor]) -> Optional[Tensor]:
-    """t contiguous, at an address the kernels' 16-byte loads take (a slice of a buffer may start anywhere)."""
+def _as(t: Optional[Tensor], dtype: torch.dtype) -> Optional[Tensor]:
+    """t in `dtype`, contiguous, at an address the kernels' 16-byte loads take (a slice of a buffer may start anywhere)."""
     if t is None:
         return None
-    t = t.contiguous()
+    if t.dtype != dtype or not t.is_contiguous():
+        t = t.to(dtype).contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _at(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """The device of `t` made the current one for a launch, where it is not already."""
+
+    def __init__(self, t: Tensor):
+        index = t.device.index
+        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+        self.index = index
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
 
 
 def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
                 tau: float) -> None:
+    _require_gpu(h, W, y, ids, z)
     if h.dim() != 2 or W.dim() != 2:
         raise PragnosiaError(f"{op}: h (..., d) and W (V, d) expected, got {tuple(h.shape)} and {tuple(W.shape)}")
     n, d = h.shape
@@ -63,131 +90,175 @@ def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optiona
         raise PragnosiaError(f"{op}: tau must be positive and finite, got {tau}")
 
 
-@torch.library.custom_op("pragnosia::head_loss", mutates_args=())
-def head_loss(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
-              tau: float) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """h (n, d), W (V, d), y (n) or None, ids and z (n, K) or None. Returns (ce, lse, kd, then what the backward takes:
-    lse_t, psum, entry, p, zl, and the bf16 operands); ce and lse are empty without y, kd and its share without ids."""
-    _require_gpu(h, W, y, ids, z)
-    _check_head("head_loss", h, W, y, ids, z, tau)
+def _forward(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor], tau: float):
+    """h (n, d), W (V, d) bf16; y (n) int64 or None; ids int64 and z fp32 (n, K) or None, all contiguous. Returns (ce,
+    lse, kd, stats): fp32, None where not asked for; stats holds lse_t, psum, entry, p and zl for the backward."""
     n, d = h.shape
     V, K = W.shape[0], 0 if ids is None else ids.shape[1]
-    e = lambda *s, dt=torch.float32: torch.empty(*s, device=h.device, dtype=dt)
-    ny, nk = (0 if y is None else n), (0 if ids is None else n)
-    ce, lse, kd, lse_t, psum = e(ny), e(ny), e(nk), e(nk), e(nk)
-    entry, p, zl = e(nk, K, dt=torch.int32), e(nk, K), e(nk, K)
-    hb, Wb = h.new_empty(0), W.new_empty(0)
+    e = lambda s: torch.empty(s, device=h.device, dtype=_F32)
+    ce, lse = (None, None) if y is None else (e(n), e(n))
+    kd, stats = (None, None) if ids is None else (e(n), e(n * (2 + 3 * K)))
     if n == 0:
-        return ce, lse, kd, lse_t, psum, entry, p, zl, hb, Wb
-    h16, W16 = _aligned(_bf16(h)), _aligned(_bf16(W))
-    y = None if y is None else y.to(torch.int64).contiguous()
-    ids, z = (None, None) if ids is None else (ids.to(torch.int64).contiguous(), _f32(z))
-    with torch.cuda.device(h.device):
-        L = lm_lib()
-        nbytes = L.pragnosia_head_fwd_workspace_bytes(n, V, d, K)
-        if nbytes < 0:
-            raise PragnosiaError(f"head_loss: shape n={n} V={V} d={d} K={K} rejected")
-        ws = e(nbytes, dt=torch.uint8)
-        opt = lambda t, on: _ptr(t) if on else None
-        check(L.pragnosia_head_fwd(_ptr(h16), _ptr(W16), _ptr(y), _ptr(ids), _ptr(z), float(tau), opt(ce, ny),
-                                   opt(lse, ny), opt(kd, nk), opt(lse_t, nk), opt(psum, nk), opt(entry, nk),
-                                   opt(p, nk), opt(zl, nk), _ptr(ws), nbytes, n, V, d, K, _stream(h)),
-              "pragnosia_head_fwd")
-    return (ce, lse, kd, lse_t, psum, entry, p, zl, hb if h16.data_ptr() == h.data_ptr() else h16,
-            Wb if W16.data_ptr() == W.data_ptr() else W16)
+        return ce, lse, kd, stats
+    L = lm_lib()
+    nbytes = L.pragnosia_head_fwd_workspace_bytes(n, V, d, K)
+    if nbytes < 0:
+        raise PragnosiaError(f"head_loss: shape n={n} V={V} d={d} K={K} rejected")
+    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    with _on(h) as stream:
+        check(L.pragnosia_head_fwd(_at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce), _at(lse), _at(kd),
+                                   *_stats_at(stats, n, K), _at(ws), nbytes, n, V, d, K, stream), "pragnosia_head_fwd")
+    return ce, lse, kd, stats
+
+
+def _stats_at(stats: Optional[Tensor], n: int, K: int):
+    """Addresses of lse_t, psum, entry, p, zl in `stats`."""
+    if stats is None:
+        return (None,) * 5
+    a = stats.data_ptr()
+    return a, a + 4 * n, a + 8 * n, a + 8 * n + 4 * n * K, a + 8 * n + 8 * n * K
+
+
+def _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, K: int, tau: float, need_h: bool, need_W: bool, dw_f32: bool):
+    """Gradients of ce, lse and kd ((n,) or None) -> (dh bf16, dW bf16 or fp32), None where not needed."""
+    n, d = h.shape
+    V = W.shape[0]
+    dW_type = _F32 if dw_f32 else _BF16
+    if n == 0 or (g_ce is None and g_lse is None and g_kd is None):
+        return (h.new_zeros(n, d) if need_h else None,
+                W.new_zeros(V, d, dtype=dW_type) if need_W else None)
+    dh = torch.empty_like(h) if need_h else None
+    dW = torch.empty(V, d, device=h.device, dtype=dW_type) if need_W else None
+    g_ce, g_lse, g_kd = _as(g_ce, _F32), _as(g_lse, _F32), _as(g_kd, _F32)
+    L = lm_lib()
+    nbytes = L.pragnosia_head_bwd_workspace_bytes(n, V, d)
+    if nbytes < 0:
+        raise PragnosiaError(f"head_loss_bwd: shape n={n} V={V} d={d} rejected")
+    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    with _on(h) as stream:
+        check(L.pragnosia_head_bwd(_at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W), _at(y), _at(lse),
+                                   *_stats_at(stats, n, K), tau, _at(dh), _at(dW), int(dw_f32), _at(ws), nbytes, n, V,
+                                   d, K, stream), "pragnosia_head_bwd")
+    return dh, dW
+
+
+def _operands(h, W, y, ids, z):
+    return _as(h, _BF16), _as(W, _BF16), _as(y, _I64), _as(ids, _I64), _as(z, _F32)
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, W, y, ids, z, tau):
+        h16, W16, y, ids, z = _operands(h, W, y, ids, z)
+        ce, lse, kd, stats = _forward(h16, W16, y, ids, z, tau)
+        ctx.save_for_backward(h16, W16, y, lse, stats)
+        ctx.tau, ctx.K, ctx.types = tau, 0 if ids is None else ids.shape[1], (h.dtype, W.dtype)
+        ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
+        return ce, lse, kd
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_ce, g_lse, g_kd):
+        h, W, y, lse, stats = ctx.saved_tensors
+        dh, dW = _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, ctx.K, ctx.tau, ctx.needs_input_grad[0],
+                           ctx.needs_input_grad[1], ctx.types[1] == _F32)
+        if dh is not None and ctx.types[0] != _BF16:
+            dh = dh.to(ctx.types[0])
+        return dh, dW, None, None, None, None
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the same as custom ops, for traces
+@torch.library.custom_op("pragnosia::head_loss", mutates_args=())
+def head_loss(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
+              tau: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """h (n, d), W (V, d), y (n) or None, ids and z (n, K) or None. Returns (ce, lse, kd, stats), empty where there are
+    no labels or no teacher; stats is what the backward takes."""
+    _check_head("head_loss", h, W, y, ids, z, tau)
+    got = _forward(*_operands(h, W, y, ids, z), float(tau))
+    return tuple(t if t is not None else torch.empty(0, device=h.device) for t in got)
 
 
 @head_loss.register_fake
 def _(h, W, y, ids, z, tau):
     n, K = h.shape[0], 0 if ids is None else ids.shape[1]
+    e = lambda s: h.new_empty(s, dtype=_F32)
     ny, nk = (0 if y is None else n), (0 if ids is None else n)
-    e = lambda *s, dt=torch.float32: h.new_empty(*s, dtype=dt)
-    return (e(ny), e(ny), e(nk), e(nk), e(nk), e(nk, K, dt=torch.int32), e(nk, K), e(nk, K),
-            h.new_empty(0) if h.dtype == torch.bfloat16 else e(*h.shape, dt=torch.bfloat16),
-            W.new_empty(0) if W.dtype == torch.bfloat16 else e(*W.shape, dt=torch.bfloat16))
+    return e(ny), e(ny), e(nk), e(nk * (2 + 3 * K))
 
 
 @torch.library.custom_op("pragnosia::head_loss_bwd", mutates_args=())
 def head_loss_bwd(g_ce: Optional[Tensor], g_lse: Optional[Tensor], g_kd: Optional[Tensor], h: Tensor, W: Tensor,
-                  y: Optional[Tensor], lse: Tensor, lse_t: Tensor, psum: Tensor, entry: Tensor, p: Tensor, zl: Tensor,
-                  tau: float, need_h: bool, need_W: bool, dw_f32: bool) -> tuple[Tensor, Tensor]:
-    """Gradients of head_loss's ce, lse and kd -> (dh (n, d) bf16, dW (V, d) bf16 or fp32); empty where not needed. h
-    and W bf16."""
-    _require_gpu(g_ce, g_lse, g_kd, h, W, y, lse, lse_t, psum, entry, p, zl)
-    if h.dim() != 2 or W.dim() != 2:
+                  y: Optional[Tensor], lse: Tensor, stats: Tensor, tau: float, need_h: bool,
+                  need_W: bool) -> tuple[Tensor, Tensor]:
+    """Gradients of head_loss's ce, lse and kd -> (dh, dW) in h's and W's types; empty where not needed. y as given to
+    head_loss, lse and stats as it returned them."""
+    _require_gpu(g_ce, g_lse, g_kd, h, W, y, lse, stats)
+    if h.dim() != 2 or W.dim() != 2 or h.dtype not in _FLOATS or W.dtype not in _FLOATS:
         raise PragnosiaError(f"head_loss_bwd: h (n, d) and W (V, d) expected, got {tuple(h.shape)}, {tuple(W.shape)}")
     n, d = h.shape
-    V, K = W.shape[0], entry.shape[-1] if g_kd is not None else 0
-    nk = n if g_kd is not None else None
     _expect("head_loss_bwd", h.device, W=(W, (None, d)), g_ce=(g_ce, (n,)), g_lse=(g_lse, (n,)), g_kd=(g_kd, (n,)),
-            y=(y, (n,)), lse=(lse if g_ce is not None or g_lse is not None else None, (n,)))
-    if g_kd is not None:
-        _expect("head_loss_bwd", h.device, lse_t=(lse_t, (nk,)), psum=(psum, (nk,)), entry=(entry, (nk, K)),
-                p=(p, (nk, K)), zl=(zl, (nk, K)))
-    if h.dtype != torch.bfloat16 or W.dtype != torch.bfloat16 or entry.dtype != torch.int32:
-        raise PragnosiaError("head_loss_bwd: h and W must be bf16 and entry int32, as head_loss returns them")
-    if g_ce is not None and y is None:
-        raise PragnosiaError("head_loss_bwd: g_ce without labels")
-    dh = torch.empty(n if need_h else 0, d, device=h.device, dtype=torch.bfloat16)
-    dW = torch.empty(V if need_W else 0, d, device=h.device, dtype=torch.float32 if dw_f32 else torch.bfloat16)
-    if n == 0 or not (need_h or need_W) or (g_ce is None and g_lse is None and g_kd is None):
-        return dh.zero_(), dW.zero_()
-    h, W = _aligned(h), _aligned(W)
-    y = None if y is None else y.to(torch.int64).contiguous()
-    g_ce, g_lse, g_kd, lse, lse_t, psum, p, zl = (_f32(t) for t in (g_ce, g_lse, g_kd, lse, lse_t, psum, p, zl))
-    entry = entry.contiguous()
-    with torch.cuda.device(h.device):
-        L = lm_lib()
-        nbytes = L.pragnosia_head_bwd_workspace_bytes(n, V, d)
-        if nbytes < 0:
-            raise PragnosiaError(f"head_loss_bwd: shape n={n} V={V} d={d} rejected")
-        ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-        opt = lambda t, on: _ptr(t) if on else None
-        kd = g_kd is not None
-        check(L.pragnosia_head_bwd(_ptr(g_ce), _ptr(g_lse), _ptr(g_kd), _ptr(h), _ptr(W), _ptr(y),
-                                   opt(lse, g_ce is not None or g_lse is not None), opt(lse_t, kd), opt(psum, kd),
-                                   opt(entry, kd), opt(p, kd), opt(zl, kd), float(tau), opt(dh, need_h),
-                                   opt(dW, need_W), int(dw_f32), _ptr(ws), nbytes, n, V, d, K, _stream(h)),
-              "pragnosia_head_bwd")
-    return dh, dW
+            y=(y, (n,)), lse=(lse if y is not None else None, (n,)), stats=(stats, (None,)))
+    K = (stats.numel() // n - 2) // 3 if n and stats.numel() else 0
+    if stats.numel() not in (0, n * (2 + 3 * K)) or lse.dtype != _F32 or stats.dtype != _F32:
+        raise PragnosiaError("head_loss_bwd: lse and stats must be head_loss's")
+    if (y is None and (g_ce is not None or g_lse is not None)) or (K == 0 and g_kd is not None):
+        raise PragnosiaError("head_loss_bwd: a gradient of a loss that was not computed")
+    dh, dW = _backward(g_ce, g_lse, g_kd, _as(h, _BF16), _as(W, _BF16), _as(y, _I64),
+                       None if y is None else _as(lse, _F32), _as(stats, _F32) if K else None, K, float(tau), need_h,
+                       need_W, W.dtype == _F32)
+    return (h.new_empty(0, d) if dh is None else dh.to(h.dtype)), (W.new_empty(0, d) if dW is None else dW)
 
 
 @head_loss_bwd.register_fake
-def _(g_ce, g_lse, g_kd, h, W, y, lse, lse_t, psum, entry, p, zl, tau, need_h, need_W, dw_f32):
+def _(g_ce, g_lse, g_kd, h, W, y, lse, stats, tau, need_h, need_W):
     n, d = h.shape
-    return (h.new_empty(n if need_h else 0, d, dtype=torch.bfloat16),
-            h.new_empty(W.shape[0] if need_W else 0, d, dtype=torch.float32 if dw_f32 else torch.bfloat16))
+    return h.new_empty(n if need_h else 0, d), W.new_empty(W.shape[0] if need_W else 0, d)
 
 
 def _head_setup(ctx, inputs, output):
-    ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
+    ctx.set_materialize_grads(False)
     h, W, y, ids, z, tau = inputs
-    _, lse, _, lse_t, psum, entry, p, zl, h16, W16 = output
-    ctx.tau, ctx.dtypes, ctx.has = tau, (h.dtype, W.dtype), (y is not None, ids is not None)
-    ctx.save_for_backward(h16 if h16.dim() == 2 else h, W16 if W16.dim() == 2 else W, y, lse, lse_t, psum, entry, p, zl)
-    ctx.mark_non_differentiable(lse_t, psum, entry, p, zl, h16, W16)
+    _, lse, _, stats = output
+    ctx.tau, ctx.has = tau, (y is not None, ids is not None)
+    ctx.save_for_backward(h, W, y, lse, stats)
+    ctx.mark_non_differentiable(stats)
 
 
-def _head_backward(ctx, g_ce, g_lse, g_kd, *_):
-    h, W, y, lse, lse_t, psum, entry, p, zl = ctx.saved_tensors
+def _head_backward(ctx, g_ce, g_lse, g_kd, _):
+    h, W, y, lse, stats = ctx.saved_tensors
     need_h, need_W = ctx.needs_input_grad[:2]
     has_y, has_kd = ctx.has
     dh, dW = head_loss_bwd(g_ce if has_y else None, g_lse if has_y else None, g_kd if has_kd else None, h, W, y, lse,
-                           lse_t, psum, entry, p, zl, ctx.tau, need_h, need_W, ctx.dtypes[1] == torch.float32)
-    return dh.to(ctx.dtypes[0]) if need_h else None, dW if need_W else None, None, None, None, None
+                           stats, ctx.tau, need_h, need_W)
+    return dh if need_h else None, dW if need_W else None, None, None, None, None
 
 
 head_loss.register_autograd(_head_backward, setup_context=_head_setup)
 
 
-def _rows(op: str, h: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor]):
+def _losses(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
+            tau: float):
+    """(ce, lse, kd) in h's leading shape."""
     lead = h.shape[:-1]
     if h.dim() < 1 or (y is not None and y.shape != lead) or any(
             t is not None and (t.dim() != h.dim() or t.shape[:-1] != lead) for t in (ids, z)):
         raise PragnosiaError(f"{op}: the labels' and the teacher's leading sizes must be h's {tuple(lead)}, got "
                              f"{[None if t is None else tuple(t.shape) for t in (y, ids, z)]}")
-    flat = lambda t: None if t is None else t.reshape(-1, t.shape[-1])
-    return flat(h), None if y is None else y.reshape(-1), flat(ids), flat(z)
+    flat = h.dim() == 2
+    if not flat:
+        h = h.reshape(-1, h.shape[-1])
+        y = None if y is None else y.reshape(-1)
+        ids, z = (None, None) if ids is None else (ids.reshape(-1, ids.shape[-1]), z.reshape(-1, z.shape[-1]))
+    if torch.compiler.is_compiling():
+        got = head_loss(h, W, y, ids, z, tau)[:3]
+    else:
+        _check_head(op, h, W, y, ids, z, tau)
+        if torch.is_grad_enabled() and (h.requires_grad or W.requires_grad):
+            got = _HeadLoss.apply(h, W, y, ids, z, tau)
+        else:
+            got = _forward(*_operands(h, W, y, ids, z), tau)[:3]
+    return got if flat else tuple(t if t is None else t.view(lead) if t.numel() or 0 in lead else t for t in got)
 
 
 def linear_cross_entropy(h: Tensor, W: Tensor, y: Tensor) -> tuple[Tensor, Tensor]:
@@ -196,9 +267,7 @@ def linear_cross_entropy(h: Tensor, W: Tensor, y: Tensor) -> tuple[Tensor, Tenso
 
     A label outside [0, V) (padding, such as -100) has loss 0 and adds no gradient. Such rows of h still enter dW's
     sums, times zero: they have to be finite there."""
-    h2, y2, _, _ = _rows("linear_cross_entropy", h, y, None, None)
-    out = head_loss(h2, W, y2, None, None, 1.0)
-    return out[0].view(y.shape), out[1].view(y.shape)
+    return _losses("linear_cross_entropy", h, W, y, None, None, 1.0)[:2]
 
 
 def linear_distill(h: Tensor, W: Tensor, ids: Tensor, logits: Tensor, tau: float = 1.0,
@@ -211,6 +280,5 @@ def linear_distill(h: Tensor, W: Tensor, ids: Tensor, logits: Tensor, tau: float
     at tau. An id outside [0, V) marks an entry that is not there (lists of different lengths); a logit of -inf has
     probability zero; a token with no entry left has loss 0 and no gradient. A repeated id has the sum of its entries'
     probabilities. The teacher gets no gradient."""
-    h2, y2, i2, z2 = _rows("linear_distill", h, y, ids, logits)
-    out = head_loss(h2, W, y2, i2, z2.detach(), float(tau))
-    return out[2].view(h.shape[:-1]), None if y is None else out[0].view(y.shape)
+    ce, _, kd = _losses("linear_distill", h, W, y, ids, logits.detach(), float(tau))
+    return kd, None if y is None else ce
