@@ -14,8 +14,8 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from ._lib import PragnosiaError, check, lm_lib
-from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _on
+from ._lib import PragnosiaError, lm_lib
+from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _once
 from .ops import _expect, _require_gpu
 
 
@@ -36,9 +36,8 @@ def _forward(ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype) -> Tensor
     """ids (n) int64, W (V, d), both contiguous."""
     n, (V, d) = ids.shape[0], W.shape
     y = torch.empty(n, d, device=W.device, dtype=dtype)
-    with _on(W) as stream:
-        check(lm_lib().pragnosia_embed_fwd(_at(ids), _at(W), W.dtype == _BF16, scale, _at(y), dtype == _BF16, n, V, d,
-                                           stream), "pragnosia_embed_fwd")
+    _call("pragnosia_embed_fwd", lm_lib().pragnosia_embed_fwd, W, _at(ids), _at(W), W.dtype == _BF16, scale, _at(y),
+          dtype == _BF16, n, V, d)
     return y
 
 
@@ -52,9 +51,8 @@ def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) 
     if nbytes < 0:
         raise PragnosiaError(f"embed_bwd: shape n={n} V={V} d={d} rejected")
     ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
-    with _on(g) as stream:
-        check(L.pragnosia_embed_bwd(_at(g), g.dtype == _BF16, _at(ids), scale, _at(dW), dtype == _BF16, _at(ws), nbytes,
-                                    n, V, d, stream), "pragnosia_embed_bwd")
+    _call("pragnosia_embed_bwd", L.pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(ids), scale, _at(dW),
+          dtype == _BF16, _at(ws), nbytes, n, V, d)
     return dW
 
 
@@ -67,7 +65,7 @@ class _Embedding(torch.autograd.Function):
         return _forward(ids, _as(W, W.dtype), scale, dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         ids, = ctx.saved_tensors
         return None, _backward(g, ids, ctx.V, ctx.scale, ctx.dtype), None, None

@@ -46,22 +46,30 @@ def _at(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The device of `t` made the current one for a launch, where it is not already."""
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(i).cuda_stream without the Python object
 
-    def __init__(self, t: Tensor):
-        index = t.device.index
-        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
-        self.index = index
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.index).cuda_stream
+def _call(what: str, fn, t: Tensor, *args) -> None:
+    """fn(*args, the current stream of t's device), with that device the current one."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+
+def _once(backward):
+    """A backward whose results cannot be differentiated again: refused (once_differentiable, whose wrapper costs as
+    much as a short call's launches) where a graph of the backward is built, direct otherwise."""
+    refusing = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
 
 
 def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
@@ -105,9 +113,8 @@ def _forward(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z
     if nbytes < 0:
         raise PragnosiaError(f"head_loss: shape n={n} V={V} d={d} K={K} rejected")
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-    with _on(h) as stream:
-        check(L.pragnosia_head_fwd(_at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce), _at(lse), _at(kd),
-                                   *_stats_at(stats, n, K), _at(ws), nbytes, n, V, d, K, stream), "pragnosia_head_fwd")
+    _call("pragnosia_head_fwd", L.pragnosia_head_fwd, h, _at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce), _at(lse),
+          _at(kd), *_stats_at(stats, n, K), _at(ws), nbytes, n, V, d, K)
     return ce, lse, kd, stats
 
 
@@ -135,10 +142,8 @@ def _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, K: int, tau: float, need_h
     if nbytes < 0:
         raise PragnosiaError(f"head_loss_bwd: shape n={n} V={V} d={d} rejected")
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-    with _on(h) as stream:
-        check(L.pragnosia_head_bwd(_at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W), _at(y), _at(lse),
-                                   *_stats_at(stats, n, K), tau, _at(dh), _at(dW), int(dw_f32), _at(ws), nbytes, n, V,
-                                   d, K, stream), "pragnosia_head_bwd")
+    _call("pragnosia_head_bwd", L.pragnosia_head_bwd, h, _at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W), _at(y),
+          _at(lse), *_stats_at(stats, n, K), tau, _at(dh), _at(dW), dw_f32, _at(ws), nbytes, n, V, d, K)
     return dh, dW
 
 
@@ -157,7 +162,7 @@ class _HeadLoss(torch.autograd.Function):
         return ce, lse, kd
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g_ce, g_lse, g_kd):
         h, W, y, lse, stats = ctx.saved_tensors
         dh, dW = _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, ctx.K, ctx.tau, ctx.needs_input_grad[0],
