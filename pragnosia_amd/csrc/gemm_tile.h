@@ -9,9 +9,9 @@
 //     read the second half's fragments;  multiply the first half
 //     wait until stage s + 1 has arrived; barrier (every wave has read all of stage s)
 //     issue the loads of stage s + NS into the buffer of stage s;  read stage s + 1's first half;  multiply the second
-// so that fragment reads run beside products (spread among them by the scheduler's group barriers: 1268 TFLOP/s at 8192^3
-// against 1217 with the reads first), one barrier a step, and a stage has NS - 1 steps to arrive. Stages past the
-// last are issued too, from offsets past the resource (zeros, no memory traffic), so that the wait counts are constants.
+// so that fragment reads run beside products, one barrier a step, and a stage has NS - 1 steps to arrive. Reads and loads
+// are spread among the products by hand. Stages past the last are issued too, from offsets past the resource (zeros, no
+// memory traffic), so that the wait counts are constants.
 //
 // A buffer load to LDS writes its 64 lanes' 16 bytes consecutively, so the arrangement against bank conflicts is made by
 // which 16 bytes each lane fetches:
@@ -41,6 +41,20 @@ struct Operand {
   const __bf16* p;
   int64_t ld, rows;
 };
+
+// 16 bytes a lane from base + off (zero past `records` bytes) to LDS address lds + 16 lane; base, records and lds uniform.
+// As an instruction of its own, not the builtin: before a transposing LDS read the compiler waits for every load to LDS
+// that it knows of, which would leave a stage no time to arrive. No register is written, so nothing of the compiler's is
+// in flight; the arrival is waited for by wait_loads, and a wait for another access only becomes stricter by these. (The
+// s_nop covers the five wait states from a lane read into a scalar register to its use as a resource.)
+PGN_DEVICE void load_to_lds(const char* base, int records, int off, unsigned lds) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const i32x4 r = {(int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xffffu), records, 0x00020000};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r)
+               : "memory", "m0");
+}
+
+PGN_DEVICE unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(lds_void*)p; }
 
 // One operand's staging: R rows (KR = false) or columns (KR = true) of the tile, T threads.
 template <bool KR, int R, int T>
@@ -99,25 +113,24 @@ struct Stager {
     }
   }
 
-  // Stage s of the range [k_begin, k_end) into lds (wave w's share). A stage past the last loads nothing.
-  PGN_DEVICE void load(int s, int64_t k_count, unsigned char* lds, int w) const {
-    const int64_t at = s * step;
-    const char* p = reinterpret_cast<const char*>(base) + at;
-    const int records = (int)max((int64_t)0, min(bytes - at, (int64_t)0x7fff0000));
-    int beyond = 0;
+  // Stage s of the range [k_begin, k_end): aim() at it, then its kLoads loads into lds (wave w's share). A stage past the
+  // last loads nothing.
+  const char* at;
+  int records, beyond;
+  PGN_DEVICE void aim(int s, int64_t k_count) {
+    at = reinterpret_cast<const char*>(base) + s * step;
+    records = (int)max((int64_t)0, min(bytes - s * step, (int64_t)0x7fff0000));
+    beyond = 0;
     if constexpr (!KR) {
       // all ones past the range's end: the offset is then past the resource
       const int room = (int)min(k_count - (int64_t)s * kGemmK, (int64_t)kGemmK);
       beyond = ((room - 1 - k_seg) >> 31) & 0x7ffffff0;
     }
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int ahead = kSame ? u * kLoadRows * pitch : 0;
-      const __amdgpu_buffer_rsrc_t r =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p + ahead), (short)0, max(0, records - ahead), 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + u * T * 16 + w * 1024), 16,
-                                               off[kSame ? 0 : u] | beyond, 0, 0, 0);
-    }
+  }
+  template <int U>
+  PGN_DEVICE void load(unsigned lds, int w) const {
+    const int ahead = kSame ? U * kLoadRows * pitch : 0;
+    load_to_lds(at + ahead, max(0, records - ahead), off[kSame ? 0 : U] | beyond, lds + U * T * 16 + w * 1024);
   }
 };
 
@@ -177,22 +190,35 @@ struct Frags {
   PGN_DEVICE void init(const WaveIdx& t) {
     rx.init(16 * C::NA * (t.w % C::WX), t.g, t.i), ry.init(16 * C::NB * (t.w / C::WX), t.g, t.i);
   }
+  // Fragment Q of half KB: Y's, then X's.
+  template <int KB, int Q>
+  PGN_DEVICE void read_one(const unsigned char* p) {
+    if constexpr (Q < C::NB)
+      fy[KB][Q] = ry.template get<Q, KB>(p + kX);
+    else
+      fx[KB][Q - C::NB] = rx.template get<Q - C::NB, KB>(p);
+  }
   template <int KB>
   PGN_DEVICE void read(const unsigned char* p) {
-    static_for<0, C::NB>([&](auto b) { fy[KB][b.value] = ry.template get<b.value, KB>(p + kX); });
-    static_for<0, C::NA>([&](auto a) { fx[KB][a.value] = rx.template get<a.value, KB>(p); });
+    static_for<0, C::NA + C::NB>([&](auto q) { read_one<KB, q.value>(p); });
   }
-  // The products of half KB, the reads of the other half (issued before) spread among them: one read, then products.
-  template <int KB>
-  PGN_DEVICE void multiply(f32x4 (&acc)[C::NA][C::NB]) {
+  // The products of half KB, NB at a time, and among them the fragments of the other half read from p (unless null) and
+  // loads(u), u < kLoads: the fragments before the last group, so that they have arrived when the half ends.
+  template <int KB, bool READ, int kLoads, class L>
+  PGN_DEVICE void multiply(f32x4 (&acc)[C::NA][C::NB], const unsigned char* p, L&& loads) {
+    constexpr int kFrags = C::NA + C::NB, kGroups = C::NA > 1 ? C::NA - 1 : 1;
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this half's fragments, read during the half before
+    static_for<0, C::NA>([&](auto a) {
+      constexpr int A = decltype(a)::value;
+      static_for<A * kLoads / C::NA, (A + 1) * kLoads / C::NA>([&](auto u) { loads(u); });
+      if constexpr (READ) {
+        constexpr int lo = A * kFrags / kGroups, hi = (A + 1) * kFrags / kGroups;
+        static_for<(lo < kFrags ? lo : kFrags), (hi < kFrags ? hi : kFrags)>(
+            [&](auto q) { read_one<1 - KB, decltype(q)::value>(p); });
+      }
 #pragma unroll
-    for (int a = 0; a < C::NA; ++a)
-#pragma unroll
-      for (int b = 0; b < C::NB; ++b) acc[a][b] = pgn_mfma(fx[KB][a], fy[KB][b], acc[a][b]);
-    constexpr int kReads = C::NA * (XKR ? 2 : 1) + C::NB * (YKR ? 2 : 1), kEach = C::NA * C::NB / kReads;
-    static_for<0, kReads>([&](auto) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
-      __builtin_amdgcn_sched_group_barrier(0x8, kEach > 0 ? kEach : 1, 0);  // products
+      for (int b = 0; b < C::NB; ++b) acc[A][b] = pgn_mfma(fx[KB][A], fy[KB][b], acc[A][b]);
+      __builtin_amdgcn_sched_barrier(0);
     });
   }
 };
@@ -221,26 +247,35 @@ PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_
   const int64_t k_count = k_end - k_begin;
   const int steps = (int)((k_count + kGemmK - 1) / kGemmK);
   zero_acc<C>(acc);
-  auto stage = [&](int s, int buf) {
-    unsigned char* p = lds + buf * C::kStage;
-    sx.load(s, k_count, p, t.w), sy.load(s, k_count, p + F::kX, t.w);
+  const unsigned lds0 = lds_address(lds);
+  constexpr int kLx = Stager<XKR, C::X, C::kThreads>::kLoads;
+  auto aim = [&](int s) { sx.aim(s, k_count), sy.aim(s, k_count); };
+  auto load = [&](auto u_c, int buf) {
+    constexpr int u = decltype(u_c)::value;
+    const unsigned p = lds0 + buf * C::kStage;
+    if constexpr (u < kLx)
+      sx.template load<u>(p, t.w);
+    else
+      sy.template load<u - kLx>(p + F::kX, t.w);
   };
-  for (int s = 0; s < C::NS; ++s) stage(s, s);
+  for (int s = 0; s < C::NS; ++s) {
+    aim(s);
+    static_for<0, C::kLoads>([&](auto u) { load(u, s); });
+  }
   wait_loads<C::kLoads * (C::NS - 1)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   f.template read<0>(lds);
   int buf = 0;
   for (int s = 0; s < steps; ++s) {
-    f.template read<1>(lds + buf * C::kStage);
-    f.template multiply<0>(acc);
+    const int next = buf + 1 == C::NS ? 0 : buf + 1;
+    f.template multiply<0, true, 0>(acc, lds + buf * C::kStage, [](auto) {});
+    aim(s + C::NS);
     wait_loads<C::kLoads * (C::NS - 2)>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    stage(s + C::NS, buf);
-    buf = buf + 1 == C::NS ? 0 : buf + 1;
-    f.template read<0>(lds + buf * C::kStage);
-    f.template multiply<1>(acc);
+    f.template multiply<1, true, C::kLoads>(acc, lds + next * C::kStage, [&](auto u) { load(u, buf); });
+    buf = next;
   }
   // nothing in flight into the buffers, nothing being read: they may be used again
   wait_loads<0>();
@@ -280,12 +315,21 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
     sx.tile(X, x0, 0), sy.tile(Y, y0, 0);
     if (li >= items) sx.bytes = sy.bytes = 0;  // loads nothing
   };
-  auto stage = [&](int buf) {
-    unsigned char* p = lds + buf * C::kStage;
-    sx.load(ls, d, p, t.w), sy.load(ls, d, p + F::kX, t.w);
-    if (++ls == steps) {
-      ls = 0, li += stride;
-      aim();
+  const unsigned lds0 = lds_address(lds);
+  constexpr int kLx = Stager<false, C::X, C::kThreads>::kLoads;
+  auto load = [&](auto u_c, int buf) {
+    constexpr int u = decltype(u_c)::value;
+    const unsigned p = lds0 + buf * C::kStage;
+    if constexpr (u == 0) sx.aim(ls, d), sy.aim(ls, d);
+    if constexpr (u < kLx)
+      sx.template load<u>(p, t.w);
+    else
+      sy.template load<u - kLx>(p + F::kX, t.w);
+    if constexpr (u == C::kLoads - 1) {
+      if (++ls == steps) {
+        ls = 0, li += stride;
+        aim();
+      }
     }
   };
   unsigned char* const info = lds + C::kLds;
@@ -293,15 +337,12 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
     int64_t x0 = 0, y0 = 0;
     if (item < items) at(item, x0, y0);
     const int64_t left = item < items && rows != nullptr ? min((int64_t)C::Y, row_count - y0) : 0;
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(static_cast<const char*>(rows) + (left > 0 ? y0 * kInfo : 0)), (short)0, (int)(left * kInfo),
-        0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(info + place * C::kThreads * 16 + t.w * 1024), 16, tid * 16,
-                                             0, 0, 0);
+    load_to_lds(static_cast<const char*>(rows) + (left > 0 ? y0 * kInfo : 0), (int)(left * kInfo), tid * 16,
+                lds0 + C::kLds + place * C::kThreads * 16 + t.w * 1024);
   };
   aim();
   load_info(first, 0);
-  for (int s = 0; s < C::NS; ++s) stage(s);
+  for (int s = 0; s < C::NS; ++s) static_for<0, C::kLoads>([&](auto u) { load(u, s); });
   wait_loads<C::kLoads * (C::NS - 1)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -312,8 +353,7 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
     f32x4 acc[C::NA][C::NB];
     zero_acc<C>(acc);
     auto half = [&](int s) {
-      f.template read<1>(lds + buf * C::kStage);
-      f.template multiply<0>(acc);
+      f.template multiply<0, true, 0>(acc, lds + buf * C::kStage, [](auto) {});
       if (s == 0 && item == first)
         wait_loads<0>();
       else if (s == 0)
@@ -323,18 +363,18 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       if (s == 0) load_info(item + stride, place ^ 1);
-      stage(buf);
-      buf = buf + 1 == C::NS ? 0 : buf + 1;
     };
     f.template read<0>(lds + buf * C::kStage);
     for (int s = 0; s + 1 < steps; ++s) {
       half(s);
-      f.template read<0>(lds + buf * C::kStage);
-      f.template multiply<1>(acc);
+      const int next = buf + 1 == C::NS ? 0 : buf + 1;
+      f.template multiply<1, true, C::kLoads>(acc, lds + next * C::kStage, [&](auto u) { load(u, buf); });
+      buf = next;
     }
     // the next tile's first fragments are read after the epilogue, which needs their registers
     half(steps - 1);
-    f.template multiply<1>(acc);
+    f.template multiply<1, false, C::kLoads>(acc, nullptr, [&](auto u) { load(u, buf); });
+    buf = buf + 1 == C::NS ? 0 : buf + 1;
     epilogue(acc, x0, y0, info + place * C::kThreads * 16);
     place ^= 1;
   }
