@@ -35,6 +35,7 @@ constexpr int kGemmK = 64;    // k a step
 constexpr int kXcdCount = 8;  // XCDs of an MI355X, taking workgroups in turn
 
 typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) const bf16x8 lds_bf16x8;
 
 // A matrix operand: `rows` rows of pitch `ld` elements (a multiple of 8) at p (16-byte aligned).
 struct Operand {
@@ -138,12 +139,13 @@ struct Stager {
 template <bool KR, int R>
 struct Reader {
   static constexpr int kRowBytes = KR ? 2 * R : 128;
-  int at[KR ? 8 : 2];  // byte offsets: KR = false: by k block; KR = true: by granule within an aligned eight (or four)
+  // byte offsets; KR = false: in k block 0 (the other is 64 bytes away, by an exchange); KR = true: by granule within an
+  // aligned eight (or four)
+  int at[KR ? 8 : 1];
 
   PGN_DEVICE void init(int x0, int g, int i) {
     if constexpr (!KR) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) at[kb] = (x0 + i) * 128 + ((4 * kb + g) ^ (i & 7)) * 16;
+      at[0] = (x0 + i) * 128 + (g ^ (i & 7)) * 16;
     } else {
       const int f = kRowBytes % 256 == 0 ? (i >> 2) | ((g & 1) << 2) : ((i >> 3) & 1) | ((g & 1) << 1);
 #pragma unroll
@@ -152,14 +154,15 @@ struct Reader {
     }
   }
 
-  // fragment q: rows (columns) x0 + 16 q ..; q < 8
+  // fragment Q: rows (columns) x0 + 16 Q ..; Q < 8. lds: address of the buffer.
   template <int Q, int KB>
-  PGN_DEVICE bf16x8 get(const unsigned char* lds) const {
+  PGN_DEVICE bf16x8 get(unsigned lds) const {
     if constexpr (!KR) {
-      return *reinterpret_cast<const bf16x8*>(lds + at[KB] + Q * 16 * 128);
+      return *(lds_bf16x8*)(lds + (KB ? at[0] ^ 64 : at[0]) + Q * 16 * 128);
     } else {
-      const __bf16* p = reinterpret_cast<const __bf16*>(lds + at[Q] + 32 * KB * kRowBytes);
-      return cat8(ds_read_tr(p), ds_read_tr(p + 4 * kRowBytes / 2));
+      const unsigned p = lds + at[Q] + 32 * KB * kRowBytes;
+      return cat8(__builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p),
+                  __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p + 4 * kRowBytes)));
     }
   }
 };
@@ -192,20 +195,21 @@ struct Frags {
   }
   // Fragment Q of half KB: Y's, then X's.
   template <int KB, int Q>
-  PGN_DEVICE void read_one(const unsigned char* p) {
+  PGN_DEVICE void read_one(unsigned p) {
     if constexpr (Q < C::NB)
       fy[KB][Q] = ry.template get<Q, KB>(p + kX);
     else
       fx[KB][Q - C::NB] = rx.template get<Q - C::NB, KB>(p);
   }
   template <int KB>
-  PGN_DEVICE void read(const unsigned char* p) {
+  PGN_DEVICE void read(unsigned p) {
     static_for<0, C::NA + C::NB>([&](auto q) { read_one<KB, q.value>(p); });
   }
-  // The products of half KB, NB at a time, and among them the fragments of the other half read from p (unless null) and
+  // The products of half KB, NB at a time, and among them the fragments of the other half read from p (READ) and
   // loads(u), u < kLoads: the fragments before the last group, so that they have arrived when the half ends.
-  template <int KB, bool READ, int kLoads, class L>
-  PGN_DEVICE void multiply(f32x4 (&acc)[C::NA][C::NB], const unsigned char* p, L&& loads) {
+  // ZERO: onto zeros, whatever acc holds.
+  template <int KB, bool READ, int kLoads, bool ZERO = false, class L>
+  PGN_DEVICE void multiply(f32x4 (&acc)[C::NA][C::NB], unsigned p, L&& loads) {
     constexpr int kFrags = C::NA + C::NB, kGroups = C::NA > 1 ? C::NA - 1 : 1;
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this half's fragments, read during the half before
     static_for<0, C::NA>([&](auto a) {
@@ -217,7 +221,7 @@ struct Frags {
             [&](auto q) { read_one<1 - KB, decltype(q)::value>(p); });
       }
 #pragma unroll
-      for (int b = 0; b < C::NB; ++b) acc[A][b] = pgn_mfma(fx[KB][A], fy[KB][b], acc[A][b]);
+      for (int b = 0; b < C::NB; ++b) acc[A][b] = pgn_mfma(fx[KB][A], fy[KB][b], ZERO ? zero4() : acc[A][b]);
       __builtin_amdgcn_sched_barrier(0);
     });
   }
@@ -265,16 +269,16 @@ PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_
   wait_loads<C::kLoads * (C::NS - 1)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  f.template read<0>(lds);
+  f.template read<0>(lds0);
   int buf = 0;
   for (int s = 0; s < steps; ++s) {
     const int next = buf + 1 == C::NS ? 0 : buf + 1;
-    f.template multiply<0, true, 0>(acc, lds + buf * C::kStage, [](auto) {});
+    f.template multiply<0, true, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
     aim(s + C::NS);
     wait_loads<C::kLoads * (C::NS - 2)>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    f.template multiply<1, true, C::kLoads>(acc, lds + next * C::kStage, [&](auto u) { load(u, buf); });
+    f.template multiply<1, true, C::kLoads>(acc, lds0 + next * C::kStage, [&](auto u) { load(u, buf); });
     buf = next;
   }
   // nothing in flight into the buffers, nothing being read: they may be used again
@@ -283,8 +287,18 @@ PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_
   asm volatile("" ::: "memory");
 }
 
-// The same for a run of tiles with both operands along their rows, k from 0 to d: tiles at(item) = (x0, y0) for item =
-// first, first + stride, .. below items (first < items), epilogue(acc, x0, y0, info) after each. The stages of the next
+// Workgroup `wg` runs on XCD wg % 8. An XCD takes a contiguous run of the items, its workgroups neighbours in it at any
+// time, so they share operands in its L2: the items are first, first + stride, .. below end.
+struct XcdRun {
+  int first, stride, end;
+};
+PGN_DEVICE XcdRun xcd_run(int items) {
+  const int per = (items + kXcdCount - 1) / kXcdCount, x = blockIdx.x % kXcdCount;
+  return {x * per + (int)blockIdx.x / kXcdCount, (int)gridDim.x / kXcdCount, min(items, (x + 1) * per)};
+}
+
+// The same for a run of tiles with both operands along their rows, k from 0 to d: the run's items (at least one), at(item,
+// ix, iy) giving their tiles, epilogue(acc, x0, y0, info) after each. The stages of the next
 // tile are under way while a tile's last steps and its epilogue run.
 //
 // info: kInfo bytes of data of each of the tile's Y rows (row y's at rows + y kInfo, row_count of them; the rest reads as
@@ -295,8 +309,7 @@ PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_
 // stages are read: those loads were issued before them, and memory operations are counted in order.
 template <class C, int kInfo, int kStores, class At, class Epilogue>
 PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const void* rows, int64_t row_count,
-                           int64_t first, int64_t stride, int64_t items, unsigned char* lds, At&& at,
-                           Epilogue&& epilogue) {
+                           const XcdRun& run, unsigned char* lds, At&& at, Epilogue&& epilogue) {
   static_assert(C::Y * kInfo <= C::kThreads * 16 && kInfo % 8 == 0, "one load a thread");
   const WaveIdx t = wave_idx();
   const int tid = threadIdx.x, steps = (int)((d + kGemmK - 1) / kGemmK);
@@ -307,13 +320,12 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
   F f;
   f.init(t);
   // the next stage to load: step ls of tile item `li`
-  int64_t li = first;
-  int ls = 0;
+  int li = run.first, ls = 0;
   auto aim = [&]() {
-    int64_t x0 = 0, y0 = 0;
-    if (li < items) at(li, x0, y0);
-    sx.tile(X, x0, 0), sy.tile(Y, y0, 0);
-    if (li >= items) sx.bytes = sy.bytes = 0;  // loads nothing
+    int ix = 0, iy = 0;
+    if (li < run.end) at(li, ix, iy);
+    sx.tile(X, (int64_t)ix * C::X, 0), sy.tile(Y, (int64_t)iy * C::Y, 0);
+    if (li >= run.end) sx.bytes = sy.bytes = 0;  // loads nothing
   };
   const unsigned lds0 = lds_address(lds);
   constexpr int kLx = Stager<false, C::X, C::kThreads>::kLoads;
@@ -327,77 +339,69 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
       sy.template load<u - kLx>(p + F::kX, t.w);
     if constexpr (u == C::kLoads - 1) {
       if (++ls == steps) {
-        ls = 0, li += stride;
+        ls = 0, li += run.stride;
         aim();
       }
     }
   };
   unsigned char* const info = lds + C::kLds;
-  auto load_info = [&](int64_t item, int place) {
-    int64_t x0 = 0, y0 = 0;
-    if (item < items) at(item, x0, y0);
-    const int64_t left = item < items && rows != nullptr ? min((int64_t)C::Y, row_count - y0) : 0;
+  auto load_info = [&](int item, int place) {
+    int ix = 0, iy = 0;
+    if (item < run.end) at(item, ix, iy);
+    const int64_t y0 = (int64_t)iy * C::Y;
+    const int64_t left = item < run.end && rows != nullptr ? min((int64_t)C::Y, row_count - y0) : 0;
     load_to_lds(static_cast<const char*>(rows) + (left > 0 ? y0 * kInfo : 0), (int)(left * kInfo), tid * 16,
                 lds0 + C::kLds + place * C::kThreads * 16 + t.w * 1024);
   };
   aim();
-  load_info(first, 0);
+  load_info(run.first, 0);
   for (int s = 0; s < C::NS; ++s) static_for<0, C::kLoads>([&](auto u) { load(u, s); });
   wait_loads<C::kLoads * (C::NS - 1)>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   int buf = 0, place = 0;
-  for (int64_t item = first; item < items; item += stride) {
-    int64_t x0, y0;
-    at(item, x0, y0);
+  for (int item = run.first; item < run.end; item += run.stride) {
+    int ix, iy;
+    at(item, ix, iy);
     f32x4 acc[C::NA][C::NB];
     zero_acc<C>(acc);
+    // The first half of step s. Stage s + 1 has arrived at its end, and every wave's reads of stage s are done. The stages
+    // that were issued before the last epilogue's stores need not wait for those.
     auto half = [&](int s) {
-      f.template multiply<0, true, 0>(acc, lds + buf * C::kStage, [](auto) {});
-      if (s == 0 && item == first)
+      f.template multiply<0, true, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
+      if (steps < C::NS)  // the row data of this tile may be among the last loads
         wait_loads<0>();
-      else if (s == 0)
-        wait_loads<kStores>();
+      else if (s < C::NS - 1 && item != run.first)
+        wait_loads<C::kLoads * (C::NS - 2) + kStores>();
       else
         wait_loads<C::kLoads * (C::NS - 2)>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (s == 0) load_info(item + stride, place ^ 1);
+      if (s == 0) load_info(item + run.stride, place ^ 1);
     };
-    f.template read<0>(lds + buf * C::kStage);
-    for (int s = 0; s + 1 < steps; ++s) {
+    f.template read<0>(lds0 + buf * C::kStage);
+    // (the last step reads the next tile's first fragments for nothing: held over the epilogue they would cost it the
+    // registers, and a copy of the step without the reads costs more of them)
+    for (int s = 0; s < steps; ++s) {
       half(s);
       const int next = buf + 1 == C::NS ? 0 : buf + 1;
-      f.template multiply<1, true, C::kLoads>(acc, lds + next * C::kStage, [&](auto u) { load(u, buf); });
+      f.template multiply<1, true, C::kLoads>(acc, lds0 + next * C::kStage, [&](auto u) { load(u, buf); });
       buf = next;
     }
-    // the next tile's first fragments are read after the epilogue, which needs their registers
-    half(steps - 1);
-    f.template multiply<1, false, C::kLoads>(acc, nullptr, [&](auto u) { load(u, buf); });
-    buf = buf + 1 == C::NS ? 0 : buf + 1;
-    epilogue(acc, x0, y0, info + place * C::kThreads * 16);
+    epilogue(acc, (int64_t)ix * C::X, (int64_t)iy * C::Y, info + place * C::kThreads * 16);
     place ^= 1;
   }
   wait_loads<0>();
 }
 
 // Tile `item` of a grid of tx x ty tiles (x tiles, y tiles), so ordered that consecutive items share operands: bands of
-// eight y tiles, within a band y fastest.
-PGN_DEVICE void band_tile(int64_t item, int64_t tx, int64_t ty, int64_t& ix, int64_t& iy) {
-  constexpr int64_t kBand = 8;
-  const int64_t band = item / (tx * kBand), y0 = band * kBand, h = min(kBand, ty - y0), in = item - band * tx * kBand;
-  ix = in / h;
-  iy = y0 + in - ix * h;
-}
-
-// Workgroup `wg` runs on XCD wg % 8. An XCD takes a contiguous run of the items, its workgroups neighbours in it at any
-// time, so they share operands in its L2: the items are first, first + stride, .. below end.
-struct XcdRun {
-  int64_t first, stride, end;
-};
-PGN_DEVICE XcdRun xcd_run(int64_t items) {
-  const int64_t per = (items + kXcdCount - 1) / kXcdCount, x = blockIdx.x % kXcdCount;
-  return {x * per + blockIdx.x / kXcdCount, gridDim.x / kXcdCount, min(items, (x + 1) * per)};
+// eight y tiles, within a band y fastest. In 32 bits and scalar registers (a division runs in the vector unit).
+PGN_DEVICE void band_tile(int item, int tx, int ty, int& ix, int& iy) {
+  constexpr unsigned kBand = 8;
+  const unsigned band = (unsigned)item / (tx * kBand), y0 = band * kBand, h = min(kBand, ty - y0);
+  const unsigned in = item - band * tx * kBand, x = in / h;
+  ix = __builtin_amdgcn_readfirstlane(x);
+  iy = __builtin_amdgcn_readfirstlane(y0 + in - x * h);
 }
 
 // Workgroups for `items` items with one each, or at most `most`, a whole number an XCD.

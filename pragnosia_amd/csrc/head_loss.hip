@@ -180,20 +180,17 @@ template <class C, int NEXP>
 __global__ __launch_bounds__(C::kThreads) void head_logits(Operand h, Operand W, const int64_t* __restrict__ y,
                                                            float scale0, float scale1, FwdOut out, int64_t d) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t tx = (W.rows + C::X - 1) / C::X, ty = (h.rows + C::Y - 1) / C::Y, n = h.rows;
+  const int64_t n = h.rows;
+  const int tx = (int)((W.rows + C::X - 1) / C::X), ty = (int)((n + C::Y - 1) / C::Y);
   const XcdRun run = xcd_run(tx * ty);
   if (run.first >= run.end) return;
-  const WaveIdx t = wave_idx();
-  const int wx = t.w % C::WX, wy = t.w / C::WX;
   constexpr int kWords = 16 * C::NA;
   const float c0 = scale0 * kLog2e, c1 = scale1 * kLog2e;
   gemm_tiles<C, 8, 0>(
-      W, h, d, y, n, run.first, run.stride, run.end, smem,
-      [&](int64_t item, int64_t& x0, int64_t& y0) {
-        band_tile(item, tx, ty, x0, y0);
-        x0 *= C::X, y0 *= C::Y;
-      },
+      W, h, d, y, n, run, smem, [&](int item, int& ix, int& iy) { band_tile(item, tx, ty, ix, iy); },
       [&](f32x4(&acc)[C::NA][C::NB], int64_t x0, int64_t y0, const unsigned char* info) {
+        const WaveIdx t = wave_idx_opaque();  // (its addresses are made here, not held in registers over the steps)
+        const int wx = t.w % C::WX, wy = t.w / C::WX;
         const int64_t v0 = x0 + kWords * wx;
         if (v0 + kWords > W.rows) {
 #pragma unroll
@@ -351,20 +348,17 @@ __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W
                                                             float scale0, float scale1, __bf16* __restrict__ dl,
                                                             int64_t ld, int64_t v_begin, int64_t n_pad, int64_t d) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t tx = ld / C::X, ty = n_pad / C::Y, words = min(ld, W.rows - v_begin);
+  const int64_t words = min(ld, W.rows - v_begin);
+  const int tx = (int)(ld / C::X), ty = (int)(n_pad / C::Y);
   const XcdRun run = xcd_run(tx * ty);
   if (run.first >= run.end) return;
-  const WaveIdx t = wave_idx();
-  const int wx = t.w % C::WX, wy = t.w / C::WX;
   const float e0 = scale0 * kLog2e, e1 = scale1 * kLog2e;
   const Operand Wp{W.p + v_begin * W.ld, W.ld, words};
   gemm_tiles<C, sizeof(RowInfo), C::NB * C::NA / 2>(
-      Wp, h, d, rows, h.rows, run.first, run.stride, run.end, smem,
-      [&](int64_t item, int64_t& x0, int64_t& y0) {
-        band_tile(item, tx, ty, x0, y0);
-        x0 *= C::X, y0 *= C::Y;
-      },
+      Wp, h, d, rows, h.rows, run, smem, [&](int item, int& ix, int& iy) { band_tile(item, tx, ty, ix, iy); },
       [&](f32x4(&acc)[C::NA][C::NB], int64_t x0, int64_t y0, const unsigned char* info) {
+        const WaveIdx t = wave_idx_opaque();
+        const int wx = t.w % C::WX, wy = t.w / C::WX;
         const int64_t c0 = x0 + 16 * C::NA * wx;
         const bool partial = c0 + 16 * C::NA > words;
 #pragma unroll
@@ -542,7 +536,9 @@ int launch_grads(const GradArgs& ga, hipStream_t st) {
 
 bool head_shape_ok(int64_t n, int64_t V, int64_t d, int64_t K) {
   return n > 0 && n <= (int64_t)1 << 24 && V > 0 && V <= (int64_t)1 << 24 && d > 0 && d % 8 == 0 && d <= 65536 &&
-         K >= 0 && K <= 65536 && n * K < (int64_t)1 << 31;  // launches of fewer than 2^32 threads
+         K >= 0 && K <= 65536 &&
+         // launches of fewer than 2^32 threads; tiles counted in 32 bits
+         n * K < (int64_t)1 << 31 && tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31;
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p % 16) == 0; }
