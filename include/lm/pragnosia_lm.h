@@ -28,9 +28,11 @@ int pragnosia_lm_abi_version(void);
  *                                     entry is left
  *
  * h (n, d) and W (V, d) bf16, d a multiple of 8; y (n) int64 or NULL (no ce); ids (n, K) int64 and z (n, K) fp32, or
- * both NULL with K = 0 (no kd); at least one of y and ids; tau > 0. Outputs, all fp32 but `entry`: ce and lse (n) with
+ * both NULL with K = 0 (no kd), K at most 1024; at least one of y and ids; tau > 0. Outputs, all fp32 but `entry`: ce and lse (n) with
  * y; kd, lse_t and psum (n), entry (n, K) int32, p and zl (n, K) with ids -- lse, lse_t, psum (1, or 0 where no entry is
- * left), entry (the id, or -1), p and zl (the student's logit of the entry) are what the backward takes. */
+ * left), entry (the
+ * id at its first place in the list, or -1), p (an id's whole probability there, or 0) and zl (the student's logit of the
+ * entry) are what the backward takes. */
 int64_t pragnosia_head_fwd_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t K);
 int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y, const int64_t* ids, const float* z, float tau,
                        float* ce, float* lse, float* kd, float* lse_t, float* psum, int32_t* entry, float* p, float* zl,
@@ -51,16 +53,16 @@ int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd,
 
 /* ---------------------------------------------------------------------------------------------------------
  * Rows of a token table: y_i = scale W[ids_i], n rows; an id outside [0, V) gives a zero row. W (V, d) and y (n, d) fp32
- * or bf16 (w_bf16, y_bf16), d a multiple of 8; ids (n) int64. n = 0 does nothing. Replaces nn.Embedding of
- * src/model.py:822-826 (scale 1). */
-int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16, int64_t n,
-                        int64_t V, int64_t d, void* stream);
+ * or bf16 (w_bf16, y_bf16), d a multiple of 8; ids (n) int64. kept (n) int32 or NULL: the ids as the backward takes them
+ * (-1 outside the table). n = 0 does nothing. Replaces nn.Embedding of src/model.py:822-826 (scale 1). */
+int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16, int32_t* kept,
+                        int64_t n, int64_t V, int64_t d, void* stream);
 
-/* Its gradient: dW[v] = scale sum of g_i over the tokens with ids_i = v, in fp32 in the order of their positions (blocks
- * of 32 where there are more), zero where there is none; g (n, d) and dW (V, d) fp32 or bf16. No atomics on values, no
- * memset: the same bits each time, also in a captured step. */
+/* Its gradient: dW[v] = scale sum of g_i over the tokens with kept_i = v, in fp32 in a fixed order, zero where there is
+ * none; g (n, d) and dW (V, d) fp32 or bf16; kept's ids below V. No atomics on values, no memset: the same bits each
+ * time, also in a captured step. */
 int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d);
-int pragnosia_embed_bwd(const void* g, int g_bf16, const int64_t* ids, float scale, void* dW, int w_bf16,
+int pragnosia_embed_bwd(const void* g, int g_bf16, const int32_t* kept, float scale, void* dW, int w_bf16,
                         void* workspace, int64_t workspace_bytes, int64_t n, int64_t V, int64_t d, void* stream);
 
 #ifdef __cplusplus

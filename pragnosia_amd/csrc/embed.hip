@@ -1,16 +1,17 @@
 // The token table's two directions: y_i = scale W[id_i], and dW[v] = scale sum over the tokens i with id_i = v of g_i.
 //
 // Both are bound by memory: the lookup moves n rows in and out, the gradient reads n rows and writes V. The gradient
-// sorts the tokens by id (a stable counting sort: a row's terms are added in the order of their positions, so the sum
-// has one order and no atomics) in one launch, sums in a second and joins long runs in a third:
+// sorts the tokens by id (a stable counting sort: a row's terms are added in one order, with no atomics on values) in one
+// launch, sums in a second and joins long runs in a third:
 //
 //   sort  Every workgroup owns a range of ids. It reads all n ids (they stay in the L2), counts those below its range
-//         -- where its tokens start in the order -- and lists its own tokens' positions in order of position; then
-//         places them by id. No workgroup waits for another.
-//   sum   Ids with at most kRun tokens are summed whole, one workgroup a few ids, zeros where there is no token. A longer
-//         run (a frequent word) is summed in blocks of kRun places of the order by other workgroups, each into a partial
-//         row of its own.
-//   join  A long run's partial rows are added in order.
+//         -- where its tokens start in the order -- and lists its own tokens in order of position; then places them by
+//         id. No workgroup waits for another.
+//   sum   An id with at most kShort tokens (most of a vocabulary, zeros where there is none) is summed by one thread a
+//         column vector, all its rows loaded at once. A longer run is summed in blocks of kBlock places of the order,
+//         four waves a block, its rows shared among them; what is left of a run that goes on in another block is a
+//         partial row.
+//   join  A run's partial rows are added in order.
 #include <algorithm>
 
 #include "../../include/lm/pragnosia_lm.h"
@@ -19,7 +20,9 @@
 namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kRun = 32;  // tokens summed by one workgroup
+constexpr int kList = 8192;  // tokens of a sorting workgroup's range that fit its LDS
+constexpr int kShort = 8;    // tokens of an id summed by one thread
+constexpr int kBlock = 64;   // places of the order summed by one workgroup: a lane each
 
 template <class T>
 struct Vec {};
@@ -34,10 +37,11 @@ struct Vec<__bf16> {
   typedef bf16x8 raw;
 };
 
-// y = scale W[id], one vector of 16 bytes of W a thread.
+// y = scale W[id], one vector of 16 bytes of W a thread. kept: the ids in 32 bits, -1 outside the table, or null.
 template <class T, class O>
 __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ ids, const T* __restrict__ W, float scale,
-                                                  O* __restrict__ y, int64_t n, int64_t V, int d) {
+                                                  O* __restrict__ y, int32_t* __restrict__ kept, int64_t n, int64_t V,
+                                                  int d) {
   constexpr int N = Vec<T>::N;
   const int per = d / N;
   const int64_t total = n * per;
@@ -47,6 +51,7 @@ __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ id
     const int64_t id = ids[i];
     typename Vec<T>::raw w{};
     const bool in = id >= 0 && id < V;
+    if (kept != nullptr && c == 0) kept[i] = in ? (int32_t)id : -1;
     if (in) w = *reinterpret_cast<const typename Vec<T>::raw*>(W + id * d + c);
     typedef O out_t __attribute__((__vector_size__(N * sizeof(O))));
     out_t o;
@@ -56,45 +61,93 @@ __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ id
   }
 }
 
-// Ids [blockIdx.x * range, ..): start[v] = the place of id v's first token in the order (start[V] the number of tokens
-// with an id in the table), order[place] = position. list: n entries, the unplaced positions and their ids.
-__global__ __launch_bounds__(kSortThreads) void embed_sort(const int64_t* __restrict__ ids, int32_t* __restrict__ order,
-                                                           int32_t* __restrict__ start, int32_t* __restrict__ list,
-                                                           int n, int64_t V, int range) {
-  extern __shared__ int32_t count_lds[];  // range: an id's tokens, then its next place
-  volatile int32_t* count = count_lds;    // (read and written by different lanes of a wave)
+// Ids [blockIdx.x * range, ..): start[v] = the place of id v's first token in the order (start[V]: the number of tokens
+// with an id), order[place] = position, sorted[place] = id. list: n entries of scratch, for ranges past kList.
+// HELD: n <= 4 * 4 * kSortThreads, the ids stay in registers between the passes over them.
+template <bool HELD>
+__global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __restrict__ ids, int32_t* __restrict__ order,
+                                                           int32_t* __restrict__ sorted, int32_t* __restrict__ start,
+                                                           int2* __restrict__ list, int n, int V, int range) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  int2* const near = reinterpret_cast<int2*>(smem);                            // (id - v0, position) of up to kList tokens
+  volatile int32_t* count = reinterpret_cast<int32_t*>(smem + 8 * kList);      // range: an id's tokens, then its next place
   __shared__ int32_t waves[2][kSortWaves];
+  constexpr int kHeld = 4;
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  const int64_t v0 = (int64_t)blockIdx.x * range, v1 = min(V, v0 + range);
-  // a wave reads a contiguous share of the ids, in order
-  const int share = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64, a = min(n, w * share), b = min(n, a + share);
+  const int v0 = blockIdx.x * range, v1 = min(V, v0 + range);
+  // a wave reads a contiguous share of the ids, in order, four a lane
+  const int share = ((n + kSortWaves - 1) / kSortWaves + 255) / 256 * 256, a = min(n, w * share), b = min(n, a + share);
+  auto load = [&](int i0) {
+    const int i = i0 + 4 * l;
+    i32x4 x = {-1, -1, -1, -1};
+    if (i + 4 <= b) {
+      x = *reinterpret_cast<const i32x4*>(ids + i);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u < b) x[u] = ids[i + u];
+    }
+    return x;
+  };
+  i32x4 held[kHeld];
   int below = 0, mine = 0;
-  for (int i = a + l; i < b; i += 64) {
-    const int64_t id = ids[i];
-    below += id >= 0 && id < v0;
-    mine += id >= v0 && id < v1;
+  auto tally = [&](i32x4 x) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      below += x[u] >= 0 && x[u] < v0;
+      mine += x[u] >= v0 && x[u] < v1;
+    }
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q) held[q] = load(a + 256 * q);
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q) tally(held[q]);
+  } else {
+#pragma unroll 4
+    for (int i0 = a; i0 < b; i0 += 256) tally(load(i0));
   }
   for (int o = 1; o < 64; o *= 2) below += __shfl_xor(below, o), mine += __shfl_xor(mine, o);
   if (l == 0) waves[0][w] = below, waves[1][w] = mine;
   for (int r = tid; r < range; r += kSortThreads) count[r] = 0;
   __syncthreads();
-  int base = 0, before = 0, all = 0;
+  int base = 0, at = 0, all = 0;
   for (int q = 0; q < kSortWaves; ++q) {
     base += waves[0][q];
-    if (q < w) before += waves[1][q];
+    if (q < w) at += waves[1][q];
     all += waves[1][q];
   }
-  // the range's tokens in order of position: list[base ..), counted by id
-  int at = base + before;
-  for (int i0 = a; i0 < b; i0 += 64) {
-    const int64_t id = i0 + l < b ? ids[i0 + l] : -1;
-    const bool in = id >= v0 && id < v1;
-    const unsigned long long m = __ballot(in);
-    if (in) {
-      list[at + __popcll(m & ((1ull << l) - 1))] = i0 + l;
-      atomicAdd(&count_lds[(int)(id - v0)], 1);
-    }
-    at += __popcll(m);
+  const bool fits = all <= kList;
+  int2* const far = list + base;
+  // the range's tokens in order of position, counted by id
+  auto append = [&](int i0, i32x4 x) {
+    bool in[4];
+    unsigned long long m[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) in[u] = x[u] >= v0 && x[u] < v1, m[u] = __ballot(in[u]);
+    if (!(m[0] | m[1] | m[2] | m[3])) return;
+    const unsigned long long lower = (1ull << l) - 1;
+    int to = at + __popcll(m[0] & lower) + __popcll(m[1] & lower) + __popcll(m[2] & lower) + __popcll(m[3] & lower);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (in[u]) {
+        const int2 e = {x[u] - v0, i0 + 4 * l + u};
+        if (fits)
+          near[to] = e;
+        else
+          far[to] = e;
+        ++to;
+        atomicAdd(const_cast<int32_t*>(&count[e.x]), 1);
+      }
+    at += __popcll(m[0]) + __popcll(m[1]) + __popcll(m[2]) + __popcll(m[3]);
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q)
+      if (a + 256 * q < b) append(a + 256 * q, held[q]);
+  } else {
+#pragma unroll 2
+    for (int i0 = a; i0 < b; i0 += 256) append(i0, load(i0));
   }
   __syncthreads();
   // places: an exclusive sum over the range's counts, by the first wave
@@ -115,36 +168,47 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int64_t* __rest
   }
   __syncthreads();
   // each id's tokens placed in order: a wave takes the ids of its residue
+  auto entry = [&](int i) { return i < all ? (fits ? near[i] : far[i]) : int2{-1, 0}; };
+  int2 next = entry(l);
   for (int i0 = 0; i0 < all; i0 += 64) {
-    const int i = i0 + l < all ? list[base + i0 + l] : -1;
-    const int r = i >= 0 ? (int)(ids[i] - v0) : -1;
-    bool todo = r >= 0 && r % kSortWaves == w;
+    const int2 e = next;
+    next = entry(i0 + 64 + l);
+    bool todo = e.x >= 0 && e.x % kSortWaves == w;
     unsigned long long left = __ballot(todo);
     while (left) {
-      const int lead = __ffsll((unsigned long long)left) - 1, rl = __shfl(r, lead);
-      const unsigned long long same = __ballot(todo && r == rl);
-      const int place = count[rl];
-      if (todo && r == rl) {
-        order[place + __popcll(same & ((1ull << l) - 1))] = i;
+      const int lead = __ffsll((long long)left) - 1, r = __shfl(e.x, lead);
+      const unsigned long long same = __ballot(todo && e.x == r);
+      const int place = count[r];
+      if (todo && e.x == r) {
+        const int to = place + __popcll(same & ((1ull << l) - 1));
+        order[to] = e.y;
+        sorted[to] = v0 + r;
         todo = false;
       }
-      if (l == lead) count[rl] = place + __popcll(same);
+      if (l == lead) count[r] = place + __popcll(same);
       left &= ~same;
     }
   }
 }
 
-// Sum of the gradient rows of places [a, b), columns c ..
-template <class G>
+// s += the gradient rows of places [a, b), columns c .., U loaded at a time.
+template <int U, class G>
 PGN_DEVICE void sum_rows(const G* __restrict__ g, const int32_t* __restrict__ order, int a, int b, int64_t d, int c,
                          float (&s)[Vec<G>::N]) {
   constexpr int N = Vec<G>::N;
+  for (int k = a; k < b; k += U) {
+    typename Vec<G>::raw x[U];
+    int at[U];
 #pragma unroll
-  for (int u = 0; u < N; ++u) s[u] = 0.f;
-  for (int k = a; k < b; ++k) {
-    const typename Vec<G>::raw x = *reinterpret_cast<const typename Vec<G>::raw*>(g + (int64_t)order[k] * d + c);
+    for (int u = 0; u < U; ++u) at[u] = order[min(k + u, b - 1)];
 #pragma unroll
-    for (int u = 0; u < N; ++u) s[u] += (float)x[u];
+    for (int u = 0; u < U; ++u)
+      if (k + u < b) x[u] = *reinterpret_cast<const typename Vec<G>::raw*>(g + (int64_t)at[u] * d + c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u < b)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += (float)x[u][i];
   }
 }
 
@@ -158,135 +222,184 @@ PGN_DEVICE void put_row(T* p, const float (&s)[Vec<G>::N], float scale) {
   *reinterpret_cast<out_t*>(p) = o;
 }
 
-// Workgroups [0, blocks): the places [kRun q, kRun q + kRun) of long runs, each into a partial row (the run that began
-// earlier: row 2 q; the one that begins here: 2 q + 1). The others: whole ids, `per` threads' columns of one id each.
-template <class G, class T>
-__global__ __launch_bounds__(256) void embed_sum(const G* __restrict__ g, const int64_t* __restrict__ ids,
-                                                 const int32_t* __restrict__ order, const int32_t* __restrict__ start,
-                                                 float scale, T* __restrict__ dW, float* __restrict__ part, int64_t V,
-                                                 int d, int blocks) {
-  constexpr int N = Vec<G>::N;
-  const int per = d / N;
-  float s[N];
-  if ((int)blockIdx.x < blocks) {
-    const int q = blockIdx.x, lo = q * kRun, hi = min(lo + kRun, start[V]);
-    if (lo >= hi) return;
-    for (int side = 0; side < 2; ++side) {
-      const int64_t v = ids[order[side ? hi - 1 : lo]];
-      const int a = start[v], b = start[v + 1];
-      if (b - a <= kRun) continue;
-      if ((a < lo) != (side == 0)) continue;  // side 0: the run that began before this block; 1: the one that begins here
-      for (int c = threadIdx.x * N; c < d; c += 256 * N) {
-        sum_rows<G>(g, order, max(a, lo), min(b, hi), d, c, s);
+// The sums of four waves in order, in the first one's s. lds: 4 x 64 x N.
+template <int N>
+PGN_DEVICE void add_waves(float* lds, float (&s)[N], int w, int l) {
+  __syncthreads();
 #pragma unroll
-        for (int u = 0; u < N; ++u) part[(int64_t)(2 * q + side) * d + c + u] = s[u];
+  for (int u = 0; u < N; ++u) lds[(w * N + u) * 64 + l] = s[u];
+  __syncthreads();
+  if (w == 0)
+    for (int q = 1; q < 4; ++q)
+#pragma unroll
+      for (int u = 0; u < N; ++u) s[u] += lds[(q * N + u) * 64 + l];
+}
+
+// Workgroups [0, blocks * chunks): places [kBlock q, kBlock q + kBlock) and a chunk of 64 column vectors, runs of more
+// than kShort; a run that began in an earlier block leaves its partial row at 2 q, one that goes on in the next at
+// 2 q + 1. The others: short runs, a thread an id and column vector.
+template <class G, class T>
+__global__ __launch_bounds__(256) void embed_sum(const G* __restrict__ g, const int32_t* __restrict__ order,
+                                                 const int32_t* __restrict__ sorted, const int32_t* __restrict__ start,
+                                                 float scale, T* __restrict__ dW, float* __restrict__ part, int V, int d,
+                                                 int blocks, int chunks) {
+  constexpr int N = Vec<G>::N;
+  __shared__ float lds[4 * 64 * N];
+  const int per = d / N;
+  if ((int)blockIdx.x < blocks * chunks) {
+    const int q = blockIdx.x / chunks, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int col = (blockIdx.x - q * chunks) * 64 + l, c = min(col, per - 1) * N;
+    const int lo = q * kBlock, hi = min(lo + kBlock, start[V]);
+    // lane l: place lo + l, and its run
+    const int v = lo + l < hi ? sorted[lo + l] : -1;
+    const int from = v >= 0 ? start[v] : 0, to = v >= 0 ? start[v + 1] : 0;
+    unsigned long long runs = __ballot(to - from > kShort && max(from, lo) == lo + l);
+    while (runs) {
+      const int lead = __ffsll((long long)runs) - 1;
+      runs &= runs - 1;
+      const int id = __shfl(v, lead), ra = __shfl(from, lead), rb = __shfl(to, lead), a = max(ra, lo), b = min(rb, hi);
+      // a wave's share of the rows
+      const int each = (b - a + 3) / 4, wa = min(b, a + w * each), wb = min(b, wa + each);
+      float s[N] = {};
+      sum_rows<8, G>(g, order, wa, wb, d, c, s);
+      add_waves<N>(lds, s, w, l);
+      if (w == 0 && col < per) {
+        if (ra >= lo && rb <= hi) {
+          put_row<G>(dW + (int64_t)id * d + c, s, scale);
+        } else {
+          float* p = part + (int64_t)(2 * q + (ra >= lo)) * d + c;
+#pragma unroll
+          for (int u = 0; u < N; ++u) p[u] = s[u];
+        }
       }
     }
     return;
   }
-  const int64_t total = V * per;
-  for (int64_t e = (int64_t)(blockIdx.x - blocks) * 256 + threadIdx.x; e < total;
-       e += (int64_t)(gridDim.x - blocks) * 256) {
+  const int64_t total = (int64_t)V * per, stride = (int64_t)(gridDim.x - blocks * chunks) * 256;
+  for (int64_t e = (int64_t)(blockIdx.x - blocks * chunks) * 256 + threadIdx.x; e < total; e += stride) {
     const int64_t v = e / per;
     const int c = (int)(e - v * per) * N, a = start[v], b = start[v + 1];
-    if (b - a > kRun) continue;
-    sum_rows<G>(g, order, a, b, d, c, s);
+    if (b - a > kShort) continue;
+    float s[N] = {};
+    if (b - a <= 2)
+      sum_rows<2, G>(g, order, a, b, d, c, s);
+    else
+      sum_rows<kShort, G>(g, order, a, b, d, c, s);
     put_row<G>(dW + v * d + c, s, scale);
   }
 }
 
-// The long run that begins in block q: its partial rows in order.
+// The run that begins in block q and goes on past it: its partial rows in order, four waves a chunk of columns.
 template <class G, class T>
-__global__ __launch_bounds__(256) void embed_join(const int64_t* __restrict__ ids, const int32_t* __restrict__ order,
-                                                  const int32_t* __restrict__ start, float scale, T* __restrict__ dW,
-                                                  const float* __restrict__ part, int64_t V, int d) {
+__global__ __launch_bounds__(256) void embed_join(const int32_t* __restrict__ sorted, const int32_t* __restrict__ start,
+                                                  float scale, T* __restrict__ dW, const float* __restrict__ part, int V,
+                                                  int d, int chunks) {
   constexpr int N = Vec<G>::N;
-  const int q = blockIdx.x, lo = q * kRun, hi = min(lo + kRun, start[V]);
-  if (lo >= hi) return;
-  const int64_t v = ids[order[hi - 1]];
-  const int a = start[v], b = start[v + 1];
-  if (b - a <= kRun || a < lo) return;
-  const int last = (b - 1) / kRun;
-  for (int c = threadIdx.x * N; c < d; c += 256 * N) {
-    float s[N];
+  __shared__ float lds[4 * 64 * N];
+  const int q = blockIdx.x / chunks, l = threadIdx.x & 63, w = threadIdx.x >> 6, per = d / N;
+  const int lo = q * kBlock, hi = lo + kBlock;
+  if (hi >= start[V]) return;
+  const int v = sorted[hi - 1], from = start[v], to = start[v + 1];
+  if (to - from <= kShort || from < lo || to <= hi) return;
+  const int col = (blockIdx.x - q * chunks) * 64 + l, c = min(col, per - 1) * N;
+  // block q's row at 2 q + 1, those of the blocks after it at 2 k
+  const int rows = (to - 1) / kBlock - q + 1, each = (rows + 3) / 4, a = min(rows, w * each), b = min(rows, a + each);
+  float s[N] = {};
+  for (int k = a; k < b; k += 4) {
+    f32x4 x[4][N / 4];
 #pragma unroll
-    for (int u = 0; u < N; ++u) s[u] = part[(int64_t)(2 * q + 1) * d + c + u];
-    for (int k = q + 1; k <= last; ++k)
+    for (int u = 0; u < 4; ++u) {
+      const int at = min(k + u, b - 1);
+      const float* p = part + (int64_t)(2 * (q + at) + (at == 0)) * d + c;
 #pragma unroll
-      for (int u = 0; u < N; ++u) s[u] += part[(int64_t)(2 * k) * d + c + u];
-    put_row<G>(dW + v * d + c, s, scale);
+      for (int i = 0; i < N / 4; ++i) x[u][i] = *reinterpret_cast<const f32x4*>(p + 4 * i);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (k + u < b)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += x[u][i / 4][i % 4];
   }
+  add_waves<N>(lds, s, w, l);
+  if (w == 0 && col < per) put_row<G>(dW + (int64_t)v * d + c, s, scale);
 }
 
-constexpr int64_t kMaxTokens = (int64_t)1 << 28;  // launches of fewer than 2^32 threads
+constexpr int64_t kMaxTokens = (int64_t)1 << 28;
 
-// Ids a sorting workgroup owns: about 512 workgroups, their counters at most 16 KB.
-int64_t sort_range(int64_t V) { return std::min<int64_t>(std::max<int64_t>((V + 511) / 512, 32), 4096); }
+// Ids a sorting workgroup owns: about 256 workgroups (each reads all ids), their counters at most 16 KB.
+int64_t sort_range(int64_t V) { return std::min<int64_t>(std::max<int64_t>((V + 255) / 256, 32), 4096); }
 
 bool embed_shape_ok(int64_t n, int64_t V, int64_t d) {
-  return n >= 0 && n <= kMaxTokens && V > 0 && V <= kMaxTokens && d > 0 && d % 8 == 0 && d <= 65536;
+  return n >= 0 && n <= kMaxTokens && V > 0 && V <= kMaxTokens && d > 0 && d % 8 == 0 && d <= 65536 &&
+         (n / kBlock + 1) * (d / 256 + 1) < (int64_t)1 << 22;  // launches of fewer than 2^32 threads
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
-int64_t runs(int64_t n) { return (n + kRun - 1) / kRun; }
+int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
 int64_t up4(int64_t x) { return (x + 3) / 4 * 4; }
 
 template <class T, class O>
-int launch_rows(const int64_t* ids, const void* W, float scale, void* y, int64_t n, int64_t V, int64_t d,
+int launch_rows(const int64_t* ids, const void* W, float scale, void* y, int32_t* kept, int64_t n, int64_t V, int64_t d,
                 hipStream_t st) {
   const int64_t blocks = (n * (d / Vec<T>::N) + 255) / 256;
   hipLaunchKernelGGL((embed_rows<T, O>), dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, st, ids,
-                     (const T*)W, scale, (O*)y, n, V, (int)d);
+                     (const T*)W, scale, (O*)y, kept, n, V, (int)d);
   PGN_RETURN_LAUNCH();
 }
 
 template <class G, class T>
-int launch_grad(const void* g, const int64_t* ids, float scale, void* dW, int32_t* ws, int64_t n, int64_t V, int64_t d,
+int launch_grad(const void* g, const int32_t* ids, float scale, void* dW, int32_t* ws, int64_t n, int64_t V, int64_t d,
                 hipStream_t st) {
-  int32_t *order = ws, *list = ws + up4(n), *start = ws + 2 * up4(n);
+  int2* list = (int2*)ws;
+  int32_t *order = ws + 2 * up4(n), *sorted = order + up4(n), *start = sorted + up4(n);
   float* part = (float*)(start + up4(V + 1));
   const int range = (int)sort_range(V);
-  hipLaunchKernelGGL(embed_sort, dim3((unsigned)((V + range - 1) / range)), dim3(kSortThreads), range * 4, st, ids,
-                     order, start, list, (int)n, V, range);
-  const int64_t blocks = runs(n), whole = std::min<int64_t>((V * (d / Vec<G>::N) + 255) / 256, 1 << 20);
-  hipLaunchKernelGGL((embed_sum<G, T>), dim3((unsigned)(blocks + whole)), dim3(256), 0, st, (const G*)g, ids, order,
-                     start, scale, (T*)dW, part, V, (int)d, (int)blocks);
-  if (n > kRun)
-    hipLaunchKernelGGL((embed_join<G, T>), dim3((unsigned)blocks), dim3(256), 0, st, ids, order, start, scale, (T*)dW,
-                       part, V, (int)d);
+  const auto sort = n <= 16 * kSortThreads ? embed_sort<true> : embed_sort<false>;
+  const int lds = 8 * kList + 4 * range;
+  const hipError_t e = pgn_lds_limit((const void*)sort, 8 * kList + 4 * 4096);
+  if (e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL(sort, dim3((unsigned)((V + range - 1) / range)), dim3(kSortThreads), lds, st, ids, order, sorted,
+                     start, list, (int)n, (int)V, range);
+  const int64_t per = d / Vec<G>::N, chunks = (per + 63) / 64, blocks = blocks_of(n);
+  const int64_t whole = std::min<int64_t>((V * per + 255) / 256, 1 << 20);
+  hipLaunchKernelGGL((embed_sum<G, T>), dim3((unsigned)(blocks * chunks + whole)), dim3(256), 0, st, (const G*)g, order,
+                     sorted, start, scale, (T*)dW, part, (int)V, (int)d, (int)blocks, (int)chunks);
+  if (blocks > 1)
+    hipLaunchKernelGGL((embed_join<G, T>), dim3((unsigned)((blocks - 1) * chunks)), dim3(256), 0, st, sorted, start,
+                       scale, (T*)dW, part, (int)V, (int)d, (int)chunks);
   PGN_RETURN_LAUNCH();
 }
 
 }  // namespace
 
 extern "C" int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16,
-                                   int64_t n, int64_t V, int64_t d, void* stream) {
+                                   int32_t* kept, int64_t n, int64_t V, int64_t d, void* stream) {
   PGN_CHECK_ARG(embed_shape_ok(n, V, d) && W && aligned(W));
   if (n == 0) return PRAGNOSIA_OK;
   PGN_CHECK_ARG(ids && y && aligned(y));
   hipStream_t st = (hipStream_t)stream;
-  if (w_bf16) return y_bf16 ? launch_rows<__bf16, __bf16>(ids, W, scale, y, n, V, d, st)
-                            : launch_rows<__bf16, float>(ids, W, scale, y, n, V, d, st);
-  return y_bf16 ? launch_rows<float, __bf16>(ids, W, scale, y, n, V, d, st)
-                : launch_rows<float, float>(ids, W, scale, y, n, V, d, st);
+  if (w_bf16) return y_bf16 ? launch_rows<__bf16, __bf16>(ids, W, scale, y, kept, n, V, d, st)
+                            : launch_rows<__bf16, float>(ids, W, scale, y, kept, n, V, d, st);
+  return y_bf16 ? launch_rows<float, __bf16>(ids, W, scale, y, kept, n, V, d, st)
+                : launch_rows<float, float>(ids, W, scale, y, kept, n, V, d, st);
 }
 
 extern "C" int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!embed_shape_ok(n, V, d)) return -1;
-  return (2 * up4(n) + up4(V + 1) + (n > kRun ? 2 * runs(n) * d : 0)) * 4;
+  return (4 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
 }
 
-extern "C" int pragnosia_embed_bwd(const void* g, int g_bf16, const int64_t* ids, float scale, void* dW, int w_bf16,
+extern "C" int pragnosia_embed_bwd(const void* g, int g_bf16, const int32_t* kept, float scale, void* dW, int w_bf16,
                                    void* workspace, int64_t workspace_bytes, int64_t n, int64_t V, int64_t d,
                                    void* stream) {
-  PGN_CHECK_ARG(embed_shape_ok(n, V, d) && dW && aligned(dW) && (n == 0 || (g && ids && aligned(g))));
+  PGN_CHECK_ARG(embed_shape_ok(n, V, d) && dW && aligned(dW) && (n == 0 || (g && kept && aligned(g) && aligned(kept))));
   PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_embed_bwd_workspace_bytes(n, V, d));
   hipStream_t st = (hipStream_t)stream;
   int32_t* ws = (int32_t*)workspace;
-  if (g_bf16) return w_bf16 ? launch_grad<__bf16, __bf16>(g, ids, scale, dW, ws, n, V, d, st)
-                            : launch_grad<__bf16, float>(g, ids, scale, dW, ws, n, V, d, st);
-  return w_bf16 ? launch_grad<float, __bf16>(g, ids, scale, dW, ws, n, V, d, st)
-                : launch_grad<float, float>(g, ids, scale, dW, ws, n, V, d, st);
+  if (g_bf16) return w_bf16 ? launch_grad<__bf16, __bf16>(g, kept, scale, dW, ws, n, V, d, st)
+                            : launch_grad<__bf16, float>(g, kept, scale, dW, ws, n, V, d, st);
+  return w_bf16 ? launch_grad<float, __bf16>(g, kept, scale, dW, ws, n, V, d, st)
+                : launch_grad<float, float>(g, kept, scale, dW, ws, n, V, d, st);
 }

@@ -109,32 +109,46 @@ PGN_DEVICE float column_max(float x) {
 PGN_DEVICE float column_sum(float x) { return swap_add<32>(swap_add<16>(x, x), swap_add<16>(x, x)); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The teacher's distribution over its entries, a wave a row.
+// The teacher's distribution over its entries, a wave a row. A repeated id's probabilities are added into its first entry,
+// the others leave the list, so that every later kernel meets an id once.
+constexpr int kMaxEntries = 1024;
+constexpr int64_t kSliceBytes = (int64_t)2 << 20;
+
 __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ ids, const float* __restrict__ z,
                                                     float inv_tau, int32_t* __restrict__ entry,
                                                     float* __restrict__ p, float* __restrict__ psum,
-                                                    float* __restrict__ ent, int64_t n, int64_t V, int64_t K) {
-  const int l = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                                    float* __restrict__ ent, int64_t n, int64_t V, int K) {
+  extern __shared__ __align__(16) unsigned char smem[];  // a wave's ids and probabilities
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * 4 + w;
   if (row >= n) return;
+  const int K4 = (K + 3) / 4 * 4;
+  int32_t* const id_of = reinterpret_cast<int32_t*>(smem) + w * 2 * K4;
+  float* const p_of = reinterpret_cast<float*>(id_of + K4);
   ids += row * K, z += row * K, entry += row * K, p += row * K;
   float m = -INFINITY;
-  for (int64_t k = l; k < K; k += 64)
-    if (ids[k] >= 0 && ids[k] < V) m = fmaxf(m, z[k] * inv_tau);
+  for (int k = l; k < K; k += 64) {
+    const int64_t id = ids[k];
+    const bool on = id >= 0 && id < V;
+    const float x = on ? z[k] * inv_tau : -INFINITY;
+    id_of[k] = on ? (int32_t)id : -1;
+    p_of[k] = x;
+    m = fmaxf(m, x);
+  }
   for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
   const bool some = m > -INFINITY;
   float sum = 0.f;
-  for (int64_t k = l; k < K; k += 64)
-    if (some && ids[k] >= 0 && ids[k] < V) sum += expf(z[k] * inv_tau - m);
+  for (int k = l; k < K; k += 64)
+    if (some && id_of[k] >= 0) sum += expf(p_of[k] - m);
   for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
   const float inv = some ? 1.f / sum : 0.f, log_sum = some ? logf(sum) : 0.f;
   float e = 0.f;
-  for (int64_t k = l; k < K; k += 64) {
-    const bool on = some && ids[k] >= 0 && ids[k] < V;
-    const float x = on ? z[k] * inv_tau - m : -INFINITY;
+  for (int k = l; k < K; k += 64) {
+    const float x = p_of[k] - m;
+    const bool on = some && id_of[k] >= 0;
     const float pk = on ? expf(x) * inv : 0.f;
-    entry[k] = on ? (int32_t)ids[k] : -1;
-    p[k] = pk;
+    if (!on) id_of[k] = -1;
+    p_of[k] = pk;
     if (pk > 0.f) e += pk * (x - log_sum);
   }
   for (int o = 1; o < 64; o *= 2) e += __shfl_xor(e, o);
@@ -142,30 +156,106 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
     psum[row] = some ? 1.f : 0.f;
     ent[row] = e;
   }
+  if (l < K4 - K) id_of[K + l] = -1;
+  // (the lists are the wave's own: its LDS operations are in order)
+  __builtin_amdgcn_wave_barrier();
+  for (int k = l; k < K + l; k += 64) {  // every lane takes part in every turn
+    const int id = k < K ? id_of[k] : -1;
+    float pk = k < K ? p_of[k] : 0.f;
+    int earlier = 0, equal = 0;
+#pragma unroll 4
+    for (int j = 0; j < K4; j += 4) {
+      const i32x4 o = *reinterpret_cast<const i32x4*>(id_of + j);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) equal += o[u] == id;
+    }
+    if (__ballot(id >= 0 && equal > 1)) {  // a repeated id
+      float all = 0.f;
+      for (int j = 0; j < K; ++j)
+        if (id_of[j] == id) {
+          all += p_of[j];
+          earlier += j < k;
+        }
+      pk = earlier == 0 ? all : 0.f;
+    }
+    if (k < K) {
+      entry[k] = earlier == 0 ? id : -1;
+      p[k] = id >= 0 ? pk : 0.f;
+    }
+  }
 }
 
-// The student's logits of the teacher's entries, zl[i][k] = h_i . W_entry; a wave a row, 16 lanes an entry.
+// The student's logits of the teacher's entries, zl[i][k] = h_i . W_entry: 16 lanes a row and slice of the vocabulary, two
+// entries at a time. Bound by the rows of W fetched (n K d values). An XCD takes every eighth slice, all rows of one before
+// the next, so that the words' rows stay in its L2 (a slice is at most 2 MB).
+template <int CHUNKS>  // 128 values of d each, h's held in registers; 0: any d
 __global__ __launch_bounds__(256) void head_entry_logits(const __bf16* __restrict__ h, const __bf16* __restrict__ W,
                                                          const int32_t* __restrict__ entry, float* __restrict__ zl,
-                                                         int64_t n, int64_t d, int64_t K) {
+                                                         int64_t n, int d, int K, int blocks, int slice) {
+  constexpr int R = CHUNKS > 0 ? CHUNKS : 1;
   const int l = threadIdx.x & 63, q = l >> 4, j = l & 15;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= n) return;
-  const __bf16* hr = h + row * d;
-  for (int64_t k0 = 0; k0 < K; k0 += 4) {
-    const int64_t k = k0 + q;
-    const int e = k < K ? entry[row * K + k] : -1;
-    float s = 0.f;
-    if (e >= 0) {
-      const __bf16* wr = W + (int64_t)e * d;
-      for (int64_t c = 8 * j; c < d; c += 128) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(hr + c), b = *reinterpret_cast<const bf16x8*>(wr + c);
+  const int turn = blockIdx.x / kXcdCount / blocks, block = blockIdx.x / kXcdCount % blocks;
+  const int lo = (turn * kXcdCount + blockIdx.x % kXcdCount) * slice;
+  const int64_t row = (int64_t)block * 16 + (threadIdx.x >> 4);
+  const bool live = row < n;
+  const int64_t at = live ? row : n - 1;
+  const __bf16* hr = h + at * d;
+  entry += at * K, zl += at * K;
+  bf16x8 x[R];
+  if constexpr (CHUNKS > 0) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s += (float)a[u] * (float)b[u];
+    for (int c = 0; c < R; ++c)
+      x[c] = 8 * j + 128 * c < d ? *reinterpret_cast<const bf16x8*>(hr + 8 * j + 128 * c) : bf16x8{};
+  }
+  for (int k0 = 0; k0 < K; k0 += 64) {
+    // the row's entries within the slice, a bit each
+    unsigned long long left = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int k = k0 + 16 * c + j, e = live && k < K ? entry[k] : -1;
+      left |= (__ballot(e >= lo && e - lo < slice) >> (16 * q) & 0xffffull) << (16 * c);
+    }
+    while (__ballot(left != 0)) {
+      int k[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        k[u] = left ? k0 + __ffsll((long long)left) - 1 : -1;
+        left &= left - 1;
+      }
+      const __bf16* wr[2];
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) wr[u] = W + (int64_t)(k[u] >= 0 ? entry[k[u]] : lo) * d + 8 * j;
+      if constexpr (CHUNKS > 0) {
+        bf16x8 w[2][R];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < R; ++c)
+            w[u][c] = 8 * j + 128 * c < d ? *reinterpret_cast<const bf16x8*>(wr[u] + 128 * c) : bf16x8{};
+#pragma unroll
+        for (int c = 0; c < R; ++c)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[u] += (float)x[c][i] * (float)w[u][c][i];
+      } else {
+        for (int c = 0; 8 * j + c < d; c += 128) {
+          const bf16x8 a = *reinterpret_cast<const bf16x8*>(hr + 8 * j + c);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bf16x8 b = *reinterpret_cast<const bf16x8*>(wr[u] + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[u] += (float)a[i] * (float)b[i];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = group_sum<16>(s[u]);
+        if (j == 0 && k[u] >= 0) zl[k[u]] = s[u];
       }
     }
-    s = group_sum<16>(s);
-    if (j == 0 && k < K) zl[row * K + k] = s;
   }
 }
 
@@ -244,7 +334,8 @@ __global__ __launch_bounds__(C::kThreads) void head_logits(Operand h, Operand W,
       });
 }
 
-// Rows' pieces joined: 16 rows a workgroup, 16 threads a row (thread 16 q + r: every 16th piece of row r from q).
+// Rows' pieces joined: R rows a workgroup, T = 256 / R threads a row (thread R q + r: every T-th piece of row r from q),
+// each in one pass with a running maximum. Few rows take more threads each.
 struct JoinArgs {
   const int64_t* y;
   float *ce, *lse;
@@ -255,35 +346,47 @@ struct JoinArgs {
   int64_t pieces, n, V, K;
 };
 
+template <int R>
 __global__ __launch_bounds__(256) void head_join(FwdOut in, JoinArgs j) {
-  __shared__ float parts[4][16][17];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t row = (int64_t)blockIdx.x * 16 + r, n = j.n;
-  const bool live = row < n;
-  float m = -INFINITY, s0 = 0.f, s1 = 0.f, dot = 0.f;
-  if (live) {
-    for (int64_t k = q; k < j.pieces; k += 16) m = fmaxf(m, in.m[k * n + row]);
-    for (int64_t k = q; k < j.K; k += 16) {
-      const float pk = j.p[row * j.K + k];
-      if (pk > 0.f) dot += pk * j.zl[row * j.K + k];
+  constexpr int T = 256 / R;
+  __shared__ float part[4][256];
+  const int tid = threadIdx.x, r = tid % R, q = tid / R;
+  const int64_t n = j.n, row = min((int64_t)blockIdx.x * R + r, n - 1);
+  float m = -INFINITY, s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+  for (int64_t k = q; k < j.pieces; k += T) {
+    const float mk = in.m[k * n + row], a0 = in.s0[k * n + row], a1 = j.second ? in.s1[k * n + row] : 0.f;
+    const float top = fmaxf(m, mk), base = top > -INFINITY ? top : 0.f;
+    s0 = s0 * expf((m - base) * j.scale0) + a0 * expf((mk - base) * j.scale0);
+    if (j.second) s1 = s1 * expf((m - base) * j.scale1) + a1 * expf((mk - base) * j.scale1);
+    m = top;
+  }
+  // the row's sum over the entries: consecutive threads take consecutive entries
+  float dot = 0.f;
+  if (j.K > 0) {
+    const int64_t at = min((int64_t)blockIdx.x * R + tid / T, n - 1) * j.K;
+    for (int64_t k = tid % T; k < j.K; k += T) {
+      const float pk = j.p[at + k];
+      if (pk > 0.f) dot += pk * j.zl[at + k];
     }
   }
-  parts[0][q][r] = m;
-  parts[3][q][r] = dot;
-  __syncthreads();
-  for (int k = 0; k < 16; ++k) m = fmaxf(m, parts[0][k][r]);
-  if (live)
-    for (int64_t k = q; k < j.pieces; k += 16) {
-      const float mk = in.m[k * n + row] - m;
-      s0 += in.s0[k * n + row] * expf(mk * j.scale0);
-      if (j.second) s1 += in.s1[k * n + row] * expf(mk * j.scale1);
+  part[0][tid] = m, part[1][tid] = s0, part[2][tid] = s1, part[3][tid] = dot;
+  for (int half = T / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (q < half) {
+      const float mk = part[0][tid + half * R], top = fmaxf(m, mk), base = top > -INFINITY ? top : 0.f;
+      const float f0 = expf((m - base) * j.scale0), g0 = expf((mk - base) * j.scale0);
+      s0 = s0 * f0 + part[1][tid + half * R] * g0;
+      if (j.second)
+        s1 = s1 * expf((m - base) * j.scale1) + part[2][tid + half * R] * expf((mk - base) * j.scale1);
+      m = top;
+      part[0][tid] = m, part[1][tid] = s0, part[2][tid] = s1;
     }
-  parts[1][q][r] = s0;
-  parts[2][q][r] = s1;
+    if (tid % T < half) part[3][tid] += part[3][tid + half];
+  }
   __syncthreads();
-  if (q != 0 || !live) return;
-  s0 = s1 = dot = 0.f;
-  for (int k = 0; k < 16; ++k) s0 += parts[1][k][r], s1 += parts[2][k][r], dot += parts[3][k][r];
+  if (q != 0 || (int64_t)blockIdx.x * R + r >= n) return;
+  dot = part[3][r * T];
   const float l0 = m * j.scale0 + logf(s0), l1 = j.second ? m * j.scale1 + logf(s1) : l0;
   if (j.y != nullptr) {
     const int64_t label = j.y[row];
@@ -404,7 +507,7 @@ __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W
       });
 }
 
-// dl at the teacher's entries, whole: a thread an entry. Repeated ids write the same value.
+// dl at the teacher's entries, whole: a thread an entry.
 __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const int32_t* __restrict__ entry,
                                                      const float* __restrict__ p, const float* __restrict__ zl,
                                                      __bf16* __restrict__ dl, int64_t ld, int64_t v_begin, int64_t n,
@@ -420,11 +523,8 @@ __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const int32_t* __
   const float w_ce = gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f), gk = in.g_kd[row] * in.tau;
   float x = 0.f;
   if (w_ce != 0.f || gk != 0.f || gc != 0.f) {
-    float pk = 0.f;
-    for (int64_t k = 0; k < K; ++k)
-      if (entry[row * K + k] == v) pk += p[row * K + k];
     const float l = zl[e];
-    x = gk * (in.psum[row] * expf(l / in.tau - in.lse_t[row]) - pk);
+    x = gk * (in.psum[row] * expf(l / in.tau - in.lse_t[row]) - p[e]);
     if (w_ce != 0.f) x += w_ce * expf(l - in.lse[row]);
     if (label == v) x -= gc;
   }
@@ -536,9 +636,9 @@ int launch_grads(const GradArgs& ga, hipStream_t st) {
 
 bool head_shape_ok(int64_t n, int64_t V, int64_t d, int64_t K) {
   return n > 0 && n <= (int64_t)1 << 24 && V > 0 && V <= (int64_t)1 << 24 && d > 0 && d % 8 == 0 && d <= 65536 &&
-         K >= 0 && K <= 65536 &&
+         K >= 0 && K <= kMaxEntries &&
          // launches of fewer than 2^32 threads; tiles counted in 32 bits
-         n * K < (int64_t)1 << 31 && tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31;
+         n * K < (int64_t)1 << 31 && (K == 0 || tiles(n, 4) * (V * d >> 20) < (int64_t)1 << 23) && tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31;
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p % 16) == 0; }
@@ -577,10 +677,15 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
   float* ent = f + (3 * pieces + 1) * n;
   const Operand ho{(const __bf16*)h, d, n}, Wo{(const __bf16*)W, d, V};
   if (K > 0) {
-    hipLaunchKernelGGL(head_teacher, dim3((unsigned)tiles(n, 4)), dim3(256), 0, st, ids, z, 1.f / tau, entry, p, psum,
-                       ent, n, V, K);
-    hipLaunchKernelGGL(head_entry_logits, dim3((unsigned)tiles(n, 4)), dim3(256), 0, st, ho.p, Wo.p, entry, zl, n, d,
-                       K);
+    hipLaunchKernelGGL(head_teacher, dim3((unsigned)tiles(n, 4)), dim3(256), (unsigned)(4 * 8 * round_up(K, 4)), st, ids, z,
+                       1.f / tau, entry, p, psum, ent, n, V, (int)K);
+    // slices of at most 2 MB of W, eight a turn
+    const int64_t turns = tiles(V * d * 2, kXcdCount * kSliceBytes), blocks = tiles(n, 16);
+    const int64_t slice = tiles(V, kXcdCount * turns);
+    const auto fn = d <= 512 ? head_entry_logits<4>
+                             : d <= 768 ? head_entry_logits<6> : d <= 1024 ? head_entry_logits<8> : head_entry_logits<0>;
+    hipLaunchKernelGGL(fn, dim3((unsigned)(kXcdCount * turns * blocks)), dim3(256), 0, st, ho.p, Wo.p, entry, zl, n,
+                       (int)d, (int)K, (int)blocks, (int)slice);
   }
   const int second = y && K > 0 && tau != 1.f;
   const float scale0 = y ? 1.f : 1.f / tau, scale1 = 1.f / tau;
@@ -596,7 +701,10 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
   });
   if (rc) return rc;
   const JoinArgs j{y, ce, lse, ent, psum, p, zl, kd, lse_t, tau, scale0, scale1, second, pieces, n, V, K};
-  hipLaunchKernelGGL(head_join, dim3((unsigned)tiles(n, 16)), dim3(256), 0, st, out, j);
+  if (n <= 4096)
+    hipLaunchKernelGGL(head_join<4>, dim3((unsigned)tiles(n, 4)), dim3(256), 0, st, out, j);
+  else
+    hipLaunchKernelGGL(head_join<16>, dim3((unsigned)tiles(n, 16)), dim3(256), 0, st, out, j);
   PGN_RETURN_LAUNCH();
 }
 

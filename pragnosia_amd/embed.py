@@ -32,17 +32,17 @@ def _check_embed(op: str, ids: Tensor, W: Tensor, scale: float, dtype: torch.dty
         raise PragnosiaError(f"{op}: scale must be finite, got {scale}")
 
 
-def _forward(ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
-    """ids (n) int64, W (V, d), both contiguous."""
+def _forward(ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype, kept: Optional[Tensor] = None) -> Tensor:
+    """ids (n) int64, W (V, d), both contiguous. kept: (n) int32 for the ids as the backward takes them, or None."""
     n, (V, d) = ids.shape[0], W.shape
     y = torch.empty(n, d, device=W.device, dtype=dtype)
     _call("pragnosia_embed_fwd", lm_lib().pragnosia_embed_fwd, W, _at(ids), _at(W), W.dtype == _BF16, scale, _at(y),
-          dtype == _BF16, n, V, d)
+          dtype == _BF16, _at(kept), n, V, d)
     return y
 
 
-def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) -> Tensor:
-    """g (n, d), ids (n) int64 -> dW (V, d) in `dtype`."""
+def _backward(g: Tensor, kept: Tensor, V: int, scale: float, dtype: torch.dtype) -> Tensor:
+    """g (n, d), kept (n) int32 (ids, negative outside the table) -> dW (V, d) in `dtype`."""
     g = _as(g, g.dtype)
     n, d = g.shape
     dW = torch.empty(V, d, device=g.device, dtype=dtype)
@@ -51,7 +51,7 @@ def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) 
     if nbytes < 0:
         raise PragnosiaError(f"embed_bwd: shape n={n} V={V} d={d} rejected")
     ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
-    _call("pragnosia_embed_bwd", L.pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(ids), scale, _at(dW),
+    _call("pragnosia_embed_bwd", L.pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(kept), scale, _at(dW),
           dtype == _BF16, _at(ws), nbytes, n, V, d)
     return dW
 
@@ -59,16 +59,16 @@ def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, W, scale, dtype):
-        ids = _as(ids, _I64)
-        ctx.save_for_backward(ids)
+        kept = torch.empty(ids.shape[0], device=W.device, dtype=torch.int32)
+        ctx.save_for_backward(kept)
         ctx.V, ctx.scale, ctx.dtype = W.shape[0], scale, W.dtype
-        return _forward(ids, _as(W, W.dtype), scale, dtype)
+        return _forward(_as(ids, _I64), _as(W, W.dtype), scale, dtype, kept)
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        ids, = ctx.saved_tensors
-        return None, _backward(g, ids, ctx.V, ctx.scale, ctx.dtype), None, None
+        kept, = ctx.saved_tensors
+        return None, _backward(g, kept, ctx.V, ctx.scale, ctx.dtype), None, None
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -95,7 +95,8 @@ def embed_bwd(g: Tensor, ids: Tensor, V: int, scale: float, bf16: bool) -> Tenso
     if ids.dtype not in _INTS:
         raise PragnosiaError(f"embed_bwd: ids must be integers, got {ids.dtype}")
     _expect("embed_bwd", g.device, ids=(ids, (g.shape[0],)))
-    return _backward(g, _as(ids, _I64), V, float(scale), _BF16 if bf16 else _F32)
+    kept = torch.where((ids >= 0) & (ids < V), ids, -1).to(torch.int32)
+    return _backward(g, _as(kept, torch.int32), V, float(scale), _BF16 if bf16 else _F32)
 
 
 @embed_bwd.register_fake

@@ -91,8 +91,8 @@ def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optiona
         raise PragnosiaError(f"{op}: labels, or a teacher's ids and logits together, expected")
     if ids is not None:
         _expect(op, h.device, logits=(z, tuple(ids.shape)))
-        if ids.shape[1] == 0 or not z.is_floating_point():
-            raise PragnosiaError(f"{op}: ids and logits (..., K) with K > 0 and floating logits expected, got "
+        if not 0 < ids.shape[1] <= 1024 or not z.is_floating_point():
+            raise PragnosiaError(f"{op}: ids and logits (..., K) with K from 1 to 1024 and floating logits expected, got "
                                  f"{tuple(ids.shape)} and {z.dtype}")
     if not (tau > 0 and math.isfinite(tau)):
         raise PragnosiaError(f"{op}: tau must be positive and finite, got {tau}")
@@ -280,7 +280,7 @@ def linear_distill(h: Tensor, W: Tensor, ids: Tensor, logits: Tensor, tau: float
     """Per-token distillation loss of the head h W^T from a teacher's top logits, and with labels y the cross entropy
     (else None) from the same pass over the vocabulary; fp32, h's leading shape, differentiable in h and W.
 
-    ids and logits (..., K): the teacher's words, in any order, and its logits there. Its distribution p is their softmax
+    ids and logits (..., K), K up to 1024: the teacher's words, in any order, and its logits there. Its distribution p is their softmax
     at temperature tau; the loss is tau^2 KL(p || q) with q the softmax of the student's logits over the whole vocabulary
     at tau. An id outside [0, V) marks an entry that is not there (lists of different lengths); a logit of -inf has
     probability zero; a token with no entry left has loss 0 and no gradient. A repeated id has the sum of its entries'
