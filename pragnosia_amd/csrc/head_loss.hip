@@ -67,7 +67,7 @@ struct GradPlan {
   int64_t dl_bytes, part_h, part_w;  // bytes of the workspace's three parts
 };
 
-GradPlan choose_grads(int64_t n, int64_t V, int64_t d) {
+GradPlan search_grads(int64_t n, int64_t V, int64_t d) {
   GradPlan p;
   p.n_pad = round_up(n, kPad);
   const int64_t v_pad = round_up(V, kPad), most = std::max(kPad, kPieceBytes / (2 * p.n_pad) / kPad * kPad);
@@ -99,6 +99,16 @@ GradPlan choose_grads(int64_t n, int64_t V, int64_t d) {
   p.part_h = p.split_h > 1 || p.pieces > 1 ? p.split_h * n * d * 4 : 0;
   p.part_w = p.split_w > 1 ? p.split_w * words * d * 4 : 0;
   return p;
+}
+
+// (The search takes microseconds of the host; a program's sizes repeat.)
+GradPlan choose_grads(int64_t n, int64_t V, int64_t d) {
+  thread_local struct {
+    int64_t n = 0, V = 0, d = 0;
+    GradPlan plan;
+  } last;
+  if (last.n != n || last.V != V || last.d != d) last = {n, V, d, search_grads(n, V, d)};
+  return last.plan;
 }
 
 // Lane exchange of the groups of 16: the maximum, and the sum, over a column's four lane groups, in every one of them.

@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from ._lib import PragnosiaError, lm_lib
-from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _once
+from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _once, _workspace
 from .ops import _expect, _require_gpu
 
 
@@ -46,12 +46,9 @@ def _backward(g: Tensor, kept: Tensor, V: int, scale: float, dtype: torch.dtype)
     g = _as(g, g.dtype)
     n, d = g.shape
     dW = torch.empty(V, d, device=g.device, dtype=dtype)
-    L = lm_lib()
-    nbytes = L.pragnosia_embed_bwd_workspace_bytes(n, V, d)
-    if nbytes < 0:
-        raise PragnosiaError(f"embed_bwd: shape n={n} V={V} d={d} rejected")
+    nbytes = _workspace("pragnosia_embed_bwd_workspace_bytes", n, V, d)
     ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
-    _call("pragnosia_embed_bwd", L.pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(kept), scale, _at(dW),
+    _call("pragnosia_embed_bwd", lm_lib().pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(kept), scale, _at(dW),
           dtype == _BF16, _at(ws), nbytes, n, V, d)
     return dW
 
@@ -123,7 +120,11 @@ def embedding(ids: Tensor, W: Tensor, scale: float = 1.0, dtype: Optional[torch.
     multiple of 8. An id outside [0, V) gives a row of zeros and takes no part in W's gradient."""
     dtype, scale = dtype or W.dtype, float(scale)
     flat = ids if ids.dim() == 1 else ids.reshape(-1)
-    _check_embed("embedding", flat, W, scale, dtype)
+    # (the usual call, without the checks' share of a short one)
+    if not (W.is_cuda and flat.device == W.device and flat.dtype is _I64 and W.dim() == 2 and W.dtype in _FLOATS
+            and dtype in _FLOATS and W.shape[0] > 0 and W.shape[1] > 0 and W.shape[1] % 8 == 0
+            and math.isfinite(scale)):
+        _check_embed("embedding", flat, W, scale, dtype)
     if torch.compiler.is_compiling():
         y = embed(flat, W, scale, dtype == _BF16)
     elif torch.is_grad_enabled() and W.requires_grad:

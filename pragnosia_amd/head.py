@@ -19,6 +19,7 @@ ops, whose dispatch costs tens of microseconds a call.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -72,6 +73,32 @@ def _once(backward):
     return run
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(what: str, *sizes: int) -> int:
+    """A workspace query of the C ABI: a function of the sizes alone."""
+    nbytes = getattr(lm_lib(), what)(*sizes)
+    if nbytes < 0:
+        raise PragnosiaError(f"{what}: sizes {sizes} rejected")
+    return nbytes
+
+
+def _plain_call(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
+                tau: float) -> bool:
+    """Whether _check_head has nothing to say, at a fraction of its cost on the host."""
+    if not (h.is_cuda and h.dim() == 2 and W.dim() == 2 and h.dtype in _FLOATS and W.dtype in _FLOATS):
+        return False
+    (n, d), dev = h.shape, h.device
+    if not (W.device == dev and W.shape[1] == d and W.shape[0] > 0 and d > 0 and d % 8 == 0):
+        return False
+    if y is not None and not (y.device == dev and y.dtype is _I64 and y.dim() == 1 and y.shape[0] == n):
+        return False
+    if ids is None:
+        return y is not None and z is None
+    return (z is not None and ids.device == dev and z.device == dev and ids.dtype is _I64 and z.dtype is _F32
+            and ids.dim() == 2 and ids.shape[0] == n and 0 < ids.shape[1] <= 1024 and z.shape == ids.shape
+            and 0 < tau < math.inf)
+
+
 def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
                 tau: float) -> None:
     _require_gpu(h, W, y, ids, z)
@@ -108,12 +135,9 @@ def _forward(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z
     kd, stats = (None, None) if ids is None else (e(n), e(n * (2 + 3 * K)))
     if n == 0:
         return ce, lse, kd, stats
-    L = lm_lib()
-    nbytes = L.pragnosia_head_fwd_workspace_bytes(n, V, d, K)
-    if nbytes < 0:
-        raise PragnosiaError(f"head_loss: shape n={n} V={V} d={d} K={K} rejected")
+    nbytes = _workspace("pragnosia_head_fwd_workspace_bytes", n, V, d, K)
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-    _call("pragnosia_head_fwd", L.pragnosia_head_fwd, h, _at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce), _at(lse),
+    _call("pragnosia_head_fwd", lm_lib().pragnosia_head_fwd, h, _at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce), _at(lse),
           _at(kd), *_stats_at(stats, n, K), _at(ws), nbytes, n, V, d, K)
     return ce, lse, kd, stats
 
@@ -137,12 +161,9 @@ def _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, K: int, tau: float, need_h
     dh = torch.empty_like(h) if need_h else None
     dW = torch.empty(V, d, device=h.device, dtype=dW_type) if need_W else None
     g_ce, g_lse, g_kd = _as(g_ce, _F32), _as(g_lse, _F32), _as(g_kd, _F32)
-    L = lm_lib()
-    nbytes = L.pragnosia_head_bwd_workspace_bytes(n, V, d)
-    if nbytes < 0:
-        raise PragnosiaError(f"head_loss_bwd: shape n={n} V={V} d={d} rejected")
+    nbytes = _workspace("pragnosia_head_bwd_workspace_bytes", n, V, d)
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-    _call("pragnosia_head_bwd", L.pragnosia_head_bwd, h, _at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W), _at(y),
+    _call("pragnosia_head_bwd", lm_lib().pragnosia_head_bwd, h, _at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W), _at(y),
           _at(lse), *_stats_at(stats, n, K), tau, _at(dh), _at(dW), dw_f32, _at(ws), nbytes, n, V, d, K)
     return dh, dW
 
@@ -258,7 +279,8 @@ def _losses(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Te
     if torch.compiler.is_compiling():
         got = head_loss(h, W, y, ids, z, tau)[:3]
     else:
-        _check_head(op, h, W, y, ids, z, tau)
+        if not _plain_call(h, W, y, ids, z, tau):
+            _check_head(op, h, W, y, ids, z, tau)
         if torch.is_grad_enabled() and (h.requires_grad or W.requires_grad):
             got = _HeadLoss.apply(h, W, y, ids, z, tau)
         else:
