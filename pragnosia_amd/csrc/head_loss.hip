@@ -30,13 +30,13 @@ struct KindInfo {
   int x, y, slots;    // tile, and workgroups that run at once
   float step, fixed;  // microseconds of a step of 64, and of a tile beside its steps, as measured on a full chip
 };
-constexpr KindInfo kLogitsKinds[] = {{Large::X, Large::Y, 256, 1.7f, 6.f},
-                                     {0, 0, 0, 0.f, 0.f},
-                                     {Mid::X, Mid::Y, 512, 1.2f, 3.f},
-                                     {Small::X, Small::Y, 512, 0.45f, 1.5f}};
-constexpr KindInfo kGradKinds[] = {{Large::X, Large::Y, 256, 1.95f, 8.f},
-                                   {Wide::X, Wide::Y, 256, 1.55f, 7.f},
-                                   {Mid::X, Mid::Y, 512, 1.3f, 4.f}};
+constexpr KindInfo kLogitsKinds[] = {{Large::X, Large::Y, 256, 1.45f, 5.f},
+                                     {Wide::X, Wide::Y, 256, 1.2f, 4.f},
+                                     {Mid::X, Mid::Y, 512, 0.85f, 3.f},
+                                     {Small::X, Small::Y, 512, 0.4f, 1.5f}};
+constexpr KindInfo kGradKinds[] = {{Large::X, Large::Y, 256, 1.6f, 6.f},
+                                   {Wide::X, Wide::Y, 256, 1.36f, 6.f},
+                                   {Mid::X, Mid::Y, 512, 1.0f, 4.f}};
 
 int64_t tiles(int64_t x, int64_t m) { return (x + m - 1) / m; }
 int64_t round_up(int64_t x, int64_t m) { return tiles(x, m) * m; }
@@ -45,7 +45,7 @@ int64_t round_up(int64_t x, int64_t m) { return tiles(x, m) * m; }
 Kind choose_logits(int64_t n, int64_t V, int64_t d) {
   Kind best = kLarge;
   float least = INFINITY;
-  for (Kind k : {kLarge, kMid, kSmall}) {
+  for (Kind k : {kLarge, kWide, kMid, kSmall}) {
     const KindInfo& i = kLogitsKinds[k];
     const float t = (float)tiles(tiles(n, i.y) * tiles(V, i.x), i.slots) * (tiles(d, kGemmK) * i.step + i.fixed);
     if (t < least) least = t, best = k;
@@ -53,26 +53,46 @@ Kind choose_logits(int64_t n, int64_t V, int64_t d) {
   return best;
 }
 
-// The workspace of one piece's dl: at most this many bytes (but at least one column of tiles).
-constexpr int64_t kPieceBytes = (int64_t)128 << 20;
-constexpr int64_t kPad = 256;  // dl's rows and columns are padded to whole tiles of any kind
+// The workspace of one piece's dl: about this many bytes at most (but 1024 words). It stays in the memory-side cache; half
+// of it costs 12 - 18% more time, twice or four times gain under 1%.
+constexpr int64_t kPieceBytes = (int64_t)144 << 20;
 
 // How the gradients' products are laid out: the pieces of the vocabulary; the tile; the ranges that the contracted
 // dimension is cut into (words for dh, tokens for dW), each a multiple of 64, so that few output tiles still fill the
 // chip: the ranges' partial sums, fp32, are added in order by head_sum.
 struct GradPlan {
-  int64_t n_pad, v_piece, pieces;
-  Kind kind;
+  int64_t v_piece, pieces;
+  Kind logits;        // the tile that forms dl
+  int64_t n_pad, ld;  // dl's rows and pitch: whole tiles
+  Kind kind;          // the products' tile
   int64_t len_h, split_h, len_w, split_w;
   int64_t dl_bytes, part_h, part_w;  // bytes of the workspace's three parts
 };
 
+// When `slots` workers have done n1 items of c1, then n2 of c2 <= c1, each taking the next as it comes free.
+float makespan(int64_t n1, float c1, int64_t n2, float c2, int64_t slots) {
+  const int64_t full = n1 / slots, rest = n1 - full * slots;
+  const float at = full * c1, done = rest ? at + c1 : at;
+  auto room = [&](float t) {
+    return (slots - rest) * (int64_t)std::max(0.f, (t - at) / c2 + 1e-3f) +
+           rest * (int64_t)std::max(0.f, (t - at - c1) / c2 + 1e-3f);
+  };
+  float lo = 0.f, hi = at + c1 + c2 * (n2 / slots + 1);
+  for (int u = 0; u < 16; ++u) {
+    const float mid = 0.5f * (lo + hi);
+    (room(mid) >= n2 ? hi : lo) = mid;
+  }
+  return std::max(done, hi);
+}
+
 GradPlan search_grads(int64_t n, int64_t V, int64_t d) {
   GradPlan p;
-  p.n_pad = round_up(n, kPad);
-  const int64_t v_pad = round_up(V, kPad), most = std::max(kPad, kPieceBytes / (2 * p.n_pad) / kPad * kPad);
-  p.v_piece = round_up(tiles(v_pad, tiles(v_pad, most)), kPad);
-  p.pieces = tiles(v_pad, p.v_piece);
+  const int64_t most = std::max<int64_t>(1024, kPieceBytes / (2 * round_up(n, Large::Y))), count = tiles(V, most);
+  p.logits = choose_logits(n, tiles(V, count), d);
+  p.v_piece = count == 1 ? V : round_up(tiles(V, count), kLogitsKinds[p.logits].x);
+  p.pieces = tiles(V, p.v_piece);
+  p.n_pad = round_up(n, kLogitsKinds[p.logits].y);
+  p.ld = round_up(p.v_piece, kLogitsKinds[p.logits].x);
   const int64_t words = std::min(V, p.v_piece), steps_h = tiles(words, kGemmK), steps_w = tiles(n, kGemmK);
   float least = INFINITY;
   for (Kind k : {kLarge, kWide, kMid}) {
@@ -81,9 +101,8 @@ GradPlan search_grads(int64_t n, int64_t V, int64_t d) {
     for (int64_t len = 4; ; len *= 2) {  // steps of an item, at most
       const int64_t sh = tiles(steps_h, len), sw = tiles(steps_w, len);
       const int64_t lh = tiles(steps_h, sh), lw = tiles(steps_w, sw);
-      const float ch = lh * i.step + i.fixed, cw = lw * i.step + i.fixed, sum = th * sh * ch + tw * sw * cw;
-      float t = std::max(ch, cw);
-      if (th * sh + tw * sw > i.slots) t = std::max(t, sum / i.slots + 0.5f * std::min(ch, cw));
+      const float ch = lh * i.step + i.fixed, cw = lw * i.step + i.fixed;
+      float t = ch >= cw ? makespan(th * sh, ch, tw * sw, cw, i.slots) : makespan(tw * sw, cw, th * sh, ch, i.slots);
       // partial sums: written and read at about 4 bytes a picosecond, and a launch
       const float part = (sh > 1 ? 8.f * sh * n * d : 0.f) + (sw > 1 ? 8.f * sw * words * d : 0.f);
       if (part > 0.f) t += part * 0.25e-6f + 3.f;
@@ -95,7 +114,7 @@ GradPlan search_grads(int64_t n, int64_t V, int64_t d) {
       if (sh == 1 && sw == 1) break;
     }
   }
-  p.dl_bytes = p.n_pad * p.v_piece * 2;
+  p.dl_bytes = round_up(p.n_pad * p.ld * 2, 256);
   p.part_h = p.split_h > 1 || p.pieces > 1 ? p.split_h * n * d * 4 : 0;
   p.part_w = p.split_w > 1 ? p.split_w * words * d * 4 : 0;
   return p;
@@ -195,6 +214,15 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
   }
 }
 
+// s + a . b of eight bf16 pairs, in fp32 two products at a time.
+PGN_DEVICE float dot8(bf16x8 a, bf16x8 b, float s) {
+  typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a[2 * i], a[2 * i + 1]}, bf16x2{b[2 * i], b[2 * i + 1]}, s, false);
+  return s;
+}
+
 // The student's logits of the teacher's entries, zl[i][k] = h_i . W_entry: 16 lanes a row and slice of the vocabulary, two
 // entries at a time. Bound by the rows of W fetched (n K d values). An XCD takes every eighth slice, all rows of one before
 // the next, so that the words' rows stay in its L2 (a slice is at most 2 MB).
@@ -246,18 +274,12 @@ __global__ __launch_bounds__(256) void head_entry_logits(const __bf16* __restric
 #pragma unroll
         for (int c = 0; c < R; ++c)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[u] += (float)x[c][i] * (float)w[u][c][i];
+          for (int u = 0; u < 2; ++u) s[u] = dot8(x[c], w[u][c], s[u]);
       } else {
         for (int c = 0; 8 * j + c < d; c += 128) {
           const bf16x8 a = *reinterpret_cast<const bf16x8*>(hr + 8 * j + c);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const bf16x8 b = *reinterpret_cast<const bf16x8*>(wr[u] + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[u] += (float)a[i] * (float)b[i];
-          }
+          for (int u = 0; u < 2; ++u) s[u] = dot8(a, *reinterpret_cast<const bf16x8*>(wr[u] + c), s[u]);
         }
       }
 #pragma unroll
@@ -454,8 +476,8 @@ PGN_DEVICE bf16x8 eight_rows(f32x4 lo, f32x4 hi) {
   return __builtin_bit_cast(bf16x8, i32x4{(int)p0, (int)q0, (int)p1, (int)q1});
 }
 
-// dl of a piece of the vocabulary: words v_begin .. v_begin + ld (ld a multiple of kPad) of the workspace's rows (n
-// padded likewise). Word and token rows past the ends get zeros.
+// dl of a piece of the vocabulary: words v_begin .. v_begin + ld (whole tiles) of the workspace's n_pad rows (likewise).
+// Word and token rows past the ends get zeros.
 template <class C, int NEXP>
 __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W, const RowInfo* __restrict__ rows,
                                                             float scale0, float scale1, __bf16* __restrict__ dl,
@@ -624,7 +646,7 @@ __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ part, 
 // Logits kernels by tile kind: F<C> with the tile type.
 template <class F>
 auto by_kind(Kind k, F&& f) {
-  return k == kLarge ? f(Large{}) : k == kMid ? f(Mid{}) : f(Small{});
+  return k == kLarge ? f(Large{}) : k == kWide ? f(Wide{}) : k == kMid ? f(Mid{}) : f(Small{});
 }
 
 int launch_sum(const float* part, void* out, int f32, int64_t split, int64_t count, hipStream_t st) {
@@ -658,7 +680,7 @@ int64_t head_pieces(int64_t n, int64_t V, int64_t d) {
   const Kind k = choose_logits(n, V, d);
   return tiles(V, kLogitsKinds[k].x) * 2;
 }
-static_assert(Large::WX == 2 && Mid::WX == 2 && Small::WX == 2, "two waves along the words");
+static_assert(Large::WX == 2 && Wide::WX == 2 && Mid::WX == 2 && Small::WX == 2, "two waves along the words");
 
 }  // namespace
 
@@ -749,15 +771,15 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   float *part_h = (float*)(ws + pl.dl_bytes), *part_w = (float*)(ws + pl.dl_bytes + pl.part_h);
   RowInfo* rows = (RowInfo*)(ws + pl.dl_bytes + pl.part_h + pl.part_w);
   hipLaunchKernelGGL(head_rows, dim3((unsigned)tiles(n, 256)), dim3(256), 0, st, in, second, rows, n, V);
-  const Kind kind = choose_logits(n, pl.v_piece, d);
   for (int64_t q = 0; q < pl.pieces; ++q) {
-    const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0), ld = round_up(words, kPad);
-    int rc = by_kind(kind, [&](auto c) {
+    const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0);
+    const int64_t ld = round_up(words, kLogitsKinds[pl.logits].x);
+    int rc = by_kind(pl.logits, [&](auto c) {
       typedef decltype(c) C;
       const auto fn = second ? head_dlogits<C, 2> : head_dlogits<C, 1>;
       const hipError_t e = pgn_lds_limit((const void*)fn, C::kLdsInfo);
       if (e != hipSuccess) return (int)e;
-      hipLaunchKernelGGL(fn, dim3(xcd_grid(ld / C::X * (pl.n_pad / C::Y), kLogitsKinds[kind].slots)),
+      hipLaunchKernelGGL(fn, dim3(xcd_grid(ld / C::X * (pl.n_pad / C::Y), kLogitsKinds[pl.logits].slots)),
                          dim3(C::kThreads), C::kLdsInfo, st, ho, Wo, rows, scale0, scale1, dl, ld, v0, pl.n_pad, d);
       return (int)hipGetLastError();
     });
