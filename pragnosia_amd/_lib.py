@@ -82,7 +82,7 @@ _RET_I64 = {"pragnosia_aspin_delta_bwd_workspace_bytes", "pragnosia_aspin_prep_t
             "pragnosia_layer_norm_partials", "pragnosia_wgrad_workspace_bytes",
             "pragnosia_aspin_exact_chunk_bwd_workspace_bytes", "pragnosia_aspin_delta_par_bwd_workspace_bytes"}
 
-# the entry points of include/lm/pragnosia_lm.h, in header order
+# the entry points of pragnosia_amd/include/pragnosia_lm.h, in header order
 LM_SIGNATURES = {
     "pragnosia_lm_abi_version": [],
     "pragnosia_head_fwd_workspace_bytes": [_i64] * 4,
@@ -123,7 +123,7 @@ def lib():
 
 
 def lm_lib():
-    """The loaded library with the language model's entry points (include/lm/pragnosia_lm.h) set up too."""
+    """The loaded library with the language model's entry points (pragnosia_amd/include/pragnosia_lm.h) set up too."""
     global _lm_lib
     if _lm_lib is None:
         L = lib()

@@ -14,7 +14,7 @@
 //   join  A run's partial rows are added in order.
 #include <algorithm>
 
-#include "../../include/lm/pragnosia_lm.h"
+#include "../include/pragnosia_lm.h"
 #include "common.h"
 
 namespace {

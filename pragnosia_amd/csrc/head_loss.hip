@@ -11,7 +11,7 @@
 // piece's columns; dh += dl W and dW = dl^T h are products over it.
 #include <algorithm>
 
-#include "../../include/lm/pragnosia_lm.h"
+#include "../include/pragnosia_lm.h"
 #include "gemm_tile.h"
 
 using namespace pgn;
@@ -146,7 +146,8 @@ constexpr int64_t kSliceBytes = (int64_t)2 << 20;
 __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ ids, const float* __restrict__ z,
                                                     float inv_tau, int32_t* __restrict__ entry,
                                                     float* __restrict__ p, float* __restrict__ psum,
-                                                    float* __restrict__ ent, int64_t n, int64_t V, int K) {
+                                                    float* __restrict__ ent, float* __restrict__ zl, int64_t n,
+                                                    int64_t V, int K) {
   extern __shared__ __align__(16) unsigned char smem[];  // a wave's ids and probabilities
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t row = (int64_t)blockIdx.x * 4 + w;
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
   const int K4 = (K + 3) / 4 * 4;
   int32_t* const id_of = reinterpret_cast<int32_t*>(smem) + w * 2 * K4;
   float* const p_of = reinterpret_cast<float*>(id_of + K4);
-  ids += row * K, z += row * K, entry += row * K, p += row * K;
+  ids += row * K, z += row * K, entry += row * K, p += row * K, zl += row * K;
   float m = -INFINITY;
   for (int k = l; k < K; k += 64) {
     const int64_t id = ids[k];
@@ -210,6 +211,7 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
     if (k < K) {
       entry[k] = earlier == 0 ? id : -1;
       p[k] = id >= 0 ? pk : 0.f;
+      if (id < 0 || earlier > 0) zl[k] = 0.f;  // (the others are head_entry_logits')
     }
   }
 }
@@ -710,7 +712,7 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
   const Operand ho{(const __bf16*)h, d, n}, Wo{(const __bf16*)W, d, V};
   if (K > 0) {
     hipLaunchKernelGGL(head_teacher, dim3((unsigned)tiles(n, 4)), dim3(256), (unsigned)(4 * 8 * round_up(K, 4)), st, ids, z,
-                       1.f / tau, entry, p, psum, ent, n, V, (int)K);
+                       1.f / tau, entry, p, psum, ent, zl, n, V, (int)K);
     // slices of at most 2 MB of W, eight a turn
     const int64_t turns = tiles(V * d * 2, kXcdCount * kSliceBytes), blocks = tiles(n, 16);
     const int64_t slice = tiles(V, kXcdCount * turns);

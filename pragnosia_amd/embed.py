@@ -1,5 +1,5 @@
 """Lookup of token rows with a scale, and its gradient by sorted tokens, on hand-written kernels (csrc/embed.hip; C ABI in
-include/lm/pragnosia_lm.h).
+pragnosia_amd/include/pragnosia_lm.h).
 
     y = embedding(ids, W, scale)
 
@@ -70,7 +70,7 @@ class _Embedding(torch.autograd.Function):
 
 # ---------------------------------------------------------------------------------------------------------------
 # the same as custom ops, for traces
-@torch.library.custom_op("pragnosia::embed", mutates_args=())
+@torch.library.custom_op("pragnosia_lm::embed", mutates_args=())
 def embed(ids: Tensor, W: Tensor, scale: float, bf16: bool) -> Tensor:
     """ids (n), W (V, d) -> scale W[ids] (n, d), bf16 or fp32."""
     dtype = _BF16 if bf16 else _F32
@@ -83,7 +83,7 @@ def _(ids, W, scale, bf16):
     return W.new_empty(ids.shape[0], W.shape[1], dtype=_BF16 if bf16 else _F32)
 
 
-@torch.library.custom_op("pragnosia::embed_bwd", mutates_args=())
+@torch.library.custom_op("pragnosia_lm::embed_bwd", mutates_args=())
 def embed_bwd(g: Tensor, ids: Tensor, V: int, scale: float, bf16: bool) -> Tensor:
     """g (n, d), ids (n) -> dW (V, d), bf16 or fp32."""
     _require_gpu(g, ids)

@@ -1,5 +1,5 @@
 """The head's losses over the vocabulary, with no logits kept: cross entropy of labels and distillation from a teacher's
-top logits, forward and backward on hand-written kernels (csrc/head_loss.hip; C ABI in include/lm/pragnosia_lm.h).
+top logits, forward and backward on hand-written kernels (csrc/head_loss.hip; C ABI in pragnosia_amd/include/pragnosia_lm.h).
 
     loss, lse = linear_cross_entropy(h, W, y)
     kd, ce = linear_distill(h, W, ids, logits, tau, y)
@@ -127,12 +127,13 @@ def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optiona
 
 def _forward(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor], tau: float):
     """h (n, d), W (V, d) bf16; y (n) int64 or None; ids int64 and z fp32 (n, K) or None, all contiguous. Returns (ce,
-    lse, kd, stats): fp32, None where not asked for; stats holds lse_t, psum, entry, p and zl for the backward."""
+    lse, kd, stats): fp32, None where not asked for; stats (int32: bits) holds lse_t, psum, entry, p and zl for the
+    backward."""
     n, d = h.shape
     V, K = W.shape[0], 0 if ids is None else ids.shape[1]
     e = lambda s: torch.empty(s, device=h.device, dtype=_F32)
     ce, lse = (None, None) if y is None else (e(n), e(n))
-    kd, stats = (None, None) if ids is None else (e(n), e(n * (2 + 3 * K)))
+    kd, stats = (None, None) if ids is None else (e(n), e(n * (2 + 3 * K)).view(torch.int32))
     if n == 0:
         return ce, lse, kd, stats
     nbytes = _workspace("pragnosia_head_fwd_workspace_bytes", n, V, d, K)
@@ -195,14 +196,15 @@ class _HeadLoss(torch.autograd.Function):
 
 # ---------------------------------------------------------------------------------------------------------------
 # the same as custom ops, for traces
-@torch.library.custom_op("pragnosia::head_loss", mutates_args=())
+@torch.library.custom_op("pragnosia_lm::head_loss", mutates_args=())
 def head_loss(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
               tau: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """h (n, d), W (V, d), y (n) or None, ids and z (n, K) or None. Returns (ce, lse, kd, stats), empty where there are
     no labels or no teacher; stats is what the backward takes."""
     _check_head("head_loss", h, W, y, ids, z, tau)
     got = _forward(*_operands(h, W, y, ids, z), float(tau))
-    return tuple(t if t is not None else torch.empty(0, device=h.device) for t in got)
+    types = (_F32, _F32, _F32, torch.int32)
+    return tuple(t if t is not None else torch.empty(0, device=h.device, dtype=dt) for t, dt in zip(got, types))
 
 
 @head_loss.register_fake
@@ -210,10 +212,10 @@ def _(h, W, y, ids, z, tau):
     n, K = h.shape[0], 0 if ids is None else ids.shape[1]
     e = lambda s: h.new_empty(s, dtype=_F32)
     ny, nk = (0 if y is None else n), (0 if ids is None else n)
-    return e(ny), e(ny), e(nk), e(nk * (2 + 3 * K))
+    return e(ny), e(ny), e(nk), h.new_empty(nk * (2 + 3 * K), dtype=torch.int32)
 
 
-@torch.library.custom_op("pragnosia::head_loss_bwd", mutates_args=())
+@torch.library.custom_op("pragnosia_lm::head_loss_bwd", mutates_args=())
 def head_loss_bwd(g_ce: Optional[Tensor], g_lse: Optional[Tensor], g_kd: Optional[Tensor], h: Tensor, W: Tensor,
                   y: Optional[Tensor], lse: Tensor, stats: Tensor, tau: float, need_h: bool,
                   need_W: bool) -> tuple[Tensor, Tensor]:
@@ -226,12 +228,12 @@ def head_loss_bwd(g_ce: Optional[Tensor], g_lse: Optional[Tensor], g_kd: Optiona
     _expect("head_loss_bwd", h.device, W=(W, (None, d)), g_ce=(g_ce, (n,)), g_lse=(g_lse, (n,)), g_kd=(g_kd, (n,)),
             y=(y, (n,)), lse=(lse if y is not None else None, (n,)), stats=(stats, (None,)))
     K = (stats.numel() // n - 2) // 3 if n and stats.numel() else 0
-    if stats.numel() not in (0, n * (2 + 3 * K)) or lse.dtype != _F32 or stats.dtype != _F32:
+    if stats.numel() not in (0, n * (2 + 3 * K)) or lse.dtype != _F32 or stats.dtype != torch.int32:
         raise PragnosiaError("head_loss_bwd: lse and stats must be head_loss's")
     if (y is None and (g_ce is not None or g_lse is not None)) or (K == 0 and g_kd is not None):
         raise PragnosiaError("head_loss_bwd: a gradient of a loss that was not computed")
     dh, dW = _backward(g_ce, g_lse, g_kd, _as(h, _BF16), _as(W, _BF16), _as(y, _I64),
-                       None if y is None else _as(lse, _F32), _as(stats, _F32) if K else None, K, float(tau), need_h,
+                       None if y is None else _as(lse, _F32), _as(stats, torch.int32) if K else None, K, float(tau), need_h,
                        need_W, W.dtype == _F32)
     return (h.new_empty(0, d) if dh is None else dh.to(h.dtype)), (W.new_empty(0, d) if dW is None else dW)
 

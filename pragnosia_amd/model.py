@@ -16,7 +16,10 @@ Constructor arguments, module names and initialisation follow the reference (`sr
 
 (`src/model.py:632-660`.) The mixers run on the HIP kernels: heads of 64 and 128 on the bf16 MFMA scans, other head
 widths on the exact fp32 scan (the plain rule at any width, the delta rule with keys up to 384; in chunks, short calls
-token by token in key and value blocks that fit the LDS). Embeddings, LayerNorms, the MLPs and the tied head are torch.
+token by token in key and value blocks that fit the LDS). Embeddings, LayerNorms, the MLPs and the tied head are torch;
+with fused_ends=True the two ends of a training step are kernels too: the lookups with a gradient by sorted tokens
+(`embed.embedding`), and the losses of the tied head without its logits (`head.linear_cross_entropy` in `loss`,
+`head.linear_distill` in `distill_loss`). The parameters and their names are the same either way.
 Attention, the hybrid stacks and the other reference mixers are outside this build and raise. `short_conv=K` adds every
 carrier's short causal convolution (`src/model.py:717-726`).
 """
@@ -29,6 +32,8 @@ import torch.utils.checkpoint
 
 from ._lib import PragnosiaError
 from .assoc import AssocCarrier
+from .embed import embedding
+from .head import linear_cross_entropy, linear_distill
 from .ops import capturing, layer_norm, linear
 from .spin import SpinCarrier
 
@@ -74,11 +79,19 @@ class Embedding(nn.Embedding):
     has not taken effect here on replays after the first; the step of 4 x 2048 tokens faulted in that kernel. So a
     capture (and a traced step, which may be captured later) of more indices selects rows by index, whose gradient is
     an indexed addition: the order of a row's fp32 sum then varies from replay to replay. An eager step, and any step
-    of fewer indices, is torch's."""
+    of fewer indices, is torch's.
 
+    With `sorted_grad` every lookup on the GPU, captured or not, is `embed.embedding`: the same rows, and a gradient summed
+    in fp32 over the tokens sorted by index, the same bits each time. An index outside the table then gives a zero row."""
+
+    sorted_grad = False
     SORTED_FROM = 3073  # indices from which torch's gradient takes the sort
 
     def forward(self, x):
+        if (self.sorted_grad and self.weight.is_cuda and self.weight.dtype in (torch.float32, torch.bfloat16)
+                and self.weight.shape[1] % 8 == 0 and self.padding_idx is None and self.max_norm is None
+                and not (self.scale_grad_by_freq or self.sparse)):
+            return embedding(x, self.weight)
         if (self.weight.is_cuda and x.numel() >= self.SORTED_FROM and torch.is_grad_enabled()
                 and self.padding_idx is None and self.max_norm is None
                 and not (self.scale_grad_by_freq or self.sparse) and capturing()):
@@ -88,13 +101,14 @@ class Embedding(nn.Embedding):
 
 class LM(nn.Module):
     def __init__(self, vocab=8192, d=768, layers=12, mlp_mult=4, ctx=512, mixer="aspin", norm="ln", short_conv=0,
-                 **unused):
+                 fused_ends=False, **unused):
         super().__init__()
         if mixer not in MIXERS:
             raise PragnosiaError(f"LM: mixer {mixer!r} is outside this build (supported: {sorted(MIXERS)})")
         self.vocab, self.d, self.layers, self.ctx, self.mixer, self.norm = vocab, d, layers, ctx, mixer, norm
         self.e = Embedding(vocab, d)
         self.p = Embedding(ctx, d)
+        self.fused_ends = self.e.sorted_grad = self.p.sorted_grad = bool(fused_ends)
         self.mix = nn.ModuleList([MIXERS[mixer](d) for _ in range(layers)])
         self.mlp = nn.ModuleList([MLP(d, mlp_mult) for _ in range(layers)])
         self.n = nn.LayerNorm(d)
@@ -158,7 +172,10 @@ class LM(nn.Module):
 
     def loss(self, h, y, chunks=4):
         """Mean cross-entropy of the tied head over (B, T) targets, the logits formed chunk by chunk under
-        activation checkpointing so at most one chunk's logits exist at a time."""
+        activation checkpointing so at most one chunk's logits exist at a time. With fused_ends the kernels of
+        `head.linear_cross_entropy`: no logits at all (`chunks` says nothing then)."""
+        if self.fused_ends and h.is_cuda:
+            return linear_cross_entropy(h, self.e.weight, y)[0].sum() / y.numel()
         hf, yf = h.reshape(-1, h.shape[-1]), y.reshape(-1)
         n = hf.shape[0]
 
@@ -175,6 +192,14 @@ class LM(nn.Module):
             total = total + torch.utils.checkpoint.checkpoint(piece, hf[sl], yf[sl], self.e.weight,
                                                               use_reentrant=False)
         return total / n
+
+    def distill_loss(self, h, ids, logits, tau=1.0, y=None):
+        """Mean distillation loss of the tied head over (B, T) tokens from a teacher's top logits, ids and logits
+        (B, T, K), at temperature tau; with targets y (B, T) also their mean cross-entropy, from the same pass over the
+        vocabulary: (distillation, cross-entropy or None). See `head.linear_distill`."""
+        kd, ce = linear_distill(h, self.e.weight, ids, logits, tau, y)
+        n = kd.numel()
+        return kd.sum() / n, None if ce is None else ce.sum() / n
 
     @torch.no_grad()
     def forward_carried(self, x, window=None):
