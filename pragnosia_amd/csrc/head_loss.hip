@@ -7,8 +7,8 @@
 // the product's rows), so a token's words lie in one lane's registers and the reduction is two lane exchanges a token.
 //
 // Backward: the logits are formed again per piece of the vocabulary, turned into dl in the accumulators and rounded to
-// bf16 (relative 2^-8 of each element, the gradient of a logit, the operands' own precision) into a workspace of the
-// piece's columns; dh += dl W and dW = dl^T h are products over it.
+// bf16 (the operands' own precision: relative 2^-8 at most of each element, over a common scale, see RowInfo) into a
+// workspace of the piece's columns; dh += dl W and dW = dl^T h are products over it.
 #include <algorithm>
 
 #include "../include/pragnosia_lm.h"
@@ -440,30 +440,63 @@ struct BwdIn {
   float tau;
 };
 
-// What dl takes of a row: dl = w0 exp(l scale0 - l0) + w1 exp(l scale1 - l1) - gc [v = label], the exponents in base 2;
-// zero where not live.
+// What dl takes of a row, over the common scale G: dl / G = w0 exp(l scale0 - l0) + w1 exp(l scale1 - l1) -
+// gc [v = label], the exponents in base 2; zero where not live.
+//
+// G is the largest of the rows' weights. A mean's rows all have the same weight w, and most of a row's gradient is its
+// label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same relative error, that of w's
+// bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and mostly much nearer, and the
+// products are multiplied by G in fp32.
 struct RowInfo {
   float w0, l0, w1, l1, gc;
   int32_t label, live, unused;
 };
 
-__global__ __launch_bounds__(256) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows, int64_t n,
-                                                 int64_t V) {
-  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (row >= n) return;
-  RowInfo o{};
-  const int64_t label = in.y != nullptr ? in.y[row] : -1;
-  const bool labelled = label >= 0 && label < V;
-  o.label = labelled ? (int32_t)label : -1;
-  o.gc = labelled && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
-  const float w_ce = o.gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f);
-  const float w_kd = in.g_kd != nullptr ? in.g_kd[row] * in.tau * in.psum[row] : 0.f;
-  o.w0 = second ? w_ce : w_ce + w_kd;
-  o.w1 = w_kd;
-  o.l0 = (in.lse != nullptr ? in.lse[row] : in.lse_t[row]) * kLog2e;
-  o.l1 = second ? in.lse_t[row] * kLog2e : 0.f;
-  o.live = w_ce != 0.f || w_kd != 0.f || o.gc != 0.f;
-  rows[row] = o;
+struct RowWeights {
+  float ce, kd, gc;
+  int64_t label;  // -1: none
+};
+
+PGN_DEVICE RowWeights row_weights(const BwdIn& in, int64_t row, int64_t V) {
+  RowWeights r;
+  r.label = in.y != nullptr ? in.y[row] : -1;
+  if (r.label < 0 || r.label >= V) r.label = -1;
+  r.gc = r.label >= 0 && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
+  r.ce = r.gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f);
+  r.kd = in.g_kd != nullptr ? in.g_kd[row] * in.tau * in.psum[row] : 0.f;
+  return r;
+}
+
+// Every workgroup finds G itself, from all rows (at most 256 workgroups, `each` rows of their own); *scale = G.
+__global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows,
+                                                  float* __restrict__ scale, int64_t n, int64_t V, int64_t each) {
+  __shared__ float most[16];
+  const int tid = threadIdx.x;
+  float g = 0.f;
+#pragma unroll 4
+  for (int64_t row = tid; row < n; row += 1024) {
+    const RowWeights r = row_weights(in, row, V);
+    g = fmaxf(g, fmaxf(fabsf(r.gc), fmaxf(fabsf(r.ce), fabsf(r.kd))));
+  }
+  for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
+  if ((tid & 63) == 0) most[tid >> 6] = g;
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) g = fmaxf(g, most[k]);
+  if (!(g > 0.f && g < INFINITY)) g = 1.f;
+  if (blockIdx.x == 0 && tid == 0) *scale = g;
+  const int64_t end = min(n, (int64_t)(blockIdx.x + 1) * each);
+  for (int64_t row = blockIdx.x * each + tid; row < end; row += 1024) {
+    const RowWeights r = row_weights(in, row, V);
+    RowInfo o{};
+    o.label = (int32_t)r.label;
+    o.gc = r.gc / g;
+    o.w0 = (second ? r.ce : r.ce + r.kd) / g;
+    o.w1 = r.kd / g;
+    o.l0 = (in.lse != nullptr ? in.lse[row] : in.lse_t[row]) * kLog2e;
+    o.l1 = second ? in.lse_t[row] * kLog2e : 0.f;
+    o.live = r.ce != 0.f || r.kd != 0.f || r.gc != 0.f;
+    rows[row] = o;
+  }
 }
 
 // Two adjacent accumulator tiles (rows 0 .. 15 and 16 .. 31 of a 32-row block; lane (i, g) holds rows 4 g .. 4 g + 3 of
@@ -478,7 +511,7 @@ PGN_DEVICE bf16x8 eight_rows(f32x4 lo, f32x4 hi) {
   return __builtin_bit_cast(bf16x8, i32x4{(int)p0, (int)q0, (int)p1, (int)q1});
 }
 
-// dl of a piece of the vocabulary: words v_begin .. v_begin + ld (whole tiles) of the workspace's n_pad rows (likewise).
+// dl / G of a piece of the vocabulary: words v_begin .. v_begin + ld (whole tiles) of the workspace's n_pad rows (likewise).
 // Word and token rows past the ends get zeros.
 template <class C, int NEXP>
 __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W, const RowInfo* __restrict__ rows,
@@ -541,31 +574,28 @@ __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W
       });
 }
 
-// dl at the teacher's entries, whole: a thread an entry.
-__global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const int32_t* __restrict__ entry,
-                                                     const float* __restrict__ p, const float* __restrict__ zl,
-                                                     __bf16* __restrict__ dl, int64_t ld, int64_t v_begin, int64_t n,
-                                                     int64_t V, int64_t K) {
+// dl / G at the teacher's entries, whole: a thread an entry.
+__global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const float* __restrict__ scale,
+                                                     const int32_t* __restrict__ entry, const float* __restrict__ p,
+                                                     const float* __restrict__ zl, __bf16* __restrict__ dl, int64_t ld,
+                                                     int64_t v_begin, int64_t words, int64_t n, int64_t V, int64_t K) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= n * K) return;
   const int64_t row = e / K;
   const int v = entry[e];
-  if (v < v_begin || v >= v_begin + ld) return;
-  const int64_t label = in.y != nullptr ? in.y[row] : -1;
-  const bool labelled = label >= 0 && label < V;
-  const float gc = labelled && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
-  const float w_ce = gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f), gk = in.g_kd[row] * in.tau;
+  if (v < v_begin || v >= v_begin + words) return;
+  const RowWeights r = row_weights(in, row, V);
   float x = 0.f;
-  if (w_ce != 0.f || gk != 0.f || gc != 0.f) {
-    const float l = zl[e];
-    x = gk * (in.psum[row] * expf(l / in.tau - in.lse_t[row]) - p[e]);
-    if (w_ce != 0.f) x += w_ce * expf(l - in.lse[row]);
-    if (label == v) x -= gc;
+  if (r.ce != 0.f || r.kd != 0.f || r.gc != 0.f) {
+    const float l = zl[e], g = *scale;
+    x = r.kd / g * (expf(l / in.tau - in.lse_t[row]) - p[e]);
+    if (r.ce != 0.f) x += r.ce / g * expf(l - in.lse[row]);
+    if (r.label == v) x -= r.gc / g;
   }
   dl[row * ld + (v - v_begin)] = (__bf16)x;
 }
 
-// dh = dl W over a piece and dW = dl^T h of the piece, in one launch; either whole, or as fp32 partial sums by range of
+// dh = G (dl / G) W over a piece and dW = G (dl / G)^T h of the piece, in one launch; either whole, or as fp32 partial sums by range of
 // the contracted dimension.
 struct GradSide {
   int64_t rows, k, len, split;  // output rows; contracted length, its ranges
@@ -577,7 +607,8 @@ struct GradArgs {
   Operand dl, W, h;  // dl by rows (n_pad); W's rows of the piece
   int64_t d;
   GradSide side[2];  // dh, dW
-  int first;         // the side whose items are longer, launched first
+  const float* scale;  // G
+  int first;           // the side whose items are longer, launched first
 };
 
 template <class C>
@@ -604,8 +635,11 @@ __global__ __launch_bounds__(C::kThreads) void head_grads(GradArgs q) {
         gemm_tile<C, true, true>(q.h, q.dl, x0, y0, k0, k1, smem, acc);
       const WaveIdx t = wave_idx();
       const int64_t c0 = x0 + 16 * C::NA * (t.w % C::WX);
+      const float g = *q.scale;
 #pragma unroll
       for (int b = 0; b < C::NB; ++b) {
+#pragma unroll
+        for (int a = 0; a < C::NA; ++a) acc[a][b] *= g;
         const int64_t row = y0 + 16 * C::NB * (t.w / C::WX) + 16 * b + t.i;
         if (s.part != nullptr || s.f32) {
           float* p = (s.part != nullptr ? s.part + (range * s.rows + row) * q.d : (float*)s.out + row * q.d);
@@ -745,7 +779,7 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
 extern "C" int64_t pragnosia_head_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!head_shape_ok(n, V, d, 0)) return -1;
   const GradPlan pl = choose_grads(n, V, d);
-  return pl.dl_bytes + pl.part_h + pl.part_w + n * (int64_t)sizeof(RowInfo);
+  return pl.dl_bytes + pl.part_h + pl.part_w + n * (int64_t)sizeof(RowInfo) + 16;
 }
 
 extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd, const void* h,
@@ -772,7 +806,9 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   __bf16* dl = (__bf16*)ws;
   float *part_h = (float*)(ws + pl.dl_bytes), *part_w = (float*)(ws + pl.dl_bytes + pl.part_h);
   RowInfo* rows = (RowInfo*)(ws + pl.dl_bytes + pl.part_h + pl.part_w);
-  hipLaunchKernelGGL(head_rows, dim3((unsigned)tiles(n, 256)), dim3(256), 0, st, in, second, rows, n, V);
+  float* scale = (float*)(rows + n);
+  const int64_t each = std::max<int64_t>(1024, tiles(n, 256));
+  hipLaunchKernelGGL(head_rows, dim3((unsigned)tiles(n, each)), dim3(1024), 0, st, in, second, rows, scale, n, V, each);
   for (int64_t q = 0; q < pl.pieces; ++q) {
     const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0);
     const int64_t ld = round_up(words, kLogitsKinds[pl.logits].x);
@@ -787,14 +823,14 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
     });
     if (rc) return rc;
     if (g_kd)
-      hipLaunchKernelGGL(head_entry_dl, dim3((unsigned)tiles(n * K, 256)), dim3(256), 0, st, in, entry, p, zl, dl, ld,
-                         v0, n, V, K);
+      hipLaunchKernelGGL(head_entry_dl, dim3((unsigned)tiles(n * K, 256)), dim3(256), 0, st, in, scale, entry, p, zl,
+                         dl, ld, v0, words, n, V, K);
     void* dW_q = dW == nullptr ? nullptr
                                : dw_f32 ? (void*)((float*)dW + v0 * d) : (void*)((__bf16*)dW + v0 * d);
     GradArgs ga{Operand{dl, ld, pl.n_pad}, Operand{Wo.p + v0 * d, d, words}, ho, d,
                 {{n, words, pl.len_h, pl.split_h, dh, pl.part_h ? part_h : nullptr, 0, q > 0},
                  {words, n, pl.len_w, pl.split_w, dW_q, pl.part_w ? part_w : nullptr, dw_f32, 0}},
-                pl.len_h >= pl.len_w ? 0 : 1};
+                scale, pl.len_h >= pl.len_w ? 0 : 1};
     rc = pl.kind == kLarge ? launch_grads<Large>(ga, st)
                            : pl.kind == kWide ? launch_grads<Wide>(ga, st) : launch_grads<Mid>(ga, st);
     if (rc) return rc;
