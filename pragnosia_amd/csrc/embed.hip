@@ -5,8 +5,8 @@
 // launch, sums in a second and joins long runs in a third:
 //
 //   sort  Every workgroup owns a range of ids. It reads all n ids (they stay in the L2), counts those below its range
-//         -- where its tokens start in the order -- and lists its own tokens in order of position; then places them by
-//         id. No workgroup waits for another.
+//         -- where its tokens start in the order -- and ranks its own by id and position; then places them. No
+//         workgroup waits for another.
 //   sum   An id with at most kShort tokens (most of a vocabulary, zeros where there is none) is summed by one thread a
 //         column vector, all its rows loaded at once. A longer run is summed in blocks of kBlock places of the order,
 //         four waves a block, its rows shared among them; what is left of a run that goes on in another block is a
@@ -20,7 +20,9 @@
 namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kList = 8192;  // tokens of a sorting workgroup's range that fit its LDS
+constexpr int kList = 6144;    // tokens of a sorting workgroup's range that fit its LDS
+constexpr int kHeld = 16;      // ids a thread of it keeps in registers
+constexpr int kMaxRange = 512;
 constexpr int kShort = 8;    // tokens of an id summed by one thread
 constexpr int kBlock = 64;   // places of the order summed by one workgroup: a lane each
 
@@ -62,54 +64,46 @@ __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ id
 }
 
 // Ids [blockIdx.x * range, ..): start[v] = the place of id v's first token in the order (start[V]: the number of tokens
-// with an id), order[place] = position, sorted[place] = id. list: n entries of scratch, for ranges past kList.
-// HELD: n <= 4 * 4 * kSortThreads, the ids stay in registers between the passes over them.
+// with an id), order[place] = position, sorted[place] = id. A wave reads a contiguous share of the ids in order and counts
+// its own tokens by id, so a token's place is its id's start, the counts of the waves before, and its rank in its wave.
+// list: n entries of scratch, for ranges with more than kList tokens. HELD: n <= kHeld kSortThreads, the ids stay in
+// registers between the two passes over them.
+struct Token {
+  int id, position, rank, wave;  // id relative to the range; rank among the wave's tokens of the id
+};
+
 template <bool HELD>
 __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __restrict__ ids, int32_t* __restrict__ order,
                                                            int32_t* __restrict__ sorted, int32_t* __restrict__ start,
-                                                           int2* __restrict__ list, int n, int V, int range) {
+                                                           Token* __restrict__ list, int n, int V, int range) {
   extern __shared__ __align__(16) unsigned char smem[];
-  int2* const near = reinterpret_cast<int2*>(smem);                            // (id - v0, position) of up to kList tokens
-  volatile int32_t* count = reinterpret_cast<int32_t*>(smem + 8 * kList);      // range: an id's tokens, then its next place
+  Token* const near = reinterpret_cast<Token*>(smem);
+  // wave w's tokens of id r at [w * range + r]; then the place of the first of them
+  int32_t* const count = reinterpret_cast<int32_t*>(smem + sizeof(Token) * kList);
   __shared__ int32_t waves[2][kSortWaves];
-  constexpr int kHeld = 4;
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  __shared__ int32_t first[kMaxRange];
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int v0 = blockIdx.x * range, v1 = min(V, v0 + range);
-  // a wave reads a contiguous share of the ids, in order, four a lane
-  const int share = ((n + kSortWaves - 1) / kSortWaves + 255) / 256 * 256, a = min(n, w * share), b = min(n, a + share);
-  auto load = [&](int i0) {
-    const int i = i0 + 4 * l;
-    i32x4 x = {-1, -1, -1, -1};
-    if (i + 4 <= b) {
-      x = *reinterpret_cast<const i32x4*>(ids + i);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (i + u < b) x[u] = ids[i + u];
-    }
-    return x;
-  };
-  i32x4 held[kHeld];
+  const int share = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64, a = min(n, w * share), b = min(n, a + share);
+  auto load = [&](int i0) { return i0 + l < b ? ids[i0 + l] : -1; };
+  int held[kHeld];
   int below = 0, mine = 0;
-  auto tally = [&](i32x4 x) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      below += x[u] >= 0 && x[u] < v0;
-      mine += x[u] >= v0 && x[u] < v1;
-    }
+  auto tally = [&](int x) {
+    below += x >= 0 && x < v0;
+    mine += x >= v0 && x < v1;
   };
   if constexpr (HELD) {
 #pragma unroll
-    for (int q = 0; q < kHeld; ++q) held[q] = load(a + 256 * q);
+    for (int q = 0; q < kHeld; ++q) held[q] = load(a + 64 * q);
 #pragma unroll
     for (int q = 0; q < kHeld; ++q) tally(held[q]);
   } else {
-#pragma unroll 4
-    for (int i0 = a; i0 < b; i0 += 256) tally(load(i0));
+#pragma unroll 8
+    for (int i0 = a; i0 < b; i0 += 64) tally(load(i0));
   }
   for (int o = 1; o < 64; o *= 2) below += __shfl_xor(below, o), mine += __shfl_xor(mine, o);
   if (l == 0) waves[0][w] = below, waves[1][w] = mine;
-  for (int r = tid; r < range; r += kSortThreads) count[r] = 0;
+  for (int r = tid; r < range * kSortWaves; r += kSortThreads) count[r] = 0;
   __syncthreads();
   int base = 0, at = 0, all = 0;
   for (int q = 0; q < kSortWaves; ++q) {
@@ -118,76 +112,77 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
     all += waves[1][q];
   }
   const bool fits = all <= kList;
-  int2* const far = list + base;
-  // the range's tokens in order of position, counted by id
-  auto append = [&](int i0, i32x4 x) {
-    bool in[4];
-    unsigned long long m[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) in[u] = x[u] >= v0 && x[u] < v1, m[u] = __ballot(in[u]);
-    if (!(m[0] | m[1] | m[2] | m[3])) return;
+  Token* const far = list + base;
+  volatile int32_t* const own = count + w * range;  // (written by one lane, read by all)
+  auto append = [&](int i0, int x) {
+    const bool in = x >= v0 && x < v1;
+    const unsigned long long m = __ballot(in);
+    if (m == 0) return;
     const unsigned long long lower = (1ull << l) - 1;
-    int to = at + __popcll(m[0] & lower) + __popcll(m[1] & lower) + __popcll(m[2] & lower) + __popcll(m[3] & lower);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (in[u]) {
-        const int2 e = {x[u] - v0, i0 + 4 * l + u};
-        if (fits)
-          near[to] = e;
-        else
-          far[to] = e;
-        ++to;
-        atomicAdd(const_cast<int32_t*>(&count[e.x]), 1);
-      }
-    at += __popcll(m[0]) + __popcll(m[1]) + __popcll(m[2]) + __popcll(m[3]);
+    int rank = 0;
+    for (unsigned long long left = m; left;) {
+      const int r = __builtin_amdgcn_readlane(x, __ffsll((long long)left) - 1) - v0;
+      const unsigned long long same = __ballot(in && x - v0 == r);
+      const int before = own[r];
+      if (in && x - v0 == r) rank = before + __popcll(same & lower);
+      own[r] = before + __popcll(same);
+      left &= ~same;
+    }
+    if (in) {
+      const Token e = {x - v0, i0 + l, rank, w};
+      const int to = at + __popcll(m & lower);
+      if (fits)
+        near[to] = e;
+      else
+        far[to] = e;
+    }
+    at += __popcll(m);
   };
   if constexpr (HELD) {
 #pragma unroll
-    for (int q = 0; q < kHeld; ++q)
-      if (a + 256 * q < b) append(a + 256 * q, held[q]);
+    for (int q = 0; q < kHeld; ++q) append(a + 64 * q, held[q]);
   } else {
-#pragma unroll 2
-    for (int i0 = a; i0 < b; i0 += 256) append(i0, load(i0));
+    int next = load(a);
+    for (int i0 = a; i0 < b; i0 += 64) {
+      const int x = next;
+      next = load(i0 + 64);
+      append(i0, x);
+    }
   }
   __syncthreads();
-  // places: an exclusive sum over the range's counts, by the first wave
+  // an id's tokens by wave: the counts of the waves before; and in all
+  if (tid < range) {
+    int s = 0;
+    for (int q = 0; q < kSortWaves; ++q) {
+      const int c = count[q * range + tid];
+      count[q * range + tid] = s;
+      s += c;
+    }
+    first[tid] = s;
+  }
+  __syncthreads();
+  // an exclusive sum over the ids, by the first wave
   if (w == 0) {
     int run = base;
     for (int r0 = 0; r0 < range; r0 += 64) {
-      const int c = r0 + l < range ? count[r0 + l] : 0;
+      const int c = r0 + l < range ? first[r0 + l] : 0;
       int s = c;
       for (int o = 1; o < 64; o *= 2) {
         const int t = __shfl_up(s, o);
         if (l >= o) s += t;
       }
-      if (r0 + l < range) count[r0 + l] = run + s - c;
+      if (r0 + l < range) first[r0 + l] = run + s - c;
       if (v0 + r0 + l < v1) start[v0 + r0 + l] = run + s - c;
       run += __shfl(s, 63);
     }
     if (l == 0 && v1 == V) start[V] = run;
   }
   __syncthreads();
-  // each id's tokens placed in order: a wave takes the ids of its residue
-  auto entry = [&](int i) { return i < all ? (fits ? near[i] : far[i]) : int2{-1, 0}; };
-  int2 next = entry(l);
-  for (int i0 = 0; i0 < all; i0 += 64) {
-    const int2 e = next;
-    next = entry(i0 + 64 + l);
-    bool todo = e.x >= 0 && e.x % kSortWaves == w;
-    unsigned long long left = __ballot(todo);
-    while (left) {
-      const int lead = __ffsll((long long)left) - 1, r = __shfl(e.x, lead);
-      const unsigned long long same = __ballot(todo && e.x == r);
-      const int place = count[r];
-      if (todo && e.x == r) {
-        const int to = place + __popcll(same & ((1ull << l) - 1));
-        order[to] = e.y;
-        sorted[to] = v0 + r;
-        todo = false;
-      }
-      if (l == lead) count[r] = place + __popcll(same);
-      left &= ~same;
-    }
+  for (int i = tid; i < all; i += kSortThreads) {
+    const Token e = fits ? near[i] : far[i];
+    const int to = first[e.id] + count[e.wave * range + e.id] + e.rank;
+    order[to] = e.position;
+    sorted[to] = v0 + e.id;
   }
 }
 
@@ -324,10 +319,10 @@ __global__ __launch_bounds__(256) void embed_join(const int32_t* __restrict__ so
   if (w == 0 && col < per) put_row<G>(dW + (int64_t)v * d + c, s, scale);
 }
 
-constexpr int64_t kMaxTokens = (int64_t)1 << 28;
+constexpr int64_t kMaxTokens = (int64_t)1 << 28;  // (sorting workgroups: V / 512)
 
-// Ids a sorting workgroup owns: about 256 workgroups (each reads all ids), their counters at most 16 KB.
-int64_t sort_range(int64_t V) { return std::min<int64_t>(std::max<int64_t>((V + 255) / 256, 32), 4096); }
+// Ids a sorting workgroup owns: about 256 workgroups (each reads all ids), their counters at most 32 KB.
+int64_t sort_range(int64_t V) { return std::min<int64_t>(std::max<int64_t>((V + 255) / 256, 32), kMaxRange); }
 
 bool embed_shape_ok(int64_t n, int64_t V, int64_t d) {
   return n >= 0 && n <= kMaxTokens && V > 0 && V <= kMaxTokens && d > 0 && d % 8 == 0 && d <= 65536 &&
@@ -352,13 +347,13 @@ int launch_rows(const int64_t* ids, const void* W, float scale, void* y, int32_t
 template <class G, class T>
 int launch_grad(const void* g, const int32_t* ids, float scale, void* dW, int32_t* ws, int64_t n, int64_t V, int64_t d,
                 hipStream_t st) {
-  int2* list = (int2*)ws;
-  int32_t *order = ws + 2 * up4(n), *sorted = order + up4(n), *start = sorted + up4(n);
+  Token* list = (Token*)ws;
+  int32_t *order = ws + 4 * up4(n), *sorted = order + up4(n), *start = sorted + up4(n);
   float* part = (float*)(start + up4(V + 1));
   const int range = (int)sort_range(V);
-  const auto sort = n <= 16 * kSortThreads ? embed_sort<true> : embed_sort<false>;
-  const int lds = 8 * kList + 4 * range;
-  const hipError_t e = pgn_lds_limit((const void*)sort, 8 * kList + 4 * 4096);
+  const auto sort = n <= kHeld * kSortThreads ? embed_sort<true> : embed_sort<false>;
+  const int lds = (int)sizeof(Token) * kList + 4 * kSortWaves * range;
+  const hipError_t e = pgn_lds_limit((const void*)sort, (int)sizeof(Token) * kList + 4 * kSortWaves * kMaxRange);
   if (e != hipSuccess) return (int)e;
   hipLaunchKernelGGL(sort, dim3((unsigned)((V + range - 1) / range)), dim3(kSortThreads), lds, st, ids, order, sorted,
                      start, list, (int)n, (int)V, range);
@@ -388,7 +383,7 @@ extern "C" int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16
 
 extern "C" int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!embed_shape_ok(n, V, d)) return -1;
-  return (4 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
+  return (6 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
 }
 
 extern "C" int pragnosia_embed_bwd(const void* g, int g_bf16, const int32_t* kept, float scale, void* dW, int w_bf16,

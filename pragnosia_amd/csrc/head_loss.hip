@@ -443,7 +443,7 @@ struct BwdIn {
 // What dl takes of a row, over the common scale G: dl / G = w0 exp(l scale0 - l0) + w1 exp(l scale1 - l1) -
 // gc [v = label], the exponents in base 2; zero where not live.
 //
-// G is the largest of the rows' weights. A mean's rows all have the same weight w, and most of a row's gradient is its
+// G is the largest of the rows' gradients. A mean's rows all have the same weight w, and most of a row's gradient is its
 // label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same relative error, that of w's
 // bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and mostly much nearer, and the
 // products are multiplied by G in fp32.
@@ -467,17 +467,27 @@ PGN_DEVICE RowWeights row_weights(const BwdIn& in, int64_t row, int64_t V) {
   return r;
 }
 
-// Every workgroup finds G itself, from all rows (at most 256 workgroups, `each` rows of their own); *scale = G.
+// The largest magnitude of x[0 .. n) that this thread of 1024 meets.
+PGN_DEVICE float thread_max(const float* __restrict__ x, int64_t n, int tid) {
+  float g = 0.f;
+#pragma unroll 2
+  for (int64_t k = 4 * tid; k + 4 <= n; k += 4096) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(x + k);
+    g = fmaxf(g, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+  }
+  if (tid < n % 4) g = fmaxf(g, fabsf(x[n - 1 - tid]));
+  return g;
+}
+
+// Every workgroup finds G itself, from all rows' gradients (at most 256 workgroups, `each` rows of their own); *scale = G.
 __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows,
                                                   float* __restrict__ scale, int64_t n, int64_t V, int64_t each) {
   __shared__ float most[16];
   const int tid = threadIdx.x;
   float g = 0.f;
-#pragma unroll 4
-  for (int64_t row = tid; row < n; row += 1024) {
-    const RowWeights r = row_weights(in, row, V);
-    g = fmaxf(g, fmaxf(fabsf(r.gc), fmaxf(fabsf(r.ce), fabsf(r.kd))));
-  }
+  if (in.g_ce != nullptr) g = thread_max(in.g_ce, n, tid);
+  if (in.g_lse != nullptr) g = fmaxf(g, thread_max(in.g_lse, n, tid));
+  if (in.g_kd != nullptr) g = fmaxf(g, in.tau * thread_max(in.g_kd, n, tid));
   for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
   if ((tid & 63) == 0) most[tid >> 6] = g;
   __syncthreads();
@@ -792,7 +802,7 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   PGN_CHECK_ARG(!(g_ce || g_lse) || lse);
   PGN_CHECK_ARG(!g_ce || y);
   PGN_CHECK_ARG(!g_kd || (K > 0 && lse_t && psum && entry && p && zl));
-  PGN_CHECK_ARG(g_ce || g_lse || g_kd);
+  PGN_CHECK_ARG((g_ce || g_lse || g_kd) && aligned(g_ce) && aligned(g_lse) && aligned(g_kd));
   PGN_CHECK_ARG(tau > 0.f && tau < INFINITY);
   PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_head_bwd_workspace_bytes(n, V, d));
   hipStream_t st = (hipStream_t)stream;
@@ -807,7 +817,7 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   float *part_h = (float*)(ws + pl.dl_bytes), *part_w = (float*)(ws + pl.dl_bytes + pl.part_h);
   RowInfo* rows = (RowInfo*)(ws + pl.dl_bytes + pl.part_h + pl.part_w);
   float* scale = (float*)(rows + n);
-  const int64_t each = std::max<int64_t>(1024, tiles(n, 256));
+  const int64_t each = std::max<int64_t>(256, tiles(n, 256));
   hipLaunchKernelGGL(head_rows, dim3((unsigned)tiles(n, each)), dim3(1024), 0, st, in, second, rows, scale, n, V, each);
   for (int64_t q = 0; q < pl.pieces; ++q) {
     const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0);
