@@ -39,27 +39,44 @@ struct Vec<__bf16> {
   typedef bf16x8 raw;
 };
 
-// y = scale W[id], one vector of 16 bytes of W a thread. kept: the ids in 32 bits, -1 outside the table, or null.
+// y = scale W[id], kRows vectors of 16 bytes of W a thread, a launch's width apart: their ids, then their rows in flight
+// together. kept: the ids in 32 bits, -1 outside the table, or null.
+constexpr int kRows = 4;
+
 template <class T, class O>
 __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ ids, const T* __restrict__ W, float scale,
                                                   O* __restrict__ y, int32_t* __restrict__ kept, int64_t n, int64_t V,
                                                   int d) {
   constexpr int N = Vec<T>::N;
+  typedef O out_t __attribute__((__vector_size__(N * sizeof(O))));
   const int per = d / N;
-  const int64_t total = n * per;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-    const int64_t i = e / per;
-    const int c = (int)(e - i * per) * N;
-    const int64_t id = ids[i];
-    typename Vec<T>::raw w{};
-    const bool in = id >= 0 && id < V;
-    if (kept != nullptr && c == 0) kept[i] = in ? (int32_t)id : -1;
-    if (in) w = *reinterpret_cast<const typename Vec<T>::raw*>(W + id * d + c);
-    typedef O out_t __attribute__((__vector_size__(N * sizeof(O))));
-    out_t o;
+  const int64_t total = n * per, width = (int64_t)gridDim.x * 256;
+  for (int64_t e0 = (int64_t)blockIdx.x * 256 + threadIdx.x; e0 < total; e0 += width * kRows) {
+    int64_t row[kRows], id[kRows];
+    int c[kRows];
+    typename Vec<T>::raw w[kRows];
 #pragma unroll
-    for (int u = 0; u < N; ++u) o[u] = in ? (O)(scale * (float)w[u]) : (O)0.f;
-    *reinterpret_cast<out_t*>(y + i * d + c) = o;
+    for (int u = 0; u < kRows; ++u) {
+      const int64_t e = min(e0 + u * width, total - 1);
+      row[u] = e / per;
+      c[u] = (int)(e - row[u] * per) * N;
+      id[u] = ids[row[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const bool in = id[u] >= 0 && id[u] < V;
+      if (!in) id[u] = -1;
+      w[u] = *reinterpret_cast<const typename Vec<T>::raw*>(W + (in ? id[u] : 0) * d + c[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      if (e0 + u * width >= total) continue;
+      if (kept != nullptr && c[u] == 0) kept[row[u]] = (int32_t)id[u];
+      out_t o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = id[u] >= 0 ? (O)(scale * (float)w[u][i]) : (O)0.f;
+      *reinterpret_cast<out_t*>(y + row[u] * d + c[u]) = o;
+    }
   }
 }
 
@@ -338,7 +355,7 @@ int64_t up4(int64_t x) { return (x + 3) / 4 * 4; }
 template <class T, class O>
 int launch_rows(const int64_t* ids, const void* W, float scale, void* y, int32_t* kept, int64_t n, int64_t V, int64_t d,
                 hipStream_t st) {
-  const int64_t blocks = (n * (d / Vec<T>::N) + 255) / 256;
+  const int64_t blocks = (n * (d / Vec<T>::N) + 256 * kRows - 1) / (256 * kRows);
   hipLaunchKernelGGL((embed_rows<T, O>), dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, st, ids,
                      (const T*)W, scale, (O*)y, kept, n, V, (int)d);
   PGN_RETURN_LAUNCH();
