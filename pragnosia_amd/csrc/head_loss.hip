@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
   for (int k = l; k < K; k += 64) {
     const int64_t id = ids[k];
     const bool on = id >= 0 && id < V;
-    const float x = on ? z[k] * inv_tau : -INFINITY;
+    const float x = on ? z[k] : -INFINITY;
     id_of[k] = on ? (int32_t)id : -1;
     p_of[k] = x;
     m = fmaxf(m, x);
@@ -169,12 +169,12 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
   const bool some = m > -INFINITY;
   float sum = 0.f;
   for (int k = l; k < K; k += 64)
-    if (some && id_of[k] >= 0) sum += expf(p_of[k] - m);
+    if (some && id_of[k] >= 0) sum += expf((p_of[k] - m) * inv_tau);
   for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
   const float inv = some ? 1.f / sum : 0.f, log_sum = some ? logf(sum) : 0.f;
   float e = 0.f;
   for (int k = l; k < K; k += 64) {
-    const float x = p_of[k] - m;
+    const float x = (p_of[k] - m) * inv_tau;
     const bool on = some && id_of[k] >= 0;
     const float pk = on ? expf(x) * inv : 0.f;
     if (!on) id_of[k] = -1;
@@ -716,7 +716,8 @@ bool head_shape_ok(int64_t n, int64_t V, int64_t d, int64_t K) {
   return n > 0 && n <= (int64_t)1 << 24 && V > 0 && V <= (int64_t)1 << 24 && d > 0 && d % 8 == 0 && d <= 65536 &&
          K >= 0 && K <= kMaxEntries &&
          // launches of fewer than 2^32 threads; tiles counted in 32 bits
-         n * K < (int64_t)1 << 31 && (K == 0 || tiles(n, 4) * (V * d >> 20) < (int64_t)1 << 23) && tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31;
+         n * K < (int64_t)1 << 31 && (K == 0 || tiles(n, 4) * (V * d >> 20) < (int64_t)1 << 23) && tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31 &&
+         tiles(std::max(n, V), Mid::Y) * tiles(d, Mid::X) < (int64_t)1 << 21;
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p % 16) == 0; }

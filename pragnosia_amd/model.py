@@ -173,8 +173,9 @@ class LM(nn.Module):
     def loss(self, h, y, chunks=4):
         """Mean cross-entropy of the tied head over (B, T) targets, the logits formed chunk by chunk under
         activation checkpointing so at most one chunk's logits exist at a time. With fused_ends the kernels of
-        `head.linear_cross_entropy`: no logits at all (`chunks` says nothing then)."""
-        if self.fused_ends and h.is_cuda:
+        `head.linear_cross_entropy`, for fp32 and bf16: no logits at all (`chunks` says nothing then)."""
+        low = (torch.float32, torch.bfloat16)
+        if self.fused_ends and h.is_cuda and h.dtype in low and self.e.weight.dtype in low and self.d % 8 == 0:
             return linear_cross_entropy(h, self.e.weight, y)[0].sum() / y.numel()
         hf, yf = h.reshape(-1, h.shape[-1]), y.reshape(-1)
         n = hf.shape[0]

@@ -70,3 +70,72 @@ def test_long_runs(kind):
     """A word that is most of a long batch: the whole order in one id's run, and in runs of every length."""
     g = torch.Generator().manual_seed(2)
     check(make_ids(kind, 70001, 1500, g).view(1, -1), 1500, 24, f32, f32)
+
+
+def test_strides_offsets_and_shapes():
+    """ids of any shape and integer type, a table inside a larger buffer at an odd offset, an expanded gradient."""
+    g = torch.Generator().manual_seed(3)
+    W = torch.randn(50 * 16 + 1, generator=g).cuda()[1:].view(50, 16).requires_grad_()
+    assert W.data_ptr() % 16
+    ids = torch.randint(0, 50, (7, 2, 3), generator=g).cuda()
+    dense = W.detach().clone().requires_grad_()
+    want, = torch.autograd.grad(embedding(ids.permute(2, 0, 1).reshape(-1), dense, 2.0).sum(), dense)
+    for t in (ids.permute(2, 0, 1), ids.permute(2, 0, 1).int(), ids.permute(2, 0, 1).to(torch.uint8)):
+        y = embedding(t, W, 2.0)
+        assert y.shape == (3, 7, 2, 16) and torch.equal(y, 2 * W[t.long()])
+        assert torch.equal(torch.autograd.grad(y.sum(), W)[0], want)
+    assert torch.equal(embedding(torch.tensor(3, device="cuda"), W), W[3])
+
+
+def test_nothing_to_do():
+    W = torch.randn(5, 8, device="cuda", requires_grad=True)
+    y = embedding(torch.zeros(0, 4, dtype=torch.long, device="cuda"), W)
+    assert y.shape == (0, 4, 8)
+    dW, = torch.autograd.grad(y.sum(), W)
+    assert dW.shape == W.shape and not dW.any()
+
+
+def test_infinities_stay_in_their_rows():
+    """A NaN or infinity in one token's gradient reaches its own id's row and no other; in a padding token's, none."""
+    ids = torch.tensor([3, 1, 3, -1, 7] * 9, device="cuda")
+    W = torch.zeros(9, 8, device="cuda", requires_grad=True)
+    gy = torch.ones(45, 8, device="cuda")
+    gy[3::5] = float("nan")
+    gy[1] = float("inf")
+    dW, = torch.autograd.grad(embedding(ids, W), W, gy)
+    assert torch.equal(dW[[0, 3, 7]], torch.tensor([0.0, 18.0, 9.0], device="cuda")[:, None].expand(3, 8))
+    assert torch.isinf(dW[1]).all()
+
+
+def test_streams_and_capture():
+    """Two gradients at once on streams of their own, and one captured and replayed on new ids: the eager call's bits."""
+    g = torch.Generator().manual_seed(4)
+    W = torch.randn(700, 64, generator=g).cuda().requires_grad_()
+    ids = [make_ids("zipf", n, 700, g).cuda() for n in (5000, 3000)]
+    gy = [torch.randn(i.shape[0], 64, generator=g).cuda() for i in ids]
+
+    def grad(i, q):
+        return torch.autograd.grad(embedding(i, W, 0.5), W, q)[0]
+
+    want = [grad(i, q) for i, q in zip(ids, gy)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ids]
+    got = []
+    for s, i, q in zip(streams * 3, ids * 3, gy * 3):
+        with torch.cuda.stream(s):
+            got.append(grad(i, q))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want * 3))
+    side = streams[0]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grad(ids[0], gy[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graph, held = torch.cuda.CUDAGraph(), ids[0].clone()
+    with torch.cuda.graph(graph):
+        out = grad(held, gy[0])
+    for _ in range(3):
+        held.copy_(make_ids("padded", 5000, 700, g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, grad(held.clone(), gy[0]))
