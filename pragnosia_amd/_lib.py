@@ -91,7 +91,7 @@ LM_SIGNATURES = {
     "pragnosia_head_bwd": [_p] * 12 + [_f32] + [_p] * 2 + [_i32, _p] + [_i64] * 5 + [_p],
     "pragnosia_embed_fwd": [_p, _p, _i32, _f32, _p, _i32, _p] + [_i64] * 3 + [_p],
     "pragnosia_embed_bwd_workspace_bytes": [_i64] * 3,
-    "pragnosia_embed_bwd": [_p, _i32, _p, _f32, _p, _i32, _p] + [_i64] * 4 + [_p],
+    "pragnosia_embed_bwd": [_p, _i32, _p, _i32, _f32, _p, _i32, _p] + [_i64] * 4 + [_p],
 }
 
 _LM_RET_I64 = {"pragnosia_head_fwd_workspace_bytes", "pragnosia_head_bwd_workspace_bytes",

@@ -12,6 +12,8 @@
 //         four waves a block, its rows shared among them; what is left of a run that goes on in another block is a
 //         partial row.
 //   join  A run's partial rows are added in order.
+//
+// A few tokens (kDirect) are one launch: a wave looks its ids up among all the tokens itself.
 #include <algorithm>
 
 #include "../include/pragnosia_lm.h"
@@ -23,6 +25,7 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kList = 6144;    // tokens of a sorting workgroup's range that fit its LDS
 constexpr int kHeld = 16;      // ids a thread of it keeps in registers
 constexpr int kMaxRange = 512;
+constexpr int kDirect = 256;   // tokens up to which a gradient is one launch (8 us for 256 of 8192 x 768 fp32; three take 17)
 constexpr int kShort = 8;    // tokens of an id summed by one thread
 constexpr int kBlock = 64;   // places of the order summed by one workgroup: a lane each
 
@@ -80,6 +83,9 @@ __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ id
   }
 }
 
+// An id in 32 bits, -1 outside the table.
+PGN_DEVICE int table_id(int64_t id, int64_t V) { return id >= 0 && id < V ? (int)id : -1; }
+
 // Ids [blockIdx.x * range, ..): start[v] = the place of id v's first token in the order (start[V]: the number of tokens
 // with an id), order[place] = position, sorted[place] = id. A wave reads a contiguous share of the ids in order and counts
 // its own tokens by id, so a token's place is its id's start, the counts of the waves before, and its rank in its wave.
@@ -89,8 +95,8 @@ struct Token {
   int id, position, rank, wave;  // id relative to the range; rank among the wave's tokens of the id
 };
 
-template <bool HELD>
-__global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __restrict__ ids, int32_t* __restrict__ order,
+template <bool HELD, class I>
+__global__ __launch_bounds__(kSortThreads) void embed_sort(const I* __restrict__ ids, int32_t* __restrict__ order,
                                                            int32_t* __restrict__ sorted, int32_t* __restrict__ start,
                                                            Token* __restrict__ list, int n, int V, int range) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -102,7 +108,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int v0 = blockIdx.x * range, v1 = min(V, v0 + range);
   const int share = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64, a = min(n, w * share), b = min(n, a + share);
-  auto load = [&](int i0) { return i0 + l < b ? ids[i0 + l] : -1; };
+  auto load = [&](int i0) { return i0 + l < b ? table_id(ids[i0 + l], V) : -1; };
   int held[kHeld];
   int below = 0, mine = 0;
   auto tally = [&](int x) {
@@ -336,6 +342,58 @@ __global__ __launch_bounds__(256) void embed_join(const int32_t* __restrict__ so
   if (w == 0 && col < per) put_row<G>(dW + (int64_t)v * d + c, s, scale);
 }
 
+// n <= kDirect tokens: a wave owns kOwn ids and 64 column vectors. A row's terms are added in the order of their positions.
+constexpr int kOwn = 8;
+
+template <class G, class T, class I>
+__global__ __launch_bounds__(256) void embed_direct(const G* __restrict__ g, const I* __restrict__ ids, float scale,
+                                                    T* __restrict__ dW, int n, int V, int d) {
+  constexpr int N = Vec<G>::N, U = 8;
+  __shared__ int32_t all[kDirect];
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), per = d / N;
+  if (tid < kDirect) all[tid] = tid < n ? table_id(ids[tid], V) : -1;
+  __syncthreads();
+  const int v0 = (blockIdx.x * 4 + w) * kOwn, col = blockIdx.y * 64 + l, c = min(col, per - 1) * N;
+  // which tokens are the wave's, a bit each
+  unsigned long long mine[kDirect / 64];
+  int x[kDirect / 64];
+#pragma unroll
+  for (int q = 0; q < kDirect / 64; ++q) {
+    x[q] = all[64 * q + l];
+    mine[q] = __ballot(x[q] >= v0 && x[q] < v0 + kOwn);
+  }
+  for (int r = 0; r < kOwn; ++r) {
+    const int v = v0 + r;
+    if (v >= V) return;
+    float s[N] = {};
+#pragma unroll
+    for (int q = 0; q < kDirect / 64; ++q) {
+      if (mine[q] == 0) continue;
+      unsigned long long left = __ballot(x[q] == v);
+      while (left) {
+        int at[U];
+        typename Vec<G>::raw y[U];
+        int k = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          at[u] = left ? 64 * q + __ffsll((long long)left) - 1 : -1;
+          k += left != 0;
+          left &= left - 1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < k) y[u] = *reinterpret_cast<const typename Vec<G>::raw*>(g + (int64_t)at[u] * d + c);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] += (float)y[u][i];
+      }
+    }
+    if (col < per) put_row<G>(dW + (int64_t)v * d + c, s, scale);
+  }
+}
+
 constexpr int64_t kMaxTokens = (int64_t)1 << 28;  // (sorting workgroups: V / 512)
 
 // Ids a sorting workgroup owns: about 256 workgroups (each reads all ids), their counters at most 32 KB.
@@ -361,27 +419,40 @@ int launch_rows(const int64_t* ids, const void* W, float scale, void* y, int32_t
   PGN_RETURN_LAUNCH();
 }
 
-template <class G, class T>
-int launch_grad(const void* g, const int32_t* ids, float scale, void* dW, int32_t* ws, int64_t n, int64_t V, int64_t d,
+template <class G, class T, class I>
+int launch_grad(const void* g, const I* ids, float scale, void* dW, int32_t* ws, int64_t n, int64_t V, int64_t d,
                 hipStream_t st) {
+  const int64_t per = d / Vec<G>::N, chunks = (per + 63) / 64, blocks = blocks_of(n);
+  if (n <= kDirect) {
+    hipLaunchKernelGGL((embed_direct<G, T, I>), dim3((unsigned)((V + 4 * kOwn - 1) / (4 * kOwn)), (unsigned)chunks),
+                       dim3(256), 0, st, (const G*)g, ids, scale, (T*)dW, (int)n, (int)V, (int)d);
+    PGN_RETURN_LAUNCH();
+  }
   Token* list = (Token*)ws;
   int32_t *order = ws + 4 * up4(n), *sorted = order + up4(n), *start = sorted + up4(n);
   float* part = (float*)(start + up4(V + 1));
   const int range = (int)sort_range(V);
-  const auto sort = n <= kHeld * kSortThreads ? embed_sort<true> : embed_sort<false>;
+  const auto sort = n <= kHeld * kSortThreads ? embed_sort<true, I> : embed_sort<false, I>;
   const int lds = (int)sizeof(Token) * kList + 4 * kSortWaves * range;
   const hipError_t e = pgn_lds_limit((const void*)sort, (int)sizeof(Token) * kList + 4 * kSortWaves * kMaxRange);
   if (e != hipSuccess) return (int)e;
   hipLaunchKernelGGL(sort, dim3((unsigned)((V + range - 1) / range)), dim3(kSortThreads), lds, st, ids, order, sorted,
                      start, list, (int)n, (int)V, range);
-  const int64_t per = d / Vec<G>::N, chunks = (per + 63) / 64, blocks = blocks_of(n);
   const int64_t whole = std::min<int64_t>((V * per + 255) / 256, 1 << 20);
   hipLaunchKernelGGL((embed_sum<G, T>), dim3((unsigned)(blocks * chunks + whole)), dim3(256), 0, st, (const G*)g, order,
                      sorted, start, scale, (T*)dW, part, (int)V, (int)d, (int)blocks, (int)chunks);
-  if (blocks > 1)
-    hipLaunchKernelGGL((embed_join<G, T>), dim3((unsigned)((blocks - 1) * chunks)), dim3(256), 0, st, sorted, start,
-                       scale, (T*)dW, part, (int)V, (int)d, (int)chunks);
+  hipLaunchKernelGGL((embed_join<G, T>), dim3((unsigned)((blocks - 1) * chunks)), dim3(256), 0, st, sorted, start, scale,
+                     (T*)dW, part, (int)V, (int)d, (int)chunks);
   PGN_RETURN_LAUNCH();
+}
+
+template <class I>
+int launch_grad_types(const void* g, int g_bf16, const I* ids, float scale, void* dW, int w_bf16, int32_t* ws, int64_t n,
+                      int64_t V, int64_t d, hipStream_t st) {
+  if (g_bf16) return w_bf16 ? launch_grad<__bf16, __bf16>(g, ids, scale, dW, ws, n, V, d, st)
+                            : launch_grad<__bf16, float>(g, ids, scale, dW, ws, n, V, d, st);
+  return w_bf16 ? launch_grad<float, __bf16>(g, ids, scale, dW, ws, n, V, d, st)
+                : launch_grad<float, float>(g, ids, scale, dW, ws, n, V, d, st);
 }
 
 }  // namespace
@@ -400,18 +471,17 @@ extern "C" int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16
 
 extern "C" int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!embed_shape_ok(n, V, d)) return -1;
-  return (6 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
+  return n <= kDirect ? 0 : (6 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
 }
 
-extern "C" int pragnosia_embed_bwd(const void* g, int g_bf16, const int32_t* kept, float scale, void* dW, int w_bf16,
-                                   void* workspace, int64_t workspace_bytes, int64_t n, int64_t V, int64_t d,
+extern "C" int pragnosia_embed_bwd(const void* g, int g_bf16, const void* ids, int ids_64, float scale, void* dW,
+                                   int w_bf16, void* workspace, int64_t workspace_bytes, int64_t n, int64_t V, int64_t d,
                                    void* stream) {
-  PGN_CHECK_ARG(embed_shape_ok(n, V, d) && dW && aligned(dW) && (n == 0 || (g && kept && aligned(g) && aligned(kept))));
-  PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_embed_bwd_workspace_bytes(n, V, d));
+  PGN_CHECK_ARG(embed_shape_ok(n, V, d) && dW && aligned(dW) && (n == 0 || (g && ids && aligned(g) && aligned(ids))));
+  const int64_t need = pragnosia_embed_bwd_workspace_bytes(n, V, d);
+  PGN_CHECK_ARG(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace))));
   hipStream_t st = (hipStream_t)stream;
   int32_t* ws = (int32_t*)workspace;
-  if (g_bf16) return w_bf16 ? launch_grad<__bf16, __bf16>(g, kept, scale, dW, ws, n, V, d, st)
-                            : launch_grad<__bf16, float>(g, kept, scale, dW, ws, n, V, d, st);
-  return w_bf16 ? launch_grad<float, __bf16>(g, kept, scale, dW, ws, n, V, d, st)
-                : launch_grad<float, float>(g, kept, scale, dW, ws, n, V, d, st);
+  return ids_64 ? launch_grad_types(g, g_bf16, (const int64_t*)ids, scale, dW, w_bf16, ws, n, V, d, st)
+                : launch_grad_types(g, g_bf16, (const int32_t*)ids, scale, dW, w_bf16, ws, n, V, d, st);
 }

@@ -443,7 +443,8 @@ struct BwdIn {
 // What dl takes of a row, over the common scale G: dl / G = w0 exp(l scale0 - l0) + w1 exp(l scale1 - l1) -
 // gc [v = label], the exponents in base 2; zero where not live.
 //
-// G is the largest of the rows' gradients. A mean's rows all have the same weight w, and most of a row's gradient is its
+// G is the largest of the rows' gradients of the cross entropy (of the distillation loss, where there is no label: a
+// teacher's probabilities are no constants, and round at random). A mean's rows all have the same weight w, and most of a row's gradient is its
 // label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same relative error, that of w's
 // bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and mostly much nearer, and the
 // products are multiplied by G in fp32.
@@ -485,13 +486,17 @@ __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo*
   __shared__ float most[16];
   const int tid = threadIdx.x;
   float g = 0.f;
-  if (in.g_ce != nullptr) g = thread_max(in.g_ce, n, tid);
-  if (in.g_lse != nullptr) g = fmaxf(g, thread_max(in.g_lse, n, tid));
-  if (in.g_kd != nullptr) g = fmaxf(g, in.tau * thread_max(in.g_kd, n, tid));
-  for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
-  if ((tid & 63) == 0) most[tid >> 6] = g;
-  __syncthreads();
-  for (int k = 0; k < 16; ++k) g = fmaxf(g, most[k]);
+  for (const float* x : {in.g_ce, in.g_kd, in.g_lse}) {
+    if (x == nullptr) continue;
+    g = thread_max(x, n, tid);
+    for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
+    __syncthreads();
+    if ((tid & 63) == 0) most[tid >> 6] = g;
+    __syncthreads();
+    for (int k = 0; k < 16; ++k) g = fmaxf(g, most[k]);
+    if (x == in.g_kd) g *= in.tau;
+    if (g > 0.f && g < INFINITY) break;
+  }
   if (!(g > 0.f && g < INFINITY)) g = 1.f;
   if (blockIdx.x == 0 && tid == 0) *scale = g;
   const int64_t end = min(n, (int64_t)(blockIdx.x + 1) * each);

@@ -41,31 +41,35 @@ def _forward(ids: Tensor, W: Tensor, scale: float, dtype: torch.dtype, kept: Opt
     return y
 
 
-def _backward(g: Tensor, kept: Tensor, V: int, scale: float, dtype: torch.dtype) -> Tensor:
-    """g (n, d), kept (n) int32 (ids, negative outside the table) -> dW (V, d) in `dtype`."""
+def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) -> Tensor:
+    """g (n, d), ids (n) int64 or int32 -> dW (V, d) in `dtype`."""
     g = _as(g, g.dtype)
     n, d = g.shape
     dW = torch.empty(V, d, device=g.device, dtype=dtype)
     nbytes = _workspace("pragnosia_embed_bwd_workspace_bytes", n, V, d)
-    ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
-    _call("pragnosia_embed_bwd", lm_lib().pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(kept), scale, _at(dW),
-          dtype == _BF16, _at(ws), nbytes, n, V, d)
+    ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8) if nbytes else None
+    _call("pragnosia_embed_bwd", lm_lib().pragnosia_embed_bwd, g, _at(g), g.dtype == _BF16, _at(ids), ids.dtype == _I64,
+          scale, _at(dW), dtype == _BF16, _at(ws), nbytes, n, V, d)
     return dW
+
+
+_KEPT_FROM = 16385  # tokens whose ids the sort reads twice: kept in 32 bits by the lookup
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, W, scale, dtype):
-        kept = torch.empty(ids.shape[0], device=W.device, dtype=torch.int32)
-        ctx.save_for_backward(kept)
+        ids, n = _as(ids, _I64), ids.shape[0]
+        kept = torch.empty(n, device=W.device, dtype=torch.int32) if n >= _KEPT_FROM else None
+        ctx.save_for_backward(ids if kept is None else kept)
         ctx.V, ctx.scale, ctx.dtype = W.shape[0], scale, W.dtype
-        return _forward(_as(ids, _I64), _as(W, W.dtype), scale, dtype, kept)
+        return _forward(ids, _as(W, W.dtype), scale, dtype, kept)
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        kept, = ctx.saved_tensors
-        return None, _backward(g, kept, ctx.V, ctx.scale, ctx.dtype), None, None
+        ids, = ctx.saved_tensors
+        return None, _backward(g, ids, ctx.V, ctx.scale, ctx.dtype), None, None
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -92,8 +96,7 @@ def embed_bwd(g: Tensor, ids: Tensor, V: int, scale: float, bf16: bool) -> Tenso
     if ids.dtype not in _INTS:
         raise PragnosiaError(f"embed_bwd: ids must be integers, got {ids.dtype}")
     _expect("embed_bwd", g.device, ids=(ids, (g.shape[0],)))
-    kept = torch.where((ids >= 0) & (ids < V), ids, -1).to(torch.int32)
-    return _backward(g, _as(kept, torch.int32), V, float(scale), _BF16 if bf16 else _F32)
+    return _backward(g, _as(ids, _I64), V, float(scale), _BF16 if bf16 else _F32)
 
 
 @embed_bwd.register_fake

@@ -53,16 +53,16 @@ int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd,
 
 /* ---------------------------------------------------------------------------------------------------------
  * Rows of a token table: y_i = scale W[ids_i], n rows; an id outside [0, V) gives a zero row. W (V, d) and y (n, d) fp32
- * or bf16 (w_bf16, y_bf16), d a multiple of 8; ids (n) int64. kept (n) int32 or NULL: the ids as the backward takes them
- * (-1 outside the table). n = 0 does nothing. Replaces nn.Embedding of src/model.py:822-826 (scale 1). */
+ * or bf16 (w_bf16, y_bf16), d a multiple of 8; ids (n) int64. kept (n) int32 or NULL: the ids in 32 bits for the
+ * backward, which then reads half as much (-1 outside the table). n = 0 does nothing. Replaces nn.Embedding of src/model.py:822-826 (scale 1). */
 int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16, int32_t* kept,
                         int64_t n, int64_t V, int64_t d, void* stream);
 
-/* Its gradient: dW[v] = scale sum of g_i over the tokens with kept_i = v, in fp32 in a fixed order, zero where there is
- * none; g (n, d) and dW (V, d) fp32 or bf16; kept's ids below V. No atomics on values, no memset: the same bits each
- * time, also in a captured step. */
+/* Its gradient: dW[v] = scale sum of g_i over the tokens with ids_i = v, in fp32 in a fixed order, zero where there is
+ * none; g (n, d) and dW (V, d) fp32 or bf16; ids (n) int64 (ids_64) or int32, ids outside the table taking no part. No
+ * atomics on values, no memset: the same bits each time, also in a captured step. No workspace up to 256 tokens. */
 int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d);
-int pragnosia_embed_bwd(const void* g, int g_bf16, const int32_t* kept, float scale, void* dW, int w_bf16,
+int pragnosia_embed_bwd(const void* g, int g_bf16, const void* ids, int ids_64, float scale, void* dW, int w_bf16,
                         void* workspace, int64_t workspace_bytes, int64_t n, int64_t V, int64_t d, void* stream);
 
 #ifdef __cplusplus

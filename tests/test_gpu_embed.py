@@ -53,7 +53,8 @@ def check(ids, V, d, wt, yt, gt_scale=1.0, scale=1.7, seed=0):
 
 
 @pytest.mark.parametrize("kind", ["uniform", "one", "zipf", "none", "padded"])
-@pytest.mark.parametrize("n,V,d", [(1, 1, 8), (33, 5, 8), (100, 40, 72), (1000, 257, 264), (5000, 20011, 64)])
+@pytest.mark.parametrize("n,V,d", [(1, 1, 8), (33, 5, 8), (100, 40, 72), (256, 100, 264), (257, 100, 264),
+                                   (1000, 257, 264), (5000, 20011, 64)])
 def test_values_and_gradient(kind, n, V, d):
     g = torch.Generator().manual_seed(n + V)
     check(make_ids(kind, n, V, g), V, d, f32, f32)

@@ -63,9 +63,9 @@ def test_embed_refuses(L):
         assert f(**bad) == -1, bad
     assert f(n=0, ids=null, y=null) == 0  # nothing to do
     b = lambda n=4, V=10, d=8, g=one, k=one, dW=one, ws=one, size=1 << 30: L.pragnosia_embed_bwd(
-        g, 0, k, 1.0, dW, 0, ws, size, n, V, d, null)
-    for bad in (dict(n=-1), dict(d=4), dict(g=null), dict(g=odd), dict(k=null), dict(dW=null), dict(ws=null),
-                dict(size=64)):
+        g, 0, k, 1, 1.0, dW, 0, ws, size, n, V, d, null)
+    for bad in (dict(n=-1), dict(d=4), dict(g=null), dict(g=odd), dict(k=null), dict(dW=null), dict(n=300, ws=null),
+                dict(n=300, size=64)):
         assert b(**bad) == -1, bad
 
 
@@ -73,6 +73,7 @@ def test_workspace_queries(L):
     assert L.pragnosia_head_fwd_workspace_bytes(0, 8, 8, 0) == -1
     assert L.pragnosia_head_bwd_workspace_bytes(8, 8, 9) == -1
     assert L.pragnosia_embed_bwd_workspace_bytes(8, 0, 8) == -1
+    assert L.pragnosia_embed_bwd_workspace_bytes(256, 8, 8) == 0 < L.pragnosia_embed_bwd_workspace_bytes(257, 8, 8)
     # the backward's space stays near its limit whatever the vocabulary, and grows with the tokens only by what they need
     for n, V, d in ((16384, 32768, 768), (8192, 262144, 1024), (100, 1 << 20, 512), (1, 1, 8)):
         assert 0 < L.pragnosia_head_bwd_workspace_bytes(n, V, d) < (512 << 20) + 16 * n * d
