@@ -1,20 +1,22 @@
-// A workgroup's bf16 matrix product over a tile of outputs, shared by the head's kernels: acc(x, y) = sum_k X(x, k) Y(y, k)
-// on v_mfma_f32_16x16x32_bf16, WX x WY waves of 16 NA x 16 NB outputs each.
+// A workgroup's bf16 matrix product over a tile of outputs, shared by the head's kernels: acc(x, y) = sum_k X(x, k)
+// Y(y, k) on v_mfma_f32_16x16x32_bf16, WX x WY waves of 16 NA x 16 NB outputs each.
 //
 // Either operand comes in one of two layouts: with the contracted index k running along its rows in memory (KR = false:
 // h, W or dl read along their rows), or down its rows (KR = true: the same matrices contracted over tokens or words).
 //
-// A step contracts 64 values of k, staged into one of NS LDS buffers straight from memory (buffer loads to LDS, 16 bytes
-// a lane). Step s, in a wave (its first half's fragments are in registers already):
+// A step contracts 64 values of k, staged into one of NS LDS buffers straight from memory (buffer loads to LDS, 16
+// bytes a lane). Step s, in a wave (its first half's fragments are in registers already):
 //     read the second half's fragments;  multiply the first half
 //     wait until stage s + 1 has arrived; barrier (every wave has read all of stage s)
 //     issue the loads of stage s + NS into the buffer of stage s;  read stage s + 1's first half;  multiply the second
-// so that fragment reads run beside products, one barrier a step, and a stage has NS - 1 steps to arrive. Reads and loads
-// are spread among the products by hand. Stages past the last are issued too, from offsets past the resource (zeros, no
-// memory traffic), so that the wait counts are constants.
+// so that fragment reads run beside products, one barrier a step, and a stage has NS - 1 steps to arrive. Reads and
+// loads are spread among the products by hand (reads first: 5% slower; in fewer groups: 0 - 4%). Measured with 256 x
+// 256 tiles at 8192^3: 1.33 - 1.36 PFLOP/s in every pair of layouts a tile a workgroup, 1.44 - 1.55 with a run of
+// tiles (gemm_tiles), the library's product 1.35 and 1.18. Stages past the last are issued too, from offsets past the
+// resource (zeros, no memory traffic), so that the wait counts are constants.
 //
-// A buffer load to LDS writes its 64 lanes' 16 bytes consecutively, so the arrangement against bank conflicts is made by
-// which 16 bytes each lane fetches:
+// A buffer load to LDS writes its 64 lanes' 16 bytes consecutively, so the arrangement against bank conflicts is made
+// by which 16 bytes each lane fetches:
 //   KR = false: an LDS row is one row's 64 k (128 bytes, eight segments of 16); segment s of row r holds k segment
 //     s ^ (r % 8).
 //   KR = true: an LDS row is one k's columns, in granules of 16 columns (32 bytes); granule s of row k holds granule
@@ -24,8 +26,9 @@
 // Both measured 240 - 250 bytes a clock and compute unit, the rate of consecutive reads. Within a 32-wide k block lane
 // group g holds k = 8 g .. 8 g + 7 of both operands.
 //
-// Range checks: a buffer resource covers exactly the rows that exist, so rows past the operand read as zero; a k segment
-// past the end of a row, or a column past it, is fetched from an offset past the resource (zero), whatever follows there.
+// Range checks: a buffer resource covers exactly the rows that exist, so rows past the operand read as zero; a k
+// segment past the end of a row, or a column past it, is fetched from an offset past the resource (zero), whatever
+// follows there.
 #pragma once
 #include "mfma_tile.h"
 
@@ -43,11 +46,12 @@ struct Operand {
   int64_t ld, rows;
 };
 
-// 16 bytes a lane from base + off (zero past `records` bytes) to LDS address lds + 16 lane; base, records and lds uniform.
-// As an instruction of its own, not the builtin: before a transposing LDS read the compiler waits for every load to LDS
-// that it knows of, which would leave a stage no time to arrive. No register is written, so nothing of the compiler's is
-// in flight; the arrival is waited for by wait_loads, and a wait for another access only becomes stricter by these. (The
-// s_nop covers the five wait states from a lane read into a scalar register to its use as a resource.)
+// 16 bytes a lane from base + off (zero past `records` bytes) to LDS address lds + 16 lane; base, records and lds
+// uniform. As an instruction of its own, not the builtin: before a transposing LDS read the compiler waits for every
+// load to LDS that it knows of, which would leave a stage no time to arrive. No register is written, so nothing of the
+// compiler's is in flight; the arrival is waited for by wait_loads, and a wait for another access only becomes
+// stricter by these. (The s_nop covers the five wait states from a lane read into a scalar register to its use as a
+// resource.)
 PGN_DEVICE void load_to_lds(const char* base, int records, int off, unsigned lds) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   const i32x4 r = {(int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xffffu), records, 0x00020000};
@@ -63,8 +67,8 @@ struct Stager {
   static constexpr int kBytes = R * kGemmK * 2;
   static constexpr int kLoads = kBytes / (T * 16);
   static constexpr int kRowBytes = KR ? 2 * R : 128;
-  // Rows that a load of all threads covers: where they are whole and the arrangement repeats after them, a lane's offset
-  // is the same for every load, from a base that moves by kLoadRows rows.
+  // Rows that a load of all threads covers: where they are whole and the arrangement repeats after them, a lane's
+  // offset is the same for every load, from a base that moves by kLoadRows rows.
   static constexpr int kLoadRows = T * 16 / kRowBytes;
   static constexpr bool kSame = T * 16 % kRowBytes == 0 && kLoadRows % 16 == 0;
   static constexpr int kOffs = kSame ? 1 : kLoads;
@@ -114,8 +118,8 @@ struct Stager {
     }
   }
 
-  // Stage s of the range [k_begin, k_end): aim() at it, then its kLoads loads into lds (wave w's share). A stage past the
-  // last loads nothing.
+  // Stage s of the range [k_begin, k_end): aim() at it, then its kLoads loads into lds (wave w's share). A stage past
+  // the last loads nothing.
   const char* at;
   int records, beyond;
   PGN_DEVICE void aim(int s, int64_t k_count) {
@@ -139,8 +143,8 @@ struct Stager {
 template <bool KR, int R>
 struct Reader {
   static constexpr int kRowBytes = KR ? 2 * R : 128;
-  // byte offsets; KR = false: in k block 0 (the other is 64 bytes away, by an exchange); KR = true: by granule within an
-  // aligned eight (or four)
+  // byte offsets; KR = false: in k block 0 (the other is 64 bytes away, by an exchange); KR = true: by granule within
+  // an aligned eight (or four)
   int at[KR ? 8 : 1];
 
   PGN_DEVICE void init(int x0, int g, int i) {
@@ -235,8 +239,8 @@ PGN_DEVICE void zero_acc(f32x4 (&acc)[C::NA][C::NB]) {
     for (int b = 0; b < C::NB; ++b) acc[a][b] = zero4();
 }
 
-// acc[a][b]: outputs x = x0 + 16 NA wx + 16 a + 4 g + r, y = y0 + 16 NB wy + 16 b + i of wave (wx, wy) = (w % WX, w / WX),
-// summed over k in [k_begin, k_end); for KR = false k_end <= ld.
+// acc[a][b]: outputs x = x0 + 16 NA wx + 16 a + 4 g + r, y = y0 + 16 NB wy + 16 b + i of wave (wx, wy) = (w % WX, w /
+// WX), summed over k in [k_begin, k_end); for KR = false k_end <= ld.
 template <class C, bool XKR, bool YKR>
 PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_t y0, int64_t k_begin, int64_t k_end,
                           unsigned char* lds, f32x4 (&acc)[C::NA][C::NB]) {
@@ -297,16 +301,16 @@ PGN_DEVICE XcdRun xcd_run(int items) {
   return {x * per + (int)blockIdx.x / kXcdCount, (int)gridDim.x / kXcdCount, min(items, (x + 1) * per)};
 }
 
-// The same for a run of tiles with both operands along their rows, k from 0 to d: the run's items (at least one), at(item,
-// ix, iy) giving their tiles, epilogue(acc, x0, y0, info) after each. The stages of the next
-// tile are under way while a tile's last steps and its epilogue run.
+// The same for a run of tiles with both operands along their rows, k from 0 to d: the run's items (at least one),
+// at(item, ix, iy) giving their tiles, epilogue(acc, x0, y0, info) after each. The stages of the next tile are under
+// way while a tile's last steps and its epilogue run.
 //
-// info: kInfo bytes of data of each of the tile's Y rows (row y's at rows + y kInfo, row_count of them; the rest reads as
-// zero), copied to LDS a tile ahead: into one of two places by the tile's parity, from a tile's first barrier on, when
-// the tile before, that place's last reader, is done; complete at the tile's own first barrier.
+// info: kInfo bytes of data of each of the tile's Y rows (row y's at rows + y kInfo, row_count of them; the rest reads
+// as zero), copied to LDS a tile ahead: into one of two places by the tile's parity, from a tile's first barrier on,
+// when the tile before, that place's last reader, is done; complete at the tile's own first barrier.
 //
-// kStores: how many stores every wave's epilogue issues, last of all. They need not have left before the next tile's first
-// stages are read: those loads were issued before them, and memory operations are counted in order.
+// kStores: how many stores every wave's epilogue issues, last of all. They need not have left before the next tile's
+// first stages are read: those loads were issued before them, and memory operations are counted in order.
 template <class C, int kInfo, int kStores, class At, class Epilogue>
 PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const void* rows, int64_t row_count,
                            const XcdRun& run, unsigned char* lds, At&& at, Epilogue&& epilogue) {
@@ -365,8 +369,8 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
     at(item, ix, iy);
     f32x4 acc[C::NA][C::NB];
     zero_acc<C>(acc);
-    // The first half of step s. Stage s + 1 has arrived at its end, and every wave's reads of stage s are done. The stages
-    // that were issued before the last epilogue's stores need not wait for those.
+    // The first half of step s. Stage s + 1 has arrived at its end, and every wave's reads of stage s are done. The
+    // stages that were issued before the last epilogue's stores need not wait for those.
     auto half = [&](int s) {
       f.template multiply<0, true, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
       if (steps < C::NS)  // the row data of this tile may be among the last loads

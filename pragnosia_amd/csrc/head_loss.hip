@@ -9,6 +9,12 @@
 // Backward: the logits are formed again per piece of the vocabulary, turned into dl in the accumulators and rounded to
 // bf16 (the operands' own precision: relative 2^-8 at most of each element, over a common scale, see RowInfo) into a
 // workspace of the piece's columns; dh += dl W and dW = dl^T h are products over it.
+//
+// Bounds. All large products here run at the card's power limit: on these operands' random values the clock falls to
+// about 1.8 GHz (2.3 on zeros), and taking stalls out of a kernel lowers the clock instead of the time. At 8192 tokens
+// x 8192 words x 768 (103 GFLOP a product): head_logits 94 us (1.1 PFLOP/s; the library's plain product of these
+// operands 92), head_dlogits 107 (the second exponential pass and 134 MB written), head_grads 165 for its two products
+// (1.25 PFLOP/s; the library's two 296). Few tokens are bound by launches: at 64 tokens every kernel takes 4 to 15 us.
 #include <algorithm>
 
 #include "../include/pragnosia_lm.h"
@@ -18,8 +24,8 @@ using namespace pgn;
 
 namespace {
 
-// Tiles of the logits (words x tokens), and of the gradients' products (columns of h or W x rows). A large one reaches the
-// matrix cores' rate; smaller ones fill the chip where there are few tokens (choose_logits, choose_grads).
+// Tiles of the logits (words x tokens), and of the gradients' products (columns of h or W x rows). A large one reaches
+// the matrix cores' rate; smaller ones fill the chip where there are few tokens (choose_logits, choose_grads).
 typedef Tile<8, 4, 2, 4, 2> Large;  // 256 x 256, 8 waves
 typedef Tile<6, 4, 2, 4, 2> Wide;   // 192 x 256, 8 waves: four cover widths of 704 and 768 with less left over
 typedef Tile<4, 4, 2, 2, 2> Mid;    // 128 x 128, 4 waves, two workgroups a compute unit
@@ -53,8 +59,8 @@ Kind choose_logits(int64_t n, int64_t V, int64_t d) {
   return best;
 }
 
-// The workspace of one piece's dl: about this many bytes at most (but 1024 words). It stays in the memory-side cache; half
-// of it costs 12 - 18% more time, twice or four times gain under 1%.
+// The workspace of one piece's dl: about this many bytes at most (but 1024 words). It stays in the memory-side cache;
+// half of it costs 12 - 18% more time, twice or four times gain under 1%.
 constexpr int64_t kPieceBytes = (int64_t)144 << 20;
 
 // How the gradients' products are laid out: the pieces of the vocabulary; the tile; the ranges that the contracted
@@ -137,9 +143,10 @@ PGN_DEVICE float column_max(float x) {
 }
 PGN_DEVICE float column_sum(float x) { return swap_add<32>(swap_add<16>(x, x), swap_add<16>(x, x)); }
 
-// ---------------------------------------------------------------------------------------------------------------
-// The teacher's distribution over its entries, a wave a row. A repeated id's probabilities are added into its first entry,
-// the others leave the list, so that every later kernel meets an id once.
+// --------------------------------------------------------------------------------------------------------------- The
+// teacher's distribution over its entries, a wave a row; bound by latency (8192 rows of 32 entries: 7 us). A repeated
+// id's probabilities are added into its first entry, the others leave the list, so that every later kernel meets an id
+// once.
 constexpr int kMaxEntries = 1024;
 constexpr int64_t kSliceBytes = (int64_t)2 << 20;
 
@@ -225,9 +232,10 @@ PGN_DEVICE float dot8(bf16x8 a, bf16x8 b, float s) {
   return s;
 }
 
-// The student's logits of the teacher's entries, zl[i][k] = h_i . W_entry: 16 lanes a row and slice of the vocabulary, two
-// entries at a time. Bound by the rows of W fetched (n K d values). An XCD takes every eighth slice, all rows of one before
-// the next, so that the words' rows stay in its L2 (a slice is at most 2 MB).
+// The student's logits of the teacher's entries, zl[i][k] = h_i . W_entry: 16 lanes a row and slice of the vocabulary,
+// two entries at a time. Bound by the rows of W fetched (n K d values). An XCD takes every eighth slice, all rows of
+// one before the next, so that the words' rows stay in its L2 (a slice is at most 2 MB): 8192 rows of 32 entries, 768
+// wide, 31 us, 13 TB/s of rows; without slices, a wave a row, 44.
 template <int CHUNKS>  // 128 values of d each, h's held in registers; 0: any d
 __global__ __launch_bounds__(256) void head_entry_logits(const __bf16* __restrict__ h, const __bf16* __restrict__ W,
                                                          const int32_t* __restrict__ entry, float* __restrict__ zl,
@@ -298,8 +306,9 @@ struct FwdOut {
   float* label;        // n: the label's logit (written only where the label is in range)
 };
 
-// Tiles of logits, reduced: a wave's words are one piece of its tokens' rows. NEXP sums of exponentials, of scale0 l and
-// scale1 l. y: labels, or null.
+// Tiles of logits, reduced: a wave's words are one piece of its tokens' rows. The exponentials and maxima of a tile
+// are 7% of its cycles, its twelve steps at d = 768 the rest. NEXP sums of exponentials, of scale0 l and scale1 l. y:
+// labels, or null.
 template <class C, int NEXP>
 __global__ __launch_bounds__(C::kThreads) void head_logits(Operand h, Operand W, const int64_t* __restrict__ y,
                                                            float scale0, float scale1, FwdOut out, int64_t d) {
@@ -368,8 +377,9 @@ __global__ __launch_bounds__(C::kThreads) void head_logits(Operand h, Operand W,
       });
 }
 
-// Rows' pieces joined: R rows a workgroup, T = 256 / R threads a row (thread R q + r: every T-th piece of row r from q),
-// each in one pass with a running maximum. Few rows take more threads each.
+// Rows' pieces joined: R rows a workgroup, T = 256 / R threads a row (thread R q + r: every T-th piece of row r from
+// q), each in one pass with a running maximum. Few rows take more threads each (7 rows of 256 pieces: 9 us with 16
+// threads a row, 4 with 64; 8192 rows of 64 pieces: 5.5 us with 16).
 struct JoinArgs {
   const int64_t* y;
   float *ce, *lse;
@@ -444,10 +454,10 @@ struct BwdIn {
 // gc [v = label], the exponents in base 2; zero where not live.
 //
 // G is the largest of the rows' gradients of the cross entropy (of the distillation loss, where there is no label: a
-// teacher's probabilities are no constants, and round at random). A mean's rows all have the same weight w, and most of a row's gradient is its
-// label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same relative error, that of w's
-// bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and mostly much nearer, and the
-// products are multiplied by G in fp32.
+// teacher's probabilities are no constants, and round at random). A mean's rows all have the same weight w, and most
+// of a row's gradient is its label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same
+// relative error, that of w's bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and
+// mostly much nearer, and the products are multiplied by G in fp32.
 struct RowInfo {
   float w0, l0, w1, l1, gc;
   int32_t label, live, unused;
@@ -480,7 +490,8 @@ PGN_DEVICE float thread_max(const float* __restrict__ x, int64_t n, int tid) {
   return g;
 }
 
-// Every workgroup finds G itself, from all rows' gradients (at most 256 workgroups, `each` rows of their own); *scale = G.
+// Every workgroup finds G itself (4 us at 8192 rows, launch and latency), from all rows' gradients (at most 256
+// workgroups, `each` rows of their own); *scale = G.
 __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows,
                                                   float* __restrict__ scale, int64_t n, int64_t V, int64_t each) {
   __shared__ float most[16];
@@ -514,9 +525,9 @@ __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo*
   }
 }
 
-// Two adjacent accumulator tiles (rows 0 .. 15 and 16 .. 31 of a 32-row block; lane (i, g) holds rows 4 g .. 4 g + 3 of
-// column i of both) rounded to bf16, exchanged between lane groups so that a lane ends with eight consecutive rows of its
-// column, first_of(g) ..: one 16-byte store, 64 bytes a column.
+// Two adjacent accumulator tiles (rows 0 .. 15 and 16 .. 31 of a 32-row block; lane (i, g) holds rows 4 g .. 4 g + 3
+// of column i of both) rounded to bf16, exchanged between lane groups so that a lane ends with eight consecutive rows
+// of its column, first_of(g) ..: one 16-byte store, 64 bytes a column.
 PGN_DEVICE int first_of(int g) { return 16 * (g & 1) + 8 * (g >> 1); }
 PGN_DEVICE bf16x8 eight_rows(f32x4 lo, f32x4 hi) {
   const i32x2 x = __builtin_bit_cast(i32x2, to_bf16x4(lo)), y = __builtin_bit_cast(i32x2, to_bf16x4(hi));
@@ -526,8 +537,8 @@ PGN_DEVICE bf16x8 eight_rows(f32x4 lo, f32x4 hi) {
   return __builtin_bit_cast(bf16x8, i32x4{(int)p0, (int)q0, (int)p1, (int)q1});
 }
 
-// dl / G of a piece of the vocabulary: words v_begin .. v_begin + ld (whole tiles) of the workspace's n_pad rows (likewise).
-// Word and token rows past the ends get zeros.
+// dl / G of a piece of the vocabulary: words v_begin .. v_begin + ld (whole tiles) of the workspace's n_pad rows
+// (likewise). Word and token rows past the ends get zeros.
 template <class C, int NEXP>
 __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W, const RowInfo* __restrict__ rows,
                                                             float scale0, float scale1, __bf16* __restrict__ dl,
@@ -589,7 +600,8 @@ __global__ __launch_bounds__(C::kThreads) void head_dlogits(Operand h, Operand W
       });
 }
 
-// dl / G at the teacher's entries, whole: a thread an entry.
+// dl / G at the teacher's entries, whole: a thread an entry, from the fp32 logit, so rounded once. Scattered two-byte
+// stores: 6 us for 8192 x 32.
 __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const float* __restrict__ scale,
                                                      const int32_t* __restrict__ entry, const float* __restrict__ p,
                                                      const float* __restrict__ zl, __bf16* __restrict__ dl, int64_t ld,
@@ -610,8 +622,9 @@ __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const float* __re
   dl[row * ld + (v - v_begin)] = (__bf16)x;
 }
 
-// dh = G (dl / G) W over a piece and dW = G (dl / G)^T h of the piece, in one launch; either whole, or as fp32 partial sums by range of
-// the contracted dimension.
+// dh = G (dl / G) W over a piece and dW = G (dl / G)^T h of the piece, in one launch; either whole, or as fp32 partial
+// sums by range of the contracted dimension. One launch, so that neither's last tiles leave the chip idle: at 8192 x
+// 8192 x 768 it is 256 workgroups of 192 x 256 for 256 compute units.
 struct GradSide {
   int64_t rows, k, len, split;  // output rows; contracted length, its ranges
   void* out;                    // rows x d, where one range is all
@@ -721,7 +734,8 @@ bool head_shape_ok(int64_t n, int64_t V, int64_t d, int64_t K) {
   return n > 0 && n <= (int64_t)1 << 24 && V > 0 && V <= (int64_t)1 << 24 && d > 0 && d % 8 == 0 && d <= 65536 &&
          K >= 0 && K <= kMaxEntries &&
          // launches of fewer than 2^32 threads; tiles counted in 32 bits
-         n * K < (int64_t)1 << 31 && (K == 0 || tiles(n, 4) * (V * d >> 20) < (int64_t)1 << 23) && tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31 &&
+         n * K < (int64_t)1 << 31 && (K == 0 || tiles(n, 4) * (V * d >> 20) < (int64_t)1 << 23) &&
+         tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31 &&
          tiles(std::max(n, V), Mid::Y) * tiles(d, Mid::X) < (int64_t)1 << 21;
 }
 
@@ -761,13 +775,15 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
   float* ent = f + (3 * pieces + 1) * n;
   const Operand ho{(const __bf16*)h, d, n}, Wo{(const __bf16*)W, d, V};
   if (K > 0) {
-    hipLaunchKernelGGL(head_teacher, dim3((unsigned)tiles(n, 4)), dim3(256), (unsigned)(4 * 8 * round_up(K, 4)), st, ids, z,
-                       1.f / tau, entry, p, psum, ent, zl, n, V, (int)K);
+    hipLaunchKernelGGL(head_teacher, dim3((unsigned)tiles(n, 4)), dim3(256), (unsigned)(4 * 8 * round_up(K, 4)), st,
+                       ids, z, 1.f / tau, entry, p, psum, ent, zl, n, V, (int)K);
     // slices of at most 2 MB of W, eight a turn
     const int64_t turns = tiles(V * d * 2, kXcdCount * kSliceBytes), blocks = tiles(n, 16);
     const int64_t slice = tiles(V, kXcdCount * turns);
-    const auto fn = d <= 512 ? head_entry_logits<4>
-                             : d <= 768 ? head_entry_logits<6> : d <= 1024 ? head_entry_logits<8> : head_entry_logits<0>;
+    const auto fn = d <= 512    ? head_entry_logits<4>
+                    : d <= 768  ? head_entry_logits<6>
+                    : d <= 1024 ? head_entry_logits<8>
+                                : head_entry_logits<0>;
     hipLaunchKernelGGL(fn, dim3((unsigned)(kXcdCount * turns * blocks)), dim3(256), 0, st, ho.p, Wo.p, entry, zl, n,
                        (int)d, (int)K, (int)blocks, (int)slice);
   }
