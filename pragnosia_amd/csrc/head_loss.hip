@@ -143,11 +143,12 @@ PGN_DEVICE float column_max(float x) {
 }
 PGN_DEVICE float column_sum(float x) { return swap_add<32>(swap_add<16>(x, x), swap_add<16>(x, x)); }
 
-// --------------------------------------------------------------------------------------------------------------- The
-// teacher's distribution over its entries, a wave a row; bound by latency (8192 rows of 32 entries: 7 us). A repeated
-// id's probabilities are added into its first entry, the others leave the list, so that every later kernel meets an id
-// once.
+// ---------------------------------------------------------------------------------------------------------------
+// The teacher's distribution over its entries, a wave a row; bound by latency (8192 rows of 32 entries: 7 us). A
+// repeated id's probabilities are added into its first entry, the others leave the list, so that every later kernel
+// meets an id once.
 constexpr int kMaxEntries = 1024;
+constexpr float kTauLeast = 0x1p-10f;
 constexpr int64_t kSliceBytes = (int64_t)2 << 20;
 
 __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ ids, const float* __restrict__ z,
@@ -164,6 +165,7 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
   float* const p_of = reinterpret_cast<float*>(id_of + K4);
   ids += row * K, z += row * K, entry += row * K, p += row * K, zl += row * K;
   float m = -INFINITY;
+  bool nan = false;
   for (int k = l; k < K; k += 64) {
     const int64_t id = ids[k];
     const bool on = id >= 0 && id < V;
@@ -171,9 +173,11 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
     id_of[k] = on ? (int32_t)id : -1;
     p_of[k] = x;
     m = fmaxf(m, x);
+    nan = nan || x != x;
   }
   for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-  const bool some = m > -INFINITY;
+  if (__ballot(nan)) m = NAN;  // (a maximum passes over it; the row's probabilities and loss are NaN)
+  const bool some = m != -INFINITY;
   float sum = 0.f;
   for (int k = l; k < K; k += 64)
     if (some && id_of[k] >= 0) sum += expf((p_of[k] - m) * inv_tau);
@@ -186,7 +190,7 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
     const float pk = on ? expf(x) * inv : 0.f;
     if (!on) id_of[k] = -1;
     p_of[k] = pk;
-    if (pk > 0.f) e += pk * (x - log_sum);
+    if (pk != 0.f) e += pk * (x - log_sum);
   }
   for (int o = 1; o < 64; o *= 2) e += __shfl_xor(e, o);
   if (l == 0) {
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(256) void head_join(FwdOut in, JoinArgs j) {
     const int64_t at = min((int64_t)blockIdx.x * R + tid / T, n - 1) * j.K;
     for (int64_t k = tid % T; k < j.K; k += T) {
       const float pk = j.p[at + k];
-      if (pk > 0.f) dot += pk * j.zl[at + k];
+      if (pk != 0.f) dot += pk * j.zl[at + k];
     }
   }
   part[0][tid] = m, part[1][tid] = s0, part[2][tid] = s1, part[3][tid] = dot;
@@ -735,7 +739,7 @@ bool head_shape_ok(int64_t n, int64_t V, int64_t d, int64_t K) {
          K >= 0 && K <= kMaxEntries &&
          // launches of fewer than 2^32 threads; tiles counted in 32 bits
          n * K < (int64_t)1 << 31 && (K == 0 || tiles(n, 4) * (V * d >> 20) < (int64_t)1 << 23) &&
-         tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 31 &&
+         tiles(n, Small::Y) * tiles(V, Small::X) < (int64_t)1 << 30 &&
          tiles(std::max(n, V), Mid::Y) * tiles(d, Mid::X) < (int64_t)1 << 21;
 }
 
@@ -766,7 +770,7 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
   PGN_CHECK_ARG(!y || (ce && lse));
   PGN_CHECK_ARG((ids != nullptr) == (K > 0) && (z != nullptr) == (K > 0));
   PGN_CHECK_ARG(K == 0 || (kd && lse_t && psum && entry && p && zl));
-  PGN_CHECK_ARG(tau > 0.f && tau < INFINITY);
+  PGN_CHECK_ARG(tau >= kTauLeast && tau <= 1.f / kTauLeast);
   PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_head_fwd_workspace_bytes(n, V, d, K));
   hipStream_t st = (hipStream_t)stream;
   const int64_t pieces = head_pieces(n, V, d);
@@ -825,7 +829,7 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   PGN_CHECK_ARG(!g_ce || y);
   PGN_CHECK_ARG(!g_kd || (K > 0 && lse_t && psum && entry && p && zl));
   PGN_CHECK_ARG((g_ce || g_lse || g_kd) && aligned(g_ce) && aligned(g_lse) && aligned(g_kd));
-  PGN_CHECK_ARG(tau > 0.f && tau < INFINITY);
+  PGN_CHECK_ARG(tau >= kTauLeast && tau <= 1.f / kTauLeast);
   PGN_CHECK_ARG(workspace && aligned(workspace) && workspace_bytes >= pragnosia_head_bwd_workspace_bytes(n, V, d));
   hipStream_t st = (hipStream_t)stream;
   const GradPlan pl = choose_grads(n, V, d);

@@ -1,5 +1,6 @@
 """The head's losses over the vocabulary, with no logits kept: cross entropy of labels and distillation from a teacher's
-top logits, forward and backward on hand-written kernels (csrc/head_loss.hip; C ABI in pragnosia_amd/include/pragnosia_lm.h).
+top logits, forward and backward on hand-written kernels (csrc/head_loss.hip; C ABI in
+pragnosia_amd/include/pragnosia_lm.h).
 
     loss, lse = linear_cross_entropy(h, W, y)
     kd, ce = linear_distill(h, W, ids, logits, tau, y)
@@ -32,10 +33,11 @@ from .ops import _expect, _require_gpu
 _FLOATS = (torch.bfloat16, torch.float32)
 _INTS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 _F32, _BF16, _I64 = torch.float32, torch.bfloat16, torch.int64
+_TAU = (2.0 ** -10, 2.0 ** 10)  # past these tau^2 kd or the scaled logits' rounding leaves little of an fp32 loss
 
 
 def _as(t: Optional[Tensor], dtype: torch.dtype) -> Optional[Tensor]:
-    """t in `dtype`, contiguous, at an address the kernels' 16-byte loads take (a slice of a buffer may start anywhere)."""
+    """t in `dtype`, contiguous, at an address the kernels' 16-byte loads take (a slice may start anywhere)."""
     if t is None:
         return None
     if t.dtype != dtype or not t.is_contiguous():
@@ -96,7 +98,7 @@ def _plain_call(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor]
         return y is not None and z is None
     return (z is not None and ids.device == dev and z.device == dev and ids.dtype is _I64 and z.dtype is _F32
             and ids.dim() == 2 and ids.shape[0] == n and 0 < ids.shape[1] <= 1024 and z.shape == ids.shape
-            and 0 < tau < math.inf)
+            and _TAU[0] <= tau <= _TAU[1])
 
 
 def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor],
@@ -119,10 +121,10 @@ def _check_head(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optiona
     if ids is not None:
         _expect(op, h.device, logits=(z, tuple(ids.shape)))
         if not 0 < ids.shape[1] <= 1024 or not z.is_floating_point():
-            raise PragnosiaError(f"{op}: ids and logits (..., K) with K from 1 to 1024 and floating logits expected, got "
-                                 f"{tuple(ids.shape)} and {z.dtype}")
-    if not (tau > 0 and math.isfinite(tau)):
-        raise PragnosiaError(f"{op}: tau must be positive and finite, got {tau}")
+            raise PragnosiaError(f"{op}: ids and logits (..., K) with K from 1 to 1024 and floating logits expected, "
+                                 f"got {tuple(ids.shape)} and {z.dtype}")
+    if not _TAU[0] <= tau <= _TAU[1]:
+        raise PragnosiaError(f"{op}: tau must be from {_TAU[0]} to {_TAU[1]}, got {tau}")
 
 
 def _forward(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z: Optional[Tensor], tau: float):
@@ -138,8 +140,8 @@ def _forward(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], z
         return ce, lse, kd, stats
     nbytes = _workspace("pragnosia_head_fwd_workspace_bytes", n, V, d, K)
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-    _call("pragnosia_head_fwd", lm_lib().pragnosia_head_fwd, h, _at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce), _at(lse),
-          _at(kd), *_stats_at(stats, n, K), _at(ws), nbytes, n, V, d, K)
+    _call("pragnosia_head_fwd", lm_lib().pragnosia_head_fwd, h, _at(h), _at(W), _at(y), _at(ids), _at(z), tau, _at(ce),
+          _at(lse), _at(kd), *_stats_at(stats, n, K), _at(ws), nbytes, n, V, d, K)
     return ce, lse, kd, stats
 
 
@@ -164,8 +166,8 @@ def _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, K: int, tau: float, need_h
     g_ce, g_lse, g_kd = _as(g_ce, _F32), _as(g_lse, _F32), _as(g_kd, _F32)
     nbytes = _workspace("pragnosia_head_bwd_workspace_bytes", n, V, d)
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-    _call("pragnosia_head_bwd", lm_lib().pragnosia_head_bwd, h, _at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W), _at(y),
-          _at(lse), *_stats_at(stats, n, K), tau, _at(dh), _at(dW), dw_f32, _at(ws), nbytes, n, V, d, K)
+    _call("pragnosia_head_bwd", lm_lib().pragnosia_head_bwd, h, _at(g_ce), _at(g_lse), _at(g_kd), _at(h), _at(W),
+          _at(y), _at(lse), *_stats_at(stats, n, K), tau, _at(dh), _at(dW), dw_f32, _at(ws), nbytes, n, V, d, K)
     return dh, dW
 
 
@@ -233,8 +235,8 @@ def head_loss_bwd(g_ce: Optional[Tensor], g_lse: Optional[Tensor], g_kd: Optiona
     if (y is None and (g_ce is not None or g_lse is not None)) or (K == 0 and g_kd is not None):
         raise PragnosiaError("head_loss_bwd: a gradient of a loss that was not computed")
     dh, dW = _backward(g_ce, g_lse, g_kd, _as(h, _BF16), _as(W, _BF16), _as(y, _I64),
-                       None if y is None else _as(lse, _F32), _as(stats, torch.int32) if K else None, K, float(tau), need_h,
-                       need_W, W.dtype == _F32)
+                       None if y is None else _as(lse, _F32), _as(stats, torch.int32) if K else None, K, float(tau),
+                       need_h, need_W, W.dtype == _F32)
     return (h.new_empty(0, d) if dh is None else dh.to(h.dtype)), (W.new_empty(0, d) if dW is None else dW)
 
 
@@ -304,10 +306,11 @@ def linear_distill(h: Tensor, W: Tensor, ids: Tensor, logits: Tensor, tau: float
     """Per-token distillation loss of the head h W^T from a teacher's top logits, and with labels y the cross entropy
     (else None) from the same pass over the vocabulary; fp32, h's leading shape, differentiable in h and W.
 
-    ids and logits (..., K), K up to 1024: the teacher's words, in any order, and its logits there. Its distribution p is their softmax
-    at temperature tau; the loss is tau^2 KL(p || q) with q the softmax of the student's logits over the whole vocabulary
-    at tau. An id outside [0, V) marks an entry that is not there (lists of different lengths); a logit of -inf has
-    probability zero; a token with no entry left has loss 0 and no gradient. A repeated id has the sum of its entries'
+    ids and logits (..., K), K up to 1024: the teacher's words, in any order, and its logits there. Its distribution p
+    is their softmax at temperature tau (2^-10 to 2^10); the loss is tau^2 KL(p || q) with q the softmax of the
+    student's logits over the whole vocabulary at tau. An id outside [0, V) marks an entry that is not there (lists of
+    different lengths), whatever its logit; a logit of -inf has probability zero; a token with no entry left has loss 0
+    and no gradient; a NaN among a token's logits makes its loss NaN. A repeated id has the sum of its entries'
     probabilities. The teacher gets no gradient."""
     ce, _, kd = _losses("linear_distill", h, W, y, ids, logits.detach(), float(tau))
     return kd, None if y is None else ce

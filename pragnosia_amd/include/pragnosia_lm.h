@@ -28,11 +28,11 @@ int pragnosia_lm_abi_version(void);
  *                                     entry is left
  *
  * h (n, d) and W (V, d) bf16, d a multiple of 8; y (n) int64 or NULL (no ce); ids (n, K) int64 and z (n, K) fp32, or
- * both NULL with K = 0 (no kd), K at most 1024; at least one of y and ids; tau > 0. Outputs, all fp32 but `entry`: ce and lse (n) with
- * y; kd, lse_t and psum (n), entry (n, K) int32, p and zl (n, K) with ids -- lse, lse_t, psum (1, or 0 where no entry is
- * left), entry (the
- * id at its first place in the list, or -1), p (an id's whole probability there, or 0) and zl (the student's logit of the
- * entry) are what the backward takes. */
+ * both NULL with K = 0 (no kd), K at most 1024; at least one of y and ids; tau from 2^-10 to 2^10. n and V at most
+ * 2^24, d at most 65536, n K below 2^31. Outputs, all fp32 but `entry`: ce and lse (n) with y; kd, lse_t and psum (n),
+ * entry (n, K) int32, p and zl (n, K) with ids -- lse, lse_t, psum (1, or 0 where no entry is left), entry (the id at
+ * its first place in the list, or -1), p (an id's whole probability there, or 0) and zl (the student's logit of the
+ * entry) are what the backward takes. A NaN among a row's present z makes its kd NaN. */
 int64_t pragnosia_head_fwd_workspace_bytes(int64_t n, int64_t V, int64_t d, int64_t K);
 int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y, const int64_t* ids, const float* z, float tau,
                        float* ce, float* lse, float* kd, float* lse_t, float* psum, int32_t* entry, float* p, float* zl,
@@ -52,9 +52,10 @@ int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd,
                        int64_t workspace_bytes, int64_t n, int64_t V, int64_t d, int64_t K, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
- * Rows of a token table: y_i = scale W[ids_i], n rows; an id outside [0, V) gives a zero row. W (V, d) and y (n, d) fp32
- * or bf16 (w_bf16, y_bf16), d a multiple of 8; ids (n) int64. kept (n) int32 or NULL: the ids in 32 bits for the
- * backward, which then reads half as much (-1 outside the table). n = 0 does nothing. Replaces nn.Embedding of src/model.py:822-826 (scale 1). */
+ * Rows of a token table: y_i = scale W[ids_i], n rows; an id outside [0, V) gives a zero row. W (V, d) and y (n, d)
+ * fp32 or bf16 (w_bf16, y_bf16), d a multiple of 8, n and V at most 2^28; ids (n) int64. kept (n) int32 or NULL: the
+ * ids in 32 bits for the backward, which then reads half as much (-1 outside the table). n = 0 does nothing. Replaces
+ * nn.Embedding of src/model.py:822-826 (scale 1). */
 int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16, int32_t* kept,
                         int64_t n, int64_t V, int64_t d, void* stream);
 

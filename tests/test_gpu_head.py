@@ -259,6 +259,21 @@ def test_teacher_edges():
         near(dh, want["dh"], "dh", 2.0 ** -8), near(dW, want["dW"], "dW", 2.0 ** -8)
 
 
+def test_teacher_that_is_no_distribution():
+    """A NaN or +inf among a token's present logits (and a whole row of NaN) is a NaN loss of that token; the others
+    keep their bits, the cross entropy too."""
+    n, V, d = 7, 90, 64
+    h, W, y, g = inputs(n, V, d, seed=17, pad=0)
+    ids = torch.stack([torch.randperm(V, generator=g)[:70] for _ in range(n)]).cuda()
+    z = torch.randn(n, 70, generator=g).cuda()
+    want = linear_distill(h, W, ids, z, 2.0, y)
+    bad = z.clone()
+    bad[1, 3], bad[2, 69], bad[4], bad[5, 0] = float("nan"), float("nan"), float("nan"), float("inf")
+    kd, ce = linear_distill(h, W, ids, bad, 2.0, y)
+    assert kd[[1, 2, 4, 5]].isnan().all()
+    assert torch.equal(kd[[0, 3, 6]], want[0][[0, 3, 6]]) and torch.equal(ce, want[1])
+
+
 def test_gradient_against_differences():
     """The directional derivative of the summed losses, by central differences of the formula in 64 bits, along random
     directions: the kernel's gradient gives it to its bf16 rounding (2^-7 of the norms of gradient and direction)."""

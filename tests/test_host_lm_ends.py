@@ -31,20 +31,23 @@ def test_header_exports_and_binding(L):
     assert f"ABI version of this header ({L.pragnosia_lm_abi_version()})" in open(HEADER).read()
 
 
-def fwd(L, n=4, V=10, d=16, K=0, h=one, W=one, y=one, ids=null, z=null, tau=1.0, out=one, kd=null, ws=one, size=1 << 30):
+def fwd(L, n=4, V=10, d=16, K=0, h=one, W=one, y=one, ids=null, z=null, tau=1.0, out=one, kd=null, ws=one,
+        size=1 << 30):
     return L.pragnosia_head_fwd(h, W, y, ids, z, tau, out, out, kd, kd, kd, kd, kd, kd, ws, size, n, V, d, K, null)
 
 
 @pytest.mark.parametrize("bad", [dict(n=0), dict(n=-1), dict(V=0), dict(d=12), dict(d=0), dict(K=-1), dict(h=null),
                                  dict(h=odd), dict(W=odd), dict(out=null), dict(y=null), dict(tau=0.0),
-                                 dict(tau=float("nan")), dict(tau=float("inf")), dict(ids=one), dict(K=3),
+                                 dict(tau=float("nan")), dict(tau=float("inf")), dict(tau=2.0 ** -11),
+                                 dict(tau=2.0 ** 11), dict(ids=one), dict(K=3),
                                  dict(K=3, ids=one, z=one), dict(K=1025, ids=one, z=one, kd=one), dict(ws=null),
                                  dict(ws=odd), dict(size=16), dict(n=1 << 25), dict(V=1 << 25)])
 def test_forward_refuses(L, bad):
     assert fwd(L, **bad) == -1
 
 
-def bwd(L, n=4, V=10, d=16, K=0, g=one, gk=null, y=one, lse=one, kd=null, tau=1.0, dh=one, dW=one, ws=one, size=1 << 30):
+def bwd(L, n=4, V=10, d=16, K=0, g=one, gk=null, y=one, lse=one, kd=null, tau=1.0, dh=one, dW=one, ws=one,
+        size=1 << 30):
     return L.pragnosia_head_bwd(g, null, gk, one, one, y, lse, kd, kd, kd, kd, kd, tau, dh, dW, 0, ws, size, n, V, d, K,
                                 null)
 
@@ -74,7 +77,7 @@ def test_workspace_queries(L):
     assert L.pragnosia_head_bwd_workspace_bytes(8, 8, 9) == -1
     assert L.pragnosia_embed_bwd_workspace_bytes(8, 0, 8) == -1
     assert L.pragnosia_embed_bwd_workspace_bytes(256, 8, 8) == 0 < L.pragnosia_embed_bwd_workspace_bytes(257, 8, 8)
-    # the backward's space stays near its limit whatever the vocabulary, and grows with the tokens only by what they need
+    # the backward's space stays near its limit whatever the vocabulary, and grows with the tokens by what they need
     for n, V, d in ((16384, 32768, 768), (8192, 262144, 1024), (100, 1 << 20, 512), (1, 1, 8)):
         assert 0 < L.pragnosia_head_bwd_workspace_bytes(n, V, d) < (512 << 20) + 16 * n * d
     assert L.pragnosia_head_bwd_workspace_bytes(8192, 8192, 768) < 160 << 20
@@ -108,7 +111,8 @@ L64 = dict(dtype=torch.long)
     (z(3, 16), z(5, 24), z(3, **L64), "W has shape"), (z(3, 16), z(5, 16), z(4, **L64), "leading sizes"),
     (z(3, 12), z(5, 12), z(3, **L64), "multiple of 8"), (z(3, 16), z(0, 16), z(3, **L64), "not empty"),
     (z(3, 16), z(5, 16), z(3), "integers"), (z(3, 16).half(), z(5, 16), z(3, **L64), "bf16 or fp32"),
-    (z(3, 16), z(5, 16).double(), z(3, **L64), "bf16 or fp32"), (z(2, 3, 16), z(5, 16), z(3, 2, **L64), "leading sizes"),
+    (z(3, 16), z(5, 16).double(), z(3, **L64), "bf16 or fp32"),
+    (z(2, 3, 16), z(5, 16), z(3, 2, **L64), "leading sizes"),
     (z(3, 16), z(5), z(3, **L64), "expected")])
 def test_cross_entropy_refuses(unguarded, h, W, y, what):
     with pytest.raises(PragnosiaError, match=what):
@@ -120,6 +124,7 @@ def test_cross_entropy_refuses(unguarded, h, W, y, what):
     (z(3, 0, **L64), z(3, 0), 1.0, "K from 1"), (z(3, 1025, **L64), z(3, 1025), 1.0, "K from 1"),
     (z(3, 2), z(3, 2), 1.0, "integers"), (z(3, 2, **L64), z(3, 2, **L64), 1.0, "floating"),
     (z(3, 2, **L64), z(3, 2), 0.0, "tau"), (z(3, 2, **L64), z(3, 2), float("nan"), "tau"),
+    (z(3, 2, **L64), z(3, 2), 2.0 ** -11, "tau"), (z(3, 2, **L64), z(3, 2), 1e30, "tau"),
     (z(3, **L64), z(3, 2), 1.0, "leading sizes")])
 def test_distill_refuses(unguarded, ids, lg, tau, what):
     with pytest.raises(PragnosiaError, match=what):
