@@ -209,23 +209,20 @@ struct Frags {
   PGN_DEVICE void read(unsigned p) {
     static_for<0, C::NA + C::NB>([&](auto q) { read_one<KB, q.value>(p); });
   }
-  // The products of half KB, NB at a time, and among them the fragments of the other half read from p (READ) and
-  // loads(u), u < kLoads: the fragments before the last group, so that they have arrived when the half ends.
-  // ZERO: onto zeros, whatever acc holds.
-  template <int KB, bool READ, int kLoads, bool ZERO = false, class L>
+  // The products of half KB, NB at a time, and among them the fragments of the other half read from p and loads(u), u <
+  // kLoads: the fragments before the last group, so that they have arrived when the half ends.
+  template <int KB, int kLoads, class L>
   PGN_DEVICE void multiply(f32x4 (&acc)[C::NA][C::NB], unsigned p, L&& loads) {
     constexpr int kFrags = C::NA + C::NB, kGroups = C::NA > 1 ? C::NA - 1 : 1;
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this half's fragments, read during the half before
     static_for<0, C::NA>([&](auto a) {
       constexpr int A = decltype(a)::value;
       static_for<A * kLoads / C::NA, (A + 1) * kLoads / C::NA>([&](auto u) { loads(u); });
-      if constexpr (READ) {
-        constexpr int lo = A * kFrags / kGroups, hi = (A + 1) * kFrags / kGroups;
-        static_for<(lo < kFrags ? lo : kFrags), (hi < kFrags ? hi : kFrags)>(
-            [&](auto q) { read_one<1 - KB, decltype(q)::value>(p); });
-      }
+      constexpr int lo = A * kFrags / kGroups, hi = (A + 1) * kFrags / kGroups;
+      static_for<(lo < kFrags ? lo : kFrags), (hi < kFrags ? hi : kFrags)>(
+          [&](auto q) { read_one<1 - KB, decltype(q)::value>(p); });
 #pragma unroll
-      for (int b = 0; b < C::NB; ++b) acc[A][b] = pgn_mfma(fx[KB][A], fy[KB][b], ZERO ? zero4() : acc[A][b]);
+      for (int b = 0; b < C::NB; ++b) acc[A][b] = pgn_mfma(fx[KB][A], fy[KB][b], acc[A][b]);
       __builtin_amdgcn_sched_barrier(0);
     });
   }
@@ -277,12 +274,12 @@ PGN_DEVICE void gemm_tile(const Operand& X, const Operand& Y, int64_t x0, int64_
   int buf = 0;
   for (int s = 0; s < steps; ++s) {
     const int next = buf + 1 == C::NS ? 0 : buf + 1;
-    f.template multiply<0, true, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
+    f.template multiply<0, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
     aim(s + C::NS);
     wait_loads<C::kLoads * (C::NS - 2)>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    f.template multiply<1, true, C::kLoads>(acc, lds0 + next * C::kStage, [&](auto u) { load(u, buf); });
+    f.template multiply<1, C::kLoads>(acc, lds0 + next * C::kStage, [&](auto u) { load(u, buf); });
     buf = next;
   }
   // nothing in flight into the buffers, nothing being read: they may be used again
@@ -309,8 +306,9 @@ PGN_DEVICE XcdRun xcd_run(int items) {
 // as zero), copied to LDS a tile ahead: into one of two places by the tile's parity, from a tile's first barrier on,
 // when the tile before, that place's last reader, is done; complete at the tile's own first barrier.
 //
-// kStores: how many stores every wave's epilogue issues, last of all. They need not have left before the next tile's
-// first stages are read: those loads were issued before them, and memory operations are counted in order.
+// kStores: how many stores every wave's epilogue issues at the least, whatever its tile holds. They need not have left
+// before the next tile's first stages are read: those loads were issued before them, and memory operations are counted
+// in order.
 template <class C, int kInfo, int kStores, class At, class Epilogue>
 PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const void* rows, int64_t row_count,
                            const XcdRun& run, unsigned char* lds, At&& at, Epilogue&& epilogue) {
@@ -372,7 +370,7 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
     // The first half of step s. Stage s + 1 has arrived at its end, and every wave's reads of stage s are done. The
     // stages that were issued before the last epilogue's stores need not wait for those.
     auto half = [&](int s) {
-      f.template multiply<0, true, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
+      f.template multiply<0, 0>(acc, lds0 + buf * C::kStage, [](auto) {});
       if (steps < C::NS)  // the row data of this tile may be among the last loads
         wait_loads<0>();
       else if (s < C::NS - 1 && item != run.first)
@@ -389,7 +387,7 @@ PGN_DEVICE void gemm_tiles(const Operand& X, const Operand& Y, int64_t d, const 
     for (int s = 0; s < steps; ++s) {
       half(s);
       const int next = buf + 1 == C::NS ? 0 : buf + 1;
-      f.template multiply<1, true, C::kLoads>(acc, lds0 + next * C::kStage, [&](auto u) { load(u, buf); });
+      f.template multiply<1, C::kLoads>(acc, lds0 + next * C::kStage, [&](auto u) { load(u, buf); });
       buf = next;
     }
     epilogue(acc, (int64_t)ix * C::X, (int64_t)iy * C::Y, info + place * C::kThreads * 16);

@@ -1,11 +1,12 @@
-"""Lookup of token rows with a scale, and its gradient by sorted tokens, on hand-written kernels (csrc/embed.hip; C ABI in
-pragnosia_amd/include/pragnosia_lm.h).
+"""Lookup of token rows with a scale, and its gradient by sorted tokens, on hand-written kernels (csrc/embed.hip; C ABI
+in pragnosia_amd/include/pragnosia_lm.h).
 
     y = embedding(ids, W, scale)
 
 is scale * W[ids] with a zero row where an id is outside the table (padding). The gradient of W is summed in fp32 over a
 stable order of the tokens by id: no atomics on values, so the same bits each time, and no memset in a captured step,
-where torch's embedding sorts with one past 3072 indices (`src/model.py:822-826` is the reference's lookup)."""
+where torch's embedding sorts with one from some thousands of indices on (`src/model.py:822-826` is the reference's
+lookup)."""
 from __future__ import annotations
 
 import math

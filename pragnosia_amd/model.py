@@ -81,8 +81,9 @@ class Embedding(nn.Embedding):
     an indexed addition: the order of a row's fp32 sum then varies from replay to replay. An eager step, and any step
     of fewer indices, is torch's.
 
-    With `sorted_grad` every lookup on the GPU, captured or not, is `embed.embedding`: the same rows, and a gradient summed
-    in fp32 over the tokens sorted by index, the same bits each time. An index outside the table then gives a zero row."""
+    With `sorted_grad` every lookup on the GPU, captured or not, is `embed.embedding`: the same rows, and a gradient
+    summed in fp32 over the tokens sorted by index, the same bits each time. An index outside the table then gives a
+    zero row."""
 
     sorted_grad = False
     SORTED_FROM = 3073  # indices from which torch's gradient takes the sort

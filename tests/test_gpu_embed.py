@@ -109,7 +109,7 @@ def test_infinities_stay_in_their_rows():
 
 
 def test_streams_and_capture():
-    """Two gradients at once on streams of their own, and one captured and replayed on new ids: the eager call's bits."""
+    """Two gradients at once on streams of their own, and one captured and replayed on new ids: the eager bits."""
     g = torch.Generator().manual_seed(4)
     W = torch.randn(700, 64, generator=g).cuda().requires_grad_()
     ids = [make_ids("zipf", n, 700, g).cuda() for n in (5000, 3000)]

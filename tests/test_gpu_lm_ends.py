@@ -46,7 +46,8 @@ def trunk(m, xs):
 
 
 def grads_of(m):
-    return {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}  # (a carrier may leave one unused)
+    # (a carrier may leave a parameter unused)
+    return {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
 
 
 def clear(m):
@@ -109,7 +110,8 @@ def test_training_step(mixer, kd):
             assert torch.equal(ref[k], pieces[k]), k
     for k, at in (("e.weight", xs[:, :-1].reshape(-1)), ("p.weight", torch.arange(CTX, device="cuda").repeat(3))):
         rows = ref[k].shape[0]
-        size = torch.zeros(rows, D, device="cuda", dtype=torch.float64).index_add_(0, at, gx.reshape(n, D).double().abs())
+        size = torch.zeros(rows, D, device="cuda", dtype=torch.float64)
+        size.index_add_(0, at, gx.reshape(n, D).double().abs())
         m_terms = torch.bincount(at, minlength=rows)[:, None]
         assert ((ref[k].double() - pieces[k].double()).abs() <= 2 * (m_terms + 2) * 2.0 ** -24 * size).all(), k
 
