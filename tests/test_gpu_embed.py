@@ -140,3 +140,20 @@ def test_streams_and_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, grad(held.clone(), gy[0]))
+
+
+@pytest.mark.parametrize("n,V", [(7, 33000), (300, 33000), (33000, 40)])
+def test_offsets_past_32_bits(n, V):
+    """A table, and gradient rows, of more than 2^31 elements. Whole numbers, whose sums are exact in fp32."""
+    d, g = 65536, torch.Generator(device="cuda").manual_seed(12)
+    W = torch.randint(-9, 10, (V, d), generator=g, device="cuda", dtype=torch.int8).bfloat16().requires_grad_()
+    ids = torch.randint(0, V, (n,), generator=g, device="cuda")
+    ids[0], ids[1], ids[-1] = V - 1, -1, V - 1
+    y = embedding(ids, W)
+    assert max(y.numel(), W.numel()) > 2 ** 31
+    on = ids >= 0
+    assert torch.equal(y[on], W.detach()[ids[on]]) and not y[1].any()
+    gy = torch.randint(-9, 10, (n, d), generator=g, device="cuda", dtype=torch.int8).bfloat16()
+    dW, = torch.autograd.grad(y, W, gy)
+    want = torch.zeros(V, d, device="cuda").index_add_(0, ids[on], gy[on].float()).bfloat16()
+    assert torch.equal(dW, want)

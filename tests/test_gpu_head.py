@@ -363,3 +363,23 @@ def test_tiles(n, V, d):
     loss, lse, dh, dW = ce_grads(h, W, y, gc)
     near(loss, want["ce"], "ce"), near(lse, want["lse"], "lse")
     near(dh, want["dh"], "dh", 2.0 ** -8), near(dW, want["dW"], "dW", 2.0 ** -8)
+
+
+@pytest.mark.parametrize("n,V", [(3, 33000), (33000, 24)])
+def test_offsets_past_32_bits(n, V):
+    """A table, and hidden rows, of more than 2^31 elements: losses and gradients up to the last row."""
+    d, g = 65536, torch.Generator(device="cuda").manual_seed(11)
+    h = torch.randn(n, d, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    W = torch.randn(V, d, generator=g, device="cuda", dtype=torch.bfloat16).mul_(2 * d ** -0.5).requires_grad_()
+    assert max(h.numel(), W.numel()) > 2 ** 31
+    ids = torch.randint(0, V, (n, 4), generator=g, device="cuda").sort(1).values
+    ids[:, 1:] = torch.where(ids[:, 1:] == ids[:, :-1], -1, ids[:, 1:])
+    ids[-1], z = torch.arange(V - 4, V, device="cuda"), torch.randn(n, 4, generator=g, device="cuda")
+    y = torch.randint(0, V, (n,), generator=g, device="cuda")
+    y[0], y[-1] = 0, V - 1
+    g_kd, g_ce = torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    kd, ce = linear_distill(h, W, ids, z, 2.0, y)
+    dh, dW = torch.autograd.grad((kd, ce), (h, W), (g_kd, g_ce))
+    want = oracle(h, W, y, g_ce, None, ids, z, 2.0, g_kd)
+    near(kd, want["kd"], "kd"), near(ce, want["ce"], "ce")
+    near(dh, want.pop("dh"), "dh", 2.0 ** -8), near(dW, want.pop("dW"), "dW", 2.0 ** -8)
