@@ -5,7 +5,7 @@
 // one launch, sums in a second and joins long runs in a third:
 //
 //   sort  Every workgroup owns a range of ids. It reads all n ids (they stay in the L2), counts those below its range
-//         -- where its tokens start in the order -- and ranks its own by id and position; then places them. No
+//         -- where its tokens start in the order -- and lists its own, ranked by id and position; then places them. No
 //         workgroup waits for another.
 //   sum   An id with at most kShort tokens (most of a vocabulary, zeros where there is none) is summed by one thread a
 //         column vector, all its rows loaded at once. A longer run is summed in blocks of kBlock places of the order,
@@ -16,7 +16,7 @@
 // A few tokens (kDirect) are one launch: a wave looks its ids up among all the tokens itself.
 //
 // Measured, fp32, 768 wide, word frequencies falling with the rank: 8192 tokens of 8192 words: lookup 8.3 us (50 MB: 6
-// TB/s, part of it from the cache), sort 9, sum 10.5 (50 MB), join 3.5; 65536 of 32768: 56, 39, 88 (301 MB: 3.4 TB/s,
+// TB/s, part of it from the cache), sort 9, sum 10.5 (50 MB), join 3.5; 65536 of 32768: 56, 28, 89 (301 MB: 3.4 TB/s,
 // short runs' rows and stores mixed), 6.
 #include <algorithm>
 
@@ -26,9 +26,9 @@
 namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kList = 6144;    // tokens of a sorting workgroup's range that fit its LDS
-constexpr int kHeld = 16;      // ids a thread of it keeps in registers
-constexpr int kMaxRange = 512;
+constexpr int kList = 768;     // tokens of a sorting wave that fit its LDS
+constexpr int kAhead = 16;     // ids a lane of it loads at once
+constexpr int kIdBits = 9, kMaxRange = 1 << kIdBits;  // ids of a sorting workgroup, at most
 constexpr int kDirect = 256;   // tokens up to which a gradient is one launch (256 of 8192 x 768: 8 us; three take 17)
 constexpr int kShort = 8;    // tokens of an id summed by one thread
 constexpr int kBlock = 64;   // places of the order summed by one workgroup: a lane each
@@ -91,90 +91,90 @@ __global__ __launch_bounds__(256) void embed_rows(const int64_t* __restrict__ id
 PGN_DEVICE int table_id(int64_t id, int64_t V) { return id >= 0 && id < V ? (int)id : -1; }
 
 // Ids [blockIdx.x * range, ..): start[v] = the place of id v's first token in the order (start[V]: the number of
-// tokens with an id), order[place] = position, sorted[place] = id. A wave reads a contiguous share of the ids in order
-// and counts its own tokens by id, so a token's place is its id's start, the counts of the waves before, and its rank
-// in its wave. list: n entries of scratch, for ranges with more than kList tokens. HELD: n <= kHeld kSortThreads, the
-// ids stay in registers between the two passes over them.
+// tokens with an id), order[place] = position, sorted[place] = id. A wave reads a contiguous share of the ids in order,
+// lists its tokens of the range and counts them by id, so a token's place is its id's start, the counts of the waves
+// before, and its rank in its wave. A wave's list is kList tokens of LDS; a workgroup with more in some wave reads the
+// ids again and lists them in `far` (n entries of scratch), where all of its waves know their places by then.
+//
+// Bound by the sixteen waves of each compute unit that look at every id between them: 65536 ids 28 us; counted first
+// and listed in a second pass 38, with a branch around each load 53.
 struct Token {
-  int id, position, rank, wave;  // id relative to the range; rank among the wave's tokens of the id
+  int position;
+  unsigned rank_id;  // rank among the wave's tokens of the id, and the id from the range's start in kIdBits
 };
 
-template <bool HELD, class I>
+template <class I>
 __global__ __launch_bounds__(kSortThreads) void embed_sort(const I* __restrict__ ids, int32_t* __restrict__ order,
                                                            int32_t* __restrict__ sorted, int32_t* __restrict__ start,
-                                                           Token* __restrict__ list, int n, int V, int range) {
+                                                           Token* __restrict__ far, int n, int V, int range) {
   extern __shared__ __align__(16) unsigned char smem[];
-  Token* const near = reinterpret_cast<Token*>(smem);
   // wave w's tokens of id r at [w * range + r]; then the place of the first of them
-  int32_t* const count = reinterpret_cast<int32_t*>(smem + sizeof(Token) * kList);
+  int32_t* const count = reinterpret_cast<int32_t*>(smem + sizeof(Token) * kList * kSortWaves);
   __shared__ int32_t waves[2][kSortWaves];
   __shared__ int32_t first[kMaxRange];
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int v0 = blockIdx.x * range, v1 = min(V, v0 + range);
   const int share = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64, a = min(n, w * share), b = min(n, a + share);
-  auto load = [&](int i0) { return i0 + l < b ? table_id(ids[i0 + l], V) : -1; };
-  int held[kHeld];
-  int below = 0, mine = 0;
-  auto tally = [&](int x) {
-    below += x >= 0 && x < v0;
-    mine += x >= v0 && x < v1;
+  Token* list = reinterpret_cast<Token*>(smem) + w * kList;
+  volatile int32_t* const own = count + w * range;  // (a wave's LDS operations are in order)
+  int below = 0, mine = 0;  // a lane's ids below the range; the wave's tokens
+  const unsigned long long lower = (1ull << l) - 1;
+  auto append = [&](int i0, int x, int room) {
+    const bool in = (unsigned)(x - v0) < (unsigned)(v1 - v0);
+    const unsigned long long m = __ballot(in);
+    if (m == 0) return;
+    unsigned long long same = 0;  // the lanes with this lane's id
+    for (unsigned long long left = m; left;) {
+      const int id = __builtin_amdgcn_readlane(x, __ffsll((long long)left) - 1);
+      const unsigned long long lanes = __ballot(x == id);
+      if (x == id) same = lanes;
+      left &= ~lanes;
+    }
+    if (in) {
+      const int before = own[x - v0], rank = before + __popcll(same & lower), to = mine + __popcll(m & lower);
+      if ((same & lower) == 0) own[x - v0] = before + __popcll(same);
+      if (to < room) list[to] = {i0 + l, (unsigned)rank << kIdBits | (unsigned)(x - v0)};
+    }
+    mine += __popcll(m);
   };
-  if constexpr (HELD) {
+  // kAhead ids a lane, -1 past the share or outside the table, the next ones under way; no load is behind a branch, or
+  // each would be waited for by itself
+  auto pass = [&](int room) {
+    I next[kAhead];
+    auto load = [&](int i0) {
 #pragma unroll
-    for (int q = 0; q < kHeld; ++q) held[q] = load(a + 64 * q);
+      for (int q = 0; q < kAhead; ++q) next[q] = ids[min(i0 + 64 * q + l, n - 1)];
+    };
+    for (int r = l; r < range; r += 64) own[r] = 0;
+    below = mine = 0;
+    load(a);
+    for (int i0 = a; i0 < b; i0 += 64 * kAhead) {
+      int x[kAhead];
 #pragma unroll
-    for (int q = 0; q < kHeld; ++q) tally(held[q]);
-  } else {
-#pragma unroll 8
-    for (int i0 = a; i0 < b; i0 += 64) tally(load(i0));
-  }
-  for (int o = 1; o < 64; o *= 2) below += __shfl_xor(below, o), mine += __shfl_xor(mine, o);
+      for (int q = 0; q < kAhead; ++q) x[q] = i0 + 64 * q + l < b ? table_id(next[q], V) : -1;
+      if (i0 + 64 * kAhead < b) load(i0 + 64 * kAhead);
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        if (i0 + 64 * q >= b) break;
+        below += (unsigned)x[q] < (unsigned)v0;
+        append(i0 + 64 * q, x[q], room);
+      }
+    }
+  };
+  pass(kList);
+  for (int o = 1; o < 64; o *= 2) below += __shfl_xor(below, o);
   if (l == 0) waves[0][w] = below, waves[1][w] = mine;
-  for (int r = tid; r < range * kSortWaves; r += kSortThreads) count[r] = 0;
   __syncthreads();
-  int base = 0, at = 0, all = 0;
+  int base = 0, at = 0;
+  bool fits = true;
   for (int q = 0; q < kSortWaves; ++q) {
     base += waves[0][q];
     if (q < w) at += waves[1][q];
-    all += waves[1][q];
+    fits = fits && waves[1][q] <= kList;
   }
-  const bool fits = all <= kList;
-  Token* const far = list + base;
-  volatile int32_t* const own = count + w * range;  // (written by one lane, read by all)
-  auto append = [&](int i0, int x) {
-    const bool in = x >= v0 && x < v1;
-    const unsigned long long m = __ballot(in);
-    if (m == 0) return;
-    const unsigned long long lower = (1ull << l) - 1;
-    int rank = 0;
-    for (unsigned long long left = m; left;) {
-      const int r = __builtin_amdgcn_readlane(x, __ffsll((long long)left) - 1) - v0;
-      const unsigned long long same = __ballot(in && x - v0 == r);
-      const int before = own[r];
-      if (in && x - v0 == r) rank = before + __popcll(same & lower);
-      own[r] = before + __popcll(same);
-      left &= ~same;
-    }
-    if (in) {
-      const Token e = {x - v0, i0 + l, rank, w};
-      const int to = at + __popcll(m & lower);
-      if (fits)
-        near[to] = e;
-      else
-        far[to] = e;
-    }
-    at += __popcll(m);
-  };
-  if constexpr (HELD) {
-#pragma unroll
-    for (int q = 0; q < kHeld; ++q) append(a + 64 * q, held[q]);
-  } else {
-    int next = load(a);
-    for (int i0 = a; i0 < b; i0 += 64) {
-      const int x = next;
-      next = load(i0 + 64);
-      append(i0, x);
-    }
+  if (!fits) {
+    list = far + base + at;
+    pass(n);
   }
   __syncthreads();
   // an id's tokens by wave: the counts of the waves before; and in all
@@ -205,11 +205,11 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const I* __restrict__
     if (l == 0 && v1 == V) start[V] = run;
   }
   __syncthreads();
-  for (int i = tid; i < all; i += kSortThreads) {
-    const Token e = fits ? near[i] : far[i];
-    const int to = first[e.id] + count[e.wave * range + e.id] + e.rank;
+  for (int i = l; i < mine; i += 64) {
+    const Token e = list[i];
+    const int id = e.rank_id & (kMaxRange - 1), to = first[id] + own[id] + (int)(e.rank_id >> kIdBits);
     order[to] = e.position;
-    sorted[to] = v0 + e.id;
+    sorted[to] = v0 + id;
   }
 }
 
@@ -399,13 +399,14 @@ __global__ __launch_bounds__(256) void embed_direct(const G* __restrict__ g, con
   }
 }
 
-constexpr int64_t kMaxTokens = (int64_t)1 << 28;  // (sorting workgroups: V / 512)
+constexpr int64_t kMaxTokens = (int64_t)1 << 27;  // (a rank in a wave, at most a sixteenth, is 32 - kIdBits bits)
+constexpr int64_t kMaxWords = (int64_t)1 << 28;
 
 // Ids a sorting workgroup owns: about 256 workgroups (each reads all ids), their counters at most 32 KB.
 int64_t sort_range(int64_t V) { return std::min<int64_t>(std::max<int64_t>((V + 255) / 256, 32), kMaxRange); }
 
 bool embed_shape_ok(int64_t n, int64_t V, int64_t d) {
-  return n >= 0 && n <= kMaxTokens && V > 0 && V <= kMaxTokens && d > 0 && d % 8 == 0 && d <= 65536 &&
+  return n >= 0 && n <= kMaxTokens && V > 0 && V <= kMaxWords && d > 0 && d % 8 == 0 && d <= 65536 &&
          (n / kBlock + 1) * (d / 256 + 1) < (int64_t)1 << 22;  // launches of fewer than 2^32 threads
 }
 
@@ -433,16 +434,16 @@ int launch_grad(const void* g, const I* ids, float scale, void* dW, int32_t* ws,
                        dim3(256), 0, st, (const G*)g, ids, scale, (T*)dW, (int)n, (int)V, (int)d);
     PGN_RETURN_LAUNCH();
   }
-  Token* list = (Token*)ws;
-  int32_t *order = ws + 4 * up4(n), *sorted = order + up4(n), *start = sorted + up4(n);
+  Token* far = (Token*)ws;
+  int32_t *order = ws + 2 * up4(n), *sorted = order + up4(n), *start = sorted + up4(n);
   float* part = (float*)(start + up4(V + 1));
   const int range = (int)sort_range(V);
-  const auto sort = n <= kHeld * kSortThreads ? embed_sort<true, I> : embed_sort<false, I>;
-  const int lds = (int)sizeof(Token) * kList + 4 * kSortWaves * range;
-  const hipError_t e = pgn_lds_limit((const void*)sort, (int)sizeof(Token) * kList + 4 * kSortWaves * kMaxRange);
+  const auto sort = embed_sort<I>;
+  const int lists = (int)sizeof(Token) * kList * kSortWaves, lds = lists + 4 * kSortWaves * range;
+  const hipError_t e = pgn_lds_limit((const void*)sort, lists + 4 * kSortWaves * kMaxRange);
   if (e != hipSuccess) return (int)e;
   hipLaunchKernelGGL(sort, dim3((unsigned)((V + range - 1) / range)), dim3(kSortThreads), lds, st, ids, order, sorted,
-                     start, list, (int)n, (int)V, range);
+                     start, far, (int)n, (int)V, range);
   const int64_t whole = std::min<int64_t>((V * per + 255) / 256, 1 << 20);
   hipLaunchKernelGGL((embed_sum<G, T>), dim3((unsigned)(blocks * chunks + whole)), dim3(256), 0, st, (const G*)g, order,
                      sorted, start, scale, (T*)dW, part, (int)V, (int)d, (int)blocks, (int)chunks);
@@ -476,7 +477,7 @@ extern "C" int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16
 
 extern "C" int64_t pragnosia_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!embed_shape_ok(n, V, d)) return -1;
-  return n <= kDirect ? 0 : (6 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
+  return n <= kDirect ? 0 : (4 * up4(n) + up4(V + 1) + 2 * blocks_of(n) * d) * 4;
 }
 
 extern "C" int pragnosia_embed_bwd(const void* g, int g_bf16, const void* ids, int ids_64, float scale, void* dW,

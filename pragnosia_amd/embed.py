@@ -54,7 +54,7 @@ def _backward(g: Tensor, ids: Tensor, V: int, scale: float, dtype: torch.dtype) 
     return dW
 
 
-_KEPT_FROM = 16385  # tokens whose ids the sort reads twice: kept in 32 bits by the lookup
+_KEPT_FROM = 16385  # tokens from which the lookup keeps the ids in 32 bits: every sorting workgroup reads them all
 
 
 class _Embedding(torch.autograd.Function):

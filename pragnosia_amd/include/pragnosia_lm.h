@@ -53,8 +53,8 @@ int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd,
 
 /* ---------------------------------------------------------------------------------------------------------
  * Rows of a token table: y_i = scale W[ids_i], n rows; an id outside [0, V) gives a zero row. W (V, d) and y (n, d)
- * fp32 or bf16 (w_bf16, y_bf16), d a multiple of 8, n and V at most 2^28; ids (n) int64. kept (n) int32 or NULL: the
- * ids in 32 bits for the backward, which then reads half as much (-1 outside the table). n = 0 does nothing. Replaces
+ * fp32 or bf16 (w_bf16, y_bf16), d a multiple of 8, n at most 2^27 and V 2^28; ids (n) int64. kept (n) int32 or NULL:
+ * the ids in 32 bits for the backward, which then reads half as much (-1 outside the table). n = 0 does nothing. Replaces
  * nn.Embedding of src/model.py:822-826 (scale 1). */
 int pragnosia_embed_fwd(const int64_t* ids, const void* W, int w_bf16, float scale, void* y, int y_bf16, int32_t* kept,
                         int64_t n, int64_t V, int64_t d, void* stream);
