@@ -28,6 +28,7 @@ namespace {
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kList = 768;     // tokens of a sorting wave that fit its LDS
 constexpr int kAhead = 16;     // ids a lane of it loads at once
+constexpr int kFew = 2;        // ids among 64 tokens that it tells apart one by one
 constexpr int kIdBits = 9, kMaxRange = 1 << kIdBits;  // ids of a sorting workgroup, at most
 constexpr int kDirect = 256;   // tokens up to which a gradient is one launch (256 of 8192 x 768: 8 us; three take 17)
 constexpr int kShort = 8;    // tokens of an id summed by one thread
@@ -117,18 +118,30 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const I* __restrict__
   const int share = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64, a = min(n, w * share), b = min(n, a + share);
   Token* list = reinterpret_cast<Token*>(smem) + w * kList;
   volatile int32_t* const own = count + w * range;  // (a wave's LDS operations are in order)
+  const int bits = 32 - __clz(range - 1);
   int below = 0, mine = 0;  // a lane's ids below the range; the wave's tokens
   const unsigned long long lower = (1ull << l) - 1;
   auto append = [&](int i0, int x, int room) {
     const bool in = (unsigned)(x - v0) < (unsigned)(v1 - v0);
     const unsigned long long m = __ballot(in);
     if (m == 0) return;
-    unsigned long long same = 0;  // the lanes with this lane's id
-    for (unsigned long long left = m; left;) {
+    // the lanes with this lane's id: of the first kFew ids one by one (a few hot words), of what is left bit by bit
+    // (65536 tokens of 64 ids of one range: 215 us, all one by one 460; with one hot word 33, all bit by bit 43)
+    unsigned long long same = 0, left = m;
+    for (int k = 0; k < kFew && left; ++k) {
       const int id = __builtin_amdgcn_readlane(x, __ffsll((long long)left) - 1);
       const unsigned long long lanes = __ballot(x == id);
       if (x == id) same = lanes;
       left &= ~lanes;
+    }
+    if (left) {
+      unsigned long long rest = left;
+      for (int k = 0; k < bits; ++k) {
+        const bool one = (x - v0) >> k & 1;
+        const unsigned long long ones = __ballot(one);
+        rest &= one ? ones : ~ones;
+      }
+      if (left >> l & 1) same = rest;
     }
     if (in) {
       const int before = own[x - v0], rank = before + __popcll(same & lower), to = mine + __popcll(m & lower);
@@ -327,17 +340,18 @@ __global__ __launch_bounds__(256) void embed_join(const int32_t* __restrict__ so
   // block q's row at 2 q + 1, those of the blocks after it at 2 k
   const int rows = (to - 1) / kBlock - q + 1, each = (rows + 3) / 4, a = min(rows, w * each), b = min(rows, a + each);
   float s[N] = {};
-  for (int k = a; k < b; k += 4) {
-    f32x4 x[4][N / 4];
+  constexpr int U = 8;  // rows loaded at once (an id of 65536 tokens, 768 wide: 4 40 us, 8 27)
+  for (int k = a; k < b; k += U) {
+    f32x4 x[U][N / 4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int at = min(k + u, b - 1);
       const float* p = part + (int64_t)(2 * (q + at) + (at == 0)) * d + c;
 #pragma unroll
       for (int i = 0; i < N / 4; ++i) x[u][i] = *reinterpret_cast<const f32x4*>(p + 4 * i);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
       if (k + u < b)
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] += x[u][i / 4][i % 4];
@@ -402,8 +416,9 @@ __global__ __launch_bounds__(256) void embed_direct(const G* __restrict__ g, con
 constexpr int64_t kMaxTokens = (int64_t)1 << 27;  // (a rank in a wave, at most a sixteenth, is 32 - kIdBits bits)
 constexpr int64_t kMaxWords = (int64_t)1 << 28;
 
-// Ids a sorting workgroup owns: about 256 workgroups (each reads all ids), their counters at most 32 KB.
-int64_t sort_range(int64_t V) { return std::min<int64_t>(std::max<int64_t>((V + 255) / 256, 32), kMaxRange); }
+// Ids a sorting workgroup owns: at most 256 workgroups where the counters allow (32 KB at most), as each reads all ids;
+// no fewer, so that many tokens of a small table are shared out (65536 of 512 positions: 18 us; 32 ids each, 33).
+int64_t sort_range(int64_t V) { return std::min<int64_t>((V + 255) / 256, kMaxRange); }
 
 bool embed_shape_ok(int64_t n, int64_t V, int64_t d) {
   return n >= 0 && n <= kMaxTokens && V > 0 && V <= kMaxWords && d > 0 && d % 8 == 0 && d <= 65536 &&

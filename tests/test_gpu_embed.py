@@ -73,6 +73,13 @@ def test_long_runs(kind):
     check(make_ids(kind, 70001, 1500, g).view(1, -1), 1500, 24, f32, f32)
 
 
+@pytest.mark.parametrize("n", [3000, 20000])
+def test_many_ids_of_one_range(n):
+    """Tokens of some tens of neighbouring ids in a large table: many ids among a wave's tokens, more than its list."""
+    g = torch.Generator().manual_seed(6)
+    check(torch.randint(100, 164, (n,), generator=g), 20000, 16, f32, f32)
+
+
 def test_strides_offsets_and_shapes():
     """ids of any shape and integer type, a table inside a larger buffer at an odd offset, an expanded gradient."""
     g = torch.Generator().manual_seed(3)
