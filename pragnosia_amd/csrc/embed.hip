@@ -16,7 +16,7 @@
 // A few tokens (kDirect) are one launch: a wave looks its ids up among all the tokens itself.
 //
 // Measured, fp32, 768 wide, word frequencies falling with the rank: 8192 tokens of 8192 words: lookup 8.3 us (50 MB: 6
-// TB/s, part of it from the cache), sort 9, sum 10.5 (50 MB), join 3.5; 65536 of 32768: 56, 28, 89 (301 MB: 3.4 TB/s,
+// TB/s, part of it from the cache), sort 9, sum 10.5 (50 MB), join 3.5; 65536 of 32768: 56, 29, 89 (301 MB: 3.4 TB/s,
 // short runs' rows and stores mixed), 6.
 #include <algorithm>
 
@@ -97,7 +97,7 @@ PGN_DEVICE int table_id(int64_t id, int64_t V) { return id >= 0 && id < V ? (int
 // before, and its rank in its wave. A wave's list is kList tokens of LDS; a workgroup with more in some wave reads the
 // ids again and lists them in `far` (n entries of scratch), where all of its waves know their places by then.
 //
-// Bound by the sixteen waves of each compute unit that look at every id between them: 65536 ids 28 us; counted first
+// Bound by the sixteen waves of each compute unit that look at every id between them: 65536 ids 29 us; counted first
 // and listed in a second pass 38, with a branch around each load 53.
 struct Token {
   int position;
