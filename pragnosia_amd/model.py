@@ -100,6 +100,13 @@ class Embedding(nn.Embedding):
         return super().forward(x)
 
 
+def _total(x):
+    """The sum of x. torch's, of more than 65536 values to one, is a multi-block reduction, which clears its semaphores
+    with a memset; captured in a HIP graph that has given wrong sums on replays. So the sum of sums of 32768."""
+    parts = [p.sum() for p in x.reshape(-1).split(32768)]
+    return parts[0] if len(parts) == 1 else torch.stack(parts).sum()
+
+
 class LM(nn.Module):
     def __init__(self, vocab=8192, d=768, layers=12, mlp_mult=4, ctx=512, mixer="aspin", norm="ln", short_conv=0,
                  fused_ends=False, **unused):
@@ -177,7 +184,7 @@ class LM(nn.Module):
         `head.linear_cross_entropy`, for fp32 and bf16: no logits at all (`chunks` says nothing then)."""
         low = (torch.float32, torch.bfloat16)
         if self.fused_ends and h.is_cuda and h.dtype in low and self.e.weight.dtype in low and self.d % 8 == 0:
-            return linear_cross_entropy(h, self.e.weight, y)[0].sum() / y.numel()
+            return _total(linear_cross_entropy(h, self.e.weight, y)[0]) / y.numel()
         hf, yf = h.reshape(-1, h.shape[-1]), y.reshape(-1)
         n = hf.shape[0]
 
@@ -201,7 +208,7 @@ class LM(nn.Module):
         vocabulary: (distillation, cross-entropy or None). See `head.linear_distill`."""
         kd, ce = linear_distill(h, self.e.weight, ids, logits, tau, y)
         n = kd.numel()
-        return kd.sum() / n, None if ce is None else ce.sum() / n
+        return _total(kd) / n, None if ce is None else _total(ce) / n
 
     @torch.no_grad()
     def forward_carried(self, x, window=None):

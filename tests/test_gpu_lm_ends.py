@@ -210,3 +210,33 @@ def test_lookup_is_torchs():
     x = torch.randint(0, VOCAB, (2, 50), device="cuda")
     assert torch.equal(m.e(x), F.embedding(x, m.e.weight))
     assert not m.e(torch.tensor([[-1, VOCAB]], device="cuda")).any()
+
+
+@pytest.mark.parametrize("n", [8192, 131073])
+def test_captured_losses_of_many_tokens(n):
+    """The mean losses over long batches and their gradients: no memset node, every replay the eager call's bits."""
+    _, m = models()
+    h = torch.randn(1, n, D, device="cuda").bfloat16().requires_grad_()
+    y, (ids, z) = torch.randint(0, VOCAB, (1, n), device="cuda"), teacher((1, n), 3, 6)
+
+    def losses():
+        kd, ce = m.distill_loss(h, ids, z, 1.0, y)
+        loss = m.loss(h, y)
+        return (kd.detach(), ce.detach(), loss.detach(), *torch.autograd.grad(kd + ce + loss, (h, m.e.weight)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        losses()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        out = losses()
+    assert _memset_nodes(graph) == 0
+    for _ in range(3):
+        y.random_(0, VOCAB), z.normal_()
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        for a, b in zip(got, losses()):
+            assert torch.equal(a, b)
