@@ -146,7 +146,7 @@ PGN_DEVICE float column_sum(float x) { return swap_add<32>(swap_add<16>(x, x), s
 // ---------------------------------------------------------------------------------------------------------------
 // The teacher's distribution over its entries, a wave a row; bound by latency (8192 rows of 32 entries: 7 us). A
 // repeated id's probabilities are added into its first entry, the others leave the list, so that every later kernel
-// meets an id once.
+// meets an id once, and the row's sum of p log p is that of the words (summed again where an id repeats).
 constexpr int kMaxEntries = 1024;
 constexpr float kTauLeast = 0x1p-10f;
 constexpr int64_t kSliceBytes = (int64_t)2 << 20;
@@ -192,14 +192,10 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
     p_of[k] = pk;
     if (pk != 0.f) e += pk * (x - log_sum);
   }
-  for (int o = 1; o < 64; o *= 2) e += __shfl_xor(e, o);
-  if (l == 0) {
-    psum[row] = some ? 1.f : 0.f;
-    ent[row] = e;
-  }
   if (l < K4 - K) id_of[K + l] = -1;
   // (the lists are the wave's own: its LDS operations are in order)
   __builtin_amdgcn_wave_barrier();
+  bool repeats = false;
   for (int k = l; k < K + l; k += 64) {  // every lane takes part in every turn
     const int id = k < K ? id_of[k] : -1;
     float pk = k < K ? p_of[k] : 0.f;
@@ -211,6 +207,7 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
       for (int u = 0; u < 4; ++u) equal += o[u] == id;
     }
     if (__ballot(id >= 0 && equal > 1)) {  // a repeated id
+      repeats = true;
       float all = 0.f;
       for (int j = 0; j < K; ++j)
         if (id_of[j] == id) {
@@ -224,6 +221,16 @@ __global__ __launch_bounds__(256) void head_teacher(const int64_t* __restrict__ 
       p[k] = id >= 0 ? pk : 0.f;
       if (id < 0 || earlier > 0) zl[k] = 0.f;  // (the others are head_entry_logits')
     }
+  }
+  if (repeats) {  // (p as this lane has just written it)
+    e = 0.f;
+    for (int k = l; k < K; k += 64)
+      if (p[k] != 0.f) e += p[k] * logf(p[k]);
+  }
+  for (int o = 1; o < 64; o *= 2) e += __shfl_xor(e, o);
+  if (l == 0) {
+    psum[row] = some ? 1.f : 0.f;
+    ent[row] = e;
   }
 }
 

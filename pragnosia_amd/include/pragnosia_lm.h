@@ -24,8 +24,9 @@ int pragnosia_lm_abi_version(void);
  *
  *   lse_i = log sum_v exp l_iv        ce_i = lse_i - l_{i, y_i}; 0 where y_i is outside [0, V)
  *   p_i   = softmax over k of z_ik / tau, over the entries with ids_ik in [0, V) (an id may repeat); z = -inf: p = 0
- *   lse_t = log sum_v exp(l_iv / tau) kd_i = tau^2 sum_k p_ik (log p_ik - l_{i, ids_ik} / tau + lse_t_i); 0 where no
- *                                     entry is left
+ *   lse_t = log sum_v exp(l_iv / tau) P_iv  = sum of p_ik over the k with ids_ik = v
+ *   kd_i  = tau^2 sum_v P_iv (log P_iv - l_iv / tau + lse_t_i), tau^2 KL(P_i || softmax(l_i / tau)); 0 where no entry
+ *           is left
  *
  * h (n, d) and W (V, d) bf16, d a multiple of 8; y (n) int64 or NULL (no ce); ids (n, K) int64 and z (n, K) fp32, or
  * both NULL with K = 0 (no kd), K at most 1024; at least one of y and ids; tau from 2^-10 to 2^10. n and V at most
