@@ -508,7 +508,8 @@ __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo*
   __shared__ float most[16];
   const int tid = threadIdx.x;
   float g = 0.f;
-  for (const float* x : {in.g_ce, in.g_kd, in.g_lse}) {
+  for (int which = 0; which < 3; ++which) {  // (by place: two losses' gradients may be one array)
+    const float* x = which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse;
     if (x == nullptr) continue;
     g = thread_max(x, n, tid);
     for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
@@ -516,7 +517,7 @@ __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo*
     if ((tid & 63) == 0) most[tid >> 6] = g;
     __syncthreads();
     for (int k = 0; k < 16; ++k) g = fmaxf(g, most[k]);
-    if (x == in.g_kd) g *= in.tau;
+    if (which == 1) g *= in.tau;
     if (g > 0.f && g < INFINITY) break;
   }
   if (!(g > 0.f && g < INFINITY)) g = 1.f;
