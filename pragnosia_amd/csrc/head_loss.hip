@@ -465,7 +465,7 @@ struct BwdIn {
 // gc [v = label], the exponents in base 2; zero where not live.
 //
 // G is the largest of the rows' gradients of the cross entropy (of the distillation loss, where there is no label: a
-// teacher's probabilities are no constants, and round at random). A mean's rows all have the same weight w, and most
+// teacher's probabilities are no constants, and round at random), over the rows that have a label (a teacher). A mean's rows all have the same weight w, and most
 // of a row's gradient is its label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same
 // relative error, that of w's bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and
 // mostly much nearer, and the products are multiplied by G in fp32.
@@ -485,20 +485,33 @@ PGN_DEVICE RowWeights row_weights(const BwdIn& in, int64_t row, int64_t V) {
   if (r.label < 0 || r.label >= V) r.label = -1;
   r.gc = r.label >= 0 && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
   r.ce = r.gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f);
-  r.kd = in.g_kd != nullptr ? in.g_kd[row] * in.tau * in.psum[row] : 0.f;
+  r.kd = in.g_kd != nullptr && in.psum[row] != 0.f ? in.g_kd[row] * in.tau : 0.f;
   return r;
 }
 
-// The largest magnitude of x[0 .. n) that this thread of 1024 meets.
-PGN_DEVICE float thread_max(const float* __restrict__ x, int64_t n, int tid) {
+// The largest magnitude, among the rows that this thread of 1024 meets, of the gradient of the cross entropy (which 0:
+// of rows with a label), the distillation loss (1: of rows with a teacher) or the log-denominator (2). A row whose loss
+// is a constant 0 takes no part: its weight, of any size, is no weight of dl's.
+PGN_DEVICE float thread_max(const BwdIn& in, int which, int64_t n, int64_t V, int tid) {
+  typedef int64_t i64x4_any __attribute__((__vector_size__(32), __aligned__(8)));
+  typedef float f32x4_any __attribute__((__vector_size__(16), __aligned__(4)));
+  const float* x = which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse;
   float g = 0.f;
+  auto take = [&](float v, int64_t label, float some) {
+    g = fmaxf(g, label >= 0 && label < V && some != 0.f ? fabsf(v) : 0.f);
+  };
 #pragma unroll 2
   for (int64_t k = 4 * tid; k + 4 <= n; k += 4096) {
     const f32x4 v = *reinterpret_cast<const f32x4*>(x + k);
-    g = fmaxf(g, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    i64x4_any label{};
+    f32x4_any some{1.f, 1.f, 1.f, 1.f};
+    if (which == 0) label = *reinterpret_cast<const i64x4_any*>(in.y + k);
+    if (which == 1) some = *reinterpret_cast<const f32x4_any*>(in.psum + k);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) take(v[u], label[u], some[u]);
   }
-  if (tid < n % 4) g = fmaxf(g, fabsf(x[n - 1 - tid]));
-  return g;
+  if (tid < n % 4) take(x[n - 1 - tid], which == 0 ? in.y[n - 1 - tid] : 0, which == 1 ? in.psum[n - 1 - tid] : 1.f);
+  return which == 1 ? g * in.tau : g;
 }
 
 // Every workgroup finds G itself (4 us at 8192 rows, launch and latency), from all rows' gradients (at most 256
@@ -509,15 +522,13 @@ __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo*
   const int tid = threadIdx.x;
   float g = 0.f;
   for (int which = 0; which < 3; ++which) {  // (by place: two losses' gradients may be one array)
-    const float* x = which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse;
-    if (x == nullptr) continue;
-    g = thread_max(x, n, tid);
+    if ((which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse) == nullptr) continue;
+    g = thread_max(in, which, n, V, tid);
     for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
     __syncthreads();
     if ((tid & 63) == 0) most[tid >> 6] = g;
     __syncthreads();
     for (int k = 0; k < 16; ++k) g = fmaxf(g, most[k]);
-    if (which == 1) g *= in.tau;
     if (g > 0.f && g < INFINITY) break;
   }
   if (!(g > 0.f && g < INFINITY)) g = 1.f;

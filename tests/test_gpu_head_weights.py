@@ -18,6 +18,35 @@ def kd_grads(h, W, y, ids, z, tau, g_kd, g_ce=None):
     return torch.autograd.grad(kd if y is None else (kd, ce), (a, b), g_kd if y is None else (g_kd, g_ce))
 
 
+@pytest.mark.parametrize("size", SIZES)
+def test_weights_on_padded_labels(size):
+    """Whatever the weight of a token without a label, the gradients keep their bits."""
+    h, W, y, g = inputs(300, 270, 64, seed=6, pad=0.2)
+    y[1], y[2] = 270, -1
+    gc = 1e-4 * torch.rand(300, generator=g).cuda()
+    there = (y >= 0) & (y < 270)
+    want = ce_grads(h, W, y, torch.where(there, gc, 0))
+    assert want[2].any() and want[3].any()
+    for a, b in zip(ce_grads(h, W, y, torch.where(there, gc, size)), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("labels", [False, True])
+@pytest.mark.parametrize("size", SIZES)
+def test_weights_on_tokens_without_a_teacher(size, labels):
+    """Likewise for a token whose teacher's list is empty, in the distillation loss."""
+    h, W, y, g = inputs(120, 270, 64, seed=7)
+    ids, z = teacher(120, 270, 6, g)
+    ids[::5] = -1
+    none = ~((ids >= 0) & (ids < 270)).any(1)
+    gk, gc = 1e-4 * torch.rand(120, generator=g).cuda(), 1e-4 * torch.rand(120, generator=g).cuda()
+    y = y if labels else None
+    want = kd_grads(h, W, y, ids, z, 2.0, torch.where(none, 0, gk), gc)
+    assert want[0].any() and want[1].any()
+    got = kd_grads(h, W, y, ids, z, 2.0, torch.where(none, size, gk), gc)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("tau", [1.0, 3.0])
 def test_one_weight_tensor_for_both_losses(tau):
     """The weights of the two losses in one tensor, or in two of equal values: the same bits."""
