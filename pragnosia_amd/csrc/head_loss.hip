@@ -638,7 +638,7 @@ __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const float* __re
   float x = 0.f;
   if (r.ce != 0.f || r.kd != 0.f || r.gc != 0.f) {
     const float l = zl[e], g = *scale;
-    x = r.kd / g * (expf(l / in.tau - in.lse_t[row]) - p[e]);
+    if (r.kd != 0.f) x = r.kd / g * (expf(l / in.tau - in.lse_t[row]) - p[e]);  // (a token's p may be NaN, its weight 0)
     if (r.ce != 0.f) x += r.ce / g * expf(l - in.lse[row]);
     if (r.label == v) x -= r.gc / g;
   }

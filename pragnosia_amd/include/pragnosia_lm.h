@@ -45,7 +45,7 @@ int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y, const int
  *         + tau g_kd_i (psum_i exp(l_iv / tau - lse_t_i) - sum_k p_ik [v = ids_ik])
  * rounded to bf16, then dh = dl W (n, d) bf16 and dW = dl^T h (V, d), bf16 or (dw_f32) fp32; either may be NULL. The
  * logits are formed again in pieces of the vocabulary. Rows whose three gradients are zero get a zero dl whatever h
- * holds there. */
+ * holds there, and a row whose g_kd is zero takes nothing from its p, which may be NaN. */
 int64_t pragnosia_head_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d);
 int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd, const void* h, const void* W,
                        const int64_t* y, const float* lse, const float* lse_t, const float* psum, const int32_t* entry,

@@ -55,3 +55,28 @@ def test_one_weight_tensor_for_both_losses(tau):
     gk = torch.rand(300, generator=g).cuda()
     one, two = kd_grads(h, W, y, ids, z, tau, gk, gk), kd_grads(h, W, y, ids, z, tau, gk, gk.clone())
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_teacher_taken_out_of_the_loss(bad):
+    """A token whose teacher is no distribution (its loss is NaN), its weight zero: the gradients of the token's cross
+    entropy, and of all other tokens, are those with any finite logits there."""
+    n, V, d = 40, 90, 64
+    h, W, y, g = inputs(n, V, d, seed=10, pad=0)
+    ids = torch.stack([torch.randperm(V, generator=g)[:7] for _ in range(n)]).cuda()
+    z = torch.randn(n, 7, generator=g).cuda()
+    keep = torch.arange(n, device="cuda") % 4 != 1
+    gk, gc = torch.randn(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    worse = z.clone()
+    worse[1::4, 2] = bad
+    for tau in (1.0, 2.0):
+        grads = []
+        for logits in (z, worse):
+            a, b = h.clone().requires_grad_(), W.clone().requires_grad_()
+            kd, ce = linear_distill(a, b, ids, logits, tau, y)
+            loss = (torch.where(keep, kd, 0) * gk + ce * gc).sum()
+            assert torch.isfinite(loss)
+            grads.append(torch.autograd.grad(loss, (a, b)))
+        assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(*grads))
+        want = oracle(h, W, y, gc, None, ids, z, tau, torch.where(keep, gk, 0))
+        near(grads[1][0], want["dh"], "dh", 2.0 ** -8), near(grads[1][1], want["dW"], "dW", 2.0 ** -8)
