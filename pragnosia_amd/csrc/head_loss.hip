@@ -465,27 +465,33 @@ struct BwdIn {
 // gc [v = label], the exponents in base 2; zero where not live.
 //
 // G is the largest of the rows' gradients of the cross entropy (of the distillation loss, where there is no label: a
-// teacher's probabilities are no constants, and round at random), over the rows that have a label (a teacher). A mean's rows all have the same weight w, and most
-// of a row's gradient is its label's -w (1 - p) with a small p: rounded as it stands, every row would carry the same
-// relative error, that of w's bf16 (up to 2^-8). Over G the weights are 1, the label's element is within 2^-9 and
-// mostly much nearer, and the products are multiplied by G in fp32.
+// teacher's probabilities are no constants, and round at random), over the rows that have a label (a teacher). A mean's
+// rows all have the same weight w, and most of a row's gradient is its label's -w (1 - p) with a small p: rounded as it
+// stands, every row would carry the same relative error, that of w's bf16 (up to 2^-8). Over G the weights are 1, the
+// label's element is within 2^-9 and mostly much nearer, and the products are multiplied by G in fp32. Where another
+// loss's weights are more than 2^64 times as large, or overflow with tau, G is 2^-64 of the largest: neither the large
+// ones overflow over it nor are those of a token that has only the small ones lost.
 struct RowInfo {
   float w0, l0, w1, l1, gc;
   int32_t label, live, unused;
 };
 
 struct RowWeights {
-  float ce, kd, gc;
-  int64_t label;  // -1: none
+  float ce, kd, gc;  // kd over g
+  int64_t label;     // -1: none
 };
 
-PGN_DEVICE RowWeights row_weights(const BwdIn& in, int64_t row, int64_t V) {
+PGN_DEVICE RowWeights row_weights(const BwdIn& in, int64_t row, int64_t V, float g) {
   RowWeights r;
   r.label = in.y != nullptr ? in.y[row] : -1;
   if (r.label < 0 || r.label >= V) r.label = -1;
   r.gc = r.label >= 0 && in.g_ce != nullptr ? in.g_ce[row] : 0.f;
   r.ce = r.gc + (in.g_lse != nullptr ? in.g_lse[row] : 0.f);
-  r.kd = in.g_kd != nullptr && in.psum[row] != 0.f ? in.g_kd[row] * in.tau : 0.f;
+  r.kd = 0.f;
+  if (in.g_kd != nullptr && in.psum[row] != 0.f) {
+    const float kd = in.g_kd[row], x = kd * in.tau;
+    r.kd = fabsf(x) < INFINITY ? x / g : kd / g * in.tau;
+  }
   return r;
 }
 
@@ -511,36 +517,45 @@ PGN_DEVICE float thread_max(const BwdIn& in, int which, int64_t n, int64_t V, in
     for (int u = 0; u < 4; ++u) take(v[u], label[u], some[u]);
   }
   if (tid < n % 4) take(x[n - 1 - tid], which == 0 ? in.y[n - 1 - tid] : 0, which == 1 ? in.psum[n - 1 - tid] : 1.f);
-  return which == 1 ? g * in.tau : g;
+  return g;
 }
 
-// Every workgroup finds G itself (4 us at 8192 rows, launch and latency), from all rows' gradients (at most 256
-// workgroups, `each` rows of their own); *scale = G.
+// Every workgroup finds G itself (4.5 us at 8192 rows, 5.6 with two losses: launch and latency), from all rows'
+// gradients (at most 256 workgroups, `each` rows of their own); *scale = G.
 __global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows,
                                                   float* __restrict__ scale, int64_t n, int64_t V, int64_t each) {
-  __shared__ float most[16];
+  __shared__ float most[3][16];
   const int tid = threadIdx.x;
-  float g = 0.f;
-  for (int which = 0; which < 3; ++which) {  // (by place: two losses' gradients may be one array)
-    if ((which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse) == nullptr) continue;
-    g = thread_max(in, which, n, V, tid);
-    for (int o = 1; o < 64; o *= 2) g = fmaxf(g, __shfl_xor(g, o));
-    __syncthreads();
-    if ((tid & 63) == 0) most[tid >> 6] = g;
-    __syncthreads();
-    for (int k = 0; k < 16; ++k) g = fmaxf(g, most[k]);
-    if (g > 0.f && g < INFINITY) break;
+  float v[3];  // (by place: two losses' gradients may be one array)
+#pragma unroll
+  for (int which = 0; which < 3; ++which) {
+    const bool there = (which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse) != nullptr;
+    v[which] = there ? thread_max(in, which, n, V, tid) : 0.f;
+    for (int o = 1; o < 64; o *= 2) v[which] = fmaxf(v[which], __shfl_xor(v[which], o));
+    if ((tid & 63) == 0) most[which][tid >> 6] = v[which];
   }
-  if (!(g > 0.f && g < INFINITY)) g = 1.f;
+  __syncthreads();
+  float g = 0.f, all = 0.f, raw = 0.f;
+#pragma unroll
+  for (int which = 0; which < 3; ++which) {
+    for (int k = 0; k < 16; ++k) v[which] = fmaxf(v[which], most[which][k]);
+    if (!(v[which] < INFINITY)) continue;
+    raw = fmaxf(raw, v[which]);
+    const float x = which == 1 ? v[which] * in.tau : v[which];
+    if (g == 0.f) g = x;
+    all = fmaxf(all, x);
+  }
+  if (!(all <= g * 0x1p64f && g < INFINITY)) g = raw * 0x1p-64f;
+  if (g == 0.f) g = 1.f;
   if (blockIdx.x == 0 && tid == 0) *scale = g;
   const int64_t end = min(n, (int64_t)(blockIdx.x + 1) * each);
   for (int64_t row = blockIdx.x * each + tid; row < end; row += 1024) {
-    const RowWeights r = row_weights(in, row, V);
+    const RowWeights r = row_weights(in, row, V, g);
     RowInfo o{};
     o.label = (int32_t)r.label;
     o.gc = r.gc / g;
-    o.w0 = (second ? r.ce : r.ce + r.kd) / g;
-    o.w1 = r.kd / g;
+    o.w0 = r.ce / g + (second ? 0.f : r.kd);
+    o.w1 = r.kd;
     o.l0 = (in.lse != nullptr ? in.lse[row] : in.lse_t[row]) * kLog2e;
     o.l1 = second ? in.lse_t[row] * kLog2e : 0.f;
     o.live = r.ce != 0.f || r.kd != 0.f || r.gc != 0.f;
@@ -634,11 +649,12 @@ __global__ __launch_bounds__(256) void head_entry_dl(BwdIn in, const float* __re
   const int64_t row = e / K;
   const int v = entry[e];
   if (v < v_begin || v >= v_begin + words) return;
-  const RowWeights r = row_weights(in, row, V);
+  const float g = *scale;
+  const RowWeights r = row_weights(in, row, V, g);
   float x = 0.f;
   if (r.ce != 0.f || r.kd != 0.f || r.gc != 0.f) {
-    const float l = zl[e], g = *scale;
-    if (r.kd != 0.f) x = r.kd / g * (expf(l / in.tau - in.lse_t[row]) - p[e]);  // (a token's p may be NaN, its weight 0)
+    const float l = zl[e];
+    if (r.kd != 0.f) x = r.kd * (expf(l / in.tau - in.lse_t[row]) - p[e]);  // (p may be NaN where the weight is zero)
     if (r.ce != 0.f) x += r.ce / g * expf(l - in.lse[row]);
     if (r.label == v) x -= r.gc / g;
   }

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from pragnosia_amd.head import linear_distill
+from pragnosia_amd.head import linear_cross_entropy, linear_distill
 from test_gpu_head import ce_grads, inputs, near, oracle, teacher
 
 pytestmark = pytest.mark.gpu
@@ -55,6 +55,32 @@ def test_one_weight_tensor_for_both_losses(tau):
     gk = torch.rand(300, generator=g).cuda()
     one, two = kd_grads(h, W, y, ids, z, tau, gk, gk), kd_grads(h, W, y, ids, z, tau, gk, gk.clone())
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+def near_or_past(got, want, what):
+    """near, or an infinity of the value's sign where the value may be past the type's largest (bf16's is 3.39e38; with
+    weights of 3.5e38 in all, an element of dW is 3.81e38)."""
+    ref, err = want
+    over = got.isinf() & (ref.abs() + err + 2.0 ** -8 * (ref.abs() + err) >= torch.finfo(got.dtype).max)
+    assert torch.equal(got[over] > 0, ref[over] > 0)
+    near(torch.where(over, 0, got), (torch.where(over, 0, ref), err), what, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("small,large", [(1e-30, 1e10), (1e-20, 1e15), (1e-4, 1e8), (1e-38, 1e38)])
+def test_losses_of_very_different_weights(small, large):
+    """One loss's weights may be any size beside the other's: the larger one's gradient where a token has both, and the
+    smaller one's (to 1e-30 at least) where it has only that."""
+    n, V, d = 60, 270, 64
+    h, W, y, g = inputs(n, V, d, seed=9)
+    ids, z = teacher(n, V, 6, g)
+    gk, gc = torch.randn(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    want = oracle(h, W, y, small * gc, None, ids, z, 2.0, large * gk)
+    got = kd_grads(h, W, y, ids, z, 2.0, large * gk, small * gc)
+    near_or_past(got[0], want["dh"], "dh"), near_or_past(got[1], want["dW"], "dW")
+    a, b = h.clone().requires_grad_(), W.clone().requires_grad_()
+    got = torch.autograd.grad(linear_cross_entropy(a, b, y), (a, b), (small * gc, large * gk))
+    want = oracle(h, W, y, small * gc, large * gk)
+    near_or_past(got[0], want["dh"], "dh"), near_or_past(got[1], want["dW"], "dW")
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
