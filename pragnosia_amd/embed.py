@@ -16,7 +16,7 @@ import torch
 from torch import Tensor
 
 from ._lib import PragnosiaError, lm_lib
-from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _once, _workspace
+from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _once, _watched, _workspace
 from .ops import _expect, _require_gpu
 
 
@@ -70,6 +70,8 @@ class _Embedding(torch.autograd.Function):
     @_once
     def backward(ctx, g):
         ids, = ctx.saved_tensors
+        if _watched(g):
+            return None, embed_bwd(g, ids, ctx.V, ctx.scale, ctx.dtype == _BF16), None, None
         return None, _backward(g, ids, ctx.V, ctx.scale, ctx.dtype), None, None
 
 
@@ -129,7 +131,7 @@ def embedding(ids: Tensor, W: Tensor, scale: float = 1.0, dtype: Optional[torch.
             and dtype in _FLOATS and W.shape[0] > 0 and W.shape[1] > 0 and W.shape[1] % 8 == 0
             and math.isfinite(scale)):
         _check_embed("embedding", flat, W, scale, dtype)
-    if torch.compiler.is_compiling():
+    if _watched(flat, W):
         y = embed(flat, W, scale, dtype == _BF16)
     elif torch.is_grad_enabled() and W.requires_grad:
         y = _Embedding.apply(flat, W, scale, dtype)

@@ -15,7 +15,8 @@ gradients that autograd hands back. The gradients of logits are rounded to bf16 
 (in h's type) and dW (in W's; an fp32 W gets the unrounded fp32 sums) are; sums are held in fp32 throughout and taken in
 a fixed order, so the same call gives the same bits.
 
-An eager call goes through an autograd function straight to the C ABI; a traced one (torch.compile) through the custom
+An eager call goes through an autograd function straight to the C ABI. One that something records or replaces
+(torch.compile, torch.export, make_fx, torch.jit.trace, a dispatch mode, tensors of another class) goes through the custom
 ops, whose dispatch costs tens of microseconds a call.
 """
 from __future__ import annotations
@@ -62,6 +63,22 @@ def _call(what: str, fn, t: Tensor, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, what)
+
+
+_Parameter, _compiling, _modes = torch.nn.Parameter, torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack
+_tracing, _included = torch._C._is_tracing, torch._C._dispatch_tls_is_dispatch_key_included
+_PRE = torch._C.DispatchKey.PreDispatch
+
+
+def _watched(*ts: Optional[Tensor]) -> bool:
+    """Whether torch's operations on these tensors are recorded or replaced by something other than autograd: a trace, a
+    dispatch mode, a tensor class of its own. The direct calls are no operations to it; the custom ops are."""
+    if _compiling() or _modes() or _tracing() or _included(_PRE):
+        return True
+    for t in ts:
+        if t is not None and type(t) is not Tensor and type(t) is not _Parameter:
+            return True
+    return False
 
 
 def _once(backward):
@@ -189,8 +206,15 @@ class _HeadLoss(torch.autograd.Function):
     @_once
     def backward(ctx, g_ce, g_lse, g_kd):
         h, W, y, lse, stats = ctx.saved_tensors
-        dh, dW = _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, ctx.K, ctx.tau, ctx.needs_input_grad[0],
-                           ctx.needs_input_grad[1], ctx.types[1] == _F32)
+        need_h, need_W = ctx.needs_input_grad[:2]
+        if _watched(g_ce, g_lse, g_kd):
+            none = W.new_empty(0, dtype=_F32)
+            dh, dW = head_loss_bwd(g_ce, g_lse, g_kd, h.to(ctx.types[0]), W.to(ctx.types[1]), y,
+                                   none if lse is None else lse, none.to(torch.int32) if stats is None else stats,
+                                   ctx.tau, need_h, need_W)
+            return dh if need_h else None, dW if need_W else None, None, None, None, None
+        dh, dW = _backward(g_ce, g_lse, g_kd, h, W, y, lse, stats, ctx.K, ctx.tau, need_h, need_W,
+                           ctx.types[1] == _F32)
         if dh is not None and ctx.types[0] != _BF16:
             dh = dh.to(ctx.types[0])
         return dh, dW, None, None, None, None
@@ -280,7 +304,7 @@ def _losses(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Te
         h = h.reshape(-1, h.shape[-1])
         y = None if y is None else y.reshape(-1)
         ids, z = (None, None) if ids is None else (ids.reshape(-1, ids.shape[-1]), z.reshape(-1, z.shape[-1]))
-    if torch.compiler.is_compiling():
+    if _watched(h, W, y, ids, z):
         got = head_loss(h, W, y, ids, z, tau)[:3]
     else:
         if not _plain_call(h, W, y, ids, z, tau):
