@@ -16,7 +16,8 @@ import torch
 from torch import Tensor
 
 from ._lib import PragnosiaError, lm_lib
-from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _once, _watched, _workspace
+from .head import (_BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _no_tangents, _once, _watched,
+                   _workspace)
 from .ops import _expect, _require_gpu
 
 
@@ -69,6 +70,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, g):
+        _no_tangents("embed_bwd", g)
         ids, = ctx.saved_tensors
         if _watched(g):
             return None, embed_bwd(g, ids, ctx.V, ctx.scale, ctx.dtype == _BF16), None, None
@@ -82,6 +84,7 @@ def embed(ids: Tensor, W: Tensor, scale: float, bf16: bool) -> Tensor:
     """ids (n), W (V, d) -> scale W[ids] (n, d), bf16 or fp32."""
     dtype = _BF16 if bf16 else _F32
     _check_embed("embed", ids, W, scale, dtype)
+    _no_tangents("embed", W)
     return _forward(_as(ids, _I64), _as(W, W.dtype), float(scale), dtype)
 
 
@@ -94,6 +97,7 @@ def _(ids, W, scale, bf16):
 def embed_bwd(g: Tensor, ids: Tensor, V: int, scale: float, bf16: bool) -> Tensor:
     """g (n, d), ids (n) -> dW (V, d), bf16 or fp32."""
     _require_gpu(g, ids)
+    _no_tangents("embed_bwd", g)
     if g.dtype not in _FLOATS or g.dim() != 2 or g.shape[1] % 8 or g.shape[1] == 0 or V <= 0:
         raise PragnosiaError(f"embed_bwd: gradients (n, d) in bf16 or fp32 expected, got {tuple(g.shape)} {g.dtype}")
     if ids.dtype not in _INTS:
@@ -125,6 +129,7 @@ def embedding(ids: Tensor, W: Tensor, scale: float = 1.0, dtype: Optional[torch.
     """scale * W[ids], (..., d) in `dtype` (W's by default; the product is rounded once). W (V, d) bf16 or fp32, d a
     multiple of 8. An id outside [0, V) gives a row of zeros and takes no part in W's gradient."""
     dtype, scale = dtype or W.dtype, float(scale)
+    _no_tangents("embedding", W)
     flat = ids if ids.dim() == 1 else ids.reshape(-1)
     # (the usual call, without the checks' share of a short one)
     if not (W.is_cuda and flat.device == W.device and flat.dtype is _I64 and W.dim() == 2 and W.dtype in _FLOATS

@@ -17,7 +17,8 @@ a fixed order, so the same call gives the same bits.
 
 An eager call goes through an autograd function straight to the C ABI. One that something records or replaces
 (torch.compile, torch.export, make_fx, torch.jit.trace, a dispatch mode, tensors of another class) goes through the custom
-ops, whose dispatch costs tens of microseconds a call.
+ops, whose dispatch costs tens of microseconds a call. Derivatives are reverse mode, once: forward-mode tangents, second
+derivatives and torch.func's transforms raise.
 """
 from __future__ import annotations
 
@@ -27,6 +28,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ._lib import PragnosiaError, check, lm_lib
 from .ops import _expect, _require_gpu
@@ -79,6 +81,14 @@ def _watched(*ts: Optional[Tensor]) -> bool:
         if t is not None and type(t) is not Tensor and type(t) is not _Parameter:
             return True
     return False
+
+
+def _no_tangents(op: str, *ts: Optional[Tensor]) -> None:
+    """A tensor with a forward-mode tangent is refused: the kernels have no forward derivative, and the result would go
+    on without one."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in ts):
+        raise PragnosiaError(f"{op}: forward-mode derivatives are not available (use reverse mode)")
 
 
 def _once(backward):
@@ -205,6 +215,7 @@ class _HeadLoss(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, g_ce, g_lse, g_kd):
+        _no_tangents("head_loss_bwd", g_ce, g_lse, g_kd)
         h, W, y, lse, stats = ctx.saved_tensors
         need_h, need_W = ctx.needs_input_grad[:2]
         if _watched(g_ce, g_lse, g_kd):
@@ -228,6 +239,7 @@ def head_loss(h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Tensor], 
     """h (n, d), W (V, d), y (n) or None, ids and z (n, K) or None. Returns (ce, lse, kd, stats), empty where there are
     no labels or no teacher; stats is what the backward takes."""
     _check_head("head_loss", h, W, y, ids, z, tau)
+    _no_tangents("head_loss", h, W)
     got = _forward(*_operands(h, W, y, ids, z), float(tau))
     types = (_F32, _F32, _F32, torch.int32)
     return tuple(t if t is not None else torch.empty(0, device=h.device, dtype=dt) for t, dt in zip(got, types))
@@ -248,6 +260,7 @@ def head_loss_bwd(g_ce: Optional[Tensor], g_lse: Optional[Tensor], g_kd: Optiona
     """Gradients of head_loss's ce, lse and kd -> (dh, dW) in h's and W's types; empty where not needed. y as given to
     head_loss, lse and stats as it returned them."""
     _require_gpu(g_ce, g_lse, g_kd, h, W, y, lse, stats)
+    _no_tangents("head_loss_bwd", g_ce, g_lse, g_kd, h, W)
     if h.dim() != 2 or W.dim() != 2 or h.dtype not in _FLOATS or W.dtype not in _FLOATS:
         raise PragnosiaError(f"head_loss_bwd: h (n, d) and W (V, d) expected, got {tuple(h.shape)}, {tuple(W.shape)}")
     n, d = h.shape
@@ -299,6 +312,7 @@ def _losses(op: str, h: Tensor, W: Tensor, y: Optional[Tensor], ids: Optional[Te
             t is not None and (t.dim() != h.dim() or t.shape[:-1] != lead) for t in (ids, z)):
         raise PragnosiaError(f"{op}: the labels' and the teacher's leading sizes must be h's {tuple(lead)}, got "
                              f"{[None if t is None else tuple(t.shape) for t in (y, ids, z)]}")
+    _no_tangents(op, h, W)
     flat = h.dim() == 2
     if not flat:
         h = h.reshape(-1, h.shape[-1])

@@ -1,13 +1,15 @@
 """CPU checks of the language model's ends under torch's traces and modes: what records or replaces torch's operations
-sees the custom ops. Nothing is launched: the calls into the library are left out, so results hold anything and only
-their shapes and the record are looked at."""
+sees the custom ops, and a forward-mode tangent is refused. Nothing is launched: the calls into the library are left out,
+so results hold anything and only their shapes and the record are looked at."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from pragnosia_amd import embed, head
+from pragnosia_amd._lib import PragnosiaError
 
 n, V, d, K = 6, 11, 16, 3
 
@@ -161,3 +163,46 @@ def test_an_eager_call_is_direct(calls):
                 node = node.next_functions[0][0] if node.next_functions else None
             if t is not W:
                 assert names & {"_HeadLossBackward", "_EmbeddingBackward"}, names
+
+
+OPS = [lambda h, W, y, ids, z: torch.ops.pragnosia_lm.head_loss(h, W, y, ids, z, 2.0),
+       lambda h, W, y, ids, z: torch.ops.pragnosia_lm.embed(y, W, 1.0, False)]
+
+
+@pytest.mark.parametrize("f", [f for f, _ in CALLS] + OPS)
+def test_tangents_are_refused(f):
+    """A dual tensor raises, whether it requires a gradient or not, and whichever operand it is; without a tangent a
+    forward-mode level changes nothing. (The table of ids and the teacher's logits have none to lose.)"""
+    h, W, *rest = operands()
+    with forward_ad.dual_level():
+        plain = _flat(f(h, W, *rest))
+        assert all(forward_ad.unpack_dual(t).tangent is None for t in plain if t.is_floating_point())
+        for which in (0, 1):
+            if which == 0 and (f is rows or f is OPS[1]):
+                continue
+            for grad in (False, True):
+                pair = [h.clone().requires_grad_(grad), W.clone().requires_grad_(grad)]
+                pair[which] = forward_ad.make_dual(pair[which], torch.ones_like(pair[which]))
+                with pytest.raises((PragnosiaError, NotImplementedError), match="forward"):
+                    f(*pair, *rest)
+
+
+@pytest.mark.parametrize("f,op", CALLS)
+def test_tangents_of_a_gradient_are_refused(f, op):
+    h, W, *rest = operands(True)
+    out = _flat(f(h, W, *rest))[0]
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(PragnosiaError, match="forward"):
+            torch.autograd.grad(out, W, g)
+
+
+@pytest.mark.parametrize("f,op", CALLS)
+def test_transforms_are_refused(f, op):
+    """torch.func's transforms raise."""
+    h, W, *rest = operands()
+    call = lambda w: _flat(f(h, w, *rest))[0].sum()
+    for run in (lambda: torch.func.jvp(call, (W,), (W,)), lambda: torch.func.grad(call)(W),
+                lambda: torch.func.vmap(call)(W.expand(2, V, d))):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            run()
