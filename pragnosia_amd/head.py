@@ -269,7 +269,8 @@ def head_loss_bwd(g_ce: Optional[Tensor], g_lse: Optional[Tensor], g_kd: Optiona
     K = (stats.numel() // n - 2) // 3 if n and stats.numel() else 0
     if stats.numel() not in (0, n * (2 + 3 * K)) or lse.dtype != _F32 or stats.dtype != torch.int32:
         raise PragnosiaError("head_loss_bwd: lse and stats must be head_loss's")
-    if (y is None and (g_ce is not None or g_lse is not None)) or (K == 0 and g_kd is not None):
+    # (of no tokens there are no entries to tell K by, and the gradients are zeros)
+    if (y is None and (g_ce is not None or g_lse is not None)) or (n and K == 0 and g_kd is not None):
         raise PragnosiaError("head_loss_bwd: a gradient of a loss that was not computed")
     dh, dW = _backward(g_ce, g_lse, g_kd, _as(h, _BF16), _as(W, _BF16), _as(y, _I64),
                        None if y is None else _as(lse, _F32), _as(stats, torch.int32) if K else None, K, float(tau),

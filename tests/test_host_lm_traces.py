@@ -1,6 +1,8 @@
 """CPU checks of the language model's ends under torch's traces and modes: what records or replaces torch's operations
 sees the custom ops, and a forward-mode tangent is refused. Nothing is launched: the calls into the library are left out,
 so results hold anything and only their shapes and the record are looked at."""
+import contextlib
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -206,3 +208,23 @@ def test_transforms_are_refused(f, op):
                 lambda: torch.func.vmap(call)(W.expand(2, V, d))):
         with pytest.raises((RuntimeError, NotImplementedError)):
             run()
+
+
+@pytest.mark.parametrize("f,op", CALLS)
+@pytest.mark.parametrize("way", ["eager", "mode", "compiled"])
+def test_empty_batch(f, op, way):
+    """No tokens: empty results, and gradients of zeros, by every way."""
+    h, W, *rest = operands()
+    h, W = h[:0].clone().requires_grad_(), W.requires_grad_()
+    rest = [t[:0] for t in rest]
+    if way == "compiled":
+        torch._dynamo.reset()
+        f = torch.compile(f, backend="aot_eager", fullgraph=True)
+    watch = Watch()
+    with watch if way == "mode" else contextlib.nullcontext():
+        out = _flat(f(h, W, *rest))
+        assert all(t.shape[0] == 0 for t in out)
+        sum(t.float().sum() for t in out).backward()
+    if op == "head_loss":
+        assert h.grad.shape == (0, d) and W.grad.shape == (V, d) and not W.grad.any()
+    assert W.grad.dtype == W.dtype and W.grad.shape == W.shape
