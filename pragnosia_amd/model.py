@@ -108,6 +108,8 @@ def _total(x):
 
 
 class LM(nn.Module):
+    fused_ends = False  # (of a model saved whole before there was the switch, too)
+
     def __init__(self, vocab=8192, d=768, layers=12, mlp_mult=4, ctx=512, mixer="aspin", norm="ln", short_conv=0,
                  fused_ends=False, **unused):
         super().__init__()
