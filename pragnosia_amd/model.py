@@ -186,7 +186,7 @@ class LM(nn.Module):
         `head.linear_cross_entropy`, for fp32 and bf16: no logits at all (`chunks` says nothing then)."""
         low = (torch.float32, torch.bfloat16)
         if self.fused_ends and h.is_cuda and h.dtype in low and self.e.weight.dtype in low and self.d % 8 == 0:
-            return _total(linear_cross_entropy(h, self.e.weight, y)[0]) / y.numel()
+            return _total(linear_cross_entropy(h, self.e.weight, y.reshape(h.shape[:-1]))[0]) / y.numel()
         hf, yf = h.reshape(-1, h.shape[-1]), y.reshape(-1)
         n = hf.shape[0]
 
