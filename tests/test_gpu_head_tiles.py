@@ -21,7 +21,7 @@ def words_of_tile(n, V, d, K):
 
 
 def teacher_of(n, V, K, g):
-    """K different words a token, lists cut short at random, on the GPU (a permutation a row takes the host too long)."""
+    """K different words a token, lists cut short at random, on the GPU (permutations take the host too long)."""
     gd = torch.Generator(device="cuda").manual_seed(int(torch.randint(1 << 30, (1,), generator=g)))
     ids = torch.rand(n, V, generator=gd, device="cuda").topk(K, 1).indices
     keep = torch.randint(0, K + 1, (n, 1), generator=gd, device="cuda")
@@ -113,3 +113,56 @@ def test_rows_past_32_bits(n, V):
         for part in ([slice(None), slice(past, None), slice(-1, None)] if ref.shape[0] == rows else [slice(None)]):
             r, e = (ref, err) if ref.shape[0] == rows else (ref[:, :-1], err[:, :-1])
             assert (e[part].norm() < 0.25 * r[part].norm()) and r[part].any()
+
+
+def test_longest_batch():
+    """2^24 tokens, the most there may be. Positive hidden rows and one label, so that no sum cancels: an fp32 sum over
+    the tokens, 32 products a step, is off by (2^24 / 32 + 64) 2^-24 of itself at most, 3.2%."""
+    n, V, d = 1 << 24, 24, 8
+    g = torch.Generator(device="cuda").manual_seed(31)
+    h = (0.5 + torch.rand(n, d, generator=g, device="cuda")).bfloat16().requires_grad_()
+    W = torch.randn(V, d, generator=g, device="cuda").bfloat16().requires_grad_()
+    y = torch.where(torch.rand(n, generator=g, device="cuda") < 0.1, -100, 3)
+    y[0], y[-1] = 3, 3
+    loss, lse = linear_cross_entropy(h, W, y)
+    dh, dW = torch.autograd.grad(loss.sum(), (h, W))
+    want_dW = torch.zeros(V, d, device="cuda", dtype=torch.float64)
+    with torch.no_grad():
+        for a in range(0, n, 1 << 21):
+            part = slice(a, a + (1 << 21))
+            want = oracle(h[part], W, y[part], torch.ones(1 << 21, device="cuda"))
+            near(loss[part], want["ce"], "ce"), near(lse[part], want["lse"], "lse")
+            near(dh[part], want["dh"], "dh", 2.0 ** -8)
+            want_dW += want["dW"][0]
+    # (dl's rounding and the logits' errors, 2^-7 of it in all, and the result's rounding)
+    assert ((dW.double() - want_dW).abs() <= (0.032 + 2.0 ** -7 + 2.0 ** -8) * want_dW.abs()).all()
+
+
+def test_largest_vocabulary():
+    """2^24 words. A row's 2^19 pieces of 32 words (eight a lane, two exchanges) are joined by 64 threads, 8192 one by one,
+    and six steps: the sum of exponentials is off by 8300 2^-24 of itself at most, 2^-10.9."""
+    n, V, d = 5, 1 << 24, 8
+    g = torch.Generator(device="cuda").manual_seed(32)
+    h = torch.randn(n, d, generator=g, device="cuda").bfloat16().requires_grad_()
+    W = torch.randn(V, d, generator=g, device="cuda").bfloat16().requires_grad_()
+    y = torch.tensor([0, V - 1, V, V // 2 + 1, 12345], device="cuda")
+    loss, lse = linear_cross_entropy(h, W, y)
+    dh, dW = torch.autograd.grad(loss.sum(), (h, W))
+    with torch.no_grad():
+        h64, W64 = h.double(), W.double()
+        x = h64 @ W64.t()
+        want = torch.logsumexp(x, 1)
+        assert ((lse - want).abs() <= 2.0 ** -10.9).all()
+        on = y < V
+        label = x.gather(1, y.clamp(max=V - 1)[:, None])[:, 0]
+        assert ((loss - torch.where(on, want - label, 0)).abs() <= 2.0 ** -10.9).all()
+        dl = (x - want[:, None]).exp()
+        dl[torch.arange(n), y.clamp(max=V - 1)] -= 1
+        dl *= on[:, None]
+        # an element of dl: 2^-10.9 for the sum, 2^-8 for its rounding, 2^-7.8 in all; dh sums 57 pieces of the words,
+        # in parts of at most 2^13, 32 a step: 1100 2^-24 of the magnitudes at most
+        full = dl.abs() @ W64.abs()
+        assert ((dh - dl @ W64).abs() <= (2.0 ** -7.8 + 2.0 ** -13) * full + 2.0 ** -8 * (dl @ W64).abs()).all()
+        want, full = dl.t() @ h64, dl.abs().t() @ h64.abs()
+        assert ((dW - want).abs() <= (2.0 ** -7.8 + 2.0 ** -20) * full + 2.0 ** -8 * want.abs()).all()
+        assert dW[y[on]].abs().amax(1).min() > 0.1 and dW[-2].any()
