@@ -495,10 +495,10 @@ PGN_DEVICE RowWeights row_weights(const BwdIn& in, int64_t row, int64_t V, float
   return r;
 }
 
-// The largest magnitude, among the rows that this thread of 1024 meets, of the gradient of the cross entropy (which 0:
-// of rows with a label), the distillation loss (1: of rows with a teacher) or the log-denominator (2). A row whose loss
-// is a constant 0 takes no part: its weight, of any size, is no weight of dl's.
-PGN_DEVICE float thread_max(const BwdIn& in, int which, int64_t n, int64_t V, int tid) {
+// The largest magnitude, among the rows of [a, b) that this thread of 1024 meets (a: a multiple of four), of the
+// gradient of the cross entropy (which 0: of rows with a label), the distillation loss (1: of rows with a teacher) or
+// the log-denominator (2). A row whose loss is a constant 0 takes no part: its weight, of any size, is no weight of dl's.
+PGN_DEVICE float thread_max(const BwdIn& in, int which, int64_t a, int64_t b, int64_t V, int tid) {
   typedef int64_t i64x4_any __attribute__((__vector_size__(32), __aligned__(8)));
   typedef float f32x4_any __attribute__((__vector_size__(16), __aligned__(4)));
   const float* x = which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse;
@@ -507,7 +507,7 @@ PGN_DEVICE float thread_max(const BwdIn& in, int which, int64_t n, int64_t V, in
     g = fmaxf(g, label >= 0 && label < V && some != 0.f ? fabsf(v) : 0.f);
   };
 #pragma unroll 2
-  for (int64_t k = 4 * tid; k + 4 <= n; k += 4096) {
+  for (int64_t k = a + 4 * tid; k + 4 <= b; k += 4096) {
     const f32x4 v = *reinterpret_cast<const f32x4*>(x + k);
     i64x4_any label{};
     f32x4_any some{1.f, 1.f, 1.f, 1.f};
@@ -516,29 +516,57 @@ PGN_DEVICE float thread_max(const BwdIn& in, int which, int64_t n, int64_t V, in
 #pragma unroll
     for (int u = 0; u < 4; ++u) take(v[u], label[u], some[u]);
   }
-  if (tid < n % 4) take(x[n - 1 - tid], which == 0 ? in.y[n - 1 - tid] : 0, which == 1 ? in.psum[n - 1 - tid] : 1.f);
+  const int64_t k = b - 1 - tid;
+  if (tid < (b - a) % 4) take(x[k], which == 0 ? in.y[k] : 0, which == 1 ? in.psum[k] : 1.f);
   return g;
 }
 
-// Every workgroup finds G itself (4.5 us at 8192 rows, 5.6 with two losses: launch and latency), from all rows'
-// gradients (at most 256 workgroups, `each` rows of their own); *scale = G.
-__global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows,
-                                                  float* __restrict__ scale, int64_t n, int64_t V, int64_t each) {
+// The three losses' maxima over the workgroup's 1024 threads (by place: two losses' gradients may be one array): of
+// rows [a, b), or of the `parts` triples of `part` where there are any.
+PGN_DEVICE void group_max(const BwdIn& in, const float* __restrict__ part, int parts, int64_t a, int64_t b, int64_t V,
+                          float (&v)[3]) {
   __shared__ float most[3][16];
   const int tid = threadIdx.x;
-  float v[3];  // (by place: two losses' gradients may be one array)
 #pragma unroll
   for (int which = 0; which < 3; ++which) {
     const bool there = (which == 0 ? in.g_ce : which == 1 ? in.g_kd : in.g_lse) != nullptr;
-    v[which] = there ? thread_max(in, which, n, V, tid) : 0.f;
+    v[which] = 0.f;
+    if (there && parts == 0) v[which] = thread_max(in, which, a, b, V, tid);
+    if (tid < parts) v[which] = part[3 * tid + which];
     for (int o = 1; o < 64; o *= 2) v[which] = fmaxf(v[which], __shfl_xor(v[which], o));
     if ((tid & 63) == 0) most[which][tid >> 6] = v[which];
   }
   __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 3; ++which)
+    for (int k = 0; k < 16; ++k) v[which] = fmaxf(v[which], most[which][k]);
+}
+
+// Rows' maxima by workgroup, for head_rows over many rows: part[3 b ..], `each` rows a workgroup.
+__global__ __launch_bounds__(1024) void head_most(BwdIn in, float* __restrict__ part, int64_t n, int64_t V,
+                                                  int64_t each) {
+  float v[3];
+  group_max(in, nullptr, 0, blockIdx.x * each, min(n, (int64_t)(blockIdx.x + 1) * each), V, v);
+  if (threadIdx.x < 3) part[3 * blockIdx.x + threadIdx.x] = threadIdx.x == 0 ? v[0] : threadIdx.x == 1 ? v[1] : v[2];
+}
+
+// Rows past which the maxima are found by a launch of their own, as every workgroup of head_rows would read all rows'
+// gradients and labels (32768 rows: 9.0 us in one launch, 8.5 in two; 65536: 13.6, 8.6; 2^20: 161, 18).
+constexpr int64_t kManyRows = (int64_t)1 << 15;
+constexpr int64_t kMostBytes = 256 * 3 * sizeof(float);
+
+// Every workgroup finds G itself (4.5 us at 8192 rows, 5.6 with two losses: launch and latency), from all rows'
+// gradients (at most 256 workgroups, `each` rows of their own); *scale = G. Past kManyRows rows, from `parts` maxima of
+// head_most's.
+__global__ __launch_bounds__(1024) void head_rows(BwdIn in, int second, RowInfo* __restrict__ rows,
+                                                  float* __restrict__ scale, const float* __restrict__ part, int parts,
+                                                  int64_t n, int64_t V, int64_t each) {
+  const int tid = threadIdx.x;
+  float v[3];
+  group_max(in, part, parts, 0, n, V, v);
   float g = 0.f, all = 0.f, raw = 0.f;
 #pragma unroll
   for (int which = 0; which < 3; ++which) {
-    for (int k = 0; k < 16; ++k) v[which] = fmaxf(v[which], most[which][k]);
     if (!(v[which] < INFINITY)) continue;
     raw = fmaxf(raw, v[which]);
     const float x = which == 1 ? v[which] * in.tau : v[which];
@@ -850,7 +878,7 @@ extern "C" int pragnosia_head_fwd(const void* h, const void* W, const int64_t* y
 extern "C" int64_t pragnosia_head_bwd_workspace_bytes(int64_t n, int64_t V, int64_t d) {
   if (!head_shape_ok(n, V, d, 0)) return -1;
   const GradPlan pl = choose_grads(n, V, d);
-  return pl.dl_bytes + pl.part_h + pl.part_w + n * (int64_t)sizeof(RowInfo) + 16;
+  return pl.dl_bytes + pl.part_h + pl.part_w + n * (int64_t)sizeof(RowInfo) + 16 + (n > kManyRows ? kMostBytes : 0);
 }
 
 extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const float* g_kd, const void* h,
@@ -878,8 +906,11 @@ extern "C" int pragnosia_head_bwd(const float* g_ce, const float* g_lse, const f
   float *part_h = (float*)(ws + pl.dl_bytes), *part_w = (float*)(ws + pl.dl_bytes + pl.part_h);
   RowInfo* rows = (RowInfo*)(ws + pl.dl_bytes + pl.part_h + pl.part_w);
   float* scale = (float*)(rows + n);
-  const int64_t each = std::max<int64_t>(256, tiles(n, 256));
-  hipLaunchKernelGGL(head_rows, dim3((unsigned)tiles(n, each)), dim3(1024), 0, st, in, second, rows, scale, n, V, each);
+  const int64_t each = std::max<int64_t>(256, round_up(tiles(n, 256), 4));
+  const int groups = (int)tiles(n, each), parts = n > kManyRows ? groups : 0;
+  float* most = scale + 4;
+  if (parts) hipLaunchKernelGGL(head_most, dim3(groups), dim3(1024), 0, st, in, most, n, V, each);
+  hipLaunchKernelGGL(head_rows, dim3(groups), dim3(1024), 0, st, in, second, rows, scale, most, parts, n, V, each);
   for (int64_t q = 0; q < pl.pieces; ++q) {
     const int64_t v0 = q * pl.v_piece, words = std::min(pl.v_piece, V - v0);
     const int64_t ld = round_up(words, kLogitsKinds[pl.logits].x);

@@ -106,3 +106,21 @@ def test_teacher_taken_out_of_the_loss(bad):
         assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(*grads))
         want = oracle(h, W, y, gc, None, ids, z, tau, torch.where(keep, gk, 0))
         near(grads[1][0], want["dh"], "dh", 2.0 ** -8), near(grads[1][1], want["dW"], "dW", 2.0 ** -8)
+
+
+@pytest.mark.parametrize("n", [32768, 32769, 70001])
+def test_many_tokens(n):
+    """The scale over more tokens than one workgroup looks at: padding's weights have no say, one large weight (the last
+    token's, a workgroup's first or last) does."""
+    V, d = 40, 16
+    h, W, y, g = inputs(n, V, d, seed=11, pad=0.2)
+    for at in (0, 255, 256, 1023, n - 1, None):
+        gc = 1e-4 * torch.rand(n, generator=g).cuda()
+        if at is not None:
+            y[at], gc[at] = 7, -3.0
+        here = torch.where(y >= 0, gc, 0)
+        want = ce_grads(h, W, y, here)
+        for a, b in zip(ce_grads(h, W, y, torch.where(y >= 0, gc, 3e38)), want):
+            assert torch.equal(a, b)
+        ref = oracle(h, W, y, here)
+        near(want[2], ref["dh"], "dh", 2.0 ** -8), near(want[3], ref["dW"], "dW", 2.0 ** -8)
