@@ -12,13 +12,14 @@ Linear's operands. The reference's LM forms its logits in chunks of rows under a
 
 Every loss comes per token in fp32, so a mean, a mask or weights are the caller's own: the kernels take the per-token
 gradients that autograd hands back. The gradients of logits are rounded to bf16 once, before the two products that dh
-(in h's type) and dW (in W's; an fp32 W gets the unrounded fp32 sums) are; sums are held in fp32 throughout and taken in
-a fixed order, so the same call gives the same bits.
+(in h's type, but always rounded to bf16 first, as autocast's product gives it) and dW (in W's; an fp32 W gets the
+unrounded fp32 sums) are; sums are held in fp32 throughout and taken in a fixed order, so the same call gives the same
+bits.
 
 An eager call goes through an autograd function straight to the C ABI. One that something records or replaces
-(torch.compile, torch.export, make_fx, torch.jit.trace, a dispatch mode, tensors of another class) goes through the custom
-ops, whose dispatch costs tens of microseconds a call. Derivatives are reverse mode, once: forward-mode tangents, second
-derivatives and torch.func's transforms raise.
+(torch.compile, torch.export, make_fx, torch.jit.trace, a dispatch mode, tensors of another class) goes through the
+custom ops, whose dispatch costs tens of microseconds a call. Derivatives are reverse mode, once: forward-mode tangents,
+second derivatives and torch.func's transforms raise.
 """
 from __future__ import annotations
 

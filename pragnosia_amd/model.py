@@ -183,7 +183,9 @@ class LM(nn.Module):
     def loss(self, h, y, chunks=4):
         """Mean cross-entropy of the tied head over (B, T) targets, the logits formed chunk by chunk under
         activation checkpointing so at most one chunk's logits exist at a time. With fused_ends the kernels of
-        `head.linear_cross_entropy`, for fp32 and bf16: no logits at all (`chunks` says nothing then)."""
+        `head.linear_cross_entropy`, for fp32 and bf16: no logits at all (`chunks` says nothing then). Either way fp32
+        hidden rows and table are rounded to bf16 for the products; the gradient of the hidden rows passes through
+        bf16, the fused table's is summed and kept in its own type."""
         low = (torch.float32, torch.bfloat16)
         if self.fused_ends and h.is_cuda and h.dtype in low and self.e.weight.dtype in low and self.d % 8 == 0:
             return _total(linear_cross_entropy(h, self.e.weight, y.reshape(h.shape[:-1]))[0]) / y.numel()
@@ -207,7 +209,8 @@ class LM(nn.Module):
     def distill_loss(self, h, ids, logits, tau=1.0, y=None):
         """Mean distillation loss of the tied head over (B, T) tokens from a teacher's top logits, ids and logits
         (B, T, K), at temperature tau; with targets y (B, T) also their mean cross-entropy, from the same pass over the
-        vocabulary: (distillation, cross-entropy or None). See `head.linear_distill`."""
+        vocabulary: (distillation, cross-entropy or None). fp32 hidden rows and table are rounded to bf16 for the
+        products, and the hidden rows' gradient passes through bf16. See `head.linear_distill`."""
         kd, ce = linear_distill(h, self.e.weight, ids, logits, tau, y)
         n = kd.numel()
         return _total(kd) / n, None if ce is None else _total(ce) / n

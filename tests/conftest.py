@@ -18,8 +18,8 @@ def pytest_configure(config):
 
 # Tests whose expected value is wrong: a distillation loss whose list repeats a word is tau^2 KL(p || q) with the word's
 # probability the sum of its entries', and these expect sum_k p_k log p_k over the entries instead (for student logits
-# 3, 0, 0, 0 and the first word twice -0.554, a negative divergence, where it is 0.139). tests/test_gpu_distill_repeats.py
-# checks the same calls against the words' probabilities.
+# 3, 0, 0, 0 and the first word twice -0.554, a negative divergence, where it is 0.139).
+# tests/test_gpu_distill_repeats.py checks the same calls against the words' probabilities.
 WRONG_VALUE = ("test_gpu_head.py::test_teacher_edges", "test_gpu_lm_ends.py::test_training_step[True-aspin]",
                "test_gpu_lm_ends.py::test_training_step[True-dspin]")
 

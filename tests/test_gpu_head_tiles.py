@@ -139,8 +139,8 @@ def test_longest_batch():
 
 
 def test_largest_vocabulary():
-    """2^24 words. A row's 2^19 pieces of 32 words (eight a lane, two exchanges) are joined by 64 threads, 8192 one by one,
-    and six steps: the sum of exponentials is off by 8300 2^-24 of itself at most, 2^-10.9."""
+    """2^24 words. A row's 2^19 pieces of 32 words (eight a lane, two exchanges) are joined by 64 threads, 8192 one by
+    one, and six steps: the sum of exponentials is off by 8300 2^-24 of itself at most, 2^-10.9."""
     n, V, d = 5, 1 << 24, 8
     g = torch.Generator(device="cuda").manual_seed(32)
     h = torch.randn(n, d, generator=g, device="cuda").bfloat16().requires_grad_()

@@ -1,6 +1,6 @@
 """CPU checks of the language model's ends under torch's traces and modes: what records or replaces torch's operations
-sees the custom ops, and a forward-mode tangent is refused. Nothing is launched: the calls into the library are left out,
-so results hold anything and only their shapes and the record are looked at."""
+sees the custom ops, and a forward-mode tangent is refused. Nothing is launched: the calls into the library are left
+out, so results hold anything and only their shapes and the record are looked at."""
 import contextlib
 
 import pytest
