@@ -97,8 +97,24 @@ LM_SIGNATURES = {
 _LM_RET_I64 = {"pragnosia_head_fwd_workspace_bytes", "pragnosia_head_bwd_workspace_bytes",
                "pragnosia_embed_bwd_workspace_bytes"}
 
+# the entry points of pragnosia_amd/include/pragnosia_gen.h, in header order
+GEN_SIGNATURES = {
+    "pragnosia_gen_abi_version": [],
+    "pragnosia_fp4_code_bytes": [_i64] * 2,
+    "pragnosia_fp4_scale_bytes": [_i64] * 3,
+    "pragnosia_fp4_quantize": [_p, _i32, _p, _p] + [_i64] * 3 + [_p],
+    "pragnosia_fp4_dequantize": [_p, _p, _p, _i32] + [_i64] * 3 + [_p],
+    "pragnosia_fp4_linear": [_p, _i32] + [_p] * 4 + [_f32, _p, _i32, _p, _p] + [_i64] * 4 + [_p],
+    "pragnosia_rules_workspace_bytes": [_i64] * 2,
+    "pragnosia_rules": [_p, _i32, _p, _i64, _i64, _p, _p] + [_p, _f32] * 3 + [_p, _p, _i64, _i64, _p, _i64] + [_p] * 4
+                       + [_i64] * 3 + [_p],
+}
+
+_GEN_RET_I64 = {"pragnosia_fp4_code_bytes", "pragnosia_fp4_scale_bytes", "pragnosia_rules_workspace_bytes"}
+
 _lib = None
 _lm_lib = None
+_gen_lib = None
 
 
 class PragnosiaError(RuntimeError):
@@ -133,6 +149,19 @@ def lm_lib():
             fn.restype = _i64 if name in _LM_RET_I64 else _i32
         _lm_lib = L
     return _lm_lib
+
+
+def gen_lib():
+    """The loaded library with generation's entry points (pragnosia_amd/include/pragnosia_gen.h) set up too."""
+    global _gen_lib
+    if _gen_lib is None:
+        L = lib()
+        for name, args in GEN_SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.argtypes = args
+            fn.restype = _i64 if name in _GEN_RET_I64 else _i32
+        _gen_lib = L
+    return _gen_lib
 
 
 def check(code: int, what: str) -> None:
