@@ -16,6 +16,8 @@ typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
 typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
 typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
 
+#define PGN_INLINE __attribute__((always_inline))  // of a lambda whose captured arrays have to stay in registers
+
 constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = 1024;
 
 PGN_DEVICE unsigned bits_of(float x) { return __builtin_bit_cast(unsigned, x); }
@@ -33,6 +35,13 @@ struct Raw<float> {
     b = reinterpret_cast<const f32x4*>(p)[1];
   }
   PGN_DEVICE void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  PGN_DEVICE void keep(bool k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = k ? a[e] : 0.f;
+      b[e] = k ? b[e] : 0.f;
+    }
+  }
   PGN_DEVICE float get(int e) const { return e < 4 ? a[e & 3] : b[e & 3]; }
 };
 template <>
@@ -40,6 +49,10 @@ struct Raw<__bf16> {
   u32x4 a;
   PGN_DEVICE void load(const __bf16* p) { a = *reinterpret_cast<const u32x4*>(p); }
   PGN_DEVICE void zero() { a = u32x4{0u, 0u, 0u, 0u}; }
+  PGN_DEVICE void keep(bool k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = k ? a[e] : 0u;
+  }
   PGN_DEVICE float get(int e) const { return e & 1 ? float_of(a[e >> 1] & 0xffff0000u) : bf16_bits(a[e >> 1]); }
 };
 
@@ -197,18 +210,30 @@ PGN_DEVICE void split8(const float (&z)[8], bf16x8 (&part)[P]) {
     for (int e = 0; e < 8; ++e) part[0][e] = pgn_bf16(z[e]);
   } else {
     unsigned u[P][8];
+    float r[8], any = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const unsigned b = bits_of(z[e]);
-      const bool odd = (b & 0x7f800000u) == 0x7f800000u;
-      u[0][e] = (b & 0xffff0000u) | (odd && (b & 0x7fffffu) ? 0x400000u : 0u);  // (a NaN whose bits are all low stays one)
-      float r = odd ? 0.f : z[e] - float_of(b & 0xffff0000u);
+      u[0][e] = bits_of(z[e]) & 0xffff0000u;
+      r[e] = z[e] - float_of(u[0][e]);
+      any += r[e];
+    }
+    if (any != any) {  // an infinity or NaN less itself is NaN
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned b = bits_of(z[e]);
+        if ((b & 0x7f800000u) == 0x7f800000u) {
+          u[0][e] |= b & 0x7fffffu ? 0x400000u : 0u;  // (a NaN whose bits are all low stays one)
+          r[e] = 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
       if constexpr (P == 3) {
-        u[1][e] = bits_of(r) & 0xffff0000u;
-        r -= float_of(u[1][e]);
-        u[2][e] = bits_of(r);
+        u[1][e] = bits_of(r[e]) & 0xffff0000u;
+        u[2][e] = bits_of(r[e] - float_of(u[1][e]));
       } else {
-        u[1][e] = bits_of(r);
+        u[1][e] = bits_of(r[e]);
       }
     }
 #pragma unroll
@@ -221,35 +246,274 @@ PGN_DEVICE void split8(const float (&z)[8], bf16x8 (&part)[P]) {
   }
 }
 
-// Sum over the lanes with the same l % MR, in all of them.
-template <int MR>
-PGN_DEVICE float sum_beside(float x) {
-  if constexpr (MR == 1) return group_sum<64>(x);
-  if constexpr (MR == 4) {
-    x += dpp_move<0x124>(x);  // row_ror:4
-    x += dpp_move<0x128>(x);  // row_ror:8
-  }
-  x = swap_add<16>(x, x);
-  return swap_add<32>(x, x);
+// Sixteen bytes of results.
+template <class T>
+struct Vec;
+template <>
+struct Vec<float> {
+  f32x4 a;
+  PGN_DEVICE void load(const float* p) { a = *reinterpret_cast<const f32x4*>(p); }
+  PGN_DEVICE void store(float* p) const { *reinterpret_cast<f32x4*>(p) = a; }
+  PGN_DEVICE float get(int e) const { return a[e]; }
+  PGN_DEVICE void set(int e, float v) { a[e] = v; }
+};
+template <>
+struct Vec<__bf16> {
+  bf16x8 a;
+  PGN_DEVICE void load(const __bf16* p) { a = *reinterpret_cast<const bf16x8*>(p); }
+  PGN_DEVICE void store(__bf16* p) const { *reinterpret_cast<bf16x8*>(p) = a; }
+  PGN_DEVICE float get(int e) const { return (float)a[e]; }
+  PGN_DEVICE void set(int e, float v) { a[e] = pgn_bf16(v); }
+};
+
+// Mean and 1 / sigma of a row, in all lanes of the wave that calls: the sum, then the squares about the mean. Up to 1024
+// columns the row stays in registers, longer ones are read twice.
+template <class T>
+PGN_DEVICE void row_stats(const T* row, int K, float eps, int l, float& mean, float& rstd) {
+  constexpr int H = 2;
+  Raw<T> raw[H];
+  const bool held = K <= 512 * H;
+  auto load = [&](int k0) PGN_INLINE {
+#pragma unroll
+    for (int u = 0; u < H; ++u) raw[u].load(row + min(k0 + 8 * (l + 64 * u), K - 8));
+  };
+  auto total = [&](auto&& f) PGN_INLINE {
+    float s = 0.f;
+    for (int k0 = 0; k0 < K; k0 += 512 * H) {
+      if (!held) load(k0);
+#pragma unroll
+      for (int u = 0; u < H; ++u) {
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t += f(raw[u].get(e));
+        s += k0 + 8 * (l + 64 * u) < K ? t : 0.f;
+      }
+    }
+    return group_sum<64>(s);
+  };
+  if (held) load(0);
+  mean = total([](float v) { return v; }) / (float)K;
+  const float m = mean, var = total([m](float v) { return (v - m) * (v - m); }) / (float)K;
+  rstd = 1.f / sqrtf(var + eps);
 }
 
-constexpr int kWaves = 4;
+// Eight columns of a row as P bf16 parts, normalised where there is a norm; zeros past the last column, where the load
+// was of others. (K is a multiple of 8. Loads stand under no condition: behind one the compiler cannot count them, and
+// waits for those of the next chunk before it uses this one's.)
+template <class T, int P>
+PGN_DEVICE void stage8(Raw<T> raw, const T* lnw, const T* lnb, float mean, float rstd, int k, int K,
+                       bool tail, bf16x8 (&part)[P]) {
+  if (tail) raw.keep(k < K);
+  if constexpr (P == 1) {
+    part[0] = __builtin_bit_cast(bf16x8, raw.a);
+  } else {
+    float z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = raw.get(e);
+    if (P == 2 || lnw) {
+      Raw<T> g, b;
+      g.load(lnw + min(k, K - 8));
+      b.load((lnb ? lnb : lnw) + min(k, K - 8));
+      if (tail) g.keep(k < K);
+      b.keep(k < K && lnb);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (z[e] - mean) * rstd * g.get(e) + b.get(e);
+    }
+    split8<P>(z, part);
+  }
+}
 
-// A workgroup's share: 16 RT rows (MR of each 16 read: MR = 1 or 4 where there are no more), WN NT column tiles of the
-// 16 columns, WK waves sharing the contracted columns of each (WN WK = 4). Rows go to LDS in P bf16 parts, a chunk of CB
-// blocks of 128 columns at a time, as the matrix core takes them; codes straight to registers, one chunk ahead.
-template <class T, int P, int GS, int MR, int RT, int U, int WK, int NT>
+// A tile's scales of one row: 4 / GS bf16 numbers in one or two words.
+template <int GS>
+struct Scales {
+  unsigned w[GS == 1 ? 2 : 1];
+  PGN_DEVICE void load(const __bf16* p) {
+    if constexpr (GS == 1) {
+      const i32x2 v = *reinterpret_cast<const i32x2*>(p);
+      w[0] = (unsigned)v[0];
+      w[1] = (unsigned)v[1];
+    } else if constexpr (GS == 2) {
+      w[0] = *reinterpret_cast<const unsigned*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const unsigned short*>(p);
+    }
+  }
+  PGN_DEVICE float get(int q) const {
+    const unsigned v = w[GS == 1 ? q >> 1 : 0];
+    return q & 1 ? float_of(v & 0xffff0000u) : bf16_bits(v);
+  }
+};
+
+// acc += one block of 128 columns: RT x NT tiles. x(p, r, ks) is the rows' operand, c and s the tiles' codes and scales.
+template <int P, int GS, int RT, int NT, class X>
+PGN_DEVICE void block(f32x4 (&acc)[RT][NT], const u32x4 (&c)[NT], const Scales<GS> (&s)[NT], X&& x) {
+  constexpr int G = 4 / GS;
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+  if constexpr (RT * NT < 4) {
+    // few tiles: every group's and part's sum a chain of its own, so that the products need not wait for each other
+    f32x4 d[G][P][RT][NT];
+#pragma unroll
+    for (int g = 0; g < GS; ++g)
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        const int ks = q * GS + g;
+        bf16x8 b[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) b[t] = operand(c[t][ks]);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const bf16x8 a = x(p, r, ks);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) d[q][p][r][t] = pgn_mfma(a, b[t], g ? d[q][p][r][t] : zero);
+          }
+      }
+#pragma unroll
+    for (int q = 0; q < G; ++q)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          f32x4 v = d[q][P - 1][r][t];  // the smallest parts first
+#pragma unroll
+          for (int p = P - 2; p >= 0; --p) v += d[q][p][r][t];
+          acc[r][t] += s[t].get(q) * v;
+        }
+  } else {
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+      f32x4 d[RT][NT];
+#pragma unroll
+      for (int g = 0; g < GS; ++g) {
+        const int ks = q * GS + g;
+        bf16x8 b[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) b[t] = operand(c[t][ks]);
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const bf16x8 a = x(p, r, ks);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) d[r][t] = pgn_mfma(a, b[t], g || p < P - 1 ? d[r][t] : zero);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float v = s[t].get(q);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r][t] += v * d[r][t];
+      }
+    }
+  }
+}
+
+template <class T>
+PGN_DEVICE void finish(float v, int row, int col, int N, const T* bias, int act, const T* resid, T* y) {
+  if (bias) v += (float)bias[col];
+  if (act == 1) v = pgn_gelu_erf(v);
+  const size_t off = (size_t)row * N + col;
+  if (resid) v += (float)resid[off];
+  y[off] = (T)v;
+}
+
+// Up to MR = 1 or 4 rows. One tile of 16 columns to a workgroup, its WK waves sharing the blocks of 128 contracted columns.
+// A wave stages its own columns of the rows in LDS of its own, so that only the sums' joining needs a barrier (and four
+// rows' norms another, a wave a row). A wave's loads of a chunk (CBW blocks) are all issued at once.
+template <class T, int P, int GS, int MR, int WK, int CBW>
+__global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u32x4* __restrict__ codes,
+                                               const __bf16* __restrict__ scales, const T* __restrict__ lnw,
+                                               const T* __restrict__ lnb, float eps, const T* __restrict__ bias, int act,
+                                               const T* resid, T* y, int n, int N, int K, int KB) {
+  constexpr int U = MR == 1 ? CBW / 4 : CBW;  // pieces of 8 columns a lane stages: of four blocks, or of four rows
+  static_assert((MR == 1 && CBW % 4 == 0) || (MR == 4 && WK == 4), "");
+  __shared__ bf16x8 rows[WK][P][CBW * 16][MR];
+  __shared__ float sums[WK][MR][16];
+  __shared__ float stat[MR][2];
+  const int tid = threadIdx.x, l = tid & 63, wk = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, h = l >> 4;
+  const int ct = blockIdx.x, m = MR == 1 ? 0 : l & 3;
+  const T* const xr = x + (size_t)min(m, n - 1) * K;
+  // piece u of this lane: block j of the wave's, 8 columns in it
+  auto piece = [&](int u) { return MR == 1 ? 4 * u + h : u; };
+  const int k8 = MR == 1 ? i : l >> 2;
+  Raw<T> raw[U];
+  u32x4 c[CBW][1];
+  Scales<GS> s[CBW][1];
+  auto load = [&](int kb0) PGN_INLINE {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].load(xr + min(kTileCols * (kb0 + WK * piece(u)) + 8 * k8, K - 8));
+#pragma unroll
+    for (int j = 0; j < CBW; ++j) {
+      const size_t tile = (size_t)ct * KB + min(kb0 + WK * j, KB - 1);  // (past the last: not used)
+      c[j][0] = codes[tile * 64 + l];
+      s[j][0].load(scales + (tile * 16 + i) * (4 / GS));
+    }
+  };
+  load(wk);
+  float mean = 0.f, rstd = 1.f;
+  if (P == 2 || (P == 3 && lnw)) {
+    if constexpr (MR == 1) {
+      row_stats(x, K, eps, l, mean, rstd);
+    } else {
+      row_stats(x + (size_t)min(wk, n - 1) * K, K, eps, l, mean, rstd);
+      if (l == 0) {
+        stat[wk][0] = mean;
+        stat[wk][1] = rstd;
+      }
+      __syncthreads();
+      mean = stat[m][0];
+      rstd = stat[m][1];
+    }
+  }
+  f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
+  for (int kb0 = wk; kb0 < KB; kb0 += WK * CBW) {
+    if (kb0 != wk) load(kb0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      bf16x8 part[P];
+      stage8<T, P>(raw[u], lnw, lnb, mean, rstd, kTileCols * (kb0 + WK * piece(u)) + 8 * k8, K, true, part);
+#pragma unroll
+      for (int p = 0; p < P; ++p) rows[wk][p][piece(u) * 16 + k8][m] = part[p];
+    }
+    // the wave reads what its own lanes wrote: LDS works in a wave's order, the compiler is kept to it
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < CBW; ++j)
+      if (kb0 + WK * j < KB)
+        block<P, GS>(acc, c[j], s[j], [&](int p, int, int ks) { return rows[wk][p][j * 16 + 4 * ks + h][i % MR]; });
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (h == 0)
+#pragma unroll
+    for (int r = 0; r < MR; ++r) sums[wk][r][i] = acc[0][0][r];
+  __syncthreads();
+  const int row = tid >> 4, col = ct * 16 + (tid & 15);
+  if (tid < 16 * MR && row < n && col < N) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < WK; ++k) v += sums[k][row][tid & 15];
+    finish(v, row, col, N, bias, act, resid, y);
+  }
+}
+
+// More rows. A workgroup's share: 16 RT rows, WN NT tiles of 16 columns, WK waves sharing the contracted columns of each (WN
+// WK waves). Rows go to LDS in P bf16 parts, a chunk of CB blocks of 128 columns at a time, as the matrix core takes them;
+// codes straight to registers. A chunk's loads are under way while the one before it is multiplied.
+template <class T, int P, int GS, int kWaves, int RT, int U, int WK, int NT>
 __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                       const __bf16* __restrict__ scales, const T* __restrict__ lnw,
                                                       const T* __restrict__ lnb, float eps, const T* __restrict__ bias,
                                                       int act, const T* resid, T* y, int n, int N, int K, int KB,
                                                       int ctiles, int rblocks) {
-  constexpr int WN = kWaves / WK, KL = 64 / MR, CB = U * 16 / (MR * RT), CBW = CB / WK, RW = MR * RT, CK8 = CB * 16;
-  constexpr int WR = kWaves / RT;  // waves that stage the same rows
-  static_assert(CBW * WK * MR * RT == U * 16 && (RT == 1 || MR == 16), "");
+  constexpr int WN = kWaves / WK, WR = kWaves / RT;  // WR waves stage the same rows, 4 pieces of 8 columns each
+  constexpr int CK8 = U * WR * 4, CB = CK8 / 16, CBW = CB / WK;
+  static_assert(CBW * WK * 16 == CK8, "");
   extern __shared__ __align__(16) char smem[];
-  __shared__ float red[2][kWaves][MR];
-  bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);  // [2 chunks][P][CK8][RW]
+  __shared__ float stat[2][16 * RT];
+  bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);  // [2 chunks][P][RT][CK8][16]
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = l & 15, h = l >> 4, wk = w % WK, wn = w / WK;
   // workgroups of the same columns run on one XCD (their numbers differ by multiples of 8)
@@ -259,100 +523,62 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
     rb = rest % rblocks;
     cg = rest / rblocks * 8 + (blockIdx.x & 7);
   }
-  const int ct0 = cg * WN * NT + wn * NT;
+  const int ct0 = cg * WN * NT + wn * NT, row0 = rb * 16 * RT;
   if (cg * WN * NT >= ctiles) return;
   const int nch = (KB + CB - 1) / CB;
 
-  // staging: this thread's row, and its first 8-column piece of a chunk
-  const int srt = w % RT, sm = l % MR, sk = (w / RT) * KL + l / MR;
-  const T* const xr = x + (size_t)min(rb * 16 * RT + 16 * srt + sm, n - 1) * K;
+  // staging: this thread's row, and its first 8-column piece of a chunk. Addresses are a wave's own part plus a lane's 32
+  // bits that no chunk changes: the vector unit has no arithmetic to spare (below).
+  const int srt = w % RT, sk = (w / RT) * 4 + h;
+  const T* const xb = x + (size_t)row0 * K;
+  const unsigned xrow = (unsigned)(min(16 * srt + i, n - 1 - row0) * K), xlane = xrow + 8 * sk;
+  const int full = K / (8 * CK8);  // chunks that lie in the row whole
   Raw<T> raw[U];
-  auto load_x = [&](int c) {
+  auto load_x = [&](int c) PGN_INLINE {
+    if (c < full) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = 8 * (c * CK8 + sk + u * WR * KL);
-      if (k < K) raw[u].load(xr + k);
-      else raw[u].zero();
+      for (int u = 0; u < U; ++u) raw[u].load(xb + (size_t)(8 * (c * CK8 + u * WR * 4)) + xlane);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u].load(xb + (xrow + (unsigned)min(8 * (c * CK8 + sk + u * WR * 4), K - 8)));
     }
   };
-  u32x4 cw[CBW][NT];
-  unsigned sw[CBW][NT][GS == 1 ? 2 : 1];
-  auto load_w = [&](int j, int c) {
-    const int kb = c * CB + wk + WK * j;
-    if (kb >= KB) return;
+  u32x4 cw[CBW][NT], cn[CBW][NT];  // this chunk's codes, the next one's
+  Scales<GS> sw[CBW][NT], sn[CBW][NT];
+  auto load_w = [&](int c, u32x4 (&cc)[CBW][NT], Scales<GS> (&ss)[CBW][NT]) PGN_INLINE {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const size_t tile = (size_t)min(ct0 + t, ctiles - 1) * KB + kb;
-      cw[j][t] = codes[tile * 64 + l];
-      const __bf16* sp = scales + (tile * 16 + i) * (4 / GS);
-      if constexpr (GS == 1) {
-        const i32x2 v = *reinterpret_cast<const i32x2*>(sp);
-        sw[j][t][0] = (unsigned)v[0];
-        sw[j][t][1] = (unsigned)v[1];
-      } else if constexpr (GS == 2) {
-        sw[j][t][0] = *reinterpret_cast<const unsigned*>(sp);
-      } else {
-        sw[j][t][0] = *reinterpret_cast<const unsigned short*>(sp);
+    for (int j = 0; j < CBW; ++j)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const size_t tile = (size_t)min(ct0 + t, ctiles - 1) * KB + min(c * CB + wk + WK * j, KB - 1);
+        cc[j][t] = (codes + tile * 64)[(unsigned)l];
+        ss[j][t].load(scales + tile * (16 * 4 / GS) + (unsigned)(i * (4 / GS)));
       }
-    }
   };
   load_x(0);
-#pragma unroll
-  for (int j = 0; j < CBW; ++j) load_w(j, 0);
-
-  // the row's mean and 1 / sigma: the sum, then the squares about the mean, each over the whole row
+  load_w(0, cw, sw);
   float mean = 0.f, rstd = 1.f;
-  const bool norm = P == 2 || (P == 3 && lnw != nullptr);
-  if (norm) {
-    auto total = [&](auto&& f, int slot) {
-      float s = 0.f;
-      for (int c = 0; c < nch; ++c) {
-        if (nch > 1) load_x(c);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (8 * (c * CK8 + sk + u * WR * KL) < K) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s += f(raw[u].get(e));
-          }
-        }
+  if (P == 2 || (P == 3 && lnw)) {
+    for (int r = w; r < 16 * RT; r += kWaves) {
+      row_stats(x + (size_t)min(row0 + r, n - 1) * K, K, eps, l, mean, rstd);
+      if (l == 0) {
+        stat[0][r] = mean;
+        stat[1][r] = rstd;
       }
-      s = sum_beside<MR>(s);
-      if (l < MR) red[slot][w][l] = s;
-      __syncthreads();
-      s = 0.f;
-#pragma unroll
-      for (int v = 0; v < WR; ++v) s += red[slot][srt + RT * v][sm];
-      return s;
-    };
-    mean = total([](float v) { return v; }, 0) / (float)K;
-    const float var = total([mean](float v) { return (v - mean) * (v - mean); }, 1) / (float)K;
-    rstd = 1.f / sqrtf(var + eps);
-    if (nch > 1) load_x(0);
+    }
+    __syncthreads();
+    mean = stat[0][16 * srt + i];
+    rstd = stat[1][16 * srt + i];
   }
-  auto store_x = [&](int c) {
-    bf16x8* const to = buf + (size_t)(c & 1) * P * CK8 * RW;
+  auto store_x = [&](int c) PGN_INLINE {
+    bf16x8* const to = buf + (c & 1) * P * RT * CK8 * 16;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k8 = sk + u * WR * KL, k = 8 * (c * CK8 + k8);
+      const int k8 = sk + u * WR * 4;
       bf16x8 part[P];
-      if constexpr (P == 1) {
-        part[0] = __builtin_bit_cast(bf16x8, raw[u].a);
-      } else {
-        float z[8];
+      stage8<T, P>(raw[u], lnw, lnb, mean, rstd, 8 * (c * CK8 + k8), K, c >= full, part);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = raw[u].get(e);
-        if (norm && k < K) {
-          Raw<T> g, b;
-          g.load(lnw + k);
-          if (lnb) b.load(lnb + k);
-          else b.zero();
-#pragma unroll
-          for (int e = 0; e < 8; ++e) z[e] = (z[e] - mean) * rstd * g.get(e) + b.get(e);
-        }
-        split8<P>(z, part);
-      }
-#pragma unroll
-      for (int p = 0; p < P; ++p) to[((size_t)p * CK8 + k8) * RW + 16 * srt + sm] = part[p];
+      for (int p = 0; p < P; ++p) to[((p * RT + srt) * CK8 + k8) * 16 + i] = part[p];
     }
   };
   store_x(0);
@@ -362,88 +588,93 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int c = 0; c < nch; ++c) {
-    __syncthreads();
-    if (c + 1 < nch) load_x(c + 1);
-    const bf16x8* const from = buf + (size_t)(c & 1) * P * CK8 * RW;
+  auto multiply = [&](int c, const u32x4 (&cc)[CBW][NT], const Scales<GS> (&ss)[CBW][NT]) PGN_INLINE {
+    const bf16x8* const from = buf + (c & 1) * P * RT * CK8 * 16;
 #pragma unroll
     for (int j = 0; j < CBW; ++j) {
       if (c * CB + wk + WK * j < KB) {
-        const bf16x8* const at = from + (size_t)((wk + WK * j) * 16 + h) * RW + i % MR;
-#pragma unroll
-        for (int q = 0; q < 4 / GS; ++q) {
-          f32x4 d[RT][NT];
-#pragma unroll
-          for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) d[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = q * GS; ks < (q + 1) * GS; ++ks) {
-            bf16x8 b[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) b[t] = operand(cw[j][t][ks]);
-#pragma unroll
-            for (int p = P - 1; p >= 0; --p)  // the smallest parts first
-#pragma unroll
-              for (int r = 0; r < RT; ++r) {
-                const bf16x8 a = at[((size_t)p * CK8 + 4 * ks) * RW + 16 * r];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) d[r][t] = pgn_mfma(a, b[t], d[r][t]);
-              }
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const unsigned sv = sw[j][t][GS == 1 ? q >> 1 : 0];
-            const float s = q & 1 ? float_of(sv & 0xffff0000u) : bf16_bits(sv);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) acc[r][t] += s * d[r][t];
-          }
-        }
+        const bf16x8* const at = from + ((wk + WK * j) * 16 + h) * 16 + i;
+        block<P, GS>(acc, cc[j], ss[j], [&](int p, int r, int ks) { return at[((p * RT + r) * CK8 + 4 * ks) * 16]; });
       }
-      if (c + 1 < nch) load_w(j, c + 1);
-    }
-    if (c + 1 < nch) store_x(c + 1);
-  }
-
-  auto finish = [&](float v, int row, int col) {
-    if (row < n && col < N) {
-      if (bias) v += (float)bias[col];
-      if (act == 1) v = pgn_gelu_erf(v);
-      const size_t off = (size_t)row * N + col;
-      if (resid) v += (float)resid[off];
-      y[off] = (T)v;
     }
   };
-  const int row0 = rb * 16 * RT;
-  if constexpr (WK == 1) {
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) finish(acc[r][t][e], row0 + 16 * r + 4 * h + e, (ct0 + t) * 16 + i);
+  // (two chunks a turn, so that codes need not be moved from one set of registers to the other)
+  auto turn = [&](int c, u32x4 (&c0)[CBW][NT], Scales<GS> (&s0)[CBW][NT], u32x4 (&c1)[CBW][NT],
+                  Scales<GS> (&s1)[CBW][NT]) PGN_INLINE {
+    __syncthreads();
+    load_x(c + 1);
+    load_w(c + 1, c1, s1);
+    multiply(c, c0, s0);
+    store_x(c + 1);
+  };
+  int c = 0;
+  for (; c + 2 < nch; c += 2) {
+    turn(c, cw, sw, cn, sn);
+    turn(c + 1, cn, sn, cw, sw);
+  }
+  if (c + 1 < nch) {
+    turn(c, cw, sw, cn, sn);
+    __syncthreads();
+    multiply(c + 1, cn, sn);
   } else {
-    // the waves' sums joined in order: wave wk's at [wk][wn][t][r][lane][e]
     __syncthreads();
-    f32x4* const part = reinterpret_cast<f32x4*>(smem);
-    constexpr int S = WN * NT * RT * 64;
+    multiply(c, cw, sw);
+  }
+
+  // The sums go through LDS, wave wk's at [wk][row][column], and V consecutive columns of a row to a thread: the waves' shares
+  // are added in order, and rows are read and written in whole vectors. (A pitch of 4 past 16: a store's four rows of 16
+  // columns fall on different banks.)
+  constexpr int C = WN * NT * 16, S = C + 4;
+  float* const part = reinterpret_cast<float*>(smem);
+  __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) part[wk * S + ((wn * NT + t) * RT + r) * 64 + l] = acc[r][t];
-    __syncthreads();
-    for (int o = tid; o < S * 4; o += 64 * kWaves) {
-      const int e = o & 3, lane = o >> 2 & 63, r = (o >> 8) % RT, tile = (o >> 8) / RT;
-      const int row = row0 + 16 * r + 4 * (lane >> 4) + e, col = (cg * WN * NT + tile) * 16 + (lane & 15);
-      if (row < n && col < N) {
-        float v = 0.f;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int k = 0; k < WK; ++k) v += reinterpret_cast<const float*>(part)[k * S * 4 + o];
-        finish(v, row, col);
+      for (int e = 0; e < 4; ++e)
+        part[(wk * 16 * RT + 16 * r + 4 * h + e) * S + (wn * NT + t) * 16 + i] = acc[r][t][e];
+  __syncthreads();
+  constexpr int all = 16 * RT * C / (64 * kWaves), most = 16 / (int)sizeof(T), V = all < 1 ? 1 : all < most ? all : most;
+  const bool whole = N % most == 0;  // every vector lies in a row and at a vector's address
+  for (int o = tid; o < 16 * RT * C / V; o += 64 * kWaves) {
+    const int r = o / (C / V), c = o % (C / V) * V, row = row0 + r, col = cg * C + c;
+    if (row >= n || col >= N) continue;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = part[r * S + c + e];
+#pragma unroll
+    for (int k = 1; k < WK; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += part[(k * 16 * RT + r) * S + c + e];
+    const size_t off = (size_t)row * N + col;
+    if (V == most && whole) {
+      Vec<T> q;
+      if (bias) {
+        q.load(bias + col);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += q.get(e);
       }
+      if (act == 1)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = pgn_gelu_erf(v[e]);
+      if (resid) {
+        q.load(resid + off);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += q.get(e);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) q.set(e, v[e]);
+      q.store(y + off);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (col + e < N) finish(v[e], row, col + e, N, bias, act, resid, y);
     }
   }
 }
+
+constexpr size_t kPlainLds = 60 << 10;  // dynamic LDS beside `red` that a launch may ask for without raising the limit
 
 struct Call {
   const void *x, *codes, *scales, *lnw, *lnb, *bias, *resid;
@@ -453,29 +684,51 @@ struct Call {
   hipStream_t st;
 };
 
-template <class T, int P, int GS, int MR, int RT, int U, int WK, int NT>
+template <class T, int P, int GS, int MR, int WK, int CBW>
+int launch_few(const Call& a) {
+  const int KB = (a.K + kTileCols - 1) / kTileCols, ctiles = (a.N + 15) / 16;
+  hipLaunchKernelGGL((few<T, P, GS, MR, WK, CBW>), dim3((unsigned)ctiles), dim3(64 * WK), 0, a.st, (const T*)a.x,
+                     (const u32x4*)a.codes, (const __bf16*)a.scales, (const T*)a.lnw, (const T*)a.lnb, a.eps,
+                     (const T*)a.bias, a.act, (const T*)a.resid, (T*)a.y, a.n, a.N, a.K, KB);
+  PGN_RETURN_LAUNCH();
+}
+
+template <class T, int P, int GS, int kWaves, int RT, int U, int WK, int NT>
 int launch(const Call& a) {
-  constexpr int CB = U * 16 / (MR * RT), WN = kWaves / WK;
+  constexpr int CB = U * (kWaves / RT) / 4, WN = kWaves / WK;
   const int KB = (a.K + kTileCols - 1) / kTileCols, ctiles = (a.N + 15) / 16;
   const int rblocks = (a.n + 16 * RT - 1) / (16 * RT), groups = (ctiles + WN * NT - 1) / (WN * NT);
   const int64_t blocks = rblocks > 1 ? (int64_t)(groups + 7) / 8 * 8 * rblocks : groups;
-  const size_t chunk = (size_t)P * U * 4096;
-  const size_t lds = std::max<size_t>(KB > CB ? 2 * chunk : chunk, WK > 1 ? (size_t)kWaves * NT * RT * 1024 : 0);
-  const auto fn = linear<T, P, GS, MR, RT, U, WK, NT>;
-  const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), 2 * chunk);
-  if (e != hipSuccess) return (int)e;
+  constexpr size_t chunk = (size_t)P * U * kWaves * 1024, join = (size_t)WK * 16 * RT * (WN * NT * 16 + 4) * 4;
+  const size_t lds = std::max(KB > CB ? 2 * chunk : chunk, join);
+  const auto fn = linear<T, P, GS, kWaves, RT, U, WK, NT>;
+  static_assert(std::max(2 * chunk, join) <= 159 << 10, "");
+  if (lds > kPlainLds) {
+    const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), std::max(2 * chunk, join));
+    if (e != hipSuccess) return (int)e;
+  }
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(64 * kWaves), lds, a.st, (const T*)a.x, (const u32x4*)a.codes,
                      (const __bf16*)a.scales, (const T*)a.lnw, (const T*)a.lnb, a.eps, (const T*)a.bias, a.act,
                      (const T*)a.resid, (T*)a.y, a.n, a.N, a.K, KB, ctiles, rblocks);
   PGN_RETURN_LAUNCH();
 }
 
+// Rows and columns of a workgroup. Up to four rows a workgroup is one tile of columns. Beyond, the smallest tile of rows by
+// columns that leaves no compute unit a second workgroup, as each stages its rows itself and a short row's cost is its chain
+// of barriers: 16 x 64 while there are 256 workgroups of those or fewer, 32 x 128 likewise, then 32 x 256. Measured, us, for 16 x
+// 64, 32 x 128 and 32 x 256 (fp32): 16 x 2328 x 768 5.7, 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3, 11.5; 512 x 2328 x 768 23.8,
+// 17.2, 13.0. The last with eight waves where there is one part (bf16, 512 x 16384 x 1024 23.7 against 27.7 with sixteen),
+// with sixteen where there are more (fp32, 56 against 65).
 template <class T, int P, int GS>
 int by_rows(const Call& a) {
-  if (a.n == 1) return launch<T, P, GS, 1, 1, 2, 4, 1>(a);
-  if (a.n <= 4) return launch<T, P, GS, 4, 1, 4, 4, 1>(a);
-  if (a.n <= 64) return launch<T, P, GS, 16, 1, 4, 2, 1>(a);
-  return launch<T, P, GS, 16, 4, P == 1 ? 8 : 4, 1, P == 1 ? 4 : 2>(a);
+  if (a.n == 1) return launch_few<T, P, GS, 1, 8, 4>(a);
+  if (a.n <= 4) return launch_few<T, P, GS, 4, 4, 4>(a);
+  const auto blocks = [&](int64_t rows, int64_t cols) { return (a.n + rows - 1) / rows * ((a.N + cols - 1) / cols); };
+  if (blocks(16, 64) <= 256) return launch<T, P, GS, 16, 1, 1, 4, 1>(a);
+  if (blocks(32, 128) <= 256) return launch<T, P, GS, 16, 2, 1, 2, 1>(a);
+  if constexpr (P == 1)
+    if (blocks(32, 256) > 256) return launch<T, P, GS, 8, 2, 2, 1, 2>(a);
+  return launch<T, P, GS, 16, 2, 1, 2, 2>(a);
 }
 
 template <class T, int P>
@@ -551,7 +804,7 @@ extern "C" int pragnosia_fp4_linear(const void* x, int bf16, const void* codes, 
   PGN_CHECK_ARG(x && codes && scales && y && aligned(x, codes, scales) && aligned(ln_weight, ln_bias, nullptr));
   PGN_CHECK_ARG((ln_weight || !ln_bias) && (!ln_weight || ln_eps >= 0.f));
   const uintptr_t size = bf16 ? 2 : 4, xa = (uintptr_t)x, ya = (uintptr_t)y;
-  PGN_CHECK_ARG(((ya | (uintptr_t)bias | (uintptr_t)resid) & (size - 1)) == 0);
+  PGN_CHECK_ARG(aligned(y, bias, resid));
   PGN_CHECK_ARG(xa + (uintptr_t)(n * K) * size <= ya || ya + (uintptr_t)(n * N) * size <= xa);
   const Call a{x, codes, scales, ln_weight, ln_bias, bias, resid, y, ln_eps, act, (int)n, (int)N, (int)K,
                (hipStream_t)stream};

@@ -1,11 +1,13 @@
 // Rules on logits: penalties for repeated tokens, biases, masks; the processed logits, or the best token they leave
 // (formulas and conventions in include/pragnosia_gen.h).
 //
-// One pass over the logits. A workgroup owns a tile of one row's words; it counts the row's history in its LDS (integer
-// atomics: any order gives the same counts), marks the bias entries of its words (the last of a repeated word wins, by an
-// integer maximum), and applies the rules to logits it loaded before all that. No counts are kept between calls and
-// nothing of the vocabulary's size is written but the result: a history is some kilobytes where a row of counts would be
-// as large as the row of logits.
+// One pass over the logits. A workgroup owns a tile of one row's words, whose logits it loads first. In its LDS, a 32-bit
+// word each, it marks the bias entries of its words (the last of a repeated word wins, by an integer maximum) and counts
+// the row's history (integer atomics: any order gives the same counts); whoever marks a word first puts it on a list. Then
+// the rules go over that list, not over the words: a listed word's value is formed from its logit and left in its place.
+// The pass over the tile's logits that follows takes those values, masks, and keeps the best or stores. No counts are kept
+// between calls and nothing of the vocabulary's size is written but the result: a history is some kilobytes where a row of
+// counts would be as large as the row of logits.
 #include <algorithm>
 
 #include "../include/pragnosia_gen.h"
@@ -17,7 +19,11 @@ namespace {
 typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr unsigned kInPrompt = 0x80000000u;  // of a word's count: it is in the part before `prompt`
+// A word's place in LDS: bit 31: it is in the history before `prompt`; from bit `shift` on its bias entry + 1, 0 without
+// one; below its count among the rest (shift bits hold L, the rest M).
+constexpr unsigned kInPrompt = 0x80000000u;
+constexpr int kList = 4096;  // words of a tile that its list holds
+constexpr int kAhead = 4;  // history entries a thread loads before it knows the history's length
 constexpr unsigned kNothing = 0x007fffffu;   // order_key(-inf): what a word has to exceed
 
 struct Args {
@@ -36,7 +42,7 @@ struct Args {
   void* out;
   int64_t* tokens;
   uint64_t* part;  // the best key of each row's tiles, hi above lo
-  int L, M, V, words, tiles;
+  int L, M, V, words, tiles, shift;
 };
 
 template <class T>
@@ -57,10 +63,9 @@ PGN_DEVICE void set_element(float x, u32x4& v, int e, __bf16) {
 }
 
 // Each operation rounded by itself.
-PGN_DEVICE float penalised(float x, unsigned count, float r, float p, float f) {
+PGN_DEVICE float penalised(float x, unsigned c, float r, float p, float f) {
 #pragma clang fp contract(off)
   x = x > 0.f ? x / r : x * r;
-  const unsigned c = count & ~kInPrompt;
   if (c) {
     x = x - p;
     const float fc = f * (float)c;
@@ -69,19 +74,40 @@ PGN_DEVICE float penalised(float x, unsigned count, float r, float p, float f) {
   return x;
 }
 
-// Q 16-byte vectors of logits a thread. Rows start at any element: the vectors lie at 16-byte addresses, so a row's first
-// and last may be shared with its neighbours and are then taken element by element.
-template <class T, int Q>
+// Bit e of `m` as a word of zeros or ones.
+PGN_DEVICE unsigned spread(unsigned m, int e) { return (unsigned)((int)(m << (31 - e)) >> 31); }
+
+// -infinity where `off` has a word's bit, on raw elements.
+PGN_DEVICE void mask_vector(u32x4& v, unsigned off, float) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned m = spread(off, e);
+    v[e] = (v[e] & ~m) | (0xff800000u & m);
+  }
+}
+PGN_DEVICE void mask_vector(u32x4& v, unsigned off, __bf16) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned m = (spread(off, 2 * e) & 0xffffu) | (spread(off, 2 * e + 1) & 0xffff0000u);
+    v[e] = (v[e] & ~m) | (0xff80ff80u & m);
+  }
+}
+
+// W words to a workgroup, Q 16-byte vectors of logits a thread. Rows start at any element: the vectors lie at 16-byte
+// addresses, so a row's first and last may be shared with its neighbours and are then taken element by element.
+template <class T, int W, bool TOKEN>
 __global__ __launch_bounds__(kThreads) void apply(const Args a) {
-  constexpr int E = 16 / (int)sizeof(T), TILE = kThreads * Q * E;
-  extern __shared__ __align__(16) unsigned smem[];  // counts [TILE] with a history, bias entries [TILE] with a list, mask
+  constexpr int E = 16 / (int)sizeof(T), Q = W / kThreads / E;
+  extern __shared__ __align__(16) unsigned smem[];  // with entries: words [W], settled [W / 32], list; with a mask its bits
   __shared__ Key key_s[kWaves];
-  static_assert(kWaves == 16, "the waves' keys are reduced in a row of 16 lanes");
+  __shared__ int listed;
+  static_assert(Q * kThreads * E == W && kWaves == 16, "the waves' keys are reduced in a row of 16 lanes");
   const int tid = threadIdx.x, b = blockIdx.y, V = a.V;
   const int64_t row = (int64_t)b * V;
-  const int v0 = (int)blockIdx.x * TILE - (int)(row & (E - 1));  // the first vector's first word, at least -E + 1
+  const int v0 = (int)blockIdx.x * W - (int)(row & (E - 1));  // the first vector's first word, at least -E + 1
   const T* const lr = (const T*)a.logits + row;
   T* const yr = (T*)a.out + row;
+  const bool entries = a.L || a.M;
 
   u32x4 x[Q];
 #pragma unroll
@@ -96,9 +122,15 @@ __global__ __launch_bounds__(kThreads) void apply(const Args a) {
         if (v + e >= 0 && v + e < V) set_element((float)lr[v + e], x[q], e, T());
     }
   }
-  int64_t len64 = a.lengths ? a.lengths[b] : a.L;
+  const int64_t* const hr = a.history + (int64_t)b * a.history_stride;
+  const int64_t* const br = a.bias_ids + (int64_t)b * a.bias_stride;
+  const float* const bv = a.bias_values + (int64_t)b * a.bias_stride;
+  int64_t id[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) id[u] = tid + u * kThreads < a.L ? hr[tid + u * kThreads] : -1;
+  const int64_t len64 = a.lengths ? a.lengths[b] : a.L;
   const int len = (int)(len64 < 0 ? 0 : len64 > a.L ? a.L : len64);
-  int64_t pr64 = a.prompt ? a.prompt[b] : 0;
+  const int64_t pr64 = a.prompt ? a.prompt[b] : 0;
   const int prompt = (int)(pr64 < 0 ? 0 : pr64 > len ? len : pr64);
   const float r = a.repetition ? a.repetition[b] : a.r0, p = a.presence ? a.presence[b] : a.p0,
               f = a.frequency ? a.frequency[b] : a.f0;
@@ -106,90 +138,135 @@ __global__ __launch_bounds__(kThreads) void apply(const Args a) {
   if (a.S) line = a.state ? a.state[b] : a.S == 1 ? 0 : b;
   const bool masked = line >= 0, closed = line >= a.S && masked;
 
-  unsigned* const count = smem;
-  unsigned* const entry = smem + (a.L ? TILE : 0);
-  unsigned* const bits = entry + (a.M ? TILE : 0);
-  const int arrays = (a.L ? TILE : 0) + (a.M ? TILE : 0);
-  for (int k = tid * 4; k < arrays; k += kThreads * 4) *reinterpret_cast<u32x4*>(smem + k) = u32x4{0u, 0u, 0u, 0u};
-  const int word0 = max(v0, 0) >> 5;
+  unsigned* const word = smem;
+  unsigned* const settled = smem + W;
+  unsigned short* const list = reinterpret_cast<unsigned short*>(smem + W + W / 32);
+  unsigned* const bits = smem + (entries ? W + W / 32 + kList / 2 : 0);
+  if (entries) {
+    for (int k = tid * 4; k < W + W / 32; k += kThreads * 4) *reinterpret_cast<u32x4*>(smem + k) = u32x4{0u, 0u, 0u, 0u};
+    if (tid == 0) listed = 0;
+  }
+  const int line0 = max(v0, 0) >> 5;
   if (masked && !closed) {
-    const int wordn = (min(v0 + TILE, V) + 31) >> 5;  // (none where the tile lies past the row)
+    const int linen = (min(v0 + W, V) + 31) >> 5;  // (none where the tile lies past the row)
     const uint32_t* const mr = a.mask + line * a.words;
-    for (int k = word0 + tid; k < wordn; k += kThreads) bits[k - word0] = mr[k];
+    for (int k = line0 + tid; k < linen; k += kThreads) bits[k - line0] = mr[k];
   }
   __syncthreads();
-  if (a.L) {
-    const int64_t* const hr = a.history + (int64_t)b * a.history_stride;
-    for (int t0 = tid; t0 < len; t0 += kThreads * 4) {
-      int64_t id[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) id[u] = t0 + u * kThreads < len ? hr[t0 + u * kThreads] : -1;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t k = id[u] - v0;
-        if (id[u] >= 0 && id[u] < V && k >= 0 && k < TILE) {
-          if (t0 + u * kThreads < prompt) atomicOr(count + k, kInPrompt);
-          else atomicAdd(count + k, 1u);
-        }
-      }
+  if (entries) {
+    // f(place in the tile) for an entry that lies in it
+    auto within = [&](int64_t i, auto&& f) {
+      if (i >= 0 && i < V && i >= v0 && i - v0 < W) f((int)(i - v0));
+    };
+    auto enlist = [&](int k, unsigned before) {
+      if (before) return;  // marked already
+      const int at = atomicAdd(&listed, 1);
+      if (at < kList) list[at] = (unsigned short)k;
+    };
+    if (a.M) {
+      for (int j = tid; j < a.M; j += kThreads)
+        within(br[j], [&](int k) { enlist(k, atomicMax(word + k, ((unsigned)j + 1u) << a.shift)); });
+      __syncthreads();
     }
-  }
-  if (a.M) {
-    const int64_t* const br = a.bias_ids + (int64_t)b * a.bias_stride;
-    for (int j = tid; j < a.M; j += kThreads) {
-      const int64_t id = br[j], k = id - v0;
-      if (id >= 0 && id < V && k >= 0 && k < TILE) atomicMax(entry + k, (unsigned)j + 1u);
+    if (a.L) {
+      auto count = [&](int t, int64_t i) {
+        within(i, [&](int k) { enlist(k, t < prompt ? atomicOr(word + k, kInPrompt) : atomicAdd(word + k, 1u)); });
+      };
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (tid + u * kThreads < len) count(tid + u * kThreads, id[u]);
+      for (int t = tid + kAhead * kThreads; t < len; t += kThreads) count(t, hr[t]);
+      __syncthreads();
     }
+    auto settle = [&](int k) {
+      const unsigned w = word[k], c = w & ((1u << a.shift) - 1u), e = (w & ~kInPrompt) >> a.shift;
+      float z = (float)lr[v0 + k];
+      if (c || (w & kInPrompt)) z = penalised(z, c, r, p, f);
+      if (e) z += bv[e - 1];
+      word[k] = __builtin_bit_cast(unsigned, z);
+      atomicOr(settled + (k >> 5), 1u << (k & 31));
+    };
+    const int n = listed;
+    if (n <= kList) {
+      for (int j = tid; j < n; j += kThreads) settle(list[j]);
+    } else {  // more words than the list holds: all that are marked
+      for (int k = tid; k < W; k += kThreads)
+        if (word[k]) settle(k);
+    }
+    __syncthreads();
   }
-  __syncthreads();
 
-  const float* const bv = a.bias_values + (int64_t)b * a.bias_stride;
-  unsigned best = kNothing;
-  int at = -1;
+  float best = -__builtin_inff();
+  int best_v = -1, nan_v = -1;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     const int k0 = (q * kThreads + tid) * E, v = v0 + k0;
     if (v >= V) continue;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float z = element<T>(x[q], e);
-      if (a.L) {
-        const unsigned c = count[k0 + e];
-        if (c) z = penalised(z, c, r, p, f);
-      }
-      if (a.M) {
-        const unsigned j = entry[k0 + e];
-        if (j) z += bv[j - 1];
-      }
-      const int ve = v + e;
-      if (masked && ve >= 0 && ve < V && (closed || !(bits[(ve >> 5) - word0] >> (ve & 31) & 1u))) z = -__builtin_inff();
-      if (ve >= 0 && ve < V) {
-        const unsigned key = order_key(z);
-        if (key > best) {  // words ascend, so the first among equals stays
-          best = key;
-          at = ve;
-        }
-      }
-      set_element(z, x[q], e, T());
+    const int from = max(-v, 0), to = min(V - v, E);  // the vector's words in the row
+    const unsigned set = entries ? settled[k0 >> 5] >> (k0 & 31) & ((1u << E) - 1u) : 0u;
+    // one bit a masked word
+    unsigned off = 0u;
+    if (closed) {
+      off = ~0u;
+    } else if (masked) {
+      const int u = max(v, 0), w0 = (u >> 5) - line0, w1 = ((v + to - 1) >> 5) - line0;
+      off = ~((unsigned)(((uint64_t)bits[w1] << 32 | bits[w0]) >> (u & 31)) << from);
     }
-    if (a.out) {
-      if (v >= 0 && v + E <= V) {
+    if constexpr (TOKEN) {
+      off |= ~((1u << to) - (1u << from));
+      float z[E], most = -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] = element<T>(x[q], e);
+      if (set) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (set >> e & 1u) z[e] = __builtin_bit_cast(float, word[k0 + e]);
+      }
+      bool nan = false;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const unsigned m = spread(off, e);
+        z[e] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, z[e]) & ~m) | (0xff800000u & m));
+        nan |= z[e] != z[e];
+        most = fmaxf(most, z[e]);
+      }
+      if (nan && nan_v < 0) {
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (z[e] != z[e]) nan_v = v + e;
+      }
+      if (most > best) {  // words ascend, so the first among equals stays
+        best = most;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (z[e] == most) best_v = v + e;
+      }
+    } else {
+      if (set) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (set >> e & 1u) set_element(__builtin_bit_cast(float, word[k0 + e]), x[q], e, T());
+      }
+      mask_vector(x[q], off, T());
+      if (from == 0 && to == E) {
         *reinterpret_cast<u32x4*>(yr + v) = x[q];
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (v + e >= 0 && v + e < V) yr[v + e] = (T)element<T>(x[q], e);
+          if (e >= from && e < to) yr[v + e] = (T)element<T>(x[q], e);
       }
     }
   }
-  if (!a.tokens) return;
-  const Key k = max_wave(Key{best, ~(unsigned)at});
-  if ((tid & 63) == 0) key_s[tid >> 6] = k;
-  __syncthreads();
-  const Key all = max_row(key_s[tid & 15]);
-  if (tid == 0) {
-    if (a.tiles == 1) a.tokens[b] = (int)~all.lo;
-    else a.part[(int64_t)b * a.tiles + blockIdx.x] = (uint64_t)all.hi << 32 | all.lo;
+  if constexpr (TOKEN) {
+    if (nan_v >= 0) best_v = nan_v;
+    const Key k = max_wave(Key{nan_v >= 0 ? 0xffffffffu : order_key(best), ~(unsigned)best_v});
+    if ((tid & 63) == 0) key_s[tid >> 6] = k;
+    __syncthreads();
+    const Key all = max_row(key_s[tid & (kWaves - 1)]);
+    if (tid == 0) {
+      if (a.tiles == 1) a.tokens[b] = (int)~all.lo;
+      else a.part[(int64_t)b * a.tiles + blockIdx.x] = (uint64_t)all.hi << 32 | all.lo;
+    }
   }
 }
 
@@ -208,41 +285,31 @@ __global__ __launch_bounds__(64) void pick(const uint64_t* __restrict__ part, in
   if (threadIdx.x == 0) tokens[blockIdx.x] = (int)~k.lo;
 }
 
-// Words of a tile with Q vectors a thread: 16384 at most (counts and entries are 128 KB of LDS then)
+// A row's tiles of `words` words; it may start E - 1 words into a vector.
 template <class T>
-constexpr int tile_words(int Q) { return kThreads * Q * (16 / (int)sizeof(T)); }
-template <class T>
-constexpr int kMostQ = sizeof(T) == 4 ? 4 : 2;
-constexpr int kMostWords = tile_words<float>(4);
-static_assert(kMostWords == tile_words<__bf16>(kMostQ<__bf16>), "");
-
-// A row's tiles; it may start E - 1 words into a vector.
-template <class T>
-int64_t tiles_of(int64_t V, int Q) {
+int64_t tiles_of(int64_t V, int words) {
   const int E = 16 / (int)sizeof(T);
-  return (V + (V % E ? E - 1 : 0) + tile_words<T>(Q) - 1) / tile_words<T>(Q);
+  return (V + (V % E ? E - 1 : 0) + words - 1) / words;
 }
 
-// Vectors a thread: one tile where the row fits one (no second launch), else the largest tile that leaves two workgroups a
-// compute unit (each reads its row's whole history).
-template <class T>
-int vectors(int64_t B, int64_t V) {
-  for (int Q = 1; Q <= kMostQ<T>; Q *= 2)
-    if (tiles_of<T>(V, Q) == 1) return Q;
-  int Q = kMostQ<T>;
-  while (Q > 1 && tiles_of<T>(V, Q) * B < 512) Q /= 2;
-  return Q;
+int bit_length(int64_t v) {
+  int n = 0;
+  for (; v > 0; v >>= 1) ++n;
+  return n;
 }
 
-template <class T, int Q>
-int launch(const Args& a, int64_t B, hipStream_t st) {
-  constexpr int tile = tile_words<T>(Q);
-  const size_t lds = ((size_t)(a.L ? tile : 0) + (a.M ? tile : 0) + (a.S ? tile / 32 + 4 : 0)) * 4;
-  const auto fn = apply<T, Q>;
-  const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), (size_t)(2 * tile + tile / 32 + 4) * 4);
-  if (e != hipSuccess) return (int)e;
+template <class T, int W, bool TOKEN>
+int launch(Args a, int64_t B, hipStream_t st) {
+  constexpr size_t marks = (size_t)(W + W / 32 + kList / 2) * 4, masks = (size_t)(W / 32 + 4) * 4;
+  const size_t lds = (a.L || a.M ? marks : 0) + (a.S ? masks : 0);
+  a.tiles = (int)tiles_of<T>(a.V, W);
+  const auto fn = apply<T, W, TOKEN>;
+  if (lds > 60 << 10) {  // (what a launch may ask for without raising the kernel's limit, with key_s to spare)
+    const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), marks + masks);
+    if (e != hipSuccess) return (int)e;
+  }
   hipLaunchKernelGGL(fn, dim3((unsigned)a.tiles, (unsigned)B), dim3(kThreads), lds, st, a);
-  if (a.tokens && a.tiles > 1) {
+  if (TOKEN && a.tiles > 1) {
     const hipError_t f = hipGetLastError();
     if (f != hipSuccess) return (int)f;
     hipLaunchKernelGGL(pick, dim3((unsigned)B), dim3(64), 0, st, a.part, a.tiles, a.tokens);
@@ -250,13 +317,17 @@ int launch(const Args& a, int64_t B, hipStream_t st) {
   PGN_RETURN_LAUNCH();
 }
 
-template <class T>
-int run(Args a, int64_t B, hipStream_t st) {
-  const int Q = vectors<T>(B, a.V);
-  a.tiles = (int)tiles_of<T>(a.V, Q);
-  if (Q == 1) return launch<T, 1>(a, B, st);
-  if (Q == 2) return launch<T, 2>(a, B, st);
-  return launch<T, kMostQ<T>>(a, B, st);
+// The words of a tile. A row whose token comes from one tile takes no second launch, which is worth more than the smaller
+// tiles' spread over the chip: 64 rows of 32768 with a history, a list and a mask 15.7 us eager in one tile a row, 18.0 in
+// four, though alone on the GPU 10.8 against 8.1. Longer rows, and logits for a sampler: 16384 words where that leaves two
+// workgroups a compute unit (256 rows of 131072 bf16: 39.0 us, with 8192 words 43.4, with 32768 40.8), else 8192.
+template <class T, bool TOKEN>
+int run(const Args& a, int64_t B, hipStream_t st) {
+  if (TOKEN && tiles_of<T>(a.V, 8192) > 1) {
+    if (tiles_of<T>(a.V, 16384) == 1) return launch<T, 16384, TOKEN>(a, B, st);
+    if (tiles_of<T>(a.V, 32768) == 1) return launch<T, 32768, TOKEN>(a, B, st);
+  }
+  return tiles_of<T>(a.V, 16384) * B >= 512 ? launch<T, 16384, TOKEN>(a, B, st) : launch<T, 8192, TOKEN>(a, B, st);
 }
 
 bool sizes_ok(int64_t B, int64_t V) {
@@ -267,8 +338,8 @@ bool sizes_ok(int64_t B, int64_t V) {
 
 extern "C" int64_t pragnosia_rules_workspace_bytes(int64_t B, int64_t V) {
   if (!sizes_ok(B, V)) return PRAGNOSIA_ERR_INVALID_ARGUMENT;
-  // (for either type: the most tiles are the smallest, fp32's, with the most that a row's start can be off, bf16's)
-  return V + 7 > kMostWords ? (V + 7 + tile_words<float>(1) - 1) / tile_words<float>(1) * B * (int64_t)sizeof(uint64_t) : 0;
+  // (the most tiles that either type has; bf16 rows may start furthest into a vector)
+  return V + 7 > 32768 ? (V + 7 + 8191) / 8192 * B * (int64_t)sizeof(uint64_t) : 0;
 }
 
 extern "C" int pragnosia_rules(const void* logits, int bf16, const int64_t* history, int64_t history_stride, int64_t L,
@@ -279,8 +350,9 @@ extern "C" int pragnosia_rules(const void* logits, int bf16, const int64_t* hist
                                const int64_t* state, void* out, int64_t* tokens, void* workspace,
                                int64_t workspace_bytes, int64_t B, int64_t V, void* stream) {
   PGN_CHECK_ARG(sizes_ok(B, V) && L >= 0 && L <= ((int64_t)1 << 24) && M >= 0 && M <= ((int64_t)1 << 20) && S >= 0);
-  PGN_CHECK_ARG((out || tokens) && (L == 0 || (history && history_stride >= L)) && (repetition || repetition_value != 0.f));
+  PGN_CHECK_ARG(!out != !tokens && (L == 0 || (history && history_stride >= L)) && (repetition || repetition_value != 0.f));
   PGN_CHECK_ARG(M == 0 || (bias_ids && bias_values && (bias_stride == 0 || bias_stride >= M)));
+  PGN_CHECK_ARG(bit_length(L) + bit_length(M) <= 31);
   PGN_CHECK_ARG(S == 0 || (mask && (state || S == 1 || S == B)));
   const int64_t need = tokens ? pragnosia_rules_workspace_bytes(B, V) : 0;
   PGN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0));
@@ -290,6 +362,8 @@ extern "C" int pragnosia_rules(const void* logits, int bf16, const int64_t* hist
   PGN_CHECK_ARG(!out || la == oa || la + size <= oa || oa + size <= la);
   const Args a{logits, history, history_stride, lengths, prompt, repetition, presence, frequency, repetition_value,
                presence_value, frequency_value, bias_ids, bias_values, bias_stride, mask, S, state, out, tokens,
-               (uint64_t*)workspace, (int)L, (int)M, (int)V, (int)((V + 31) / 32), 0};
-  return bf16 ? run<__bf16>(a, B, (hipStream_t)stream) : run<float>(a, B, (hipStream_t)stream);
+               (uint64_t*)workspace, (int)L, (int)M, (int)V, (int)((V + 31) / 32), 0, bit_length(L)};
+  const hipStream_t st = (hipStream_t)stream;
+  if (tokens) return bf16 ? run<__bf16, true>(a, B, st) : run<float, true>(a, B, st);
+  return bf16 ? run<__bf16, false>(a, B, st) : run<float, false>(a, B, st);
 }

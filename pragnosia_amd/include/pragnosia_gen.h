@@ -64,9 +64,11 @@ int pragnosia_fp4_linear(const void* x, int bf16, const void* codes, const void*
  * words, word v's bit v % 32 of word v / 32; state (B) int64 is each row's line of the mask (NULL: line b, or line 0 if
  * S = 1); a negative one leaves the row unmasked, one of S or more masks every word. S = 0: no mask.
  *
- * out (B, V) in l's type (may be l itself) or NULL: x, rounded once. tokens (B) int64 or NULL: the word of the largest x,
- * the lowest among equals, NaN above every number (torch.argmax's rule); -1 where every x is -inf. At least one of them.
- * V at most 2^26, B at most 65535, L at most 2^24, M at most 2^20, B V below 2^40. Only tokens take a workspace. */
+ * One of out and tokens is given, the other NULL. out (B, V) in l's type (may be l itself): x, rounded once. tokens (B)
+ * int64: the word of the largest x, the lowest among equals, NaN above every number (torch.argmax's rule); -1 where every
+ * x is -inf.
+ * V at most 2^26, B at most 65535, L at most 2^24, M at most 2^20, L and M of 31 bits together, B V below 2^40. Only tokens
+ * take a workspace, of rows past 32761 words. */
 int64_t pragnosia_rules_workspace_bytes(int64_t B, int64_t V);
 int pragnosia_rules(const void* logits, int bf16, const int64_t* history, int64_t history_stride, int64_t L,
                     const int64_t* lengths, const int64_t* prompt, const float* repetition, float repetition_value,

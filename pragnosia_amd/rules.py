@@ -22,8 +22,9 @@ from typing import Optional, Union
 import torch
 from torch import Tensor
 
-from ._lib import PragnosiaError, gen_lib
-from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _no_tangents, _watched
+from ._lib import PragnosiaError, check, gen_lib
+from .fp4 import _device, _fits, _quiet
+from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _no_tangents, _raw_stream, _watched
 from .ops import _expect, _require_gpu
 
 Penalty = Union[float, Tensor]
@@ -61,6 +62,9 @@ def _checked(op: str, logits: Tensor, history: Optional[Tensor], lengths: Option
         if ids.dim() not in (1, 2) or (ids.dim() == 2 and ids.shape[0] != B) or ids.shape[-1] > 1 << 20:
             raise PragnosiaError(f"{op}: bias ids (M) or ({B}, M) with M up to 2^20 expected, got {tuple(ids.shape)}")
         _expect(op, dev, bias_ids=(ids, tuple(ids.shape)), bias_values=(values, tuple(ids.shape)))
+        if history is not None and history.shape[1].bit_length() + ids.shape[-1].bit_length() > 31:
+            raise PragnosiaError(f"{op}: the lengths of history and bias list must have 31 bits together at most, got "
+                                 f"{history.shape[1]} and {ids.shape[-1]}")
         if not values.is_floating_point():
             raise PragnosiaError(f"{op}: bias values must be floating, got {values.dtype}")
     words = (V + 31) // 32
@@ -129,6 +133,9 @@ def _rules(op: str, logits, history, lengths, prompt, repetition, presence, freq
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in floats):
         raise PragnosiaError(f"{op}: rules have no backward; call it under torch.no_grad()")
     _no_tangents(op, *floats)
+    got = _plain(logits, history, lengths, prompt, (repetition, presence, frequency), ids, values, mask, state, choose)
+    if got is not None:
+        return got
     _checked(op, logits, history, lengths, prompt, penalties, ids, values, mask, state)
     if _watched(*floats, history, lengths, prompt, ids, mask, state):
         # (the ops take penalties as tensors or numbers, and bias as two tensors)
@@ -137,6 +144,69 @@ def _rules(op: str, logits, history, lengths, prompt, repetition, presence, freq
         call = rules_token if choose else rules_apply
         return call(logits, history, lengths, prompt, t[0], v[0], t[1], v[1], t[2], v[2], ids, values, mask, state)
     return _run(logits, history, lengths, prompt, (repetition, presence, frequency), ids, values, mask, state, choose)
+
+
+def _plain(logits, history, lengths, prompt, penalties, ids, values, mask, state, choose: bool) -> Optional[Tensor]:
+    """The usual call, all of whose tensors the kernels take as they are: no conversions, and no refusals to look for, which
+    is most of what the host does in the general path (19 us for one row with a history; this one 11). None: not such a
+    call."""
+    if logits.dim() != 2:
+        return None
+    (B, V), index, dt = logits.shape, logits.get_device(), logits.dtype
+    if not (logits.is_cuda and 0 < B <= 65535 and 0 < V <= 1 << 26 and dt in _FLOATS and index == _device()
+            and logits.is_contiguous() and not logits.data_ptr() & 15):
+        return None
+    row = (B,)
+    L = stride = M = bias_stride = S = 0
+    if history is not None:
+        if not (history.dim() == 2 and history.dtype is _I64 and history.get_device() == index and history.shape[0] == B):
+            return None
+        L, (stride, inner) = history.shape[1], history.stride()
+        if inner != 1 or not 0 < L <= 1 << 24 or stride < L:
+            return None
+        for t in (lengths, prompt):
+            if t is not None and not _fits(t, _I64, index, row):
+                return None
+    elif lengths is not None or prompt is not None:
+        return None
+    args = []
+    for p in penalties:
+        if isinstance(p, Tensor):
+            if not _fits(p, _F32, index, row):
+                return None
+            args += [p.data_ptr(), 1.0]
+        else:
+            args += [None, p]
+    if not (isinstance(args[1], float) and 0.0 < args[1] < math.inf and math.isfinite(args[3]) and math.isfinite(args[5])):
+        return None
+    if ids is not None:
+        M = ids.shape[-1]
+        shape = row + (M,) if ids.dim() == 2 else (M,)
+        if not (0 < M <= 1 << 20 and L.bit_length() + M.bit_length() <= 31 and values is not None and _fits(ids, _I64, index, shape) and _fits(values, _F32, index, shape)):
+            return None
+        bias_stride = M if ids.dim() == 2 else 0
+    elif values is not None:
+        return None
+    if mask is not None:
+        S = mask.shape[0] if mask.dim() else 0
+        if not (S and _fits(mask, torch.int32, index, (S, (V + 31) // 32))
+                and (S in (1, B) if state is None else _fits(state, _I64, index, row))):
+            return None
+    elif state is not None:
+        return None
+    if not _quiet({type(t) for t in (logits, history, lengths, prompt, *penalties, ids, values, mask, state)}):
+        return None
+    got = logits.new_empty(B, dtype=_I64) if choose else torch.empty_like(logits)
+    nbytes = _gen_workspace(B, V) if choose else 0
+    ws = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    at = got.data_ptr()
+    rc = gen_lib().pragnosia_rules(logits.data_ptr(), dt is _BF16, _at(history), stride, L, _at(lengths), _at(prompt),
+                                   *args, _at(ids), _at(values), M, bias_stride, _at(mask), S, _at(state),
+                                   None if choose else at, at if choose else None, _at(ws), nbytes, B, V,
+                                   _raw_stream(index))
+    if rc:
+        check(rc, "pragnosia_rules")
+    return got
 
 
 def _run(logits, history, lengths, prompt, penalties, ids, values, mask, state, choose: bool) -> Tensor:
@@ -157,7 +227,7 @@ def apply_rules(logits: Tensor, history: Optional[Tensor] = None, lengths: Optio
     prompt[b] (0 by default) on were generated; ids outside [0, V) take no part, lengths and prompt are clamped to
     [0, L]. repetition (above 0), presence and frequency: a number, or a (B,) tensor for each row its own. bias: (ids,
     values), both (M) or (B, M): the last entry of a repeated id counts, ids outside [0, V) are skipped, -inf bans a
-    word. mask (S, ceil(V / 32)) int32: word v is allowed where bit v % 32 of word v // 32 is set; state (B) picks each
+    word; L and M must have 31 bits together at most (2^15 entries on 2^15 tokens). mask (S, ceil(V / 32)) int32: word v is allowed where bit v % 32 of word v // 32 is set; state (B) picks each
     row's line (by default its own of B, or the only one): a negative state leaves the row unmasked, one of S or more
     masks every word. For inference: no input may require a gradient where gradients are recorded."""
     return _rules("apply_rules", logits, history, lengths, prompt, repetition, presence, frequency, bias, mask, state,

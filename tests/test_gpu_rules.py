@@ -133,6 +133,13 @@ def test_histories(L, dtype):
     check(inputs(3, 1000, L, dtype=dtype, seed=L))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,L,M", [(40000, 20000, 0), (9000, 6000, 5000)])
+def test_many_words_repeated(V, L, M, dtype):
+    """More words of one tile under rules than its list of them holds."""
+    check(inputs(2, V, L, M=M, S=2, dtype=dtype, seed=7))
+
+
 @pytest.mark.parametrize("M", [1, 300, 2500])
 def test_lists(M):
     check(inputs(2, 3001, 5, M=M, seed=M))

@@ -42,7 +42,7 @@ def test_sizes(L):
     assert fp4._sizes("", 1000, 1000, 64) == (L.pragnosia_fp4_code_bytes(1000, 1000),
                                               L.pragnosia_fp4_scale_bytes(1000, 1000, 64) // 2)
     # of tokens alone, and only where a row has several tiles
-    assert L.pragnosia_rules_workspace_bytes(4, 16377) == 0 < L.pragnosia_rules_workspace_bytes(4, 16378)
+    assert L.pragnosia_rules_workspace_bytes(4, 32761) == 0 < L.pragnosia_rules_workspace_bytes(4, 32762)
     assert L.pragnosia_rules_workspace_bytes(0, 9) == 0
     for B, V in ((-1, 9), (65536, 9), (1, 0), (1, (1 << 26) + 1), (65535, 1 << 26)):
         assert L.pragnosia_rules_workspace_bytes(B, V) == -1
@@ -80,11 +80,13 @@ def rule(L, logits=one, history=null, stride=0, n=0, r=1.0, ids=null, values=nul
 
 
 @pytest.mark.parametrize("bad", [
-    dict(logits=null), dict(logits=odd), dict(out=odd), dict(out=null), dict(out=ctypes.c_void_p(32)), dict(r=0.0), dict(n=5),
+    dict(logits=null), dict(logits=odd), dict(out=odd), dict(out=null), dict(tokens=one), dict(out=ctypes.c_void_p(32)), dict(r=0.0), dict(n=5),
     dict(n=-1), dict(n=5, history=one, stride=4), dict(n=(1 << 24) + 1, history=one, stride=1 << 30), dict(M=3),
     dict(M=3, ids=one), dict(M=3, ids=one, values=one, bstride=2), dict(M=-1), dict(M=(1 << 20) + 1, ids=one, values=one),
     dict(S=1), dict(S=3, mask=one), dict(S=-1), dict(B=-1), dict(B=1 << 16), dict(V=0), dict(V=(1 << 26) + 1),
-    dict(tokens=one, V=20000), dict(tokens=one, V=20000, ws=one, size=79), dict(tokens=one, V=20000, ws=odd, size=1 << 20)])
+    dict(n=1 << 20, history=one, stride=1 << 20, M=1 << 10, ids=one, values=one),
+    dict(out=null, tokens=one, V=40000), dict(out=null, tokens=one, V=40000, ws=one, size=79),
+    dict(out=null, tokens=one, V=40000, ws=odd, size=1 << 20)])
 def test_rules_entry_refuses(L, bad):
     assert rule(L, **bad) == -1
 
@@ -206,6 +208,7 @@ H = z(2, 3, **L64)
     (dict(bias=(z(3, 4, **L64), z(3, 4))), "bias ids"), (dict(bias=(z(4), z(4))), "bias ids must be integers"),
     (dict(bias=(z(2, 4, **L64), z(4))), "bias_values has shape"), (dict(bias=(z(4, **L64), z(4, **L64))), "floating"),
     (dict(bias=(z(1, **L64).expand((1 << 20) + 1), z(1).expand((1 << 20) + 1))), "2\\^20"),
+    (dict(history=z(1, **L64).expand(2, 1 << 20), bias=(z(1 << 10, **L64), z(1 << 10))), "31 bits"),
     (dict(bias=(z(4, **L64), None)), "ids, values"), (dict(state=z(2, **L64)), "there is none"),
     (dict(mask=z(2, 2, dtype=torch.int32)), "mask has shape"), (dict(mask=z(2, 1)), "mask"),
     (dict(mask=z(0, 1, dtype=torch.int32)), "S > 0"), (dict(mask=z(3, 1, dtype=torch.int32)), "without a state"),
