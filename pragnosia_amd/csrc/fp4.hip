@@ -15,6 +15,7 @@ namespace {
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
 typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
 typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
+typedef __attribute__((__vector_size__(2 * sizeof(unsigned short)))) unsigned short u16x2;
 
 #define PGN_INLINE __attribute__((always_inline))  // of a lambda whose captured arrays have to stay in registers
 
@@ -34,7 +35,6 @@ struct Raw<float> {
     a = reinterpret_cast<const f32x4*>(p)[0];
     b = reinterpret_cast<const f32x4*>(p)[1];
   }
-  PGN_DEVICE void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
   PGN_DEVICE void keep(bool k) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -43,17 +43,29 @@ struct Raw<float> {
     }
   }
   PGN_DEVICE float get(int e) const { return e < 4 ? a[e & 3] : b[e & 3]; }
+  // the largest absolute value, as its bits (their order is the values', a NaN above an infinity)
+  PGN_DEVICE unsigned most() const {
+    unsigned m = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, bits_of(get(e)) & 0x7fffffffu);
+    return m;
+  }
 };
 template <>
 struct Raw<__bf16> {
   u32x4 a;
   PGN_DEVICE void load(const __bf16* p) { a = *reinterpret_cast<const u32x4*>(p); }
-  PGN_DEVICE void zero() { a = u32x4{0u, 0u, 0u, 0u}; }
   PGN_DEVICE void keep(bool k) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) a[e] = k ? a[e] : 0u;
   }
   PGN_DEVICE float get(int e) const { return e & 1 ? float_of(a[e >> 1] & 0xffff0000u) : bf16_bits(a[e >> 1]); }
+  PGN_DEVICE unsigned most() const {  // (two at a time)
+    u16x2 m{0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, a[e] & 0x7fff7fffu));
+    return (unsigned)max(m[0], m[1]) << 16;
+  }
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -76,9 +88,12 @@ PGN_DEVICE unsigned exact_code(float w, float s) {
   return c | (bits_of(w) >> 31) << 3;
 }
 
-// One wave a tile. The codes come from the hardware's conversion of w / s, with the quotient a little too large and a
-// little too small: where both give the same eight codes no border lies within the quotient's error, elsewhere (about
-// one lane in 10^4, and every exact tie) exact_code decides.
+// One wave a tile. A code is the hardware's rounding of w / s, to nearest even as the definition has it, of the quotient
+// rounded once: a quotient that is not a border between codes does not round to one, as |w - t s| is at least a step of w for
+// the exact product t s. Quotients come by a product with the reciprocal and one correction (correctly rounded, as the
+// reciprocal is: all scales' mantissas were tried), where neither can leave the range; elsewhere by division and
+// exact_code. Deciding the doubtful ones by exact_code instead (two quotients, a little too large and too small, that give
+// different codes) took that path in every other wave of bf16 weights, which often lie on a border: 32768 x 4096 in 82 us.
 template <class T, int GS>
 __global__ __launch_bounds__(256) void quantize(const T* __restrict__ W, u32x4* __restrict__ codes,
                                                 __bf16* __restrict__ scales, int64_t N, int K, int KB, int64_t tiles) {
@@ -92,16 +107,13 @@ __global__ __launch_bounds__(256) void quantize(const T* __restrict__ W, u32x4* 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int k = kTileCols * kb + 32 * j + 8 * h;
-    if (row < N && k < K) w[j].load(W + row * K + k);
-    else w[j].zero();
+    w[j].load(W + min(row, N - 1) * K + min(k, K - 8));
+    w[j].keep(row < N && k < K);
   }
   unsigned m[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    m[j] = 0u;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m[j] = max(m[j], bits_of(w[j].get(e)) & 0x7fffffffu);
-    m[j] = max_over_h(m[j]);
+    m[j] = max_over_h(w[j].most());
   }
   u32x4 out;
   float s[4 / GS];
@@ -110,21 +122,28 @@ __global__ __launch_bounds__(256) void quantize(const T* __restrict__ W, u32x4* 
     unsigned g = m[q * GS];
 #pragma unroll
     for (int j = 1; j < GS; ++j) g = max(g, m[q * GS + j]);
-    s[q] = g >= 0x7f800000u ? __builtin_nanf("") : pgn_f32(pgn_bf16(float_of(g) / 6.f));
-    const bool fast = s[q] > 0x1p-100f && s[q] < 0x1p100f;
-    const float inv = __builtin_amdgcn_rcpf(s[q]), hi = inv * (1.f + 0x1p-20f), lo = inv * (1.f - 0x1p-20f);
+    const float top = float_of(g);
+    const bool fast = top > 0x1p-96f && top < 0x1p96f;
+    // top / 6, correctly rounded in the same way
+    constexpr float sixth = 1.f / 6.f;
+    float ratio = top * sixth;
+    ratio = __builtin_fmaf(__builtin_fmaf(-6.f, ratio, top), sixth, ratio);
+    if (!fast) ratio = top / 6.f;
+    s[q] = g >= 0x7f800000u ? __builtin_nanf("") : pgn_f32(pgn_bf16(ratio));
+    float inv = __builtin_amdgcn_rcpf(s[q]);
+    inv = __builtin_fmaf(__builtin_fmaf(-s[q], inv, 1.f), inv, inv);
+    const auto over = [&](float w) {
+      const float t = w * inv;
+      return __builtin_fmaf(__builtin_fmaf(-t, s[q], w), inv, t);
+    };
 #pragma unroll
     for (int j = q * GS; j < (q + 1) * GS; ++j) {
-      unsigned a = 0u, b = 0u;
-#define PGN_PAIR(P)                                                                                              \
-  a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, w[j].get(2 * P) * hi, w[j].get(2 * P + 1) * hi, 1.f, P);       \
-  b = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(b, w[j].get(2 * P) * lo, w[j].get(2 * P + 1) * lo, 1.f, P);
-      PGN_PAIR(0)
-      PGN_PAIR(1)
-      PGN_PAIR(2)
-      PGN_PAIR(3)
-#undef PGN_PAIR
-      if (!(fast && a == b)) {
+      unsigned a = 0u;
+      a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, over(w[j].get(0)), over(w[j].get(1)), 1.f, 0);
+      a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, over(w[j].get(2)), over(w[j].get(3)), 1.f, 1);
+      a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, over(w[j].get(4)), over(w[j].get(5)), 1.f, 2);
+      a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, over(w[j].get(6)), over(w[j].get(7)), 1.f, 3);
+      if (!fast) {
         a = 0u;
         if (s[q] > 0.f)  // (zeros and NaN scales: codes 0)
 #pragma unroll
@@ -141,53 +160,65 @@ __global__ __launch_bounds__(256) void quantize(const T* __restrict__ W, u32x4* 
   }
 }
 
-// The eight values of a word of codes, times s.
-PGN_DEVICE void decode8(unsigned c, float s, float (&v)[8]) {
-#define PGN_PAIR(P)                                                              \
-  {                                                                              \
-    const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, P);         \
-    v[2 * P] = s * p[0];                                                         \
-    v[2 * P + 1] = s * p[1];                                                     \
+// How a wave writes the weights of a tile: 16 bytes to a lane, a row's 128 columns side by side, so that memory is written in
+// whole lines (with the lanes of the codes' layout a row's piece is 64 bytes: 32768 x 4096 bf16 in 77 us, so in 67), and past
+// the caches where the rows are whole lines (50; rows of 2000 bytes 7.6 instead of 6.8).
+template <class T>
+struct Rows {
+  static constexpr int kCols = 16 / (int)sizeof(T), kLanes = kTileCols / kCols, kAtOnce = 64 / kLanes,
+                       kTurns = kTileRows / kAtOnce;
+  int row, col;  // of the lane's first vector; the next one's row is kAtOnce further
+  PGN_DEVICE explicit Rows(int l) : row(l / kLanes), col(l % kLanes * kCols) {}
+  // where codes of these columns lie in the tile: the 32-bit word, and its shift
+  PGN_DEVICE int word(int turn) const {
+    const int k8 = col >> 3;
+    return ((k8 & 3) * 16 + row + kAtOnce * turn) * 4 + (k8 >> 2);
   }
-  PGN_PAIR(0)
-  PGN_PAIR(1)
-  PGN_PAIR(2)
-  PGN_PAIR(3)
-#undef PGN_PAIR
-}
-
-PGN_DEVICE void store8(float* p, const float (&v)[8]) {
-  reinterpret_cast<f32x4*>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
-  reinterpret_cast<f32x4*>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
-}
-PGN_DEVICE void store8(__bf16* p, const float (&v)[8]) {
-  bf16x8 o;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = pgn_bf16(v[e]);
-  *reinterpret_cast<bf16x8*>(p) = o;
-}
-
-// One wave a tile.
-template <class T, int GS>
-__global__ __launch_bounds__(256) void dequantize(const u32x4* __restrict__ codes, const __bf16* __restrict__ scales,
+  PGN_DEVICE int shift() const { return (col & 7) * 4; }
+};
+// One wave a tile. LINES: the weight's rows are whole lines of 128 bytes.
+template <class T, int GS, bool LINES>
+__global__ __launch_bounds__(256) void dequantize(const unsigned* __restrict__ codes, const __bf16* __restrict__ scales,
                                                   T* __restrict__ W, int64_t N, int K, int KB, int64_t tiles) {
-  const int l = threadIdx.x & 63, i = l & 15, h = l >> 4;
+  using R = Rows<T>;
+  const int l = threadIdx.x & 63;
   const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (tile >= tiles) return;
   const int64_t rt = tile / KB;
-  const int kb = (int)(tile - rt * KB);
-  const int64_t row = rt * kTileRows + i;
-  const u32x4 c = codes[tile * 64 + l];
-  const __bf16* sp = scales + (tile * kTileRows + i) * (4 / GS);
-  float s[4 / GS];
+  const int k = kTileCols * (int)(tile - rt * KB);
+  const R at(l);
+  unsigned c[R::kTurns];
+  float s[R::kTurns];
 #pragma unroll
-  for (int q = 0; q < 4 / GS; ++q) s[q] = pgn_f32(sp[q]);
+  for (int u = 0; u < R::kTurns; ++u) {
+    c[u] = codes[tile * 256 + at.word(u)] >> at.shift();
+    s[u] = pgn_f32(scales[(tile * kTileRows + at.row + R::kAtOnce * u) * (4 / GS) + at.col / (32 * GS)]);
+  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int k = kTileCols * kb + 32 * j + 8 * h;
-    float v[8];
-    decode8(c[j], s[j / GS], v);
-    if (row < N && k < K) store8(W + row * K + k, v);
+  for (int u = 0; u < R::kTurns; ++u) {
+    const int64_t row = rt * kTileRows + at.row + R::kAtOnce * u;
+    u32x4 o;
+#define PGN_PAIR(P)                                                                                          \
+  if constexpr (2 * P < R::kCols) {                                                                          \
+    const f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, P);                                  \
+    if constexpr (R::kCols == 8) {                                                                           \
+      const bf16x2 r{pgn_bf16(s[u] * v[0]), pgn_bf16(s[u] * v[1])};                                          \
+      o[P] = __builtin_bit_cast(unsigned, r);                                                                \
+    } else {                                                                                                 \
+      o[2 * P & 3] = bits_of(s[u] * v[0]);                                                                   \
+      o[(2 * P + 1) & 3] = bits_of(s[u] * v[1]);                                                             \
+    }                                                                                                        \
+  }
+    PGN_PAIR(0)
+    PGN_PAIR(1)
+    PGN_PAIR(2)
+    PGN_PAIR(3)
+#undef PGN_PAIR
+    if (row < N && k + at.col < K) {
+      u32x4* const to = reinterpret_cast<u32x4*>(W + row * K + k + at.col);
+      if constexpr (LINES) __builtin_nontemporal_store(o, to);
+      else *to = o;
+    }
   }
 }
 
@@ -759,38 +790,45 @@ extern "C" int64_t pragnosia_fp4_scale_bytes(int64_t N, int64_t K, int64_t group
   return weight_ok(N, K, group) ? tiles_of(N, K) * kTileRows * (kTileCols / group) * 2 : PRAGNOSIA_ERR_INVALID_ARGUMENT;
 }
 
-#define PGN_BY_TYPE(FN, SRC, ...)                                                                             \
-  const dim3 grid((unsigned)((tiles + 3) / 4));                                                               \
-  const hipStream_t st = (hipStream_t)stream;                                                                 \
-  if (bf16) {                                                                                                 \
-    if (group == 32) hipLaunchKernelGGL((FN<__bf16, 1>), grid, dim3(256), 0, st, __VA_ARGS__(__bf16));        \
-    else if (group == 64) hipLaunchKernelGGL((FN<__bf16, 2>), grid, dim3(256), 0, st, __VA_ARGS__(__bf16));   \
-    else hipLaunchKernelGGL((FN<__bf16, 4>), grid, dim3(256), 0, st, __VA_ARGS__(__bf16));                    \
-  } else {                                                                                                    \
-    if (group == 32) hipLaunchKernelGGL((FN<float, 1>), grid, dim3(256), 0, st, __VA_ARGS__(float));          \
-    else if (group == 64) hipLaunchKernelGGL((FN<float, 2>), grid, dim3(256), 0, st, __VA_ARGS__(float));     \
-    else hipLaunchKernelGGL((FN<float, 4>), grid, dim3(256), 0, st, __VA_ARGS__(float));                      \
+namespace {
+
+template <class T, int GS>
+void launch_quantize(const void* W, void* codes, void* scales, int64_t N, int K, int64_t tiles, hipStream_t st) {
+  hipLaunchKernelGGL((quantize<T, GS>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, st, (const T*)W, (u32x4*)codes,
+                     (__bf16*)scales, N, K, (K + kTileCols - 1) / kTileCols, tiles);
+}
+
+template <class T, int GS>
+void launch_dequantize(const void* codes, const void* scales, void* W, int64_t N, int K, int64_t tiles, hipStream_t st) {
+  const auto fn = K % (128 / (int)sizeof(T)) == 0 ? dequantize<T, GS, true> : dequantize<T, GS, false>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, st, (const unsigned*)codes,
+                     (const __bf16*)scales, (T*)W, N, K, (K + kTileCols - 1) / kTileCols, tiles);
+}
+
+}  // namespace
+
+#define PGN_BY_TYPE(FN, ...)                                     \
+  if (bf16) {                                                    \
+    if (group == 32) FN<__bf16, 1>(__VA_ARGS__);                 \
+    else if (group == 64) FN<__bf16, 2>(__VA_ARGS__);            \
+    else FN<__bf16, 4>(__VA_ARGS__);                             \
+  } else {                                                       \
+    if (group == 32) FN<float, 1>(__VA_ARGS__);                  \
+    else if (group == 64) FN<float, 2>(__VA_ARGS__);             \
+    else FN<float, 4>(__VA_ARGS__);                              \
   }
 
 extern "C" int pragnosia_fp4_quantize(const void* W, int bf16, void* codes, void* scales, int64_t N, int64_t K,
                                       int64_t group, void* stream) {
   PGN_CHECK_ARG(W && codes && scales && weight_ok(N, K, group) && aligned(W, codes, scales));
-  const int64_t tiles = tiles_of(N, K);
-  const int KB = (int)((K + kTileCols - 1) / kTileCols);
-#define PGN_ARGS(T) (const T*)W, (u32x4*)codes, (__bf16*)scales, N, (int)K, KB, tiles
-  PGN_BY_TYPE(quantize, W, PGN_ARGS)
-#undef PGN_ARGS
+  PGN_BY_TYPE(launch_quantize, W, codes, scales, N, (int)K, tiles_of(N, K), (hipStream_t)stream)
   PGN_RETURN_LAUNCH();
 }
 
 extern "C" int pragnosia_fp4_dequantize(const void* codes, const void* scales, void* W, int bf16, int64_t N, int64_t K,
                                         int64_t group, void* stream) {
   PGN_CHECK_ARG(W && codes && scales && weight_ok(N, K, group) && aligned(W, codes, scales));
-  const int64_t tiles = tiles_of(N, K);
-  const int KB = (int)((K + kTileCols - 1) / kTileCols);
-#define PGN_ARGS(T) (const u32x4*)codes, (const __bf16*)scales, (T*)W, N, (int)K, KB, tiles
-  PGN_BY_TYPE(dequantize, W, PGN_ARGS)
-#undef PGN_ARGS
+  PGN_BY_TYPE(launch_dequantize, codes, scales, W, N, (int)K, tiles_of(N, K), (hipStream_t)stream)
   PGN_RETURN_LAUNCH();
 }
 
