@@ -108,6 +108,8 @@ GEN_SIGNATURES = {
     "pragnosia_rules_workspace_bytes": [_i64] * 2,
     "pragnosia_rules": [_p, _i32, _p, _i64, _i64, _p, _p] + [_p, _f32] * 3 + [_p, _p, _i64, _i64, _p, _i64] + [_p] * 4
                        + [_i64] * 3 + [_p],
+    "pragnosia_rules_tail": [_p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i64] + [_p] * 5
+                            + [_i64, _p, _p, _p, _i64, _i64, _i64, _p],
 }
 
 _GEN_RET_I64 = {"pragnosia_fp4_code_bytes", "pragnosia_fp4_scale_bytes", "pragnosia_rules_workspace_bytes"}

@@ -330,6 +330,68 @@ int run(const Args& a, int64_t B, hipStream_t st) {
   return tiles_of<T>(a.V, 16384) * B >= 512 ? launch<T, 16384, TOKEN>(a, B, st) : launch<T, 8192, TOKEN>(a, B, st);
 }
 
+// What follows a chosen token, one workgroup a row: the token joins the row's history and moves its grammar's state, and
+// (emb) what decode_tail does after its argmax: the token written out, the position advanced, the next step's input.
+constexpr int kTailThreads = 256;
+
+struct Tail {
+  const int64_t* tokens;
+  int64_t* history;
+  int64_t history_stride, cap;
+  int64_t* lengths;
+  const int32_t* next;
+  int64_t S, V;
+  int64_t* state;
+  const float *emb, *pemb;
+  int d, ctx;
+  const int64_t* ctr_in;
+  int64_t* ctr_out;
+  const int64_t* pos_in;
+  int64_t* pos_out;
+  int64_t* out;
+  int64_t n_rows;
+  int64_t* tok;
+  float* h;
+  float* p0s;
+  int L, B;
+};
+
+__global__ __launch_bounds__(kTailThreads) void tail(const Tail a) {
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int64_t t = a.tokens[b];
+  const bool known = t >= 0 && t < a.V;
+  if (tid == 0 && known) {
+    if (a.lengths) {
+      const int64_t n = a.lengths[b];
+      if (n >= 0 && n < a.cap) {
+        a.history[b * a.history_stride + n] = t;
+        a.lengths[b] = n + 1;
+      }
+    }
+    if (a.state) {
+      const int64_t s = a.state[b];
+      if (s >= 0 && s < a.S) a.state[b] = a.next[s * a.V + t];
+    }
+  }
+  if (!a.emb) return;
+  const int64_t c = *a.ctr_in, p = (*a.pos_in + 1) % a.ctx;
+  if (tid == 0) {
+    a.tok[b] = t;
+    if (c >= 0 && c < a.n_rows) a.out[c * a.B + b] = t;
+  }
+  const float* const er = a.emb + (known ? t : 0) * a.d;
+  const float* const pr = a.pemb + p * a.d;
+  float* const hr = a.h + (int64_t)b * a.d;
+  for (int k = tid; k < a.d; k += kTailThreads) hr[k] = (known ? er[k] : 0.f) + pr[k];
+  if (b == 0) {
+    if (tid == 0) {
+      *a.pos_out = p;
+      *a.ctr_out = c + 1;
+    }
+    for (int k = tid; k < a.L; k += kTailThreads) a.p0s[k] = 1.f;
+  }
+}
+
 bool sizes_ok(int64_t B, int64_t V) {
   return B >= 0 && B <= 65535 && V > 0 && V <= ((int64_t)1 << 26) && B * V < ((int64_t)1 << 40);
 }
@@ -366,4 +428,25 @@ extern "C" int pragnosia_rules(const void* logits, int bf16, const int64_t* hist
   const hipStream_t st = (hipStream_t)stream;
   if (tokens) return bf16 ? run<__bf16, true>(a, B, st) : run<float, true>(a, B, st);
   return bf16 ? run<__bf16, false>(a, B, st) : run<float, false>(a, B, st);
+}
+
+extern "C" int pragnosia_rules_tail(const int64_t* tokens, int64_t* history, int64_t history_stride, int64_t cap,
+                                    int64_t* lengths, const int32_t* next, int64_t S, int64_t* state, const float* emb,
+                                    const float* pemb, int64_t d, int64_t ctx, const int64_t* ctr_in, int64_t* ctr_out,
+                                    const int64_t* pos_in, int64_t* pos_out, int64_t* out, int64_t n_rows, int64_t* tok,
+                                    float* h, float* p0s, int64_t L, int64_t B, int64_t V, void* stream) {
+  PGN_CHECK_ARG(sizes_ok(B, V) && (!history == !lengths) && (!history || (cap > 0 && history_stride >= cap)));
+  PGN_CHECK_ARG((!next == !state) && (!next || (S > 0 && S * V < ((int64_t)1 << 40))));
+  PGN_CHECK_ARG(history || next || emb);
+  if (emb) {
+    PGN_CHECK_ARG(pemb && ctr_in && ctr_out && pos_in && pos_out && out && tok && h && d > 0 && d < (1 << 30) && ctx > 0 &&
+                  ctx < (1 << 30) && n_rows > 0 && L >= 0 && L < (1 << 30) && (L == 0 || p0s));
+    PGN_CHECK_ARG(ctr_in != ctr_out && pos_in != pos_out && tok != tokens);
+  }
+  if (B == 0) return PRAGNOSIA_OK;
+  PGN_CHECK_ARG(tokens);
+  const Tail a{tokens, history, history_stride, cap, lengths, next, S, V, state, emb, pemb, (int)d, (int)ctx, ctr_in,
+               ctr_out, pos_in, pos_out, out, n_rows, tok, h, p0s, (int)L, (int)B};
+  hipLaunchKernelGGL(tail, dim3((unsigned)B), dim3(kTailThreads), 0, (hipStream_t)stream, a);
+  PGN_RETURN_LAUNCH();
 }

@@ -17,13 +17,21 @@ layers run on the fp32 matrix cores (decode_gemm, the norms, biases, GELU and re
 a layer (LayerNorm kernel and torch GEMMs where a width is not covered). Other mixers
 run the modules' own T = 1 path. The concatenated weights are copied from the parameters at every `start`, so the
 graph always sees the current parameters.
+
+With weights="fp4" the fused step's projections, both MLP layers and the head run on 4-bit weights (`fp4.linear`, with their
+norms, biases, GELU and residuals inside), rounded from the parameters at every `start`; the gated o-projection stays fp32,
+inside the carrier step's kernels. With `rules` (`rules.TokenRules`) every token, the first included, is the best that
+penalties, biases and a grammar leave (`rules.next_token`), -1 from where nothing is left; the history and the grammar's
+states are kept on the device, so replays still need no host.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
 
+from . import fp4
 from .assoc import AssocCarrier
+from .rules import RuleState, TokenRules
 from .ops import DecodeFold, decode_gemm_ok, decode_tail, ln_supported
 
 
@@ -82,10 +90,14 @@ def _gemm_layers_ok(model) -> bool:
 
 class GreedyDecoder:
     def __init__(self, model, batch: int, steps_per_graph: int = 8, fused: bool | None = None,
-                 record_logits: bool = False):
-        """record_logits: the captured step also writes each step's logits (fp32) into a device buffer of
-        (n + steps_per_graph, batch, vocab), read with `logits(n)`; for checking the graphed path itself against a
-        reference decode, at the cost of one (batch, vocab) copy a step."""
+                 record_logits: bool = False, weights: str | None = None, group: int = 64,
+                 rules: TokenRules | None = None):
+        """record_logits: the captured step also writes each step's logits (fp32, before any rules) into a device buffer
+        of (n + steps_per_graph, batch, vocab), read with `logits(n)`; for checking the graphed path itself against a
+        reference decode, at the cost of one (batch, vocab) copy a step.
+
+        weights: None (the parameters as they are) or "fp4", 4-bit weights with a scale for each `group` columns (32, 64
+        or 128), for the fused step. rules: what tokens are chosen under; read at every `start`."""
         self.m = model
         self.B = batch
         self.K = steps_per_graph
@@ -95,6 +107,14 @@ class GreedyDecoder:
         self.fused = fused_decode_ok(model, batch) if fused is None else fused
         if self.fused and not fused_decode_ok(model, batch):
             raise ValueError("GreedyDecoder: this model's decode step cannot run fused")
+        if weights not in (None, "fp4"):
+            raise ValueError(f"GreedyDecoder: weights must be None or 'fp4', got {weights!r}")
+        if weights is not None and not self.fused:
+            raise ValueError("GreedyDecoder: 4-bit weights need the fused step")
+        if weights is not None:
+            for K in {model.d} | {mp.b.weight.shape[1] for mp in model.mlp}:
+                fp4._sizes("GreedyDecoder", 1, K, group)  # refuses widths and groups that the kernels do not take
+        self.weights, self.group, self.rules, self.rs = weights, group, rules, None
         if self.fused and steps_per_graph % 2:
             raise ValueError("GreedyDecoder: the fused step captures an even number of steps per graph (its tail "
                              "alternates two counter slots)")
@@ -161,12 +181,17 @@ class GreedyDecoder:
                     a.fill_(float(b))
         self.pos.copy_((self.pos + 1) % m.ctx)
         lg = F.linear(m.n(h), m.e.weight)[:, -1]
-        nxt = lg.argmax(-1)
+        if self.rs is None:
+            nxt = lg.argmax(-1)
+        else:
+            nxt = self.rs.choose(lg.float().contiguous())
+            self.rs.advance(nxt)
         if self.lgs is not None:
             self.lgs.index_copy_(0, self.ctr, lg.float().view(1, self.B, -1))
         self.out.index_copy_(0, self.ctr, nxt.view(1, -1))
         self.ctr.add_(1)
-        self.tok.copy_(nxt.view(-1, 1))
+        # (-1, nothing left, is -1 from then on, whatever is read in its place)
+        self.tok.copy_((nxt if self.rs is None else nxt.clamp(min=0)).view(-1, 1))
 
     def _gemm_ok(self) -> bool:
         """Whether the dense layers run on decode_gemm: past the GEMV's batch sizes, every layer's input width
@@ -272,13 +297,81 @@ class GreedyDecoder:
         th, ch, bh = self.wbuf[-1]
         self._tail(op.decode_gemm(h, th, ch.shape[0], 1, ch, m.n.eps, bh, None, 0, None), par)
 
+    def _fp4_weights(self):
+        """Per layer the concatenated input projection and both MLP layers, then the head, in 4 bits; the o-projections'
+        gates, and past GEMV batch sizes their weights as the kernels there take them. Into the same buffers every time."""
+        m, dev = self.m, self.m.e.weight.device
+        K = lambda mx: mx.h * mx.dk
+        first = getattr(self, "q4", None) is None
+        if first:
+            e = lambda *s: torch.empty(*s, device=dev, dtype=torch.float32)
+            self.gates = e(len(m.mix))
+            self.sig = [self.gates[i:i + 1] for i in range(len(m.mix))]
+            self.q4 = [[None] * 3 for _ in m.mix]
+            self.q4head = None
+            self.otile = [e((m.d + 15) // 16 * 16 * K(mx)) if self.gemm else None for mx in m.mix]
+            self.wos = [e(*mx.o.weight.shape) if self.B > GEMV_MAX_BATCH and not self.gemm else None for mx in m.mix]
+        torch.sigmoid(torch.stack([mx.gate.detach().float().reshape(()) for mx in m.mix]), out=self.gates)
+        for q, mx, mp, sig, wos in zip(self.q4, m.mix, m.mlp, self.sig, self.wos):
+            extra = [mx.wb.weight] if mx.delta else ([] if mx.write_all else [mx.wi.weight])
+            W = torch.cat([w.detach().float() for w in [mx.q.weight, mx.k.weight, mx.v.weight, mx.wa.weight] + extra])
+            for j, w in enumerate((W, mp.a.weight.detach().float(), mp.b.weight.detach().float())):
+                q[j] = fp4.quantize(w, self.group, out=q[j])
+            if wos is not None:
+                torch.mul(mx.o.weight.detach().float(), sig, out=wos)
+        self.q4head = fp4.quantize(m.e.weight.detach().float(), self.group, out=self.q4head)
+        if self.gemm:
+            src = [([mx.o.weight], mx.on.weight, None, None) for mx in m.mix]
+            if getattr(self, "fold", None) is None:
+                self.fold = DecodeFold(src, [(t, None, None) for t in self.otile])
+            self.fold.run(src)
+
+    def _one_step_fp4(self, par=0):
+        """The fused step on 4-bit weights: the carrier steps and o-projections of `_one_step_fused` and `_one_step_gemm`,
+        every other dense layer one `fp4.linear`."""
+        m, op, h = self.m, torch.ops.pragnosia, self.h
+        for i, (mx, mp) in enumerate(zip(m.mix, m.mlp)):
+            gated = not (mx.delta or mx.write_all)
+            qp, qa, qb = self.q4[i]
+            P = fp4.linear(h, qp, norm=mx.ln)
+            on_eps = mx.on.eps if mx.on.eps is not None else torch.finfo(torch.float32).eps
+            step = (P, mx.h, mx.wa.bias, mx.A, mx.la_floor if mx.hl_floor else None, mx.wi.bias if gated else None,
+                    mx.wb.bias if mx.delta else None, 0.75 if (mx.delta and mx.write_all) else 0.0, gated, mx.theta,
+                    self.p0s[i:i + 1], 0.0)
+            if self.st2[i] is not None:
+                src, dst = (self.st[i][0], self.st2[i]) if par == 0 else (self.st2[i], self.st[i][0])
+                op.aspin_decode_oproj_(src, dst, *step, mx.on.weight, on_eps, mx.o.weight, self.sig[i], h)
+                x1 = h
+            else:
+                rms = self.gemm or (self.B <= GEMV_MAX_BATCH and _rms_gemv_ok(mx.h * mx.dk))
+                o = op.aspin_decode_proj_(self.st[i][0], *step, None if rms else mx.on.weight, on_eps)
+                if self.gemm:
+                    op.decode_gemm_acc_(o, self.otile[i], 2 if mx.dk == 64 else 3, on_eps, None, self.sig[i], h)
+                    x1 = h
+                elif rms:
+                    x1 = op.decode_gemv_rms(o, mx.o.weight, mx.on.weight, on_eps, None, self.sig[i], 0, h)
+                elif self.B <= GEMV_MAX_BATCH:
+                    x1 = self._dense(o, mx.o.weight, None, scale=self.sig[i], resid=h)
+                else:
+                    x1 = torch.addmm(h, o, self.wos[i].t())
+            hm = fp4.linear(x1, qa, mp.a.bias, norm=mp.n, act="gelu")
+            h = fp4.linear(hm, qb, mp.b.bias, resid=x1)
+        self._tail(fp4.linear(h, self.q4head, norm=m.n), par)
+
     def _tail(self, lg, par):
         """The step's end in one kernel (decode_tail): argmax, the token written to the output row and the token
         buffer, the position advanced, the next step's input embedding into `self.h`, every carried state's position
         offset reset to 1 (one-token calls from here on), the logits recorded when asked. The row counter and the
         position alternate between two int64 slots (read slot `par`, write the other), so a captured graph of an even
-        number of steps replays where the last replay ended."""
+        number of steps replays where the last replay ended. With rules, the token they leave, and the same from it in a
+        second kernel."""
         m = self.m
+        if self.rs is not None:
+            if self.lgs is not None:
+                self.lgs.index_copy_(0, self.ctrb[par:par + 1], lg.view(1, self.B, -1))
+            self.rs.advance(self.rs.choose(lg), (m.e.weight, m.p.weight, self.ctrb[par], self.ctrb[1 - par], self.posb[par],
+                                                 self.posb[1 - par], self.out, self.tok, self.h, self.p0s))
+            return
         decode_tail(lg, m.e.weight, m.p.weight, self.ctrb[par], self.ctrb[1 - par], self.posb[par],
                     self.posb[1 - par], self.out, self.tok, self.h, self.p0s, self.lgs)
 
@@ -324,12 +417,15 @@ class GreedyDecoder:
             h = self._dense(hm, mp.b.weight, None, bias=mp.b.bias, resid=x1)
         self._tail(self._dense(h, m.e.weight, m.n), par)
 
+    def _load_weights(self):
+        self._fp4_weights() if self.weights else self._fused_weights()
+
     def _capture(self, states, n_max):
         dev = self.m.e.weight.device
         self.st = self._static_states(states)
         if self.fused:
             self.gemm = self._gemm_ok()
-            self._fused_weights()
+            self._load_weights()
             self.p0s = torch.stack([st[1].reshape(()) for st in self.st]).float().contiguous()
             # the one-launch step + o-projection (64-wide heads, GEMV batch sizes) writes the new state to a second
             # buffer, the two swapping roles every step
@@ -347,7 +443,8 @@ class GreedyDecoder:
             self.lgs = torch.zeros(n_max + self.K, self.B, self.m.e.weight.shape[0], dtype=torch.float32, device=dev)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        step = (self._one_step if not self.fused else self._one_step_gemm if self.gemm else self._one_step_fused)
+        step = (self._one_step if not self.fused else self._one_step_fp4 if self.weights else
+                self._one_step_gemm if self.gemm else self._one_step_fused)
         with torch.cuda.stream(side):
             for i in range(2):
                 step(i % 2)
@@ -358,23 +455,43 @@ class GreedyDecoder:
                 step(i % 2)
         self.n_max = n_max
 
+    def _load_rules(self, prompt, n):
+        """The rules and the prompt into the graph's buffers; whether they are new ones (the graph is captured again)."""
+        if self.rules is None:
+            self.rs = None
+            return False
+        V, dev = self.m.e.weight.shape[0], self.m.e.weight.device
+        need = (0 if prompt is None else prompt.shape[1]) + n + self.K
+        new = self.rs is None or self.rs.shapes != RuleState.shapes_of(self.rules) or need > self.rs.capacity
+        if new:
+            self.rs = RuleState(self.rules, self.B, V, need, dev)
+        self.rs.load(self.rules, prompt)
+        return new
+
     @torch.no_grad()
-    def start(self, states, pw, lg, n):
-        """Load a prefilled state into the static buffers (capturing the graph on first use)."""
-        if self.graph is None or n > self.n_max:
+    def start(self, states, pw, lg, n, prompt=None):
+        """Load a prefilled state into the static buffers (capturing the graph on first use). prompt (B, P): the ids that
+        rules count as the history."""
+        had = self.rs is not None
+        if self._load_rules(prompt, n) or had != (self.rs is not None) or self.graph is None or n > self.n_max:
             self._capture(states, n)
+            self._load_rules(prompt, n)  # (the capture's first steps moved the history and the states)
         self._load_states(states)
         if self.fused:
-            self._fused_weights()
+            self._load_weights()
         self.pos.fill_(pw)
-        first = lg.argmax(-1)
+        if self.rs is None:
+            first = lg.argmax(-1)
+        else:
+            first = self.rs.choose(lg.float().contiguous())
+            self.rs.advance(first)
         self.out.zero_()
         self.out[0].copy_(first)
         if self.lgs is not None:
             self.lgs.zero_()
             self.lgs[0].copy_(lg.float())
         self.ctr.fill_(1)
-        self.tok.copy_(first.view(-1, 1))
+        self.tok.copy_((first if self.rs is None else first.clamp(min=0)).view(-1, 1))
         if self.fused:
             self.ctrb.fill_(1)
             self.posb.fill_(pw)
@@ -395,9 +512,9 @@ class GreedyDecoder:
 
     @torch.no_grad()
     def generate(self, prompt, n):
-        """prompt (B, P) ids on the device; returns the n greedy tokens (B, n)."""
+        """prompt (B, P) ids on the device; returns the n greedy tokens (B, n), under rules -1 from where nothing is left."""
         states, pw, lg = self.prefill(prompt)
-        self.start(states, pw, lg, n)
+        self.start(states, pw, lg, n, prompt)
         self.replay(n)
         return self.out[:n].t().clone()
 

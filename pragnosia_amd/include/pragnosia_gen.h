@@ -77,6 +77,21 @@ int pragnosia_rules(const void* logits, int bf16, const int64_t* history, int64_
                     const uint32_t* mask, int64_t S, const int64_t* state, void* out, int64_t* tokens, void* workspace,
                     int64_t workspace_bytes, int64_t B, int64_t V, void* stream);
 
+/* What follows a chosen token in a step of generation, for rows b with tokens[b] in [0, V) (others, -1 among them, leave
+ * their history and state as they are): with history (B rows of cap entries, history_stride apart) and lengths (B), the
+ * token becomes entry lengths[b], which counts one more, while it is below cap; with next (S, V) int32 and state (B), a
+ * state s in [0, S) becomes next[s][token]. Each pair may be NULL.
+ *
+ * With emb (V, d), fp32, for all rows the end of a decode step (pragnosia_decode_tail's, after its argmax):
+ * out[c][b] = tok[b] = tokens[b] with c = *ctr_in (out has n_rows rows of B; none past them), p = (*pos_in + 1) mod ctx,
+ * h[b] = emb[token] + pemb[p] (fp32; a token outside the table adds nothing), *ctr_out = c + 1, *pos_out = p,
+ * p0s[0 .. L - 1] = 1. The two counters are read from one slot and written to another; tok is not tokens. */
+int pragnosia_rules_tail(const int64_t* tokens, int64_t* history, int64_t history_stride, int64_t cap, int64_t* lengths,
+                         const int32_t* next, int64_t S, int64_t* state, const float* emb, const float* pemb, int64_t d,
+                         int64_t ctx, const int64_t* ctr_in, int64_t* ctr_out, const int64_t* pos_in, int64_t* pos_out,
+                         int64_t* out, int64_t n_rows, int64_t* tok, float* h, float* p0s, int64_t L, int64_t B, int64_t V,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

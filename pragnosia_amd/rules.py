@@ -3,6 +3,7 @@ for repeated tokens, biases of some words, masks of what a grammar allows, in on
 
     token = next_token(logits, history, lengths, prompt, repetition=1.2, bias=(ids, values), mask=mask, state=state)
     logits = apply_rules(logits, ...)           # the same rules, the logits for a sampler of the caller's own
+    advance(token, history, lengths, next, state)    # the token joins the history and moves the grammar's state, in place
 
 For row b and word v, in fp32, each step rounded:
 
@@ -16,6 +17,7 @@ logits as they are (`src/bench.py:83`).
 """
 from __future__ import annotations
 
+import dataclasses
 import math
 from typing import Optional, Union
 
@@ -242,6 +244,128 @@ def next_token(logits: Tensor, history: Optional[Tensor] = None, lengths: Option
     above every number as in torch.argmax; -1 where nothing is left (every word masked, banned or at -inf). The fp32 values
     are compared, also of bf16 logits."""
     return _rules("next_token", logits, history, lengths, prompt, repetition, presence, frequency, bias, mask, state, True)
+
+
+def advance(tokens: Tensor, history: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
+            next: Optional[Tensor] = None, state: Optional[Tensor] = None, *, vocab: Optional[int] = None) -> None:
+    """What follows a chosen token, in place and without the host: history[b, lengths[b]] = tokens[b] and lengths[b] one
+    more (while there is room), state[b] = next[state[b], tokens[b]] (for a state in [0, S)). tokens, lengths and state (B)
+    and history (B, L) int64, next (S, V) int32; history with lengths, next with state, either pair or both. Rows whose token
+    is outside the vocabulary (-1: nothing was left) stay as they are; without next, the vocabulary is `vocab` words."""
+    if next is None and vocab is None:
+        raise PragnosiaError("advance: the vocabulary's size, as `next` or `vocab`, is needed")
+    V = next.shape[-1] if next is not None else vocab
+    _check_advance("advance", tokens, history, lengths, next, state, V)
+    if _watched(tokens, history, lengths, next, state):
+        raise PragnosiaError("advance: not available in a trace or under a dispatch mode (it works in place)")
+    _tail(tokens, history, lengths, next, state, V)
+
+
+def _check_advance(op: str, tokens, history, lengths, next, state, V: int) -> None:
+    _require_gpu(tokens, history, lengths, next, state)
+    if (history is None) != (lengths is None) or (next is None) != (state is None) or (history is None and next is None):
+        raise PragnosiaError(f"{op}: history with lengths, next with state, either pair or both expected")
+    B = tokens.numel()
+    _expect(op, tokens.device, tokens=(tokens, (B,)), history=(history, (B, None)), lengths=(lengths, (B,)),
+            next=(next, (None, V)), state=(state, (B,)))
+    for name, t in (("tokens", tokens), ("history", history), ("lengths", lengths), ("state", state)):
+        if t is not None and (t.dtype != _I64 or not (t.is_contiguous() or (name == "history" and t.stride(1) == 1 and
+                                                                            t.stride(0) >= t.shape[1]))):
+            raise PragnosiaError(f"{op}: {name} must be int64 and dense (history's rows), as it is changed in place")
+    if next is not None and (next.dtype != torch.int32 or not next.is_contiguous() or next.shape[0] == 0):
+        raise PragnosiaError(f"{op}: next (S, V) must be dense int32 with S > 0, got {tuple(next.shape)} {next.dtype}")
+    if history is not None and history.shape[1] == 0:
+        raise PragnosiaError(f"{op}: a history of no entries has no room")
+
+
+def _tail(tokens, history, lengths, next, state, V: int, step=None) -> None:
+    """The C call. step: the rest of a decode step as decode.GreedyDecoder keeps it, or None."""
+    B = tokens.shape[0]
+    if B == 0:
+        return
+    emb = [None, None, 0, 0] + [None] * 5 + [0, None, None, None, 0]
+    if step is not None:
+        e, pe, ctr_in, ctr_out, pos_in, pos_out, out, tok, h, p0s = step
+        if not (all(t.dtype == _F32 and t.is_contiguous() for t in (e, pe, h, p0s)) and e.shape == (V, h.shape[1])
+                and pe.shape[1] == e.shape[1] and h.shape[0] == B and out.shape[1] == B and tok.numel() == B):
+            raise PragnosiaError("advance: the step's buffers do not have the decoder's shapes and types")
+        emb = [_at(e), _at(pe), e.shape[1], pe.shape[0], _at(ctr_in), _at(ctr_out), _at(pos_in), _at(pos_out), _at(out),
+               out.shape[0], _at(tok), _at(h), _at(p0s), p0s.numel()]
+    _call("pragnosia_rules_tail", gen_lib().pragnosia_rules_tail, tokens, _at(tokens), _at(history),
+          0 if history is None else history.stride(0), 0 if history is None else history.shape[1], _at(lengths), _at(next),
+          0 if next is None else next.shape[0], _at(state), *emb, B, V)
+
+
+@dataclasses.dataclass
+class TokenRules:
+    """Rules that `GreedyDecoder` chooses tokens under, with the meanings of `next_token`: repetition counts the prompt,
+    presence and frequency what was generated. A grammar is an automaton on the GPU: `mask` (S, ceil(V / 32)) holds the words
+    allowed in each state, `next` (S, V) int32 the state after each word (-1: free from then on; S or more: nothing may
+    follow), `state` (B) the states to begin in (0 by default). Without `next` the states stay."""
+    repetition: Penalty = 1.0
+    presence: Penalty = 0.0
+    frequency: Penalty = 0.0
+    bias: Optional[tuple[Tensor, Tensor]] = None
+    mask: Optional[Tensor] = None
+    state: Optional[Tensor] = None
+    next: Optional[Tensor] = None
+
+
+class RuleState:
+    """TokenRules, and the history and states of B sequences they are applied to, in buffers that a captured graph reads."""
+
+    def __init__(self, rules: TokenRules, B: int, V: int, capacity: int, device):
+        self.B, self.V, self.capacity = B, V, capacity
+        self.shapes = self.shapes_of(rules)
+        e = lambda *s, dt=_I64: torch.zeros(*s, device=device, dtype=dt)  # noqa: E731
+        self.history, self.lengths, self.prompt = e(B, capacity), e(B), e(B)
+        self.penalties = [e(B, dt=_F32) for _ in range(3)]
+        ids, _, mask, state, nxt = self.shapes
+        self.bias = None if ids is None else (e(*ids), e(*ids, dt=_F32))
+        self.mask = None if mask is None else e(*mask, dt=torch.int32)
+        self.next = None if nxt is None else e(*nxt, dt=torch.int32)
+        self.state = e(B) if state is not None or nxt is not None else None
+
+    @staticmethod
+    def shapes_of(rules: TokenRules):
+        ids, values = (None, None) if rules.bias is None else rules.bias
+        return tuple(None if t is None else tuple(t.shape) for t in (ids, values, rules.mask, rules.state, rules.next))
+
+    def load(self, rules: TokenRules, prompt: Optional[Tensor]) -> None:
+        """The rules' present values, the prompt (B, P) as history, and the states to begin in."""
+        if self.shapes[0] != self.shapes[1] or (self.next is not None and (self.mask is None or self.next.shape != (
+                self.mask.shape[0], self.V))):
+            raise PragnosiaError("TokenRules: bias ids and values of one shape, and next (S, V) beside mask (S, words), "
+                                 f"expected, got {self.shapes}")
+        for name, buf in zip(("repetition", "presence", "frequency"), self.penalties):
+            p = getattr(rules, name)
+            if not isinstance(p, Tensor) and (not math.isfinite(p) or (name == "repetition" and p <= 0)):
+                raise PragnosiaError(f"TokenRules: {name} must be finite{' and above 0' if name == 'repetition' else ''}, "
+                                     f"got {p}")
+            buf.copy_(p) if isinstance(p, Tensor) else buf.fill_(float(p))
+        if self.bias is not None:
+            self.bias[0].copy_(rules.bias[0]), self.bias[1].copy_(rules.bias[1])
+        if self.mask is not None:
+            self.mask.copy_(rules.mask)
+        if self.next is not None:
+            self.next.copy_(rules.next)
+        if self.state is not None:
+            self.state.zero_() if rules.state is None else self.state.copy_(rules.state)
+        P = 0 if prompt is None else prompt.shape[1]
+        if P:
+            self.history[:, :P].copy_(prompt)
+        self.lengths.fill_(P)
+        self.prompt.fill_(P)
+
+    def choose(self, logits: Tensor) -> Tensor:
+        r, p, f = self.penalties
+        return next_token(logits, self.history, self.lengths, self.prompt, repetition=r, presence=p, frequency=f,
+                          bias=self.bias, mask=self.mask, state=self.state)
+
+    def advance(self, tokens: Tensor, step=None) -> None:
+        state = self.state if self.next is not None else None
+        _check_advance("advance", tokens, self.history, self.lengths, self.next, state, self.V)
+        _tail(tokens, self.history, self.lengths, self.next, state, self.V, step)
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -219,3 +219,37 @@ def test_rules_refuse(unguarded, kw, what):
     for f in (rules.next_token, rules.apply_rules):
         with pytest.raises(PragnosiaError, match=what):
             f(**kw)
+
+
+def tail(L, tokens=one, history=null, stride=0, cap=0, lengths=null, next=null, S=0, state=null, emb=null, d=0, ctx=0,
+         ctr=(one, far), pos=(one, far), tok=far, h=far, B=2, V=100):
+    return L.pragnosia_rules_tail(tokens, history, stride, cap, lengths, next, S, state, emb, emb, d, ctx, *ctr, *pos, far,
+                                  9, tok, h, null, 0, B, V, null)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(), dict(tokens=null, history=one, stride=4, cap=4, lengths=one), dict(history=one, stride=4, cap=4),
+    dict(lengths=one), dict(history=one, stride=3, cap=4, lengths=one), dict(history=one, lengths=one), dict(next=one, S=3),
+    dict(state=one), dict(next=one, state=one), dict(emb=one, ctx=4), dict(emb=one, d=8), dict(emb=one, d=8, ctx=4, h=null),
+    dict(emb=one, d=8, ctx=4, ctr=(one, one)), dict(emb=one, d=8, ctx=4, pos=(far, far)), dict(emb=one, d=8, ctx=4, tok=one),
+    dict(next=one, state=one, S=3, B=-1), dict(next=one, state=one, S=3, V=0)])
+def test_tail_entry_refuses(L, bad):
+    assert tail(L, **bad) == -1
+
+
+def test_tail_entry_of_no_rows(L):
+    assert tail(L, tokens=null, next=one, state=one, S=3, B=0) == 0
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(vocab=10), "either pair"), (dict(history=H, lengths=z(2, **L64)), "vocabulary's size"),
+    (dict(history=H, vocab=10), "either pair"), (dict(history=H, lengths=z(3, **L64), vocab=10), "lengths has shape"),
+    (dict(history=H, lengths=z(2, dtype=torch.int32), vocab=10), "lengths must be int64"),
+    (dict(history=z(3, 2, **L64).t(), lengths=z(2, **L64), vocab=10), "history must be int64 and dense"),
+    (dict(history=H[:, :0], lengths=z(2, **L64), vocab=10), "no room"), (dict(next=z(3, 10, dtype=torch.int32)), "either pair"),
+    (dict(next=z(3, 10, **L64), state=z(2, **L64)), "dense int32"), (dict(next=z(0, 10, dtype=torch.int32), state=z(2, **L64)),
+                                                                     "S > 0"),
+    (dict(next=z(3, 10, dtype=torch.int32), state=z(2)), "state must be int64")])
+def test_advance_refuses(unguarded, kw, what):
+    with pytest.raises(PragnosiaError, match=what):
+        rules.advance(z(2, **L64), **kw)
