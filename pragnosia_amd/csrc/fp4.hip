@@ -297,43 +297,43 @@ struct Vec<__bf16> {
   PGN_DEVICE void set(int e, float v) { a[e] = pgn_bf16(v); }
 };
 
-// Mean and 1 / sigma of a row, in all lanes of the wave that calls: the sum, then the squares about the mean. Up to 1024
-// columns the row stays in registers, longer ones are read twice.
+// Mean and 1 / sigma of a row, in all lanes of a wave: the sum, then the squares about the mean. Up to 1024 columns the row
+// stays in registers, with its loads issued long before; longer ones are read twice.
 template <class T>
-PGN_DEVICE void row_stats(const T* row, int K, float eps, int l, float& mean, float& rstd) {
-  constexpr int H = 2;
+struct RowStats {
+  static constexpr int H = 2;
   Raw<T> raw[H];
-  const bool held = K <= 512 * H;
-  auto load = [&](int k0) PGN_INLINE {
+  PGN_DEVICE void load(const T* row, int K, int l, int k0 = 0) {
 #pragma unroll
     for (int u = 0; u < H; ++u) raw[u].load(row + min(k0 + 8 * (l + 64 * u), K - 8));
-  };
-  auto total = [&](auto&& f) PGN_INLINE {
-    float s = 0.f;
-    for (int k0 = 0; k0 < K; k0 += 512 * H) {
-      if (!held) load(k0);
+  }
+  PGN_DEVICE void get(const T* row, int K, float eps, int l, float& mean, float& rstd) {
+    auto total = [&](auto&& f) PGN_INLINE {
+      float s = 0.f;
+      for (int k0 = 0; k0 < K; k0 += 512 * H) {
+        if (K > 512 * H) load(row, K, l, k0);
 #pragma unroll
-      for (int u = 0; u < H; ++u) {
-        float t = 0.f;
+        for (int u = 0; u < H; ++u) {
+          float t = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t += f(raw[u].get(e));
-        s += k0 + 8 * (l + 64 * u) < K ? t : 0.f;
+          for (int e = 0; e < 8; ++e) t += f(raw[u].get(e));
+          s += k0 + 8 * (l + 64 * u) < K ? t : 0.f;
+        }
       }
-    }
-    return group_sum<64>(s);
-  };
-  if (held) load(0);
-  mean = total([](float v) { return v; }) / (float)K;
-  const float m = mean, var = total([m](float v) { return (v - m) * (v - m); }) / (float)K;
-  rstd = 1.f / sqrtf(var + eps);
-}
+      return group_sum<64>(s);
+    };
+    mean = total([](float v) { return v; }) / (float)K;
+    const float m = mean, var = total([m](float v) { return (v - m) * (v - m); }) / (float)K;
+    rstd = 1.f / sqrtf(var + eps);
+  }
+};
 
-// Eight columns of a row as P bf16 parts, normalised where there is a norm; zeros past the last column, where the load
-// was of others. (K is a multiple of 8. Loads stand under no condition: behind one the compiler cannot count them, and
-// waits for those of the next chunk before it uses this one's.)
-template <class T, int P>
-PGN_DEVICE void stage8(Raw<T> raw, const T* lnw, const T* lnb, float mean, float rstd, int k, int K,
-                       bool tail, bf16x8 (&part)[P]) {
+// Eight columns of a row as P bf16 parts, normalised with LN; zeros past the last column (tail), where the load was of
+// others. (K is a multiple of 8. Loads stand under no condition: behind one the compiler cannot count them, and waits for
+// those of the next chunk before it uses this one's. The norm's weights are loaded here: with the row's, they took longer.)
+template <class T, int P, bool LN>
+PGN_DEVICE void stage8(Raw<T> raw, const T* lnw, const T* lnb, float mean, float rstd, int k, int K, bool tail,
+                       bf16x8 (&part)[P]) {
   if (tail) raw.keep(k < K);
   if constexpr (P == 1) {
     part[0] = __builtin_bit_cast(bf16x8, raw.a);
@@ -341,7 +341,7 @@ PGN_DEVICE void stage8(Raw<T> raw, const T* lnw, const T* lnb, float mean, float
     float z[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] = raw.get(e);
-    if (P == 2 || lnw) {
+    if constexpr (LN) {
       Raw<T> g, b;
       g.load(lnw + min(k, K - 8));
       b.load((lnb ? lnb : lnw) + min(k, K - 8));
@@ -449,31 +449,72 @@ PGN_DEVICE void finish(float v, int row, int col, int N, const T* bias, int act,
   y[off] = (T)v;
 }
 
-// Up to MR = 1 or 4 rows. One tile of 16 columns to a workgroup, its WK waves sharing the blocks of 128 contracted columns.
-// A wave stages its own columns of the rows in LDS of its own, so that only the sums' joining needs a barrier (and four
-// rows' norms another, a wave a row). A wave's loads of a chunk (CBW blocks) are all issued at once.
-template <class T, int P, int GS, int MR, int WK, int CBW>
+// The same of one result to a thread, its bias and residual loaded as the kernel starts (of x where there is none).
+template <class T>
+struct Epilogue {
+  T bias, resid;
+  PGN_DEVICE void load(const T* x, const T* bp, const T* rp, int row, int col, int n, int N) {
+    bias = *(bp ? bp + min(col, N - 1) : x);
+    resid = *(rp ? rp + (size_t)min(row, n - 1) * N + min(col, N - 1) : x);
+  }
+  PGN_DEVICE void finish(float v, int row, int col, int N, const T* bp, int act, const T* rp, T* y) const {
+    v += bp ? (float)bias : 0.f;
+    if (act == 1) v = pgn_gelu_erf(v);
+    v += rp ? (float)resid : 0.f;
+    y[(size_t)row * N + col] = (T)v;
+  }
+};
+
+// Sixteen rows are staged in whole lines: sixteen lanes take 128 neighbouring columns of a row (four lanes 32 of each row: up
+// to 1.7 times as long, 16 x 4096 x 14336 bf16 16.1 us against 9.3). Their pieces are written a pitch apart and read a row
+// apart, so a pitch of one piece past 16 keeps both off each other's banks.
+constexpr int kPitch = 17;
+
+// MR = 1, 4 or 16 rows and one tile of 16 columns to a workgroup, its WK waves sharing the blocks of 128 contracted columns.
+// A wave stages its own columns of the rows in LDS of its own, so that only the sums' joining needs a barrier (and the
+// norms of several rows another). A wave's loads of CBW blocks are issued at once; while it waits for the next, others of the
+// compute unit work (their loads issued ahead, in registers of their own: 64 x 704 x 2816 7.8 -> 9.0 us).
+template <class T, int P, bool LN, int GS, int MR, int WK, int CBW>
 __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                const __bf16* __restrict__ scales, const T* __restrict__ lnw,
                                                const T* __restrict__ lnb, float eps, const T* __restrict__ bias, int act,
-                                               const T* resid, T* y, int n, int N, int K, int KB) {
-  constexpr int U = MR == 1 ? CBW / 4 : CBW;  // pieces of 8 columns a lane stages: of four blocks, or of four rows
-  static_assert((MR == 1 && CBW % 4 == 0) || (MR == 4 && WK == 4), "");
-  __shared__ bf16x8 rows[WK][P][CBW * 16][MR];
+                                               const T* resid, T* y, int n, int N, int K, int KB, int ctiles,
+                                               int rblocks) {
+  constexpr int U = CBW * MR / 4;  // pieces of 8 columns a lane stages
+  constexpr int S = MR == 16 ? kPitch : MR;
+  static_assert(CBW * MR % 4 == 0 && (MR == 1 || MR == 4 || (MR == 16 && !LN)) && 16 * MR <= 64 * WK, "");
+  extern __shared__ __align__(16) char smem[];
   __shared__ float sums[WK][MR][16];
   __shared__ float stat[MR][2];
   const int tid = threadIdx.x, l = tid & 63, wk = __builtin_amdgcn_readfirstlane(tid >> 6), i = l & 15, h = l >> 4;
-  const int ct = blockIdx.x, m = MR == 1 ? 0 : l & 3;
-  const T* const xr = x + (size_t)min(m, n - 1) * K;
-  // piece u of this lane: block j of the wave's, 8 columns in it
-  auto piece = [&](int u) { return MR == 1 ? 4 * u + h : u; };
-  const int k8 = MR == 1 ? i : l >> 2;
+  // workgroups of the same columns run on one XCD (their numbers differ by multiples of 8)
+  int ct = blockIdx.x, rb = 0;
+  if (rblocks > 1) {
+    const int rest = blockIdx.x >> 3;
+    rb = rest % rblocks;
+    ct = rest / rblocks * 8 + (blockIdx.x & 7);
+  }
+  if (ct >= ctiles) return;
+  bf16x8* const mine = reinterpret_cast<bf16x8*>(smem) + wk * P * CBW * 16 * S;  // [P][CBW * 16][S]
+  const int row0 = rb * MR;
+  const int row = row0 + (tid >> 4), col = ct * 16 + (tid & 15);  // the result this thread ends with
+  // piece u of this lane: 8 columns k8 of the wave's blocks, all its blocks' pieces in a row, of row m
+  auto k8 = [&](int u) { return MR == 16 ? 16 * (u / 4) + i : u * (64 / MR) + l / MR; };
+  auto m = [&](int u) { return MR == 16 ? 4 * (u % 4) + h : l % MR; };
+  const T* const xb = x + (size_t)row0 * K;
+  unsigned xr[MR == 16 ? 4 : 1];
+#pragma unroll
+  for (int u = 0; u < (MR == 16 ? 4 : 1); ++u) xr[u] = (unsigned)(min(m(u), n - 1 - row0) * K);
+  auto column = [&](int kb0, int u) { return kTileCols * (kb0 + WK * (k8(u) >> 4)) + 8 * (k8(u) & 15); };
+  constexpr int kRows = LN ? (MR + WK - 1) / WK : 1;  // rows whose moments a wave forms (all form the one of MR = 1)
+  RowStats<T> stats[kRows];
+  auto stat_row = [&](int r) { return x + (size_t)min(row0 + (MR == 1 ? 0 : (wk + WK * r) % MR), n - 1) * K; };
   Raw<T> raw[U];
   u32x4 c[CBW][1];
   Scales<GS> s[CBW][1];
   auto load = [&](int kb0) PGN_INLINE {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u].load(xr + min(kTileCols * (kb0 + WK * piece(u)) + 8 * k8, K - 8));
+    for (int u = 0; u < U; ++u) raw[u].load(xb + (xr[MR == 16 ? u % 4 : 0] + (unsigned)min(column(kb0, u), K - 8)));
 #pragma unroll
     for (int j = 0; j < CBW; ++j) {
       const size_t tile = (size_t)ct * KB + min(kb0 + WK * j, KB - 1);  // (past the last: not used)
@@ -481,20 +522,26 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
       s[j][0].load(scales + (tile * 16 + i) * (4 / GS));
     }
   };
+  if constexpr (LN)
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) stats[r].load(stat_row(r), K, l);
   load(wk);
+  Epilogue<T> end;
+  if (wk < (16 * MR + 63) / 64) end.load(x, bias, resid, row, col, n, N);
   float mean = 0.f, rstd = 1.f;
-  if (P == 2 || (P == 3 && lnw)) {
-    if constexpr (MR == 1) {
-      row_stats(x, K, eps, l, mean, rstd);
-    } else {
-      row_stats(x + (size_t)min(wk, n - 1) * K, K, eps, l, mean, rstd);
-      if (l == 0) {
-        stat[wk][0] = mean;
-        stat[wk][1] = rstd;
+  if constexpr (LN) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      stats[r].get(stat_row(r), K, eps, l, mean, rstd);
+      if (MR > 1 && l == 0 && wk + WK * r < MR) {
+        stat[wk + WK * r][0] = mean;
+        stat[wk + WK * r][1] = rstd;
       }
+    }
+    if constexpr (MR > 1) {
       __syncthreads();
-      mean = stat[m][0];
-      rstd = stat[m][1];
+      mean = stat[m(0)][0];
+      rstd = stat[m(0)][1];
     }
   }
   f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
@@ -502,10 +549,11 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
     if (kb0 != wk) load(kb0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (MR > 1 && kb0 + WK * (MR == 16 ? u / 4 : u * (64 / MR) / 16) >= KB) break;  // (past the last block; of one row, lanes have different ones)
       bf16x8 part[P];
-      stage8<T, P>(raw[u], lnw, lnb, mean, rstd, kTileCols * (kb0 + WK * piece(u)) + 8 * k8, K, true, part);
+      stage8<T, P, LN>(raw[u], lnw, lnb, mean, rstd, column(kb0, u), K, K % kTileCols != 0, part);
 #pragma unroll
-      for (int p = 0; p < P; ++p) rows[wk][p][piece(u) * 16 + k8][m] = part[p];
+      for (int p = 0; p < P; ++p) mine[(p * CBW * 16 + k8(u)) * S + m(u)] = part[p];
     }
     // the wave reads what its own lanes wrote: LDS works in a wave's order, the compiler is kept to it
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -513,27 +561,27 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
 #pragma unroll
     for (int j = 0; j < CBW; ++j)
       if (kb0 + WK * j < KB)
-        block<P, GS>(acc, c[j], s[j], [&](int p, int, int ks) { return rows[wk][p][j * 16 + 4 * ks + h][i % MR]; });
+        block<P, GS>(acc, c[j], s[j],
+                     [&](int p, int, int ks) { return mine[(p * CBW * 16 + j * 16 + 4 * ks + h) * S + i % MR]; });
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
-  if (h == 0)
+  if (h < (MR + 3) / 4)
 #pragma unroll
-    for (int r = 0; r < MR; ++r) sums[wk][r][i] = acc[0][0][r];
+    for (int r = 0; r < (MR < 4 ? MR : 4); ++r) sums[wk][4 * h + r][i] = acc[0][0][r];
   __syncthreads();
-  const int row = tid >> 4, col = ct * 16 + (tid & 15);
   if (tid < 16 * MR && row < n && col < N) {
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < WK; ++k) v += sums[k][row][tid & 15];
-    finish(v, row, col, N, bias, act, resid, y);
+    for (int k = 0; k < WK; ++k) v += sums[k][tid >> 4][tid & 15];
+    end.finish(v, row, col, N, bias, act, resid, y);
   }
 }
 
 // More rows. A workgroup's share: 16 RT rows, WN NT tiles of 16 columns, WK waves sharing the contracted columns of each (WN
 // WK waves). Rows go to LDS in P bf16 parts, a chunk of CB blocks of 128 columns at a time, as the matrix core takes them;
 // codes straight to registers. A chunk's loads are under way while the one before it is multiplied.
-template <class T, int P, int GS, int kWaves, int RT, int U, int WK, int NT>
+template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
 __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                       const __bf16* __restrict__ scales, const T* __restrict__ lnw,
                                                       const T* __restrict__ lnb, float eps, const T* __restrict__ bias,
@@ -541,10 +589,10 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
                                                       int ctiles, int rblocks) {
   constexpr int WN = kWaves / WK, WR = kWaves / RT;  // WR waves stage the same rows, 4 pieces of 8 columns each
   constexpr int CK8 = U * WR * 4, CB = CK8 / 16, CBW = CB / WK;
-  static_assert(CBW * WK * 16 == CK8, "");
+  static_assert(CBW * WK * 16 == CK8 && WR % 4 == 0, "");
   extern __shared__ __align__(16) char smem[];
   __shared__ float stat[2][16 * RT];
-  bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);  // [2 chunks][P][RT][CK8][16]
+  bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);  // [2 chunks][P][RT][CK8][kPitch]
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = l & 15, h = l >> 4, wk = w % WK, wn = w / WK;
   // workgroups of the same columns run on one XCD (their numbers differ by multiples of 8)
@@ -560,9 +608,9 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
 
   // staging: this thread's row, and its first 8-column piece of a chunk. Addresses are a wave's own part plus a lane's 32
   // bits that no chunk changes: the vector unit has no arithmetic to spare (below).
-  const int srt = w % RT, sk = (w / RT) * 4 + h;
+  const int srt = w % RT, sm = w / RT % 4 * 4 + h, sk = w / RT / 4 * 16 + i;
   const T* const xb = x + (size_t)row0 * K;
-  const unsigned xrow = (unsigned)(min(16 * srt + i, n - 1 - row0) * K), xlane = xrow + 8 * sk;
+  const unsigned xrow = (unsigned)(min(16 * srt + sm, n - 1 - row0) * K), xlane = xrow + 8 * sk;
   const int full = K / (8 * CK8);  // chunks that lie in the row whole
   Raw<T> raw[U];
   auto load_x = [&](int c) PGN_INLINE {
@@ -586,30 +634,43 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
         ss[j][t].load(scales + tile * (16 * 4 / GS) + (unsigned)(i * (4 / GS)));
       }
   };
+  // one result to a thread in the smallest tiles, whose latency counts
+  constexpr int C = WN * NT * 16, all = 16 * RT * C / (64 * kWaves), most = 16 / (int)sizeof(T),
+                V = all < 1 ? 1 : all < most ? all : most;
+  constexpr bool single = V == 1 && 16 * RT * C == 64 * kWaves;
+  constexpr int kRows = LN ? 16 * RT / kWaves : 1;  // rows whose moments a wave forms
+  RowStats<T> stats[kRows];
+  auto stat_row = [&](int r) { return x + (size_t)min(row0 + w + kWaves * r, n - 1) * K; };
+  if constexpr (LN)
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) stats[r].load(stat_row(r), K, l);
   load_x(0);
   load_w(0, cw, sw);
+  Epilogue<T> end;
+  if constexpr (single) end.load(x, bias, resid, row0 + tid / C, cg * C + tid % C, n, N);
   float mean = 0.f, rstd = 1.f;
-  if (P == 2 || (P == 3 && lnw)) {
-    for (int r = w; r < 16 * RT; r += kWaves) {
-      row_stats(x + (size_t)min(row0 + r, n - 1) * K, K, eps, l, mean, rstd);
+  if constexpr (LN) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      stats[r].get(stat_row(r), K, eps, l, mean, rstd);
       if (l == 0) {
-        stat[0][r] = mean;
-        stat[1][r] = rstd;
+        stat[0][w + kWaves * r] = mean;
+        stat[1][w + kWaves * r] = rstd;
       }
     }
     __syncthreads();
-    mean = stat[0][16 * srt + i];
-    rstd = stat[1][16 * srt + i];
+    mean = stat[0][16 * srt + sm];
+    rstd = stat[1][16 * srt + sm];
   }
   auto store_x = [&](int c) PGN_INLINE {
-    bf16x8* const to = buf + (c & 1) * P * RT * CK8 * 16;
+    bf16x8* const to = buf + (c & 1) * P * RT * CK8 * kPitch;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k8 = sk + u * WR * 4;
       bf16x8 part[P];
-      stage8<T, P>(raw[u], lnw, lnb, mean, rstd, 8 * (c * CK8 + k8), K, c >= full, part);
+      stage8<T, P, LN>(raw[u], lnw, lnb, mean, rstd, 8 * (c * CK8 + k8), K, c >= full, part);
 #pragma unroll
-      for (int p = 0; p < P; ++p) to[((p * RT + srt) * CK8 + k8) * 16 + i] = part[p];
+      for (int p = 0; p < P; ++p) to[((p * RT + srt) * CK8 + k8) * kPitch + sm] = part[p];
     }
   };
   store_x(0);
@@ -620,12 +681,12 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](int c, const u32x4 (&cc)[CBW][NT], const Scales<GS> (&ss)[CBW][NT]) PGN_INLINE {
-    const bf16x8* const from = buf + (c & 1) * P * RT * CK8 * 16;
+    const bf16x8* const from = buf + (c & 1) * P * RT * CK8 * kPitch;
 #pragma unroll
     for (int j = 0; j < CBW; ++j) {
       if (c * CB + wk + WK * j < KB) {
-        const bf16x8* const at = from + ((wk + WK * j) * 16 + h) * 16 + i;
-        block<P, GS>(acc, cc[j], ss[j], [&](int p, int r, int ks) { return at[((p * RT + r) * CK8 + 4 * ks) * 16]; });
+        const bf16x8* const at = from + ((wk + WK * j) * 16 + h) * kPitch + i;
+        block<P, GS>(acc, cc[j], ss[j], [&](int p, int r, int ks) { return at[((p * RT + r) * CK8 + 4 * ks) * kPitch]; });
       }
     }
   };
@@ -655,7 +716,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
   // The sums go through LDS, wave wk's at [wk][row][column], and V consecutive columns of a row to a thread: the waves' shares
   // are added in order, and rows are read and written in whole vectors. (A pitch of 4 past 16: a store's four rows of 16
   // columns fall on different banks.)
-  constexpr int C = WN * NT * 16, S = C + 4;
+  constexpr int S = C + 4;
   float* const part = reinterpret_cast<float*>(smem);
   __syncthreads();
 #pragma unroll
@@ -666,7 +727,6 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
       for (int e = 0; e < 4; ++e)
         part[(wk * 16 * RT + 16 * r + 4 * h + e) * S + (wn * NT + t) * 16 + i] = acc[r][t][e];
   __syncthreads();
-  constexpr int all = 16 * RT * C / (64 * kWaves), most = 16 / (int)sizeof(T), V = all < 1 ? 1 : all < most ? all : most;
   const bool whole = N % most == 0;  // every vector lies in a row and at a vector's address
   for (int o = tid; o < 16 * RT * C / V; o += 64 * kWaves) {
     const int r = o / (C / V), c = o % (C / V) * V, row = row0 + r, col = cg * C + c;
@@ -679,7 +739,9 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] += part[(k * 16 * RT + r) * S + c + e];
     const size_t off = (size_t)row * N + col;
-    if (V == most && whole) {
+    if constexpr (single) {
+      end.finish(v[0], row, col, N, bias, act, resid, y);
+    } else if (V == most && whole) {
       Vec<T> q;
       if (bias) {
         q.load(bias + col);
@@ -705,7 +767,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
   }
 }
 
-constexpr size_t kPlainLds = 60 << 10;  // dynamic LDS beside `red` that a launch may ask for without raising the limit
+constexpr size_t kPlainLds = 60 << 10;  // LDS that a launch may ask for without raising the limit, statistics apart
 
 struct Call {
   const void *x, *codes, *scales, *lnw, *lnb, *bias, *resid;
@@ -715,24 +777,32 @@ struct Call {
   hipStream_t st;
 };
 
-template <class T, int P, int GS, int MR, int WK, int CBW>
+template <class T, int P, bool LN, int GS, int MR, int WK, int CBW>
 int launch_few(const Call& a) {
-  const int KB = (a.K + kTileCols - 1) / kTileCols, ctiles = (a.N + 15) / 16;
-  hipLaunchKernelGGL((few<T, P, GS, MR, WK, CBW>), dim3((unsigned)ctiles), dim3(64 * WK), 0, a.st, (const T*)a.x,
-                     (const u32x4*)a.codes, (const __bf16*)a.scales, (const T*)a.lnw, (const T*)a.lnb, a.eps,
-                     (const T*)a.bias, a.act, (const T*)a.resid, (T*)a.y, a.n, a.N, a.K, KB);
+  const int KB = (a.K + kTileCols - 1) / kTileCols, ctiles = (a.N + 15) / 16, rblocks = (a.n + MR - 1) / MR;
+  const int64_t blocks = rblocks > 1 ? (int64_t)(ctiles + 7) / 8 * 8 * rblocks : ctiles;
+  constexpr size_t lds = (size_t)WK * P * CBW * 16 * (MR == 16 ? kPitch : MR) * 16, sums = (size_t)WK * MR * 16 * 4;
+  static_assert(lds + sums <= 159 << 10, "");
+  const auto fn = few<T, P, LN, GS, MR, WK, CBW>;
+  if constexpr (lds + sums > kPlainLds) {
+    const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(64 * WK), lds, a.st, (const T*)a.x, (const u32x4*)a.codes,
+                     (const __bf16*)a.scales, (const T*)a.lnw, (const T*)a.lnb, a.eps, (const T*)a.bias, a.act,
+                     (const T*)a.resid, (T*)a.y, a.n, a.N, a.K, KB, ctiles, rblocks);
   PGN_RETURN_LAUNCH();
 }
 
-template <class T, int P, int GS, int kWaves, int RT, int U, int WK, int NT>
+template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
 int launch(const Call& a) {
   constexpr int CB = U * (kWaves / RT) / 4, WN = kWaves / WK;
   const int KB = (a.K + kTileCols - 1) / kTileCols, ctiles = (a.N + 15) / 16;
   const int rblocks = (a.n + 16 * RT - 1) / (16 * RT), groups = (ctiles + WN * NT - 1) / (WN * NT);
   const int64_t blocks = rblocks > 1 ? (int64_t)(groups + 7) / 8 * 8 * rblocks : groups;
-  constexpr size_t chunk = (size_t)P * U * kWaves * 1024, join = (size_t)WK * 16 * RT * (WN * NT * 16 + 4) * 4;
+  constexpr size_t chunk = (size_t)P * U * kWaves * 64 * kPitch, join = (size_t)WK * 16 * RT * (WN * NT * 16 + 4) * 4;
   const size_t lds = std::max(KB > CB ? 2 * chunk : chunk, join);
-  const auto fn = linear<T, P, GS, kWaves, RT, U, WK, NT>;
+  const auto fn = linear<T, P, LN, GS, kWaves, RT, U, WK, NT>;
   static_assert(std::max(2 * chunk, join) <= 159 << 10, "");
   if (lds > kPlainLds) {
     const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), std::max(2 * chunk, join));
@@ -744,27 +814,33 @@ int launch(const Call& a) {
   PGN_RETURN_LAUNCH();
 }
 
-// Rows and columns of a workgroup. Up to four rows a workgroup is one tile of columns. Beyond, the smallest tile of rows by
-// columns that leaves no compute unit a second workgroup, as each stages its rows itself and a short row's cost is its chain
-// of barriers: 16 x 64 while there are 256 workgroups of those or fewer, 32 x 128 likewise, then 32 x 256. Measured, us, for 16 x
-// 64, 32 x 128 and 32 x 256 (fp32): 16 x 2328 x 768 5.7, 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3, 11.5; 512 x 2328 x 768 23.8,
-// 17.2, 13.0. The last with eight waves where there is one part (bf16, 512 x 16384 x 1024 23.7 against 27.7 with sixteen),
-// with sixteen where there are more (fp32, 56 against 65).
-template <class T, int P, int GS>
+// Rows and columns of a workgroup, measured in us. Up to four rows a workgroup is one tile of columns. Beyond, the smallest tile
+// of rows by columns that leaves no compute unit a second workgroup, as each stages its rows itself and a short row's cost is
+// its chain of barriers. 16 x 16, no barrier between blocks, while there are 256 of those or fewer and no norm, whose moments it
+// would form once more a tile of columns: 16 x 768 x 768 fp32 3.5 against 4.1 with 16 x 64, 16 x 4096 x 4096 bf16 4.0 against
+// 6.0; 512 of them 6.7 against 6.2, with a norm 7.5 against 7.3. Then 16 x 64, 32 x 128 and 32 x 256 (fp32: 16 x 2328 x 768 5.7,
+// 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3, 11.5; 512 x 2328 x 768 23.8, 17.2, 13.0). Three parts with groups of 32 do not fit into
+// the registers of 32 x 128 (64 x 8192 x 768 13.4, with 32 x 256 11.5). The last with eight waves where there is one part (bf16,
+// 512 x 16384 x 1024 23.7 against 27.7 with sixteen), with sixteen where there are more (fp32, 56 against 65); 16 x 16 the other
+// way round, as one part leaves its loads the time (16 x 4096 x 14336 bf16 9.3 with sixteen, 11.0 with eight).
+template <class T, int P, bool LN, int GS>
 int by_rows(const Call& a) {
-  if (a.n == 1) return launch_few<T, P, GS, 1, 8, 4>(a);
-  if (a.n <= 4) return launch_few<T, P, GS, 4, 4, 4>(a);
+  if (a.n == 1) return launch_few<T, P, LN, GS, 1, 8, 4>(a);
+  if (a.n <= 4) return launch_few<T, P, LN, GS, 4, 8, 2>(a);
   const auto blocks = [&](int64_t rows, int64_t cols) { return (a.n + rows - 1) / rows * ((a.N + cols - 1) / cols); };
-  if (blocks(16, 64) <= 256) return launch<T, P, GS, 16, 1, 1, 4, 1>(a);
-  if (blocks(32, 128) <= 256) return launch<T, P, GS, 16, 2, 1, 2, 1>(a);
+  if constexpr (!LN)
+    if (blocks(16, 16) <= 256) return launch_few<T, P, LN, GS, 16, P == 1 ? 16 : 8, 1>(a);
+  if (blocks(16, 64) <= 256) return launch<T, P, LN, GS, 16, 1, 1, 4, 1>(a);
+  if constexpr (P < 3 || GS > 1)
+    if (blocks(32, 128) <= 256) return launch<T, P, LN, GS, 16, 2, 1, 2, 1>(a);
   if constexpr (P == 1)
-    if (blocks(32, 256) > 256) return launch<T, P, GS, 8, 2, 2, 1, 2>(a);
-  return launch<T, P, GS, 16, 2, 1, 2, 2>(a);
+    if (blocks(32, 256) > 256) return launch<T, P, LN, GS, 8, 2, 2, 1, 2>(a);
+  return launch<T, P, LN, GS, 16, 2, 1, 2, 2>(a);
 }
 
-template <class T, int P>
+template <class T, int P, bool LN>
 int by_group(const Call& a, int64_t group) {
-  return group == 32 ? by_rows<T, P, 1>(a) : group == 64 ? by_rows<T, P, 2>(a) : by_rows<T, P, 4>(a);
+  return group == 32 ? by_rows<T, P, LN, 1>(a) : group == 64 ? by_rows<T, P, LN, 2>(a) : by_rows<T, P, LN, 4>(a);
 }
 
 bool weight_ok(int64_t N, int64_t K, int64_t group) {
@@ -846,6 +922,6 @@ extern "C" int pragnosia_fp4_linear(const void* x, int bf16, const void* codes, 
   PGN_CHECK_ARG(xa + (uintptr_t)(n * K) * size <= ya || ya + (uintptr_t)(n * N) * size <= xa);
   const Call a{x, codes, scales, ln_weight, ln_bias, bias, resid, y, ln_eps, act, (int)n, (int)N, (int)K,
                (hipStream_t)stream};
-  if (!bf16) return by_group<float, 3>(a, group);
-  return ln_weight ? by_group<__bf16, 2>(a, group) : by_group<__bf16, 1>(a, group);
+  if (!bf16) return ln_weight ? by_group<float, 3, true>(a, group) : by_group<float, 3, false>(a, group);
+  return ln_weight ? by_group<__bf16, 2, true>(a, group) : by_group<__bf16, 1, false>(a, group);
 }
