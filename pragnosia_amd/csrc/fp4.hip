@@ -411,6 +411,30 @@ PGN_DEVICE void block(f32x4 (&acc)[RT][NT], const u32x4 (&c)[NT], const Scales<G
           for (int p = P - 2; p >= 0; --p) v += d[q][p][r][t];
           acc[r][t] += s[t].get(q) * v;
         }
+  } else if constexpr (P == 1 && RT * NT >= 16) {
+    // many tiles: a group's operands of the rows are kept, the tiles of columns taken one after the other (all at once, the
+    // sums leave no registers)
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+      bf16x8 a[GS][RT];
+#pragma unroll
+      for (int g = 0; g < GS; ++g)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) a[g][r] = x(0, r, q * GS + g);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 d[RT];
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+          const bf16x8 b = operand(c[t][q * GS + g]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) d[r] = pgn_mfma(a[g][r], b, g ? d[r] : zero);
+        }
+        const float v = s[t].get(q);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r][t] += v * d[r];
+      }
+    }
   } else {
 #pragma unroll
     for (int q = 0; q < G; ++q) {
@@ -582,14 +606,15 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
 // WK waves). Rows go to LDS in P bf16 parts, a chunk of CB blocks of 128 columns at a time, as the matrix core takes them;
 // codes straight to registers. A chunk's loads are under way while the one before it is multiplied.
 template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
-__global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
+__global__ __launch_bounds__(64 * kWaves, RT == 4 ? 2 : 4) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                       const __bf16* __restrict__ scales, const T* __restrict__ lnw,
                                                       const T* __restrict__ lnb, float eps, const T* __restrict__ bias,
                                                       int act, const T* resid, T* y, int n, int N, int K, int KB,
                                                       int ctiles, int rblocks) {
-  constexpr int WN = kWaves / WK, WR = kWaves / RT;  // WR waves stage the same rows, 4 pieces of 8 columns each
-  constexpr int CK8 = U * WR * 4, CB = CK8 / 16, CBW = CB / WK;
-  static_assert(CBW * WK * 16 == CK8 && WR % 4 == 0, "");
+  // a wave's loads of 4 rows by 128 columns: U in a chunk, of 16 rows' quarters and blocks in turn, so of R row tiles
+  constexpr int WN = kWaves / WK, CB = U * kWaves / (4 * RT), CK8 = 16 * CB, CBW = CB / WK;
+  constexpr int R = 4 * RT > kWaves ? 4 * RT / kWaves : 1, step = CK8 / (U / R);
+  static_assert(CBW * WK * 4 * RT == U * kWaves && U % R == 0 && kWaves % 4 == 0, "");
   extern __shared__ __align__(16) char smem[];
   __shared__ float stat[2][16 * RT];
   bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);  // [2 chunks][P][RT][CK8][kPitch]
@@ -608,18 +633,21 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
 
   // staging: this thread's row, and its first 8-column piece of a chunk. Addresses are a wave's own part plus a lane's 32
   // bits that no chunk changes: the vector unit has no arithmetic to spare (below).
-  const int srt = w % RT, sm = w / RT % 4 * 4 + h, sk = w / RT / 4 * 16 + i;
+  const int sm = w % 4 * 4 + h, sk = w / (4 * RT) * 16 + i;
+  auto srt = [&](int u) { return (w / 4 + u % R * (kWaves / 4)) % RT; };
   const T* const xb = x + (size_t)row0 * K;
-  const unsigned xrow = (unsigned)(min(16 * srt + sm, n - 1 - row0) * K), xlane = xrow + 8 * sk;
+  unsigned xrow[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) xrow[r] = (unsigned)(min(16 * srt(r) + sm, n - 1 - row0) * K);
   const int full = K / (8 * CK8);  // chunks that lie in the row whole
   Raw<T> raw[U];
   auto load_x = [&](int c) PGN_INLINE {
     if (c < full) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u].load(xb + (size_t)(8 * (c * CK8 + u * WR * 4)) + xlane);
+      for (int u = 0; u < U; ++u) raw[u].load(xb + (size_t)(8 * (c * CK8 + u / R * step)) + (xrow[u % R] + 8 * sk));
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u].load(xb + (xrow + (unsigned)min(8 * (c * CK8 + sk + u * WR * 4), K - 8)));
+      for (int u = 0; u < U; ++u) raw[u].load(xb + (xrow[u % R] + (unsigned)min(8 * (c * CK8 + sk + u / R * step), K - 8)));
     }
   };
   u32x4 cw[CBW][NT], cn[CBW][NT];  // this chunk's codes, the next one's
@@ -648,29 +676,32 @@ __global__ __launch_bounds__(64 * kWaves) void linear(const T* __restrict__ x, c
   load_w(0, cw, sw);
   Epilogue<T> end;
   if constexpr (single) end.load(x, bias, resid, row0 + tid / C, cg * C + tid % C, n, N);
-  float mean = 0.f, rstd = 1.f;
+  float mean[R], rstd[R];
   if constexpr (LN) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      stats[r].get(stat_row(r), K, eps, l, mean, rstd);
+      stats[r].get(stat_row(r), K, eps, l, mean[0], rstd[0]);
       if (l == 0) {
-        stat[0][w + kWaves * r] = mean;
-        stat[1][w + kWaves * r] = rstd;
+        stat[0][w + kWaves * r] = mean[0];
+        stat[1][w + kWaves * r] = rstd[0];
       }
     }
     __syncthreads();
-    mean = stat[0][16 * srt + sm];
-    rstd = stat[1][16 * srt + sm];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = stat[0][16 * srt(r) + sm];
+      rstd[r] = stat[1][16 * srt(r) + sm];
+    }
   }
   auto store_x = [&](int c) PGN_INLINE {
     bf16x8* const to = buf + (c & 1) * P * RT * CK8 * kPitch;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k8 = sk + u * WR * 4;
+      const int k8 = sk + u / R * step;
       bf16x8 part[P];
-      stage8<T, P, LN>(raw[u], lnw, lnb, mean, rstd, 8 * (c * CK8 + k8), K, c >= full, part);
+      stage8<T, P, LN>(raw[u], lnw, lnb, LN ? mean[u % R] : 0.f, LN ? rstd[u % R] : 1.f, 8 * (c * CK8 + k8), K, c >= full, part);
 #pragma unroll
-      for (int p = 0; p < P; ++p) to[((p * RT + srt) * CK8 + k8) * kPitch + sm] = part[p];
+      for (int p = 0; p < P; ++p) to[((p * RT + srt(u)) * CK8 + k8) * kPitch + sm] = part[p];
     }
   };
   store_x(0);
@@ -796,7 +827,7 @@ int launch_few(const Call& a) {
 
 template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
 int launch(const Call& a) {
-  constexpr int CB = U * (kWaves / RT) / 4, WN = kWaves / WK;
+  constexpr int CB = U * kWaves / (4 * RT), WN = kWaves / WK;
   const int KB = (a.K + kTileCols - 1) / kTileCols, ctiles = (a.N + 15) / 16;
   const int rblocks = (a.n + 16 * RT - 1) / (16 * RT), groups = (ctiles + WN * NT - 1) / (WN * NT);
   const int64_t blocks = rblocks > 1 ? (int64_t)(groups + 7) / 8 * 8 * rblocks : groups;
@@ -822,7 +853,10 @@ int launch(const Call& a) {
 // 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3, 11.5; 512 x 2328 x 768 23.8, 17.2, 13.0). Three parts with groups of 32 do not fit into
 // the registers of 32 x 128 (64 x 8192 x 768 13.4, with 32 x 256 11.5). The last with eight waves where there is one part (bf16,
 // 512 x 16384 x 1024 23.7 against 27.7 with sixteen), with sixteen where there are more (fp32, 56 against 65); 16 x 16 the other
-// way round, as one part leaves its loads the time (16 x 4096 x 14336 bf16 9.3 with sixteen, 11.0 with eight).
+// way round, as one part leaves its loads the time (16 x 4096 x 14336 bf16 9.3 with sixteen, 11.0 with eight). One part's
+// eight waves take 64 x 256, half the conversions and reads of rows, where the contracted axis is long and workgroups of one
+// to a compute unit fill the last round or nearly: 512 x 8192 x 4096 36.4 against 39.4 with 32 x 256, in groups of 32 41.9
+// against 45.6, 2048 deep 20.4 against 21.4; with the last round a quarter full, 640 x 8192 x 4096 67 against 55.
 template <class T, int P, bool LN, int GS>
 int by_rows(const Call& a) {
   if (a.n == 1) return launch_few<T, P, LN, GS, 1, 8, 4>(a);
@@ -834,7 +868,10 @@ int by_rows(const Call& a) {
   if constexpr (P < 3 || GS > 1)
     if (blocks(32, 128) <= 256) return launch<T, P, LN, GS, 16, 2, 1, 2, 1>(a);
   if constexpr (P == 1)
-    if (blocks(32, 256) > 256) return launch<T, P, LN, GS, 8, 2, 2, 1, 2>(a);
+    if (blocks(32, 256) > 256) {
+      const bool full = (blocks(64, 256) + 255) % 256 >= 224 && (a.n + 31) / 32 % 2 == 0;
+      return full && a.K >= 2048 ? launch<T, P, LN, GS, 8, 4, 4, 2, 4>(a) : launch<T, P, LN, GS, 8, 2, 2, 1, 2>(a);
+    }
   return launch<T, P, LN, GS, 16, 2, 1, 2, 2>(a);
 }
 

@@ -211,6 +211,18 @@ def test_linear_sizes(N, K, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,N,K", [(21, 1000, 264), (21, 4100, 264), (70, 4100, 264), (300, 4100, 264), (1000, 4100, 264),
+                                   (959, 4100, 2056), (960, 4096, 2048), (1024, 4096, 2048)])
+def test_linear_tiles(n, N, K, group, dtype):
+    """Numbers of rows and columns that ask for ever larger tiles, whole and with ragged edges."""
+    Q = fp4.quantize(weight(N, K, dtype), group)
+    bias, resid = rows(1, N, dtype, 4)[0], rows(n, N, dtype, 5)
+    check(rows(n, K, dtype), Q, bias=bias, resid=resid)
+    check(rows(n, K, dtype), Q, norm=layer_norm(K, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n", [1, 4, 6, 90])
 def test_linear_epilogue(n, dtype):
     N, K = 200, 512
