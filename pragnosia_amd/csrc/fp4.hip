@@ -573,7 +573,8 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
     if (kb0 != wk) load(kb0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (MR > 1 && kb0 + WK * (MR == 16 ? u / 4 : u * (64 / MR) / 16) >= KB) break;  // (past the last block; of one row, lanes have different ones)
+      // (past the last block; the lanes of one row's pieces have different ones)
+      if (MR > 1 && kb0 + WK * (MR == 16 ? u / 4 : u * (64 / MR) / 16) >= KB) break;
       bf16x8 part[P];
       stage8<T, P, LN>(raw[u], lnw, lnb, mean, rstd, column(kb0, u), K, K % kTileCols != 0, part);
 #pragma unroll

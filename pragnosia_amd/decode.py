@@ -456,24 +456,24 @@ class GreedyDecoder:
         self.n_max = n_max
 
     def _load_rules(self, prompt, n):
-        """The rules and the prompt into the graph's buffers; whether they are new ones (the graph is captured again)."""
-        if self.rules is None:
-            self.rs = None
-            return False
-        V, dev = self.m.e.weight.shape[0], self.m.e.weight.device
-        need = (0 if prompt is None else prompt.shape[1]) + n + self.K
-        new = self.rs is None or self.rs.shapes != RuleState.shapes_of(self.rules) or need > self.rs.capacity
-        if new:
-            self.rs = RuleState(self.rules, self.B, V, need, dev)
-        self.rs.load(self.rules, prompt)
-        return new
+        """The rules and the prompt into the graph's buffers; a graph of other buffers is let go."""
+        rs = None
+        if self.rules is not None:
+            V, dev = self.m.e.weight.shape[0], self.m.e.weight.device
+            need = (0 if prompt is None else prompt.shape[1]) + n + self.K
+            rs = self.rs
+            if rs is None or rs.shapes != RuleState.shapes_of(self.rules) or need > rs.capacity:
+                rs = RuleState(self.rules, self.B, V, need, dev)
+            rs.load(self.rules, prompt)
+        if rs is not self.rs:  # (rules that were refused leave the buffers, and the graph that reads them, as they were)
+            self.rs, self.graph = rs, None
 
     @torch.no_grad()
     def start(self, states, pw, lg, n, prompt=None):
         """Load a prefilled state into the static buffers (capturing the graph on first use). prompt (B, P): the ids that
         rules count as the history."""
-        had = self.rs is not None
-        if self._load_rules(prompt, n) or had != (self.rs is not None) or self.graph is None or n > self.n_max:
+        self._load_rules(prompt, n)
+        if self.graph is None or n > self.n_max:
             self._capture(states, n)
             self._load_rules(prompt, n)  # (the capture's first steps moved the history and the states)
         self._load_states(states)

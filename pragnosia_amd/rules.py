@@ -184,7 +184,8 @@ def _plain(logits, history, lengths, prompt, penalties, ids, values, mask, state
     if ids is not None:
         M = ids.shape[-1]
         shape = row + (M,) if ids.dim() == 2 else (M,)
-        if not (0 < M <= 1 << 20 and L.bit_length() + M.bit_length() <= 31 and values is not None and _fits(ids, _I64, index, shape) and _fits(values, _F32, index, shape)):
+        if not (0 < M <= 1 << 20 and L.bit_length() + M.bit_length() <= 31 and values is not None
+                and _fits(ids, _I64, index, shape) and _fits(values, _F32, index, shape)):
             return None
         bias_stride = M if ids.dim() == 2 else 0
     elif values is not None:
@@ -229,9 +230,10 @@ def apply_rules(logits: Tensor, history: Optional[Tensor] = None, lengths: Optio
     prompt[b] (0 by default) on were generated; ids outside [0, V) take no part, lengths and prompt are clamped to
     [0, L]. repetition (above 0), presence and frequency: a number, or a (B,) tensor for each row its own. bias: (ids,
     values), both (M) or (B, M): the last entry of a repeated id counts, ids outside [0, V) are skipped, -inf bans a
-    word; L and M must have 31 bits together at most (2^15 entries on 2^15 tokens). mask (S, ceil(V / 32)) int32: word v is allowed where bit v % 32 of word v // 32 is set; state (B) picks each
-    row's line (by default its own of B, or the only one): a negative state leaves the row unmasked, one of S or more
-    masks every word. For inference: no input may require a gradient where gradients are recorded."""
+    word; L and M must have 31 bits together at most (2^15 entries on 2^15 tokens). mask (S, ceil(V / 32)) int32: word v
+    is allowed where bit v % 32 of word v // 32 is set; state (B) picks each row's line (by default its own of B, or the
+    only one): a negative state leaves the row unmasked, one of S or more masks every word. For inference: no input may
+    require a gradient where gradients are recorded."""
     return _rules("apply_rules", logits, history, lengths, prompt, repetition, presence, frequency, bias, mask, state,
                   False)
 

@@ -207,6 +207,24 @@ def test_rules_change_between_generations():
     assert torch.equal(neutral, free)
 
 
+def test_refused_rules_leave_the_decoder_as_it_was():
+    m, x = plain_model(), prompt(2, 9)
+    good = TokenRules(repetition=1.3)
+    dec = GreedyDecoder(m, 2, rules=good)
+    want = dec.generate(x, 20)
+    rs, graph = dec.rs, dec.graph
+    for bad in (TokenRules(next=torch.zeros(3, 500, dtype=torch.int32)), TokenRules(repetition=0.0),
+                TokenRules(bias=(torch.zeros(3, dtype=torch.int64), torch.zeros(4)))):
+        dec.rules = bad
+        with pytest.raises(PragnosiaError):
+            dec.generate(x, 20)
+        assert dec.rs is rs and dec.graph is graph
+    dec.rules = good
+    assert torch.equal(dec.generate(x, 20), want) and dec.graph is graph
+    dec.rules = None
+    assert torch.equal(dec.generate(x, 20), GreedyDecoder(m, 2).generate(x, 20))
+
+
 @pytest.mark.parametrize("B", [1, 5])
 def test_advance(B):
     """History, lengths and states in place: room that ends, tokens and states outside their range, a strided history."""
