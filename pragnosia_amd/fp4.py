@@ -56,6 +56,9 @@ class Weight4:
     def __setattr__(self, name, value):
         raise PragnosiaError(f"Weight4: {name} cannot be changed (its sizes were checked together)")
 
+    def __reduce__(self):  # copies and pickles go through the checks too
+        return Weight4, (self.codes, self.scales, self.N, self.K, self.group, self.dtype)
+
     @property
     def shape(self):
         return torch.Size((self.N, self.K))
@@ -219,8 +222,9 @@ def _check_linear(op: str, x: Tensor, codes: Tensor, scales: Tensor, lnw: Option
 def linear(x: Tensor, Q: Weight4, bias: Optional[Tensor] = None, *, norm: Optional[torch.nn.LayerNorm] = None,
            act: Optional[str] = None, resid: Optional[Tensor] = None) -> Tensor:
     """act(norm(x) W^T + bias) + resid with the weight that Q stands for: x (..., K) fp32 or bf16, result (..., N) in its
-    type. norm: an affine LayerNorm over K; act: None or "gelu" (erf form); bias (N) and resid (..., N). For inference: any
-    input that requires a gradient is refused where gradients are recorded."""
+    type. norm: an affine LayerNorm over K; act: None or "gelu" (erf form); bias (N) and resid (..., N). Parameters and resid
+    of the other type are rounded to x's. For inference: any input that requires a gradient is refused where gradients are
+    recorded."""
     N, K = Q.N, Q.K
     lnw, lnb, eps = None, None, 0.0
     if norm is not None:

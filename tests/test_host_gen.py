@@ -1,7 +1,9 @@
 """CPU checks of generation's operators: the third header's exports, binding and version, what the entry points and the
 Python functions refuse before anything is launched, and the size queries."""
+import copy
 import ctypes
 import os
+import pickle
 import re
 
 import pytest
@@ -253,3 +255,17 @@ def test_tail_entry_of_no_rows(L):
 def test_advance_refuses(unguarded, kw, what):
     with pytest.raises(PragnosiaError, match=what):
         rules.advance(z(2, **L64), **kw)
+
+
+def test_weights_are_copied_and_saved(tmp_path):
+    codes = torch.arange(2048, dtype=torch.int64).to(torch.uint8)
+    Q = fp4.Weight4(codes, torch.arange(64).bfloat16(), 20, 128, 64, torch.bfloat16)
+    m = torch.nn.Module()
+    m.q = Q
+    for R in (copy.copy(Q), copy.deepcopy(m).q, pickle.loads(pickle.dumps(Q))):
+        assert R is not Q and (R.N, R.K, R.group, R.dtype) == (20, 128, 64, torch.bfloat16)
+        assert torch.equal(R.codes, Q.codes) and torch.equal(R.scales, Q.scales)
+    torch.save(Q, tmp_path / "q.pt")
+    with torch.serialization.safe_globals([fp4.Weight4]):
+        R = torch.load(tmp_path / "q.pt", weights_only=True)
+    assert torch.equal(R.codes, Q.codes) and R.shape == Q.shape
