@@ -94,6 +94,8 @@ PGN_DEVICE unsigned exact_code(float w, float s) {
 // reciprocal is: all scales' mantissas were tried), where neither can leave the range; elsewhere by division and
 // exact_code. Deciding the doubtful ones by exact_code instead (two quotients, a little too large and too small, that give
 // different codes) took that path in every other wave of bf16 weights, which often lie on a border: 32768 x 4096 in 82 us.
+// Bound by the weight's bytes where it is large (32768 x 4096 bf16 in 55 us, groups of 32: 6.2 TB/s, part of them from the
+// memory-side cache), by a launch and one round of loads where it is not (8192 x 768 fp32 6 us).
 template <class T, int GS>
 __global__ __launch_bounds__(256) void quantize(const T* __restrict__ W, u32x4* __restrict__ codes,
                                                 __bf16* __restrict__ scales, int64_t N, int K, int KB, int64_t tiles) {
@@ -176,7 +178,8 @@ struct Rows {
   }
   PGN_DEVICE int shift() const { return (col & 7) * 4; }
 };
-// One wave a tile. LINES: the weight's rows are whole lines of 128 bytes.
+// One wave a tile, whose four or eight vectors a lane depend on nothing but their own word and scale. LINES: the weight's rows
+// are whole lines of 128 bytes. Bound by the bytes written.
 template <class T, int GS, bool LINES>
 __global__ __launch_bounds__(256) void dequantize(const unsigned* __restrict__ codes, const __bf16* __restrict__ scales,
                                                   T* __restrict__ W, int64_t N, int K, int KB, int64_t tiles) {
@@ -497,7 +500,9 @@ constexpr int kPitch = 17;
 // MR = 1, 4 or 16 rows and one tile of 16 columns to a workgroup, its WK waves sharing the blocks of 128 contracted columns.
 // A wave stages its own columns of the rows in LDS of its own, so that only the sums' joining needs a barrier (and the
 // norms of several rows another). A wave's loads of CBW blocks are issued at once; while it waits for the next, others of the
-// compute unit work (their loads issued ahead, in registers of their own: 64 x 704 x 2816 7.8 -> 9.0 us).
+// compute unit work (their loads issued ahead, in registers of their own: 64 x 704 x 2816 7.8 -> 9.0 us). One row of 16384 x
+// 4096 in groups of 32 takes 7.8 us, 4.8 TB/s of codes and scales, and is bound by them; small products by the chain of a launch,
+// the row's moments, one round of loads and the join (1 x 2328 x 768 with a norm 3.7 us).
 template <class T, int P, bool LN, int GS, int MR, int WK, int CBW>
 __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                const __bf16* __restrict__ scales, const T* __restrict__ lnw,
@@ -605,7 +610,10 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
 
 // More rows. A workgroup's share: 16 RT rows, WN NT tiles of 16 columns, WK waves sharing the contracted columns of each (WN
 // WK waves). Rows go to LDS in P bf16 parts, a chunk of CB blocks of 128 columns at a time, as the matrix core takes them;
-// codes straight to registers. A chunk's loads are under way while the one before it is multiplied.
+// codes straight to registers. A chunk's loads are under way while the one before it is multiplied. Large products are bound by
+// instructions: beside a matrix instruction of 16 cycles stand its share of the conversions (4 / RT) and of the scaling of its
+// sums (2 in groups of 64); two vector instructions beside one cost 2 cycles, a third 4 more. 512 x 8192 x 4096 bf16 36.4
+// us, 945 TFLOP/s; fp32 rows are three such products (512 x 16384 x 1024 50 us).
 template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
 __global__ __launch_bounds__(64 * kWaves, RT == 4 ? 2 : 4) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                       const __bf16* __restrict__ scales, const T* __restrict__ lnw,
