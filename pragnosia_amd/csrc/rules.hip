@@ -11,7 +11,8 @@
 //
 // Bound by the chain within a workgroup (loads, marks, settling, the pass), two of which a compute unit overlaps: one row of
 // 8192 under a history of 600 4.7 us, 64 of 32768 with a history of 2000, a list of 100 and a mask 10.8, 256 bf16 rows of
-// 131072 with a history of 4000, 32 entries and a mask 38.6 (3.5 TB/s of logits in and out). Workgroups that go through a
+// 131072 with a history of 4000, 32 entries and a mask 33.0 (4.1 TB/s of logits in and out; 21.5 without any rule).
+// A row's tiles run on one XCD, whose L2 then has its history for all but the first (39.0 otherwise). Workgroups that go through a
 // row's tiles by themselves, the next tile's logits on their way, took 48: their registers leave room for one.
 #include <algorithm>
 
@@ -48,6 +49,7 @@ struct Args {
   int64_t* tokens;
   uint64_t* part;  // the best key of each row's tiles, hi above lo
   int L, M, V, words, tiles, shift;
+  int rows;  // B where a row's tiles are to run on one XCD, else 0
 };
 
 template <class T>
@@ -107,9 +109,16 @@ __global__ __launch_bounds__(kThreads) void apply(const Args a) {
   __shared__ Key key_s[kWaves];
   __shared__ int listed;
   static_assert(Q * kThreads * E == W && kWaves == 16, "the waves' keys are reduced in a row of 16 lanes");
-  const int tid = threadIdx.x, b = blockIdx.y, V = a.V;
+  const int tid = threadIdx.x, V = a.V;
+  int b = blockIdx.y, tile = blockIdx.x;
+  if (a.rows) {  // (workgroups whose numbers differ by multiples of 8 share an XCD)
+    const unsigned id = blockIdx.y * (unsigned)a.tiles + blockIdx.x, turn = id >> 3;
+    b = (int)(turn / (unsigned)a.tiles * 8 + (id & 7));
+    tile = (int)(turn % (unsigned)a.tiles);
+    if (b >= a.rows) return;
+  }
   const int64_t row = (int64_t)b * V;
-  const int v0 = (int)blockIdx.x * W - (int)(row & (E - 1));  // the first vector's first word, at least -E + 1
+  const int v0 = tile * W - (int)(row & (E - 1));  // the first vector's first word, at least -E + 1
   const T* const lr = (const T*)a.logits + row;
   T* const yr = (T*)a.out + row;
   const bool entries = a.L || a.M;
@@ -161,7 +170,8 @@ __global__ __launch_bounds__(kThreads) void apply(const Args a) {
   if (entries) {
     // f(place in the tile) for an entry that lies in it
     auto within = [&](int64_t i, auto&& f) {
-      if (i >= 0 && i < V && i >= v0 && i - v0 < W) f((int)(i - v0));
+      const unsigned v = (unsigned)i, k = v - (unsigned)v0;
+      if ((uint64_t)i >> 32 == 0 && v < (unsigned)V && k < (unsigned)W) f((int)k);
     };
     auto enlist = [&](int k, unsigned before) {
       if (before) return;  // marked already
@@ -270,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void apply(const Args a) {
     const Key all = max_row(key_s[tid & (kWaves - 1)]);
     if (tid == 0) {
       if (a.tiles == 1) a.tokens[b] = (int)~all.lo;
-      else a.part[(int64_t)b * a.tiles + blockIdx.x] = (uint64_t)all.hi << 32 | all.lo;
+      else a.part[(int64_t)b * a.tiles + tile] = (uint64_t)all.hi << 32 | all.lo;
     }
   }
 }
@@ -314,7 +324,10 @@ int launch(Args a, int64_t B, hipStream_t st) {
     const hipError_t e = pgn_lds_limit(reinterpret_cast<const void*>(fn), marks + masks);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(fn, dim3((unsigned)a.tiles, (unsigned)B), dim3(kThreads), lds, st, a);
+  // (rows that leave an XCD one more than another only where there are many: 65 rows of 131072 13.4 us, else 15.1)
+  const bool by_row = a.L && a.tiles > 1 && (B % 8 == 0 || (B >= 64 && B < 65528));
+  a.rows = by_row ? (int)B : 0;
+  hipLaunchKernelGGL(fn, dim3((unsigned)a.tiles, (unsigned)(by_row ? (B + 7) / 8 * 8 : B)), dim3(kThreads), lds, st, a);
   if (TOKEN && a.tiles > 1) {
     const hipError_t f = hipGetLastError();
     if (f != hipSuccess) return (int)f;
@@ -326,7 +339,7 @@ int launch(Args a, int64_t B, hipStream_t st) {
 // The words of a tile. A row whose token comes from one tile takes no second launch, which is worth more than the smaller
 // tiles' spread over the chip: 64 rows of 32768 with a history, a list and a mask 15.7 us eager in one tile a row, 18.0 in
 // four, though alone on the GPU 10.8 against 8.1. Longer rows, and logits for a sampler: 16384 words where that leaves two
-// workgroups a compute unit (256 rows of 131072 bf16: 39.0 us, with 8192 words 43.4, with 32768 40.8), else 8192.
+// workgroups a compute unit (256 rows of 131072 bf16: 33.0 us, with 8192 words 42.3, with 32768 38.7), else 8192.
 template <class T, bool TOKEN>
 int run(const Args& a, int64_t B, hipStream_t st) {
   if (TOKEN && tiles_of<T>(a.V, 8192) > 1) {
@@ -431,7 +444,7 @@ extern "C" int pragnosia_rules(const void* logits, int bf16, const int64_t* hist
   PGN_CHECK_ARG(!out || la == oa || la + size <= oa || oa + size <= la);
   const Args a{logits, history, history_stride, lengths, prompt, repetition, presence, frequency, repetition_value,
                presence_value, frequency_value, bias_ids, bias_values, bias_stride, mask, S, state, out, tokens,
-               (uint64_t*)workspace, (int)L, (int)M, (int)V, (int)((V + 31) / 32), 0, bit_length(L)};
+               (uint64_t*)workspace, (int)L, (int)M, (int)V, (int)((V + 31) / 32), 0, bit_length(L), 0};
   const hipStream_t st = (hipStream_t)stream;
   if (tokens) return bf16 ? run<__bf16, true>(a, B, st) : run<float, true>(a, B, st);
   return bf16 ? run<__bf16, false>(a, B, st) : run<float, false>(a, B, st);

@@ -160,6 +160,12 @@ def test_many_rows():
     check(inputs(40, 33000, 20, M=3, S=5, seed=3))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B", [7, 8, 24, 63, 64, 67])
+def test_many_rows_of_several_tiles(B, dtype):
+    check(inputs(B, 17000 if B > 8 else 35001, 40, M=3, S=5, dtype=dtype, seed=B))
+
+
 def test_nothing_left():
     kw = inputs(4, 9000, 10, S=3, seed=9)
     kw["state"] = torch.tensor([0, 2, 3, 1 << 40])
