@@ -511,7 +511,7 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
                                                int rblocks) {
   constexpr int U = CBW * MR / 4;  // pieces of 8 columns a lane stages
   constexpr int S = MR == 16 ? kPitch : MR;
-  static_assert(CBW * MR % 4 == 0 && (MR == 1 || MR == 4 || (MR == 16 && !LN)) && 16 * MR <= 64 * WK, "");
+  static_assert(CBW * MR % 4 == 0 && (MR == 1 || MR == 4 || MR == 16) && 16 * MR <= 64 * WK, "");
   extern __shared__ __align__(16) char smem[];
   __shared__ float sums[WK][MR][16];
   __shared__ float stat[MR][2];
@@ -531,9 +531,10 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
   auto k8 = [&](int u) { return MR == 16 ? 16 * (u / 4) + i : u * (64 / MR) + l / MR; };
   auto m = [&](int u) { return MR == 16 ? 4 * (u % 4) + h : l % MR; };
   const T* const xb = x + (size_t)row0 * K;
-  unsigned xr[MR == 16 ? 4 : 1];
+  constexpr int R = MR == 16 ? 4 : 1;  // rows that a lane stages pieces of
+  unsigned xr[R];
 #pragma unroll
-  for (int u = 0; u < (MR == 16 ? 4 : 1); ++u) xr[u] = (unsigned)(min(m(u), n - 1 - row0) * K);
+  for (int u = 0; u < R; ++u) xr[u] = (unsigned)(min(m(u), n - 1 - row0) * K);
   auto column = [&](int kb0, int u) { return kTileCols * (kb0 + WK * (k8(u) >> 4)) + 8 * (k8(u) & 15); };
   constexpr int kRows = LN ? (MR + WK - 1) / WK : 1;  // rows whose moments a wave forms (all form the one of MR = 1)
   RowStats<T> stats[kRows];
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
   Scales<GS> s[CBW][1];
   auto load = [&](int kb0) PGN_INLINE {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u].load(xb + (xr[MR == 16 ? u % 4 : 0] + (unsigned)min(column(kb0, u), K - 8)));
+    for (int u = 0; u < U; ++u) raw[u].load(xb + (xr[u % R] + (unsigned)min(column(kb0, u), K - 8)));
 #pragma unroll
     for (int j = 0; j < CBW; ++j) {
       const size_t tile = (size_t)ct * KB + min(kb0 + WK * j, KB - 1);  // (past the last: not used)
@@ -557,20 +558,23 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
   load(wk);
   Epilogue<T> end;
   if (wk < (16 * MR + 63) / 64) end.load(x, bias, resid, row, col, n, N);
-  float mean = 0.f, rstd = 1.f;
+  float mean[R], rstd[R];
   if constexpr (LN) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      stats[r].get(stat_row(r), K, eps, l, mean, rstd);
+      stats[r].get(stat_row(r), K, eps, l, mean[0], rstd[0]);
       if (MR > 1 && l == 0 && wk + WK * r < MR) {
-        stat[wk + WK * r][0] = mean;
-        stat[wk + WK * r][1] = rstd;
+        stat[wk + WK * r][0] = mean[0];
+        stat[wk + WK * r][1] = rstd[0];
       }
     }
     if constexpr (MR > 1) {
       __syncthreads();
-      mean = stat[m(0)][0];
-      rstd = stat[m(0)][1];
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        mean[u] = stat[m(u)][0];
+        rstd[u] = stat[m(u)][1];
+      }
     }
   }
   f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
       // (past the last block; the lanes of one row's pieces have different ones)
       if (MR > 1 && kb0 + WK * (MR == 16 ? u / 4 : u * (64 / MR) / 16) >= KB) break;
       bf16x8 part[P];
-      stage8<T, P, LN>(raw[u], lnw, lnb, mean, rstd, column(kb0, u), K, K % kTileCols != 0, part);
+      stage8<T, P, LN>(raw[u], lnw, lnb, LN ? mean[u % R] : 0.f, LN ? rstd[u % R] : 1.f, column(kb0, u), K, K % kTileCols != 0, part);
 #pragma unroll
       for (int p = 0; p < P; ++p) mine[(p * CBW * 16 + k8(u)) * S + m(u)] = part[p];
     }
@@ -854,25 +858,25 @@ int launch(const Call& a) {
   PGN_RETURN_LAUNCH();
 }
 
-// Rows and columns of a workgroup, measured in us. Up to four rows a workgroup is one tile of columns. Beyond, the smallest tile
-// of rows by columns that leaves no compute unit a second workgroup, as each stages its rows itself and a short row's cost is
-// its chain of barriers. 16 x 16, no barrier between blocks, while there are 256 of those or fewer and no norm, whose moments it
-// would form once more a tile of columns: 16 x 768 x 768 fp32 3.5 against 4.1 with 16 x 64, 16 x 4096 x 4096 bf16 4.0 against
-// 6.0; 512 of them 6.7 against 6.2, with a norm 7.5 against 7.3. Then 16 x 64, 32 x 128 and 32 x 256 (fp32: 16 x 2328 x 768 5.7,
-// 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3, 11.5; 512 x 2328 x 768 23.8, 17.2, 13.0). Three parts with groups of 32 do not fit into
-// the registers of 32 x 128 (64 x 8192 x 768 13.4, with 32 x 256 11.5). The last with eight waves where there is one part (bf16,
-// 512 x 16384 x 1024 23.7 against 27.7 with sixteen), with sixteen where there are more (fp32, 56 against 65); 16 x 16 the other
-// way round, as one part leaves its loads the time (16 x 4096 x 14336 bf16 9.3 with sixteen, 11.0 with eight). One part's
-// eight waves take 64 x 256, half the conversions and reads of rows, where the contracted axis is long and workgroups of one
-// to a compute unit fill the last round or nearly: 512 x 8192 x 4096 36.4 against 39.4 with 32 x 256, in groups of 32 41.9
-// against 45.6, 2048 deep 20.4 against 21.4; with the last round a quarter full, 640 x 8192 x 4096 67 against 55.
+// Rows and columns of a workgroup, measured in us. Up to four rows a workgroup is one tile of columns. Beyond, the
+// smallest tile of rows by columns that leaves no compute unit a second workgroup, as each stages its rows itself and a
+// short row's cost is its chain of barriers. 16 x 16, no barrier between blocks, while there are 256 of those or fewer
+// (fp32, against 16 x 64: 16 x 768 x 768 3.5 and 4.1, 16 x 2328 x 768 with a norm 5.8 and 6.5; 512 of them, bf16, 6.7
+// and 6.2). Then 16 x 64, 32 x 128 and 32 x 256 (fp32: 16 x 2328 x 768 5.7, 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3,
+// 11.5; 512 x 2328 x 768 23.8, 17.2, 13.0). Three parts with groups of 32 do not fit into the registers of 32 x 128 (64
+// x 8192 x 768 13.4, with 32 x 256 11.5). The last with eight waves where there is one part (bf16, 512 x 16384 x 1024
+// 23.7 against 27.7 with sixteen), with sixteen where there are more (fp32, 56 against 65); 16 x 16 the other way
+// round, as one part leaves its loads the time (16 x 4096 x 14336 bf16 9.3 with sixteen, 11.0 with eight). One part's
+// eight waves take 64 x 256, half the conversions and reads of rows, where the contracted axis is long and workgroups
+// of one to a compute unit fill the last round or nearly: 512 x 8192 x 4096 36.4 against 39.4 with 32 x 256, in groups
+// of 32 41.9 against 45.6, 2048 deep 20.4 against 21.4; with the last round a quarter full, 640 x 8192 x 4096 67
+// against 55.
 template <class T, int P, bool LN, int GS>
 int by_rows(const Call& a) {
   if (a.n == 1) return launch_few<T, P, LN, GS, 1, 8, 4>(a);
   if (a.n <= 4) return launch_few<T, P, LN, GS, 4, 8, 2>(a);
   const auto blocks = [&](int64_t rows, int64_t cols) { return (a.n + rows - 1) / rows * ((a.N + cols - 1) / cols); };
-  if constexpr (!LN)
-    if (blocks(16, 16) <= 256) return launch_few<T, P, LN, GS, 16, P == 1 ? 16 : 8, 1>(a);
+  if (blocks(16, 16) <= 256) return launch_few<T, P, LN, GS, 16, P == 1 ? 16 : 8, 1>(a);
   if (blocks(16, 64) <= 256) return launch<T, P, LN, GS, 16, 1, 1, 4, 1>(a);
   if constexpr (P < 3 || GS > 1)
     if (blocks(32, 128) <= 256) return launch<T, P, LN, GS, 16, 2, 1, 2, 1>(a);
