@@ -612,14 +612,22 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
   }
 }
 
+// Waves to a SIMD: two workgroups of eight share a compute unit, but for those whose LDS leaves room for one (64 rows; two
+// blocks of three parts) and those of several parts in groups of 32, whose scales and sums would spill (fp32 512 x 16384 x 1024
+// 70.8 us with two, 58.8 with one).
+template <int P, int GS, int kWaves, int RT, int U>
+constexpr int waves_per_simd() {
+  return RT == 4 || (kWaves == 8 && P > 1 && (P * U > 4 || GS == 1)) ? 2 : 4;
+}
+
 // More rows. A workgroup's share: 16 RT rows, WN NT tiles of 16 columns, WK waves sharing the contracted columns of each (WN
 // WK waves). Rows go to LDS in P bf16 parts, a chunk of CB blocks of 128 columns at a time, as the matrix core takes them;
 // codes straight to registers. A chunk's loads are under way while the one before it is multiplied. Large products are bound by
 // instructions: beside a matrix instruction of 16 cycles stand its share of the conversions (4 / RT) and of the scaling of its
 // sums (2 in groups of 64); two vector instructions beside one cost 2 cycles, a third 4 more. 512 x 8192 x 4096 bf16 36.4
-// us, 945 TFLOP/s; fp32 rows are three such products (512 x 16384 x 1024 50 us).
+// us, 945 TFLOP/s; fp32 rows are three such products (512 x 16384 x 1024 48 us).
 template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
-__global__ __launch_bounds__(64 * kWaves, RT == 4 ? 2 : 4) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<P, GS, kWaves, RT, U>())) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
                                                       const __bf16* __restrict__ scales, const T* __restrict__ lnw,
                                                       const T* __restrict__ lnb, float eps, const T* __restrict__ bias,
                                                       int act, const T* resid, T* y, int n, int N, int K, int KB,
@@ -862,15 +870,16 @@ int launch(const Call& a) {
 // smallest tile of rows by columns that leaves no compute unit a second workgroup, as each stages its rows itself and a
 // short row's cost is its chain of barriers. 16 x 16, no barrier between blocks, while there are 256 of those or fewer
 // (fp32, against 16 x 64: 16 x 768 x 768 3.5 and 4.1, 16 x 2328 x 768 with a norm 5.8 and 6.5; 512 of them, bf16, 6.7
-// and 6.2). Then 16 x 64, 32 x 128 and 32 x 256 (fp32: 16 x 2328 x 768 5.7, 8.4, 10.7; 128 x 2328 x 768 10.1, 9.3,
-// 11.5; 512 x 2328 x 768 23.8, 17.2, 13.0). Three parts with groups of 32 do not fit into the registers of 32 x 128 (64
-// x 8192 x 768 13.4, with 32 x 256 11.5). The last with eight waves where there is one part (bf16, 512 x 16384 x 1024
-// 23.7 against 27.7 with sixteen), with sixteen where there are more (fp32, 56 against 65); 16 x 16 the other way
-// round, as one part leaves its loads the time (16 x 4096 x 14336 bf16 9.3 with sixteen, 11.0 with eight). One part's
-// eight waves take 64 x 256, half the conversions and reads of rows, where the contracted axis is long and workgroups
-// of one to a compute unit fill the last round or nearly: 512 x 8192 x 4096 36.4 against 39.4 with 32 x 256, in groups
-// of 32 41.9 against 45.6, 2048 deep 20.4 against 21.4; with the last round a quarter full, 640 x 8192 x 4096 67
-// against 55.
+// and 6.2), with sixteen waves where there is one part, which leaves its loads the time (16 x 4096 x 14336 bf16 9.3,
+// with eight 11.0). Then 16 x 64, 32 x 128 and 32 x 256 (fp32: 16 x 2328 x 768 5.7, 8.4, 10.7; 128 x 2328 x 768 10.1,
+// 9.3, 11.5; 512 x 2328 x 768 23.8, 17.2, 13.0). 32 x 128 has sixteen waves, but eight with two tiles of columns each
+// where three parts make reading the rows the limit and no norm needs the waves (64 x 8192 x 768 8.2, with sixteen 8.8;
+// with a norm 12.3 and 11.8) or groups of 32 the registers (8.4 and 13.4). 32 x 256 has sixteen waves for one round of
+// workgroups, eight for more, two workgroups to a compute unit (512 x 16384 x 1024 bf16 23.7, with sixteen 27.7; fp32
+// 48 and 51, 511 x 16880 x 256 18.3 and 24.8; one round, 512 x 2328 x 768, 17.1 and 14.3). One part's eight waves take
+// 64 x 256, half the conversions and reads of rows, where the contracted axis is long and workgroups of one to a
+// compute unit fill the last round or nearly: 512 x 8192 x 4096 36.4 against 39.4 with 32 x 256, in groups of 32 41.9
+// against 45.6, 2048 deep 20.4 against 21.4; with the last round a quarter full, 640 x 8192 x 4096 67 against 55.
 template <class T, int P, bool LN, int GS>
 int by_rows(const Call& a) {
   if (a.n == 1) return launch_few<T, P, LN, GS, 1, 8, 4>(a);
@@ -878,13 +887,16 @@ int by_rows(const Call& a) {
   const auto blocks = [&](int64_t rows, int64_t cols) { return (a.n + rows - 1) / rows * ((a.N + cols - 1) / cols); };
   if (blocks(16, 16) <= 256) return launch_few<T, P, LN, GS, 16, P == 1 ? 16 : 8, 1>(a);
   if (blocks(16, 64) <= 256) return launch<T, P, LN, GS, 16, 1, 1, 4, 1>(a);
-  if constexpr (P < 3 || GS > 1)
-    if (blocks(32, 128) <= 256) return launch<T, P, LN, GS, 16, 2, 1, 2, 1>(a);
-  if constexpr (P == 1)
-    if (blocks(32, 256) > 256) {
-      const bool full = (blocks(64, 256) + 255) % 256 >= 224 && (a.n + 31) / 32 % 2 == 0;
-      return full && a.K >= 2048 ? launch<T, P, LN, GS, 8, 4, 4, 2, 4>(a) : launch<T, P, LN, GS, 8, 2, 2, 1, 2>(a);
-    }
+  if (blocks(32, 128) <= 256) {
+    if constexpr (P == 3 && (!LN || GS == 1)) return launch<T, P, LN, GS, 8, 2, 2, 2, 2>(a);
+    else return launch<T, P, LN, GS, 16, 2, 1, 2, 1>(a);
+  }
+  if (blocks(32, 256) > 256) {
+    if constexpr (P == 1)
+      if (a.K >= 2048 && (a.n + 31) / 32 % 2 == 0 && (blocks(64, 256) + 255) % 256 >= 224)
+        return launch<T, P, LN, GS, 8, 4, 4, 2, 4>(a);
+    return launch<T, P, LN, GS, 8, 2, P == 1 ? 2 : 1, 1, 2>(a);
+  }
   return launch<T, P, LN, GS, 16, 2, 1, 2, 2>(a);
 }
 
