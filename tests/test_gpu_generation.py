@@ -207,6 +207,22 @@ def test_rules_change_between_generations():
     assert torch.equal(neutral, free)
 
 
+def test_two_decoders_of_one_model():
+    """Weights, histories and states are each decoder's own: replays that take turns give what each gives alone."""
+    m, x = model(), prompt(2, 9)
+    decs = [GreedyDecoder(m, 2, weights="fp4", rules=TokenRules(repetition=1.5)),
+            GreedyDecoder(m, 2, weights="fp4", group=32, rules=kinds(2, 500)["grammar"]), GreedyDecoder(m, 2, weights="fp4")]
+    want = [dec.generate(x, 33) for dec in decs]
+    for dec in decs:
+        states, pw, lg = dec.prefill(x)
+        dec.start(states, pw, lg, 33, x)
+    for _ in range(4):
+        for dec in decs:
+            dec.replay(9)
+    for dec, w in zip(decs, want):
+        assert torch.equal(dec.out[:33].t(), w)
+
+
 def test_refused_rules_leave_the_decoder_as_it_was():
     m, x = plain_model(), prompt(2, 9)
     good = TokenRules(repetition=1.3)

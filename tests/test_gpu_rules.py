@@ -258,6 +258,30 @@ def test_graph_and_streams():
     assert torch.equal(other, rules.next_token(logits, **kw))
 
 
+def test_two_graphs_at_once():
+    """Rows of several tiles, whose best words pass through a workspace: two captured calls replayed on two streams, and
+    eager ones between."""
+    calls = []
+    for seed in (1, 2):
+        logits, kw = gpu(inputs(16, 70001, 40, M=3, S=4, seed=seed))
+        want = rules.next_token(logits, **kw)
+        g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g):
+            token = rules.next_token(logits, **kw)
+        calls.append((g, stream, token, want, logits, kw))
+    for _ in range(10):
+        for g, stream, token, *_ in calls:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                token.zero_()
+                for _ in range(5):
+                    g.replay()
+        eager = [rules.next_token(logits, **kw) for *_, logits, kw in calls]
+        torch.cuda.synchronize()
+        for (_, _, token, want, _, _), got in zip(calls, eager):
+            assert torch.equal(token, want) and torch.equal(got, want)
+
+
 def test_trace():
     from torch.fx.experimental.proxy_tensor import make_fx
     logits, kw = gpu(inputs(2, 100, 8, M=3, S=2, seed=6))
