@@ -585,7 +585,8 @@ __global__ __launch_bounds__(64 * WK) void few(const T* __restrict__ x, const u3
       // (past the last block; the lanes of one row's pieces have different ones)
       if (MR > 1 && kb0 + WK * (MR == 16 ? u / 4 : u * (64 / MR) / 16) >= KB) break;
       bf16x8 part[P];
-      stage8<T, P, LN>(raw[u], lnw, lnb, LN ? mean[u % R] : 0.f, LN ? rstd[u % R] : 1.f, column(kb0, u), K, K % kTileCols != 0, part);
+      stage8<T, P, LN>(raw[u], lnw, lnb, LN ? mean[u % R] : 0.f, LN ? rstd[u % R] : 1.f, column(kb0, u), K,
+                       K % kTileCols != 0, part);
 #pragma unroll
       for (int p = 0; p < P; ++p) mine[(p * CBW * 16 + k8(u)) * S + m(u)] = part[p];
     }
@@ -627,11 +628,10 @@ constexpr int waves_per_simd() {
 // sums (2 in groups of 64); two vector instructions beside one cost 2 cycles, a third 4 more. 512 x 8192 x 4096 bf16 36.4
 // us, 945 TFLOP/s; fp32 rows are three such products (512 x 16384 x 1024 48 us).
 template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
-__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<P, GS, kWaves, RT, U>())) void linear(const T* __restrict__ x, const u32x4* __restrict__ codes,
-                                                      const __bf16* __restrict__ scales, const T* __restrict__ lnw,
-                                                      const T* __restrict__ lnb, float eps, const T* __restrict__ bias,
-                                                      int act, const T* resid, T* y, int n, int N, int K, int KB,
-                                                      int ctiles, int rblocks) {
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<P, GS, kWaves, RT, U>())) void linear(
+    const T* __restrict__ x, const u32x4* __restrict__ codes, const __bf16* __restrict__ scales, const T* __restrict__ lnw,
+    const T* __restrict__ lnb, float eps, const T* __restrict__ bias, int act, const T* resid, T* y, int n, int N, int K,
+    int KB, int ctiles, int rblocks) {
   // a wave's loads of 4 rows by 128 columns: U in a chunk, of 16 rows' quarters and blocks in turn, so of R row tiles
   constexpr int WN = kWaves / WK, CB = U * kWaves / (4 * RT), CK8 = 16 * CB, CBW = CB / WK;
   constexpr int R = 4 * RT > kWaves ? 4 * RT / kWaves : 1, step = CK8 / (U / R);

@@ -12,8 +12,8 @@
 // Bound by the chain within a workgroup (loads, marks, settling, the pass), two of which a compute unit overlaps: one row of
 // 8192 under a history of 600 4.7 us, 64 of 32768 with a history of 2000, a list of 100 and a mask 10.8, 256 bf16 rows of
 // 131072 with a history of 4000, 32 entries and a mask 33.0 (4.1 TB/s of logits in and out; 21.5 without any rule).
-// A row's tiles run on one XCD, whose L2 then has its history for all but the first (39.0 otherwise). Workgroups that go through a
-// row's tiles by themselves, the next tile's logits on their way, took 48: their registers leave room for one.
+// A row's tiles run on one XCD, whose L2 then has its history for all but the first (39.0 otherwise). Workgroups that go
+// through a row's tiles by themselves, the next tile's logits on their way, took 48: their registers leave room for one.
 #include <algorithm>
 
 #include "../include/pragnosia_gen.h"

@@ -82,7 +82,8 @@ def rule(L, logits=one, history=null, stride=0, n=0, r=1.0, ids=null, values=nul
 
 
 @pytest.mark.parametrize("bad", [
-    dict(logits=null), dict(logits=odd), dict(out=odd), dict(out=null), dict(tokens=one), dict(out=ctypes.c_void_p(32)), dict(r=0.0), dict(n=5),
+    dict(logits=null), dict(logits=odd), dict(out=odd), dict(out=null), dict(tokens=one),
+    dict(out=ctypes.c_void_p(32)), dict(r=0.0), dict(n=5),
     dict(n=-1), dict(n=5, history=one, stride=4), dict(n=(1 << 24) + 1, history=one, stride=1 << 30), dict(M=3),
     dict(M=3, ids=one), dict(M=3, ids=one, values=one, bstride=2), dict(M=-1), dict(M=(1 << 20) + 1, ids=one, values=one),
     dict(S=1), dict(S=3, mask=one), dict(S=-1), dict(B=-1), dict(B=1 << 16), dict(V=0), dict(V=(1 << 26) + 1),
