@@ -235,48 +235,38 @@ PGN_DEVICE bf16x8 operand(unsigned c) {
   return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
-// z in P bf16 parts whose sum it is: exactly with three (each takes the next 8 bits, by truncation), to 16 bits with two,
-// rounded with one. An infinity or NaN is its first part alone.
-template <int P>
-PGN_DEVICE void split8(const float (&z)[8], bf16x8 (&part)[P]) {
-  if constexpr (P == 1) {
+// z in three bf16 parts whose sum it is exactly: each takes the next 8 bits, by truncation. An infinity or NaN is its first
+// part alone.
+PGN_DEVICE void split8(const float (&z)[8], bf16x8 (&part)[3]) {
+  unsigned u[3][8];
+  float r[8], any = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[0][e] = pgn_bf16(z[e]);
-  } else {
-    unsigned u[P][8];
-    float r[8], any = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      u[0][e] = bits_of(z[e]) & 0xffff0000u;
-      r[e] = z[e] - float_of(u[0][e]);
-      any += r[e];
-    }
-    if (any != any) {  // an infinity or NaN less itself is NaN
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned b = bits_of(z[e]);
-        if ((b & 0x7f800000u) == 0x7f800000u) {
-          u[0][e] |= b & 0x7fffffu ? 0x400000u : 0u;  // (a NaN whose bits are all low stays one)
-          r[e] = 0.f;
-        }
-      }
-    }
+  for (int e = 0; e < 8; ++e) {
+    u[0][e] = bits_of(z[e]) & 0xffff0000u;
+    r[e] = z[e] - float_of(u[0][e]);
+    any += r[e];
+  }
+  if (any != any) {  // an infinity or NaN less itself is NaN
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (P == 3) {
-        u[1][e] = bits_of(r[e]) & 0xffff0000u;
-        u[2][e] = bits_of(r[e] - float_of(u[1][e]));
-      } else {
-        u[1][e] = bits_of(r[e]);
+      const unsigned b = bits_of(z[e]);
+      if ((b & 0x7f800000u) == 0x7f800000u) {
+        u[0][e] |= b & 0x7fffffu ? 0x400000u : 0u;  // (a NaN whose bits are all low stays one)
+        r[e] = 0.f;
       }
     }
+  }
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      u32x4 o;
+  for (int e = 0; e < 8; ++e) {
+    u[1][e] = bits_of(r[e]) & 0xffff0000u;
+    u[2][e] = bits_of(r[e] - float_of(u[1][e]));
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = __builtin_amdgcn_perm(u[p][2 * e + 1], u[p][2 * e], 0x07060302u);
-      part[p] = __builtin_bit_cast(bf16x8, o);
-    }
+  for (int p = 0; p < 3; ++p) {
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_amdgcn_perm(u[p][2 * e + 1], u[p][2 * e], 0x07060302u);
+    part[p] = __builtin_bit_cast(bf16x8, o);
   }
 }
 
@@ -353,7 +343,7 @@ PGN_DEVICE void stage8(Raw<T> raw, const T* lnw, const T* lnb, float mean, float
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = (z[e] - mean) * rstd * g.get(e) + b.get(e);
     }
-    split8<P>(z, part);
+    split8(z, part);
   }
 }
 
@@ -985,5 +975,5 @@ extern "C" int pragnosia_fp4_linear(const void* x, int bf16, const void* codes, 
   const Call a{x, codes, scales, ln_weight, ln_bias, bias, resid, y, ln_eps, act, (int)n, (int)N, (int)K,
                (hipStream_t)stream};
   if (!bf16) return ln_weight ? by_group<float, 3, true>(a, group) : by_group<float, 3, false>(a, group);
-  return ln_weight ? by_group<__bf16, 2, true>(a, group) : by_group<__bf16, 1, false>(a, group);
+  return ln_weight ? by_group<__bf16, 3, true>(a, group) : by_group<__bf16, 1, false>(a, group);
 }

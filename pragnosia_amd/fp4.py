@@ -9,8 +9,8 @@ A weight is kept as 4-bit floating codes (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 with 
 batch, weights="fp4")` runs a model's decode step on them; the reference decodes in fp32 (`src/bench.py:241-317`).
 
 `linear` multiplies the values s v that the codes stand for, with fp32 sums, and is as exact as its operands' type lets it
-be: fp32 rows are not rounded (they go through the bf16 matrix cores in three parts), bf16 rows are taken as they are, and a
-bf16 row's LayerNorm is kept to 16 bits. Sums are taken in a fixed order: the same call gives the same bits.
+be: fp32 rows, and normalised rows of either type, are not rounded (they go through the bf16 matrix cores in three parts),
+other bf16 rows are taken as they are. Sums are taken in a fixed order: the same call gives the same bits.
 
 There is no backward: an input that requires a gradient is refused where gradients are recorded. An eager call goes
 straight to the C ABI; one that something records or replaces (torch.compile, make_fx, torch.jit.trace, a dispatch mode)
