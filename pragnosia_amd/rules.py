@@ -18,7 +18,6 @@ logits as they are (`src/bench.py:83`).
 from __future__ import annotations
 
 import dataclasses
-import math
 from typing import Optional, Union
 
 import torch
@@ -30,6 +29,17 @@ from .head import _BF16, _F32, _FLOATS, _I64, _INTS, _as, _at, _call, _no_tangen
 from .ops import _expect, _require_gpu
 
 Penalty = Union[float, Tensor]
+_MAX, _TINY = torch.finfo(torch.float32).max, 2.0 ** -149  # of what the kernels take a penalty's number in
+
+
+def _in_range(name: str, p: float) -> bool:
+    """Whether fp32 holds a penalty: finite, and above 0 where it divides. (1e39 is finite here and infinite there, and its
+    product with a logit of 0 a NaN, which is above every word.)"""
+    return _TINY <= p <= _MAX if name == "repetition" else -_MAX <= p <= _MAX
+
+
+def _out_of_range(what: str, name: str, p: float) -> PragnosiaError:
+    return PragnosiaError(f"{what}: {name} must be finite{' and above 0' if name == 'repetition' else ''} in fp32, got {p}")
 
 
 def _checked(op: str, logits: Tensor, history: Optional[Tensor], lengths: Optional[Tensor], prompt: Optional[Tensor],
@@ -56,8 +66,8 @@ def _checked(op: str, logits: Tensor, history: Optional[Tensor], lengths: Option
             _expect(op, dev, **{name: (p, (B,))})
             if not p.is_floating_point():
                 raise PragnosiaError(f"{op}: {name} must be floating, got {p.dtype}")
-        elif not math.isfinite(p) or (name == "repetition" and p <= 0):
-            raise PragnosiaError(f"{op}: {name} must be finite{' and above 0' if name == 'repetition' else ''}, got {p}")
+        elif not _in_range(name, p):
+            raise _out_of_range(op, name, p)
     if (ids is None) != (values is None):
         raise PragnosiaError(f"{op}: bias is (ids, values)")
     if ids is not None:
@@ -179,7 +189,8 @@ def _plain(logits, history, lengths, prompt, penalties, ids, values, mask, state
             args += [p.data_ptr(), 1.0]
         else:
             args += [None, p]
-    if not (isinstance(args[1], float) and 0.0 < args[1] < math.inf and math.isfinite(args[3]) and math.isfinite(args[5])):
+    if not (isinstance(args[1], float) and _TINY <= args[1] <= _MAX and -_MAX <= args[3] <= _MAX
+            and -_MAX <= args[5] <= _MAX):
         return None
     if ids is not None:
         M = ids.shape[-1]
@@ -228,7 +239,8 @@ def apply_rules(logits: Tensor, history: Optional[Tensor] = None, lengths: Optio
 
     history (B, L): each row's token ids, of which the first lengths[b] (all by default) are there and those from
     prompt[b] (0 by default) on were generated; ids outside [0, V) take no part, lengths and prompt are clamped to
-    [0, L]. repetition (above 0), presence and frequency: a number, or a (B,) tensor for each row its own. bias: (ids,
+    [0, L]. repetition (above 0), presence and frequency: a number finite in fp32, or a (B,) tensor for each row its own, whose
+    values are taken as they are. bias: (ids,
     values), both (M) or (B, M): the last entry of a repeated id counts, ids outside [0, V) are skipped, -inf bans a
     word; L and M must have 31 bits together at most (2^15 entries on 2^15 tokens). mask (S, ceil(V / 32)) int32: word v
     is allowed where bit v % 32 of word v // 32 is set; state (B) picks each row's line (by default its own of B, or the
@@ -341,9 +353,8 @@ class RuleState:
                                  f"expected, got {self.shapes}")
         for name, buf in zip(("repetition", "presence", "frequency"), self.penalties):
             p = getattr(rules, name)
-            if not isinstance(p, Tensor) and (not math.isfinite(p) or (name == "repetition" and p <= 0)):
-                raise PragnosiaError(f"TokenRules: {name} must be finite{' and above 0' if name == 'repetition' else ''}, "
-                                     f"got {p}")
+            if not isinstance(p, Tensor) and not _in_range(name, p):
+                raise _out_of_range("TokenRules", name, p)
             buf.copy_(p) if isinstance(p, Tensor) else buf.fill_(float(p))
         if self.bias is not None:
             self.bias[0].copy_(rules.bias[0]), self.bias[1].copy_(rules.bias[1])
