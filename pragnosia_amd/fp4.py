@@ -30,11 +30,8 @@ from .ops import _expect, _require_gpu
 
 GROUPS = (32, 64, 128)
 _ACTS = {None: 0, "gelu": 1}
-_U8, _empty, _new = torch.uint8, torch.empty, object.__new__
+_U8, _empty = torch.uint8, torch.empty
 _device = torch._C._cuda_getDevice  # current_device() without the check that CUDA is initialised: a GPU tensor was made
-
-
-_put = object.__setattr__
 
 
 class Weight4:
@@ -48,9 +45,10 @@ class Weight4:
         self._set(codes, scales, N, K, group, dtype)
 
     def _set(self, codes, scales, N, K, group, dtype):
-        put = _put
-        put(self, "codes", codes), put(self, "scales", scales), put(self, "dtype", dtype)
-        put(self, "N", N), put(self, "K", K), put(self, "group", group)
+        # (written out: torch.compile traces these and `Weight4.__new__(Weight4)`, and no other names for them)
+        object.__setattr__(self, "codes", codes), object.__setattr__(self, "scales", scales)
+        object.__setattr__(self, "dtype", dtype), object.__setattr__(self, "N", N)
+        object.__setattr__(self, "K", K), object.__setattr__(self, "group", group)
         return self
 
     def __setattr__(self, name, value):
@@ -122,11 +120,11 @@ def quantize(W: Tensor, group: int = 64, out: Optional[Weight4] = None) -> Weigh
     max |w| / 6 rounded to bf16, a code the nearest value (ties to the even code, past 6 to 6); a group with an infinity or
     a NaN becomes NaN throughout. `out`: a Weight4 of the same sizes, group and device to write into (one that a captured
     graph reads, say)."""
-    if W.dim() == 2 and out is None:  # the usual call, without the general path's looks at everything (10 us of host; this 7)
+    # the usual call, without the general path's looks at everything (10 us of host; this 7)
+    if W.dim() == 2 and out is None and _quiet({type(W)}):
         index, dt, (N, K) = W.get_device(), W.dtype, W.shape
         if (W.is_cuda and index == _device() and dt in _FLOATS and group in GROUPS and 0 < N <= 1 << 26 and 0 < K <= 65536
-                and K % 8 == 0 and W.is_contiguous() and not W.data_ptr() & 15 and forward_ad._current_level < 0
-                and _quiet({type(W)})):
+                and K % 8 == 0 and W.is_contiguous() and not W.data_ptr() & 15 and forward_ad._current_level < 0):
             tiles = -(-N // 16) * -(-K // 128)
             codes = _empty(tiles * 1024, device=W.device, dtype=_U8)
             scales = _empty(tiles * (2048 // group), device=W.device, dtype=_BF16)
@@ -134,7 +132,7 @@ def quantize(W: Tensor, group: int = 64, out: Optional[Weight4] = None) -> Weigh
                                                   _raw_stream(index))
             if rc:
                 check(rc, "pragnosia_fp4_quantize")
-            return _new(Weight4)._set(codes, scales, N, K, group, dt)
+            return Weight4.__new__(Weight4)._set(codes, scales, N, K, group, dt)
     nbytes, count = _check_source("quantize", W, group)
     N, K = W.shape
     if out is not None:
@@ -160,7 +158,7 @@ def dequantize(Q: Weight4, dtype: Optional[torch.dtype] = None) -> Tensor:
         raise PragnosiaError(f"dequantize: fp32 or bf16 expected, got {dtype}")
     codes, scales = Q.codes, Q.scales
     index = codes.get_device()
-    if codes.is_cuda and index == _device() and _quiet({type(codes), type(scales)}):
+    if _quiet({type(codes), type(scales)}) and codes.is_cuda and index == _device():
         W = _empty(Q.N, Q.K, device=codes.device, dtype=dtype)
         rc = gen_lib().pragnosia_fp4_dequantize(codes.data_ptr(), scales.data_ptr(), W.data_ptr(), dtype is _BF16, Q.N, Q.K,
                                                 Q.group, _raw_stream(index))
@@ -183,8 +181,9 @@ _PLAIN = {Tensor, torch.nn.Parameter, type(None), float, int}
 
 
 def _quiet(types: set) -> bool:
-    """_watched's negative, of a set of argument types."""
-    return _PLAIN.issuperset(types) and not _watched()
+    """_watched's negative, of a set of argument types. Asked before anything else of a short way: what stands behind it (the
+    current device, addresses) is neither traced nor there for a fake tensor."""
+    return not _watched() and _PLAIN.issuperset(types)
 
 
 def _linear(x: Tensor, codes: Tensor, scales: Tensor, lnw: Optional[Tensor], lnb: Optional[Tensor], eps: float,
@@ -242,11 +241,11 @@ def linear(x: Tensor, Q: Weight4, bias: Optional[Tensor] = None, *, norm: Option
     # the usual call: nothing to convert, to refuse or to record, and the host has no more to do than to see so (the general
     # path below takes 15 us of the host for a projection of one row, this one 9, its launch 5 of either)
     dt, index, n = x.dtype, x.get_device(), x.shape[0]
-    if (x.is_cuda and x.dim() == 2 and 0 < n <= 1 << 16 and n * max(N, K) < 1 << 31 and dt in _FLOATS and eps >= 0.0
+    if (_quiet({type(x), type(lnw), type(lnb), type(bias), type(resid), type(Q.codes), type(Q.scales)})
+            and x.is_cuda and x.dim() == 2 and 0 < n <= 1 << 16 and n * max(N, K) < 1 << 31 and dt in _FLOATS and eps >= 0.0
             and index == Q.codes.get_device() == _device() and _fits(x, dt, index, (n, K))
             and (lnw is None or _fits(lnw, dt, index, (K,)) and (lnb is None or _fits(lnb, dt, index, (K,))))
-            and (bias is None or _fits(bias, dt, index, (N,))) and (resid is None or _fits(resid, dt, index, (n, N)))
-            and _quiet({type(x), type(lnw), type(lnb), type(bias), type(resid), type(Q.codes), type(Q.scales)})):
+            and (bias is None or _fits(bias, dt, index, (N,))) and (resid is None or _fits(resid, dt, index, (n, N)))):
         y = x.new_empty(n, N)
         rc = gen_lib().pragnosia_fp4_linear(x.data_ptr(), dt is _BF16, Q.codes.data_ptr(), Q.scales.data_ptr(), _at(lnw),
                                             _at(lnb), eps, _at(bias), _ACTS[act], _at(resid), y.data_ptr(), n, N, K,

@@ -162,7 +162,8 @@ def _plain(logits, history, lengths, prompt, penalties, ids, values, mask, state
     """The usual call, all of whose tensors the kernels take as they are: no conversions, and no refusals to look for, which
     is most of what the host does in the general path (19 us for one row with a history; this one 11). None: not such a
     call."""
-    if logits.dim() != 2:
+    if logits.dim() != 2 or not _quiet({type(t) for t in (logits, history, lengths, prompt, *penalties, ids, values, mask,
+                                                          state)}):
         return None
     (B, V), index, dt = logits.shape, logits.get_device(), logits.dtype
     if not (logits.is_cuda and 0 < B <= 65535 and 0 < V <= 1 << 26 and dt in _FLOATS and index == _device()
@@ -207,8 +208,6 @@ def _plain(logits, history, lengths, prompt, penalties, ids, values, mask, state
                 and (S in (1, B) if state is None else _fits(state, _I64, index, row))):
             return None
     elif state is not None:
-        return None
-    if not _quiet({type(t) for t in (logits, history, lengths, prompt, *penalties, ids, values, mask, state)}):
         return None
     got = logits.new_empty(B, dtype=_I64) if choose else torch.empty_like(logits)
     nbytes = _gen_workspace(B, V) if choose else 0
