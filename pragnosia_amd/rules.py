@@ -38,6 +38,12 @@ def _in_range(name: str, p: float) -> bool:
     return _TINY <= p <= _MAX if name == "repetition" else -_MAX <= p <= _MAX
 
 
+def _marks_fit(L: int, M: int) -> bool:
+    """Whether a history of L (up to 2^24) and a list of M (up to 2^20) entries have 31 bits together at most, by comparisons
+    alone: in a trace a size is no Python number and has no bit_length."""
+    return not any(M >= 1 << k - 1 and L >= 1 << 31 - k for k in range(7, 22))
+
+
 def _out_of_range(what: str, name: str, p: float) -> PragnosiaError:
     return PragnosiaError(f"{what}: {name} must be finite{' and above 0' if name == 'repetition' else ''} in fp32, got {p}")
 
@@ -74,7 +80,7 @@ def _checked(op: str, logits: Tensor, history: Optional[Tensor], lengths: Option
         if ids.dim() not in (1, 2) or (ids.dim() == 2 and ids.shape[0] != B) or ids.shape[-1] > 1 << 20:
             raise PragnosiaError(f"{op}: bias ids (M) or ({B}, M) with M up to 2^20 expected, got {tuple(ids.shape)}")
         _expect(op, dev, bias_ids=(ids, tuple(ids.shape)), bias_values=(values, tuple(ids.shape)))
-        if history is not None and history.shape[1].bit_length() + ids.shape[-1].bit_length() > 31:
+        if history is not None and not _marks_fit(history.shape[1], ids.shape[-1]):
             raise PragnosiaError(f"{op}: the lengths of history and bias list must have 31 bits together at most, got "
                                  f"{history.shape[1]} and {ids.shape[-1]}")
         if not values.is_floating_point():

@@ -59,16 +59,18 @@ def linear(W, x, codes, scales, w, b, bias, resid, *rest):
     return fp4.linear(x, weight4(codes, scales), bias, act="gelu", resid=resid)
 
 
-def by_rules(call):
+def by_rules(call, listed=False):
     def f(W, x, codes, scales, w, b, bias, resid, logits, history, lengths, repetition, ids, values, mask, state):
-        return call(logits, history, lengths, repetition=repetition, presence=0.5, mask=mask, state=state)
+        return call(logits, history, lengths, repetition=repetition, presence=0.5, bias=(ids, values) if listed else None,
+                    mask=mask, state=state)
     return f
 
 
 CALLS = [(quantize, "fp4_quantize"), (dequantize, "fp4_dequantize"), (round_trip, "fp4_dequantize"), (linear, "fp4_linear"),
-         (by_rules(rules.next_token), "rules_token"), (by_rules(rules.apply_rules), "rules_apply")]
-each = pytest.mark.parametrize("f,op", CALLS, ids=["quantize", "dequantize", "round_trip", "linear", "next_token",
-                                                   "apply_rules"])
+         (by_rules(rules.next_token), "rules_token"), (by_rules(rules.apply_rules), "rules_apply"),
+         (by_rules(rules.next_token, True), "rules_token"), (by_rules(rules.apply_rules, True), "rules_apply")]
+each = pytest.mark.parametrize("f,op", CALLS, ids=["quantize", "dequantize", "round_trip", "linear", "next_token", "apply_rules",
+                                                   "next_token_listed", "apply_rules_listed"])
 
 
 def flat(out):
@@ -168,3 +170,12 @@ def test_exported():
     W, x, codes, scales, *rest = operands()
     got = torch.export.export(Layer(), (x, codes, scales)).graph_module.code
     assert "fp4_linear" in got
+
+
+def test_marks_of_31_bits():
+    """The comparisons are those of the lengths in bits."""
+    sizes = sorted({v for k in range(25) for v in ((1 << k) - 1, 1 << k, (1 << k) + 1) if v <= 1 << 24})
+    for L in sizes:
+        for M in sizes:
+            if M <= 1 << 20:
+                assert rules._marks_fit(L, M) == (L.bit_length() + M.bit_length() <= 31), (L, M)
