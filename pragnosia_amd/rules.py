@@ -320,7 +320,7 @@ class TokenRules:
     """Rules that `GreedyDecoder` chooses tokens under, with the meanings of `next_token`: repetition counts the prompt,
     presence and frequency what was generated. A grammar is an automaton on the GPU: `mask` (S, ceil(V / 32)) holds the words
     allowed in each state, `next` (S, V) int32 the state after each word (-1: free from then on; S or more: nothing may
-    follow), `state` (B) the states to begin in (0 by default). Without `next` the states stay."""
+    follow), `state` (B) the states to begin in (0 by default, for every sequence). Without `next` the states stay."""
     repetition: Penalty = 1.0
     presence: Penalty = 0.0
     frequency: Penalty = 0.0
@@ -339,11 +339,11 @@ class RuleState:
         e = lambda *s, dt=_I64: torch.zeros(*s, device=device, dtype=dt)  # noqa: E731
         self.history, self.lengths, self.prompt = e(B, capacity), e(B), e(B)
         self.penalties = [e(B, dt=_F32) for _ in range(3)]
-        ids, _, mask, state, nxt = self.shapes
+        ids, _, mask, _, nxt = self.shapes
         self.bias = None if ids is None else (e(*ids), e(*ids, dt=_F32))
         self.mask = None if mask is None else e(*mask, dt=torch.int32)
         self.next = None if nxt is None else e(*nxt, dt=torch.int32)
-        self.state = e(B) if state is not None or nxt is not None else None
+        self.state = e(B) if mask is not None else None  # (0, also of a mask that has as many lines as there are rows)
 
     @staticmethod
     def shapes_of(rules: TokenRules):
@@ -356,6 +356,8 @@ class RuleState:
                 self.mask.shape[0], self.V))):
             raise PragnosiaError("TokenRules: bias ids and values of one shape, and next (S, V) beside mask (S, words), "
                                  f"expected, got {self.shapes}")
+        if rules.state is not None and self.mask is None:
+            raise PragnosiaError("TokenRules: state names a line of the mask; there is none")
         for name, buf in zip(("repetition", "presence", "frequency"), self.penalties):
             p = getattr(rules, name)
             if not isinstance(p, Tensor) and not _in_range(name, p):
