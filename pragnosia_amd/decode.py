@@ -456,16 +456,18 @@ class GreedyDecoder:
         self.n_max = n_max
 
     def _load_rules(self, prompt, n):
-        """The rules and the prompt into the graph's buffers; a graph of other buffers is let go."""
+        """The rules and the prompt into the graph's buffers; a graph of other buffers is let go. Rules that are refused leave
+        the buffers, and the graph that reads them, as they were."""
         rs = None
         if self.rules is not None:
             V, dev = self.m.e.weight.shape[0], self.m.e.weight.device
-            need = (0 if prompt is None else prompt.shape[1]) + n + self.K
+            need = (0 if prompt is None else prompt.shape[-1]) + n + self.K
+            RuleState.check(self.rules, prompt, self.B, V, need)
             rs = self.rs
             if rs is None or rs.shapes != RuleState.shapes_of(self.rules) or need > rs.capacity:
                 rs = RuleState(self.rules, self.B, V, need, dev)
             rs.load(self.rules, prompt)
-        if rs is not self.rs:  # (rules that were refused leave the buffers, and the graph that reads them, as they were)
+        if rs is not self.rs:
             self.rs, self.graph = rs, None
 
     @torch.no_grad()

@@ -350,18 +350,51 @@ class RuleState:
         ids, values = (None, None) if rules.bias is None else rules.bias
         return tuple(None if t is None else tuple(t.shape) for t in (ids, values, rules.mask, rules.state, rules.next))
 
+    @staticmethod
+    def check(rules: TokenRules, prompt: Optional[Tensor], B: int, V: int, capacity: int) -> None:
+        """Refuses what `load` or a step would not take, before anything is made or written. A tensor of one value for B
+        counts for every sequence."""
+        def no(what, got):
+            raise PragnosiaError(f"TokenRules: {what} expected, got {got}")
+
+        def shown(t):
+            return f"{tuple(t.shape)} {t.dtype}"
+
+        each = ((B,), (1,), ())
+        if capacity > 1 << 24:
+            no("a prompt and a run of at most 2^24 tokens together", capacity)
+        if prompt is not None and (prompt.dim() != 2 or prompt.shape[0] not in (1, B) or prompt.dtype not in _INTS):
+            no(f"a prompt of integers ({B}, P)", shown(prompt))
+        for name in ("repetition", "presence", "frequency"):
+            p = getattr(rules, name)
+            if isinstance(p, Tensor):
+                if tuple(p.shape) not in each or not (p.is_floating_point() or p.dtype in _INTS):
+                    no(f"{name}, a number or numbers ({B},),", shown(p))
+            elif not _in_range(name, p):
+                raise _out_of_range("TokenRules", name, p)
+        if rules.bias is not None:
+            ids, values = rules.bias
+            if (ids.dim() not in (1, 2) or (ids.dim() == 2 and ids.shape[0] != B) or ids.shape[-1] > 1 << 20
+                    or ids.dtype not in _INTS):
+                no(f"bias ids, integers (M) or ({B}, M) with M up to 2^20,", shown(ids))
+            if values.shape != ids.shape or not (values.is_floating_point() or values.dtype in _INTS):
+                no(f"bias values {tuple(ids.shape)}", shown(values))
+            if not _marks_fit(capacity, ids.shape[-1]):
+                no("prompt, run and bias list of 31 bits together at most", (capacity, ids.shape[-1]))
+        mask, state, nxt, words = rules.mask, rules.state, rules.next, (V + 31) // 32
+        if mask is not None and (mask.dim() != 2 or mask.shape[0] == 0 or mask.shape[1] != words
+                                 or mask.dtype not in (torch.int32, _I64)):
+            no(f"mask (S, {words}) int32 with S > 0", shown(mask))
+        if state is not None and (mask is None or tuple(state.shape) not in each or state.dtype not in _INTS):
+            no(f"state, integers ({B},) beside a mask,", shown(state))
+        if nxt is not None and (mask is None or tuple(nxt.shape) != (mask.shape[0], V)
+                                or nxt.dtype not in (torch.int32, _I64)):
+            no("next (S, V) int32 beside mask (S, words)", shown(nxt))
+
     def load(self, rules: TokenRules, prompt: Optional[Tensor]) -> None:
-        """The rules' present values, the prompt (B, P) as history, and the states to begin in."""
-        if self.shapes[0] != self.shapes[1] or (self.next is not None and (self.mask is None or self.next.shape != (
-                self.mask.shape[0], self.V))):
-            raise PragnosiaError("TokenRules: bias ids and values of one shape, and next (S, V) beside mask (S, words), "
-                                 f"expected, got {self.shapes}")
-        if rules.state is not None and self.mask is None:
-            raise PragnosiaError("TokenRules: state names a line of the mask; there is none")
+        """The rules' present values, the prompt (B, P) as history, and the states to begin in; all checked before."""
         for name, buf in zip(("repetition", "presence", "frequency"), self.penalties):
             p = getattr(rules, name)
-            if not isinstance(p, Tensor) and not _in_range(name, p):
-                raise _out_of_range("TokenRules", name, p)
             buf.copy_(p) if isinstance(p, Tensor) else buf.fill_(float(p))
         if self.bias is not None:
             self.bias[0].copy_(rules.bias[0]), self.bias[1].copy_(rules.bias[1])

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from pragnosia_amd._lib import PragnosiaError
 from pragnosia_amd.decode import GreedyDecoder
 from pragnosia_amd.model import LM
 from pragnosia_amd.rules import TokenRules
@@ -23,12 +24,12 @@ def prompt(B, P, seed=1):
     return torch.randint(0, V, (B, P), generator=torch.Generator().manual_seed(seed)).to(DEV)
 
 
-def lines(S, share=0.1, seed=0):
+def lines(S, share=0.1, seed=0, dev=DEV):
     """Words (S, V) that a grammar allows, and the same as bits."""
     allowed = torch.rand(S, V, generator=torch.Generator().manual_seed(seed)) < share
     bits = torch.zeros(S, (V + 31) // 32 * 32, dtype=torch.long)
     bits[:, :V] = allowed
-    return allowed, (bits.view(S, -1, 32) << torch.arange(32)).sum(2).to(torch.int32).to(DEV)
+    return allowed, (bits.view(S, -1, 32) << torch.arange(32)).sum(2).to(torch.int32).to(dev)
 
 
 @pytest.mark.parametrize("mixer,d", [("aspin", 256), ("fspin", 128)])
@@ -45,3 +46,66 @@ def test_states_begin_at_zero_and_stay(S, mixer, d):
     state = torch.arange(B, device=DEV) % S
     got = GreedyDecoder(model(mixer, d), B, rules=TokenRules(mask=mask, state=state)).generate(prompt(B, 9), n).cpu()
     assert all(allowed[b % S][got[b]].all() for b in range(B))
+
+
+def refused():
+    """Rules that differ from `TokenRules(repetition=1.3, mask=, next=)` in one thing a step does not take."""
+    _, mask = lines(4, dev="cpu")
+    nxt = torch.zeros(4, V, dtype=torch.int32)
+    good = dict(repetition=9.0, mask=mask.roll(1, 0), next=nxt + 1)
+    i = lambda *s: torch.zeros(*s, dtype=torch.long)  # noqa: E731
+    return {"presence": good | dict(presence=float("inf")), "frequency": good | dict(frequency=1e39),
+            "penalties' number": good | dict(frequency=torch.zeros(5)), "mask's width": dict(repetition=9.0, mask=mask[:, 1:]),
+            "mask's type": good | dict(mask=mask.float()), "next's shape": good | dict(next=nxt[:, 1:]),
+            "next's type": good | dict(next=nxt.float()), "next alone": dict(repetition=9.0, next=nxt),
+            "state alone": dict(repetition=9.0, state=i(3)), "states' number": good | dict(state=i(5)),
+            "state's type": good | dict(state=torch.zeros(3)), "list's ids": good | dict(bias=(torch.zeros(4), torch.zeros(4))),
+            "list's rows": good | dict(bias=(i(2, 4), torch.zeros(2, 4))), "list's values": good | dict(bias=(i(4), torch.zeros(3))),
+            "list of none": good | dict(bias=(torch.tensor(3), torch.tensor(1.0)))}
+
+
+@pytest.mark.parametrize("what", list(refused()))
+def test_refused_rules_write_nothing(what):
+    """Nothing of the refused rules reaches the buffers: the run goes on as it would have."""
+    B, n = 3, 33
+    _, mask = lines(4)
+    good = TokenRules(repetition=1.3, mask=mask, next=(torch.arange(4, device=DEV) + 1).remainder(4).int()[:, None].expand(4, V))
+    x = prompt(B, 9)
+    dec = GreedyDecoder(model(), B, rules=good)
+    want = dec.generate(x, n)
+    states, pw, lg = dec.prefill(x)
+    dec.start(states, pw, lg, n, x)
+    dec.replay(17)
+    rs, graph = dec.rs, dec.graph
+    buffers = [*rs.penalties, rs.mask, rs.next, rs.state, rs.history, rs.lengths, rs.prompt]
+    before = [t.clone() for t in buffers]
+    dec.rules = TokenRules(**refused()[what])
+    with pytest.raises(PragnosiaError, match="TokenRules"):
+        dec.generate(x, n)
+    assert dec.rs is rs and dec.graph is graph and all(torch.equal(a, b) for a, b in zip(buffers, before))
+    dec.replay(17)  # (the other half of the run)
+    assert torch.equal(dec.out[:n].t(), want)
+
+
+@pytest.mark.parametrize("x", [torch.zeros(2, 9, dtype=torch.long), torch.zeros(3, 9), torch.zeros(9, dtype=torch.long)])
+def test_prompts_are_refused(x):
+    """Of another number of sequences, of numbers that are no ids, of one dimension."""
+    dec = GreedyDecoder(model(), 3, rules=TokenRules(repetition=1.3))
+    states, pw, lg = dec.prefill(prompt(3, 9))
+    with pytest.raises(PragnosiaError, match="prompt"):
+        dec.start(states, pw, lg, 20, x.to(DEV))
+    assert dec.rs is None and dec.graph is None
+
+
+def test_one_value_for_every_sequence():
+    """Penalties and states of one value, numbers of other types, successors in 64 bits, tensors on the CPU."""
+    B, n, x = 3, 20, prompt(3, 9)
+    _, mask = lines(4)
+    nxt = torch.randint(0, 4, (4, V), generator=torch.Generator().manual_seed(5))
+    ids = torch.arange(0, 60, 2)
+    m = model()
+    want = GreedyDecoder(m, B, rules=TokenRules(torch.full((B,), 1.5, device=DEV), 0.5, 1.0, (ids.to(DEV), ids.float().to(DEV)),
+                                                mask, torch.full((B,), 2, device=DEV), nxt.int().to(DEV))).generate(x, n)
+    got = GreedyDecoder(m, B, rules=TokenRules(torch.tensor(1.5).double(), torch.tensor([0.5]).half(), torch.tensor([1, 1, 1]),
+                                               (ids.int(), ids), mask.long().cpu(), torch.tensor([2]), nxt)).generate(x, n)
+    assert torch.equal(got, want)
