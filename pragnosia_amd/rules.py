@@ -401,7 +401,8 @@ class RuleState:
         if self.mask is not None:
             self.mask.copy_(rules.mask)
         if self.next is not None:
-            self.next.copy_(rules.next)
+            nxt = rules.next  # (64-bit states past 32 bits stay past the last)
+            self.next.copy_(nxt if nxt.dtype == torch.int32 else nxt.clamp(-1, nxt.shape[0]))
         if self.state is not None:
             self.state.zero_() if rules.state is None else self.state.copy_(rules.state)
         P = 0 if prompt is None else prompt.shape[1]

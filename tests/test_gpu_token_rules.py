@@ -109,3 +109,14 @@ def test_one_value_for_every_sequence():
     got = GreedyDecoder(m, B, rules=TokenRules(torch.tensor(1.5).double(), torch.tensor([0.5]).half(), torch.tensor([1, 1, 1]),
                                                (ids.int(), ids), mask.long().cpu(), torch.tensor([2]), nxt)).generate(x, n)
     assert torch.equal(got, want)
+
+
+def test_successors_past_32_bits():
+    """A state of 2^40, as one of S, lets nothing follow; one of -2^40, as -1, anything."""
+    B, n, x, (_, mask) = 2, 12, prompt(2, 9), lines(2)
+    m = model()
+    for far, near in ((1 << 40, 2), (1 << 32, 2), (-(1 << 40), -1)):
+        runs = [GreedyDecoder(m, B, rules=TokenRules(mask=mask, next=torch.full((2, V), s, device=DEV))).generate(x, n)
+                for s in (far, near)]
+        assert torch.equal(*runs)
+        assert (runs[0][:, 1:] == -1).all() == (far > 0)
