@@ -232,7 +232,7 @@ def linear(x: Tensor, Q: Weight4, bias: Optional[Tensor] = None, *, norm: Option
         lnw, lnb, eps = norm.weight, norm.bias, norm.eps
     if act not in _ACTS:
         raise PragnosiaError(f"linear: act must be None or 'gelu', got {act!r}")
-    if x.dim() == 0 or (resid is not None and resid.shape != (*x.shape[:-1], N)):
+    if x.dim() == 0 or x.shape[-1] == 0 or (resid is not None and resid.shape != (*x.shape[:-1], N)):
         raise PragnosiaError(f"linear: x (..., {K}) and resid (..., {N}) expected, got {tuple(x.shape)} and "
                              f"{None if resid is None else tuple(resid.shape)}")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lnw, lnb, bias, resid)):

@@ -200,7 +200,7 @@ def _plain(logits, history, lengths, prompt, penalties, ids, values, mask, state
             and -_MAX <= args[5] <= _MAX):
         return None
     if ids is not None:
-        M = ids.shape[-1]
+        M = ids.shape[-1] if ids.dim() else 0
         shape = row + (M,) if ids.dim() == 2 else (M,)
         if not (0 < M <= 1 << 20 and L.bit_length() + M.bit_length() <= 31 and values is not None
                 and _fits(ids, _I64, index, shape) and _fits(values, _F32, index, shape)):
@@ -273,7 +273,7 @@ def advance(tokens: Tensor, history: Optional[Tensor] = None, lengths: Optional[
     is outside the vocabulary (-1: nothing was left) stay as they are; without next, the vocabulary is `vocab` words."""
     if next is None and vocab is None:
         raise PragnosiaError("advance: the vocabulary's size, as `next` or `vocab`, is needed")
-    V = next.shape[-1] if next is not None else vocab
+    V = vocab if next is None else next.shape[-1] if next.dim() else 0
     _check_advance("advance", tokens, history, lengths, next, state, V)
     if _watched(tokens, history, lengths, next, state):
         raise PragnosiaError("advance: not available in a trace or under a dispatch mode (it works in place)")
@@ -291,8 +291,8 @@ def _check_advance(op: str, tokens, history, lengths, next, state, V: int) -> No
         if t is not None and (t.dtype != _I64 or not (t.is_contiguous() or (name == "history" and t.stride(1) == 1 and
                                                                             t.stride(0) >= t.shape[1]))):
             raise PragnosiaError(f"{op}: {name} must be int64 and dense (history's rows), as it is changed in place")
-    if next is not None and (next.dtype != torch.int32 or not next.is_contiguous() or next.shape[0] == 0):
-        raise PragnosiaError(f"{op}: next (S, V) must be dense int32 with S > 0, got {tuple(next.shape)} {next.dtype}")
+    if next is not None and (next.dtype != torch.int32 or not next.is_contiguous() or next.numel() == 0):
+        raise PragnosiaError(f"{op}: next (S, V) must be dense int32 with S > 0 and V > 0, got {tuple(next.shape)} {next.dtype}")
     if history is not None and history.shape[1] == 0:
         raise PragnosiaError(f"{op}: a history of no entries has no room")
 
