@@ -186,9 +186,10 @@ class GreedyDecoder:
         else:
             nxt = self.rs.choose(lg.float().contiguous())
             self.rs.advance(nxt)
+        at = self.ctr.clamp(max=self.out.shape[0])
         if self.lgs is not None:
-            self.lgs.index_copy_(0, self.ctr, lg.float().view(1, self.B, -1))
-        self.out.index_copy_(0, self.ctr, nxt.view(1, -1))
+            self.lgs_past.index_copy_(0, at, lg.float().view(1, self.B, -1))
+        self.out_past.index_copy_(0, at, nxt.view(1, -1))
         self.ctr.add_(1)
         # (-1, nothing left, is -1 from then on, whatever is read in its place)
         self.tok.copy_((nxt if self.rs is None else nxt.clamp(min=0)).view(-1, 1))
@@ -368,7 +369,7 @@ class GreedyDecoder:
         m = self.m
         if self.rs is not None:
             if self.lgs is not None:
-                self.lgs.index_copy_(0, self.ctrb[par:par + 1], lg.view(1, self.B, -1))
+                self.lgs_past.index_copy_(0, self.ctrb[par:par + 1].clamp(max=self.out.shape[0]), lg.view(1, self.B, -1))
             self.rs.advance(self.rs.choose(lg), (m.e.weight, m.p.weight, self.ctrb[par], self.ctrb[1 - par], self.posb[par],
                                                  self.posb[1 - par], self.out, self.tok, self.h, self.p0s))
             return
@@ -433,14 +434,17 @@ class GreedyDecoder:
                         else None for st, mx in zip(self.st, self.m.mix)]
         self.tok = torch.zeros(self.B, 1, dtype=torch.long, device=dev)
         self.pos = torch.zeros(1, dtype=torch.long, device=dev)
-        self.out = torch.zeros(n_max + self.K, self.B, dtype=torch.long, device=dev)
+        # (a row past the last, where steps past the run's end are put that index their row)
+        self.out_past = torch.zeros(n_max + self.K + 1, self.B, dtype=torch.long, device=dev)
+        self.out = self.out_past[:-1]
         self.ctr = torch.zeros(1, dtype=torch.long, device=dev)
         if self.fused:  # the fused step's input and the tail kernel's alternating counter and position slots
             self.h = torch.zeros(self.B, self.m.d, device=dev, dtype=torch.float32)
             self.ctrb = torch.zeros(2, dtype=torch.long, device=dev)
             self.posb = torch.zeros(2, dtype=torch.long, device=dev)
         if self.record:
-            self.lgs = torch.zeros(n_max + self.K, self.B, self.m.e.weight.shape[0], dtype=torch.float32, device=dev)
+            self.lgs_past = torch.zeros(n_max + self.K + 1, self.B, self.m.e.weight.shape[0], dtype=torch.float32, device=dev)
+            self.lgs = self.lgs_past[:-1]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         step = (self._one_step if not self.fused else self._one_step_fp4 if self.weights else
@@ -501,7 +505,8 @@ class GreedyDecoder:
 
     @torch.no_grad()
     def replay(self, n):
-        """Run ceil((n - 1) / steps_per_graph) graph replays (the first token came from the prefill's logits)."""
+        """Run ceil((n - 1) / steps_per_graph) graph replays (the first token came from the prefill's logits). Steps past those
+        that `start` made room for run, and leave no token, logits or history behind."""
         for _ in range(-(-(n - 1) // self.K)):
             self.graph.replay()
 

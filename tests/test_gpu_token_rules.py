@@ -120,3 +120,23 @@ def test_successors_past_32_bits():
                 for s in (far, near)]
         assert torch.equal(*runs)
         assert (runs[0][:, 1:] == -1).all() == (far > 0)
+
+
+@pytest.mark.parametrize("rules", [None, TokenRules(repetition=1.4)])
+@pytest.mark.parametrize("mixer,d,weights", [("aspin", 256, None), ("aspin", 256, "fp4"), ("fspin", 128, None)])
+def test_replays_past_the_end(mixer, d, weights, rules):
+    """More steps than a run has room for: what was recorded of it stays, and the next run is as the first."""
+    B, n, x = 2, 9, prompt(2, 12)
+    dec = GreedyDecoder(model(mixer, d), B, record_logits=True, weights=weights, rules=rules)
+    want = dec.generate(x, n)
+    states, pw, lg = dec.prefill(x)
+    dec.start(states, pw, lg, n, x)
+    dec.replay(n)
+    logits = dec.logits(n).clone()  # (of this run: the fp32 step adds with atomics, whose last bits differ by run)
+    dec.replay(n)  # (the last rows that there are)
+    out, lgs = dec.out.clone(), dec.lgs.clone()
+    for _ in range(3):
+        dec.replay(n)
+    assert torch.equal(dec.out, out) and torch.equal(dec.lgs, lgs) and dec.out.shape == (n + 8, B)
+    assert torch.equal(dec.out[:n].t(), want) and torch.equal(dec.logits(n), logits)
+    assert torch.equal(dec.generate(x, n), want)
