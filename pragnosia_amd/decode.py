@@ -423,6 +423,7 @@ class GreedyDecoder:
 
     def _capture(self, states, n_max):
         dev = self.m.e.weight.device
+        self.graph = None  # (the buffers that an earlier one reads and writes go now, also if this capture fails)
         self.st = self._static_states(states)
         if self.fused:
             self.gemm = self._gemm_ok()

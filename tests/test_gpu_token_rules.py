@@ -140,3 +140,16 @@ def test_replays_past_the_end(mixer, d, weights, rules):
     assert torch.equal(dec.out, out) and torch.equal(dec.lgs, lgs) and dec.out.shape == (n + 8, B)
     assert torch.equal(dec.out[:n].t(), want) and torch.equal(dec.logits(n), logits)
     assert torch.equal(dec.generate(x, n), want)
+
+
+def test_a_capture_that_fails_leaves_no_graph(monkeypatch):
+    """A graph whose buffers were let go cannot be replayed; the next start captures one."""
+    x = prompt(2, 9)
+    dec = GreedyDecoder(model(), 2, rules=TokenRules(repetition=1.3))
+    want = dec.generate(x, 30)
+    with monkeypatch.context() as patch:
+        patch.setattr(dec, "_load_weights", lambda: (_ for _ in ()).throw(MemoryError("no room")))
+        with pytest.raises(MemoryError):
+            dec.generate(x, 60)
+    assert dec.graph is None
+    assert torch.equal(dec.generate(x, 60)[:, :30], want)
