@@ -12,9 +12,10 @@ batch, weights="fp4")` runs a model's decode step on them; the reference decodes
 be: fp32 rows, and normalised rows of either type, are not rounded (they go through the bf16 matrix cores in three parts),
 other bf16 rows are taken as they are. Sums are taken in a fixed order: the same call gives the same bits.
 
-There is no backward: an input that requires a gradient is refused where gradients are recorded. An eager call goes
-straight to the C ABI; one that something records or replaces (torch.compile, make_fx, torch.jit.trace, a dispatch mode)
-goes through the custom ops `pragnosia_gen::fp4_*`.
+There is no backward: `linear` refuses an input that requires a gradient where gradients are recorded. `quantize` takes the
+present values of a weight, also of a parameter that is being trained; no gradient leads back through the codes. An eager
+call goes straight to the C ABI; one that something records or replaces (torch.compile, make_fx, torch.export,
+torch.jit.trace, a dispatch mode) goes through the custom ops `pragnosia_gen::fp4_*`.
 """
 from __future__ import annotations
 
@@ -118,8 +119,8 @@ def _check_source(op: str, W: Tensor, group: int) -> tuple[int, int]:
 def quantize(W: Tensor, group: int = 64, out: Optional[Weight4] = None) -> Weight4:
     """W (N, K), fp32 or bf16, in 4 bits with a scale for each `group` (32, 64 or 128) columns of a row. A scale is
     max |w| / 6 rounded to bf16, a code the nearest value (ties to the even code, past 6 to 6); a group with an infinity or
-    a NaN becomes NaN throughout. `out`: a Weight4 of the same sizes, group and device to write into (one that a captured
-    graph reads, say)."""
+    a NaN becomes NaN throughout. A W that requires a gradient is detached. `out`: a Weight4 of the same sizes, group and
+    device to write into (one that a captured graph reads, say)."""
     # the usual call, without the general path's looks at everything (10 us of host; this 7)
     if W.dim() == 2 and out is None and _quiet({type(W)}):
         index, dt, (N, K) = W.get_device(), W.dtype, W.shape

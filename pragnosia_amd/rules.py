@@ -247,10 +247,11 @@ def apply_rules(logits: Tensor, history: Optional[Tensor] = None, lengths: Optio
     [0, L]. repetition (above 0), presence and frequency: a number finite in fp32, or a (B,) tensor for each row its own, whose
     values are taken as they are. bias: (ids,
     values), both (M) or (B, M): the last entry of a repeated id counts, ids outside [0, V) are skipped, -inf bans a
-    word; L and M must have 31 bits together at most (2^15 entries on 2^15 tokens). mask (S, ceil(V / 32)) int32: word v
-    is allowed where bit v % 32 of word v // 32 is set; state (B) picks each row's line (by default its own of B, or the
-    only one): a negative state leaves the row unmasked, one of S or more masks every word. For inference: no input may
-    require a gradient where gradients are recorded."""
+    word whose logit is finite (of an infinity or a NaN it makes a NaN; a mask bans any); L and M must have 31 bits together
+    at most (2^15 entries on 2^15 tokens). mask (S, ceil(V / 32)) int32: word v is allowed where bit v % 32 of word v // 32 is
+    set; state (B) picks each row's line (by default its own of B, or the only one): a negative state leaves the row
+    unmasked, one of S or more masks every word. For inference: no input may require a gradient where gradients are
+    recorded."""
     return _rules("apply_rules", logits, history, lengths, prompt, repetition, presence, frequency, bias, mask, state,
                   False)
 
@@ -292,7 +293,8 @@ def _check_advance(op: str, tokens, history, lengths, next, state, V: int) -> No
                                                                             t.stride(0) >= t.shape[1]))):
             raise PragnosiaError(f"{op}: {name} must be int64 and dense (history's rows), as it is changed in place")
     if next is not None and (next.dtype != torch.int32 or not next.is_contiguous() or next.numel() == 0):
-        raise PragnosiaError(f"{op}: next (S, V) must be dense int32 with S > 0 and V > 0, got {tuple(next.shape)} {next.dtype}")
+        raise PragnosiaError(f"{op}: next (S, V) must be dense int32 with S > 0 and V > 0, got {tuple(next.shape)} "
+                             f"{next.dtype}")
     if history is not None and history.shape[1] == 0:
         raise PragnosiaError(f"{op}: a history of no entries has no room")
 
