@@ -345,15 +345,14 @@ class GreedyDecoder:
                 op.aspin_decode_oproj_(src, dst, *step, mx.on.weight, on_eps, mx.o.weight, self.sig[i], h)
                 x1 = h
             else:
-                rms = self.gemm or (self.B <= GEMV_MAX_BATCH and _rms_gemv_ok(mx.h * mx.dk))
+                # (heads of 128 at GEMV batch sizes: _rms_gemv_ok holds, or the step would not run fused)
+                rms = self.gemm or self.B <= GEMV_MAX_BATCH
                 o = op.aspin_decode_proj_(self.st[i][0], *step, None if rms else mx.on.weight, on_eps)
                 if self.gemm:
                     op.decode_gemm_acc_(o, self.otile[i], 2 if mx.dk == 64 else 3, on_eps, None, self.sig[i], h)
                     x1 = h
                 elif rms:
                     x1 = op.decode_gemv_rms(o, mx.o.weight, mx.on.weight, on_eps, None, self.sig[i], 0, h)
-                elif self.B <= GEMV_MAX_BATCH:
-                    x1 = self._dense(o, mx.o.weight, None, scale=self.sig[i], resid=h)
                 else:
                     x1 = torch.addmm(h, o, self.wos[i].t())
             hm = fp4.linear(x1, qa, mp.a.bias, norm=mp.n, act="gelu")

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from pragnosia_amd import decode
 from pragnosia_amd._lib import PragnosiaError
 from pragnosia_amd.decode import GreedyDecoder
 from pragnosia_amd.model import LM
@@ -153,3 +154,22 @@ def test_a_capture_that_fails_leaves_no_graph(monkeypatch):
             dec.generate(x, 60)
     assert dec.graph is None
     assert torch.equal(dec.generate(x, 60)[:, :30], want)
+
+
+@pytest.mark.parametrize("rules", [None, TokenRules(repetition=1.4)])
+@pytest.mark.parametrize("mixer", ["aspin", "dspin"])
+def test_fp4_step_where_decode_gemm_covers_no_width(monkeypatch, mixer, rules):
+    """The o-projection as a product of torch's, beside 4-bit weights: the logits of the step that covers it."""
+    B, n, x, m = 6, 25, prompt(6, 12), model(mixer)
+    runs = []
+    for covered in (True, False):
+        with monkeypatch.context() as patch:
+            if not covered:
+                patch.setattr(decode, "_gemm_layers_ok", lambda model: False)
+            dec = GreedyDecoder(m, B, record_logits=True, weights="fp4", rules=rules)
+            runs.append((dec.generate(x, n), dec.logits(n).clone()))
+            assert dec.gemm is covered
+    (want, a), (got, b) = runs
+    assert torch.equal(got, want)
+    for t in range(n):  # (a step is held to 1e-4, and states carry it on)
+        assert (a[:, t] - b[:, t]).abs().max() <= 1e-4 * (t + 2) * a[:, t].abs().max()
