@@ -10,7 +10,9 @@ batch, weights="fp4")` runs a model's decode step on them; the reference decodes
 
 `linear` multiplies the values s v that the codes stand for, with fp32 sums, and is as exact as its operands' type lets it
 be: fp32 rows, and normalised rows of either type, are not rounded (they go through the bf16 matrix cores in three parts),
-other bf16 rows are taken as they are. Sums are taken in a fixed order: the same call gives the same bits.
+other bf16 rows are taken as they are. Values of a row may lie between 2^-102, below which their last bits may be lost, and
+2^118, past which a group's sum may overflow before its scale. Sums are taken in a fixed order: the same call gives the same
+bits.
 
 There is no backward: `linear` refuses an input that requires a gradient where gradients are recorded. `quantize` takes the
 present values of a weight, also of a parameter that is being trained; no gradient leads back through the codes. An eager

@@ -43,7 +43,8 @@ int pragnosia_fp4_dequantize(const void* codes, const void* scales, void* W, int
 /* y = act(z W^T + bias) + resid for n rows: z = x, or with ln_weight (K) the LayerNorm of x's rows with ln_weight, ln_bias
  * (K, or NULL) and ln_eps; act 0: identity, 1: GELU (erf form); bias (N) and resid (n, N) may be NULL. x (n, K), the
  * norm's, bias, resid and y (n, N) all fp32 or all bf16 (bf16). Sums are fp32; fp32 rows and normalised rows of either type
- * are multiplied whole (as three bf16 parts), other bf16 rows as they are. y may be resid, and must not overlap x.
+ * are multiplied whole (as three bf16 parts; what lies below 2^-126 may be lost), other bf16 rows as they are. A group's sum
+ * of z v is formed before its scale s, so values of z past 2^118 may overflow. y may be resid, and must not overlap x.
  * n at most 2^24, n N and n K below 2^31. n = 0 does nothing. */
 int pragnosia_fp4_linear(const void* x, int bf16, const void* codes, const void* scales, const void* ln_weight,
                          const void* ln_bias, float ln_eps, const void* bias, int act, const void* resid, void* y,
