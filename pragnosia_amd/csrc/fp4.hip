@@ -614,9 +614,11 @@ constexpr int waves_per_simd() {
 // More rows. A workgroup's share: 16 RT rows, WN NT tiles of 16 columns, WK waves sharing the contracted columns of each (WN
 // WK waves). Rows go to LDS in P bf16 parts, a chunk of CB blocks of 128 columns at a time, as the matrix core takes them;
 // codes straight to registers. A chunk's loads are under way while the one before it is multiplied. Large products are bound by
-// instructions: beside a matrix instruction of 16 cycles stand its share of the conversions (4 / RT) and of the scaling of its
-// sums (2 in groups of 64); two vector instructions beside one cost 2 cycles, a third 4 more. 512 x 8192 x 4096 bf16 36.4
-// us, 945 TFLOP/s; fp32 rows are three such products (512 x 16384 x 1024 48 us).
+// instructions and by waits: beside a matrix instruction of 16 cycles stand its share of the conversions (4 / RT) and of the
+// scaling of its sums (2 in groups of 64), and two vector instructions beside one cost 2 cycles, a third 4 more; and two waves a
+// SIMD that meet at a chunk's barrier do not fill each other's waits. 512 x 8192 x 4096 bf16: 36.5 us, 945 TFLOP/s, the matrix
+// cores busy 41% of the time, a wave waiting 30% of it; fp32 rows and normalised ones are three such products (512 x 16384 x
+// 1024 48 us).
 template <class T, int P, bool LN, int GS, int kWaves, int RT, int U, int WK, int NT>
 __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<P, GS, kWaves, RT, U>())) void linear(
     const T* __restrict__ x, const u32x4* __restrict__ codes, const __bf16* __restrict__ scales, const T* __restrict__ lnw,
