@@ -21,9 +21,10 @@ graph always sees the current parameters.
 With weights="fp4" the fused step's projections, both MLP layers and the head run on 4-bit weights (`fp4.linear`, with their
 norms, biases, GELU and residuals inside), rounded from the parameters at every `start`; the gated o-projection stays fp32,
 inside the carrier step's kernels. The prompt is read on the parameters as they are, so the first token and the states that
-the steps begin with are those of fp32 weights, and the parameters stay resident beside the 4-bit weights. With `rules` (`rules.TokenRules`) every token, the first included, is the best that
-penalties, biases and a grammar leave (`rules.next_token`), -1 from where nothing is left; the history and the grammar's
-states are kept on the device, so replays still need no host.
+the steps begin with are those of fp32 weights, and the parameters stay resident beside the 4-bit weights. With `rules`
+(`rules.TokenRules`) every token, the first included, is the best that penalties, biases and a grammar leave
+(`rules.next_token`), -1 from where nothing is left; the history and the grammar's states are kept on the device, so replays
+still need no host.
 """
 from __future__ import annotations
 

@@ -390,7 +390,7 @@ class RuleState:
         if state is not None and (mask is None or tuple(state.shape) not in each or state.dtype not in _INTS):
             no(f"state, integers ({B},) beside a mask,", shown(state))
         if nxt is not None and (mask is None or tuple(nxt.shape) != (mask.shape[0], V)
-                                or nxt.dtype not in (torch.int32, _I64)):
+                                or nxt.dtype not in _INTS):
             no("next (S, V) int32 beside mask (S, words)", shown(nxt))
 
     def load(self, rules: TokenRules, prompt: Optional[Tensor]) -> None:
@@ -404,7 +404,7 @@ class RuleState:
             self.mask.copy_(rules.mask)
         if self.next is not None:
             nxt = rules.next  # (64-bit states past 32 bits stay past the last)
-            self.next.copy_(nxt if nxt.dtype == torch.int32 else nxt.clamp(-1, nxt.shape[0]))
+            self.next.copy_(nxt.clamp(-1, nxt.shape[0]) if nxt.dtype == _I64 else nxt)
         if self.state is not None:
             self.state.zero_() if rules.state is None else self.state.copy_(rules.state)
         P = 0 if prompt is None else prompt.shape[1]

@@ -173,3 +173,12 @@ def test_fp4_step_where_decode_gemm_covers_no_width(monkeypatch, mixer, rules):
     assert torch.equal(got, want)
     for t in range(n):  # (a step is held to 1e-4, and states carry it on)
         assert (a[:, t] - b[:, t]).abs().max() <= 1e-4 * (t + 2) * a[:, t].abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int64])
+def test_successors_of_other_integers(dtype):
+    B, n, x, (_, mask) = 2, 12, prompt(2, 9), lines(4)
+    nxt = torch.randint(0, 6, (4, V), generator=torch.Generator().manual_seed(6), dtype=torch.int32).to(DEV)
+    m = model()
+    want, got = (GreedyDecoder(m, B, rules=TokenRules(mask=mask, next=t)).generate(x, n) for t in (nxt, nxt.to(dtype)))
+    assert torch.equal(got, want)
